@@ -1,0 +1,276 @@
+"""Operators of libredukt_gpu.so on the caller's own device tensors (include/redukt_ops.h).
+
+The gated delta rule for one token (`delta_step`) and for whole sequences (`delta_chunk`), int8
+codes of activation rows (`quantize_rows`) and the product of codes with a scale per token and
+channel (`int8_matmul`).  Arguments are torch tensors on one GPU; work is queued on torch's
+current stream of that GPU (or on `stream`, a hipStream_t's value: outputs and workspace are
+then best passed in too, since torch frees what it allocates by its own streams).  No model
+needs to be open.  Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch
+nothing; there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import ffi
+
+NORMALIZE = 1      # REDUKT_DELTA_NORMALIZE
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+class DeltaRows(ctypes.Structure):
+    """redukt_delta_rows."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("hk", ctypes.c_uint32), ("hv", ctypes.c_uint32),
+                ("dk", ctypes.c_uint32), ("dv", ctypes.c_uint32), ("flags", ctypes.c_uint32), ("scale", ctypes.c_float),
+                ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("out_stride", ctypes.c_int64), ("g", ctypes.c_void_p), ("beta", ctypes.c_void_p),
+                ("g_stride", ctypes.c_int64), ("beta_stride", ctypes.c_int64)]
+
+
+class QuantizeRows(ctypes.Structure):
+    """redukt_quantize_rows."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("cols", ctypes.c_uint32), ("x", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
+                ("scales", ctypes.c_void_p)]
+
+
+class Int8Matmul(ctypes.Structure):
+    """redukt_int8_matmul."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("m", ctypes.c_uint32), ("n", ctypes.c_uint32), ("k", ctypes.c_uint32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("x_scales", ctypes.c_void_p),
+                ("w", ctypes.c_void_p), ("w_stride", ctypes.c_int64), ("w_scales", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64)]
+
+
+_lib = None
+
+
+def _load() -> ctypes.CDLL:
+    global _lib
+    if _lib is None:
+        L = ffi.PluginLibrary().lib
+        p, u32, u64 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
+        L.redukt_op_delta_step.argtypes = [ctypes.POINTER(DeltaRows), p, u32, p, p]
+        L.redukt_op_delta_chunk.argtypes = [ctypes.POINTER(DeltaRows), p, u32, p, p, u32, p, p, u64, p]
+        L.redukt_op_delta_chunk_workspace.argtypes = [ctypes.POINTER(DeltaRows), u32]
+        L.redukt_op_delta_chunk_workspace.restype = u64
+        L.redukt_op_quantize_rows.argtypes = [ctypes.POINTER(QuantizeRows), p]
+        L.redukt_op_int8_matmul.argtypes = [ctypes.POINTER(Int8Matmul), p]
+        for f in ("delta_step", "delta_chunk", "quantize_rows", "int8_matmul"):
+            getattr(L, "redukt_op_" + f).restype = ctypes.c_int32
+        _lib = L
+    return _lib
+
+
+def _refuse(what: str) -> None:
+    raise ffi.BackendError(ffi.BackendResult.INVALID_ARGUMENT, what)
+
+
+def _done(code: int, what: str) -> None:
+    if code:
+        raise ffi.BackendError(ffi.BackendResult.from_code(code), what)
+
+
+def _check(op: str, device, name: str, t, dtype, shape) -> None:
+    """t is a tensor on `device` of this type and shape (None: any size)."""
+    if not isinstance(t, torch.Tensor):
+        _refuse(f"{op}: {name} is not a tensor")
+    if t.device != device:
+        _refuse(f"{op}: {name} is on {t.device}, not on {device}")
+    if t.dtype != dtype:
+        _refuse(f"{op}: {name} is {t.dtype}, not {dtype}")
+    if len(t.shape) != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
+        _refuse(f"{op}: {name} has shape {tuple(t.shape)}, not {tuple('*' if w is None else w for w in shape)}")
+
+
+def _device(op: str, t):
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        _refuse(f"{op}: tensors on a GPU are needed")
+    return t.device
+
+
+def _stream(stream: Optional[int], device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+
+
+def _row_stride(op: str, name: str, t) -> int:
+    """Elements from a row of t [rows, ..., width] to the next, whose rows are contiguous."""
+    shape, strides = t.shape, t.stride()
+    want = 1
+    for i in range(len(shape) - 1, 0, -1):
+        if shape[i] != 1 and strides[i] != want:
+            _refuse(f"{op}: the rows of {name} are not contiguous")
+        want *= shape[i]
+    return strides[0] if shape[0] > 1 else want
+
+
+def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, torch.Tensor]:
+    device = _device(op, q)
+    if q.dtype not in DTYPES or q.dim() != 3:
+        _refuse(f"{op}: q [rows, key heads, dk] is bfloat16, float16 or float32")
+    T, hk, dk = q.shape
+    _check(op, device, "k", k, q.dtype, (T, hk, dk))
+    _check(op, device, "v", v, q.dtype, (T, None, None))
+    hv, dv = v.shape[1:]
+    _check(op, device, "g", g, torch.float32, (T, hv))
+    _check(op, device, "beta", beta, torch.float32, (T, hv))
+    if out is None:
+        out = torch.empty((T, hv, dv), dtype=q.dtype, device=device)
+    else:
+        _check(op, device, "out", out, q.dtype, (T, hv, dv))
+    a = DeltaRows(DTYPES[q.dtype], T, hk, hv, dk, dv, NORMALIZE if normalize else 0,
+                  dk ** -0.5 if scale is None and dk else scale or 0.0, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  out.data_ptr(), _row_stride(op, "q", q), _row_stride(op, "k", k), _row_stride(op, "v", v),
+                  _row_stride(op, "out", out), g.data_ptr(), beta.data_ptr(), _row_stride(op, "g", g),
+                  _row_stride(op, "beta", beta))
+    return a, out
+
+
+def _pool(op: str, device, name: str, t, a: DeltaRows) -> None:
+    _check(op, device, name, t, torch.float32, (None, a.hv, a.dk, a.dv))
+    if not t.is_contiguous():
+        _refuse(f"{op}: {name} is not contiguous")
+
+
+def _slots(op: str, device, slots, n: int) -> Optional[int]:
+    if slots is None:
+        return None
+    _check(op, device, "slots", slots, torch.int32, (n,))
+    if not slots.is_contiguous():
+        _refuse(f"{op}: slots is not contiguous")
+    return slots.data_ptr()
+
+
+def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[float] = None, normalize: bool = False,
+               stream: Optional[int] = None):
+    """The gated delta rule for one token of each of n entries; states are stepped in place.
+
+    q, k [n, key heads, dk] and v [n, value heads, dv] in bfloat16, float16 or float32; g (log
+    decay) and beta (write strength) [n, value heads] float32; states [slots, value heads, dk,
+    dv] float32.  Entry i steps slot slots[i] (int32; None: slot i); -1 leaves entry i's output
+    and state as they are; a slot out of range, or named by an earlier entry, gives NaN outputs
+    and touches no state.  scale: of the outputs (None: dk ** -0.5).  normalize: k and q are
+    divided by sqrt(sum of squares + 1e-6) first.  Returns out [n, value heads, dv] (allocated
+    if None).  dk is 64 or 128, dv a multiple of 32 up to 256; rows may be strided (slices of
+    one projection's output), by whole 16 bytes.
+    """
+    op = "delta_step"
+    a, out = _rows(op, q, k, v, g, beta, out, scale, normalize)
+    device = q.device
+    _pool(op, device, "states", states, a)
+    code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
+                                        _slots(op, device, slots, a.rows), _stream(stream, device))
+    _done(code, op)
+    return out
+
+
+def delta_chunk_workspace(tokens: int, sequences: int, hk: int, hv: int, dk: int, dv: int, dtype) -> int:
+    """Bytes of workspace that `delta_chunk` needs for these sizes."""
+    if dtype not in DTYPES:
+        _refuse("delta_chunk_workspace: bfloat16, float16 or float32")
+    return _load().redukt_op_delta_chunk_workspace(ctypes.byref(DeltaRows(DTYPES[dtype], tokens, hk, hv, dk, dv)), sequences)
+
+
+def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slots=None, out=None,
+                scale: Optional[float] = None, normalize: bool = False, workspace=None, stream: Optional[int] = None):
+    """The gated delta rule over packed sequences: rows cu_seqlens[i] to cu_seqlens[i + 1] of
+    q, k, v, g and beta (as in `delta_step`) are sequence i, from the state in slot slots[i]
+    (None: i) of state_in (None: zeros); its final state goes to that slot of state_out (None:
+    not wanted; state_in itself: in place).  cu_seqlens int32, none decreasing, within the rows.
+    A slot of -1 leaves the sequence out; slots out of range, or named before while state_out
+    is given, give NaN rows.  Returns out [rows, value heads, dv]; rows of no sequence are not
+    written.  workspace: a uint8 tensor of `delta_chunk_workspace` bytes that nothing else uses
+    meanwhile (allocated if None).
+    """
+    op = "delta_chunk"
+    a, out = _rows(op, q, k, v, g, beta, out, scale, normalize)
+    device = q.device
+    _check(op, device, "cu_seqlens", cu_seqlens, torch.int32, (None,))
+    n = cu_seqlens.shape[0] - 1
+    if n < 0 or not cu_seqlens.is_contiguous():
+        _refuse(f"{op}: cu_seqlens holds one value more than there are sequences")
+    n_slots = 0
+    for name, pool in (("state_in", state_in), ("state_out", state_out)):
+        if pool is not None:
+            _pool(op, device, name, pool, a)
+            n_slots = pool.shape[0]
+    if state_in is not None and state_out is not None and state_in.shape[0] != state_out.shape[0]:
+        _refuse(f"{op}: state_in and state_out differ in slots")
+    L = _load()
+    need = L.redukt_op_delta_chunk_workspace(ctypes.byref(a), n)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    else:
+        _check(op, device, "workspace", workspace, torch.uint8, (None,))
+    code = L.redukt_op_delta_chunk(ctypes.byref(a), cu_seqlens.data_ptr(), n,
+                                   None if state_in is None else state_in.data_ptr(),
+                                   None if state_out is None else state_out.data_ptr(), n_slots,
+                                   _slots(op, device, slots, n), workspace.data_ptr(), workspace.numel(),
+                                   _stream(stream, device))
+    _done(code, op)
+    return out
+
+
+def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
+    """int8 codes of each row of x [rows, cols] (bfloat16, float16 or float32) with the library's
+    recipe: scale = max|x| / 127 (1 for a row of zeros), code = x / scale rounded with halves away
+    from zero, each step in float32; NaN counts for nothing and becomes 0.  Returns (codes int8
+    [rows, cols], scales float32 [rows]), allocated if None.  Rows may be strided.
+    """
+    op = "quantize_rows"
+    device = _device(op, x)
+    if x.dtype not in DTYPES or x.dim() != 2:
+        _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
+    rows, cols = x.shape
+    if codes is None:
+        codes = torch.empty((rows, cols), dtype=torch.int8, device=device)
+    else:
+        _check(op, device, "codes", codes, torch.int8, (rows, cols))
+    if scales is None:
+        scales = torch.empty((rows,), dtype=torch.float32, device=device)
+    else:
+        _check(op, device, "scales", scales, torch.float32, (rows,))
+        if not scales.is_contiguous():
+            _refuse(f"{op}: scales is not contiguous")
+    a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x), codes.data_ptr(),
+                     _row_stride(op, "codes", codes), scales.data_ptr())
+    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), _stream(stream, device)), op)
+    return codes, scales
+
+
+def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloat16, stream: Optional[int] = None):
+    """out[i, j] = (x[i] . w[j]) x_scales[i] w_scales[j] + bias[j]: int8 codes x [tokens, k] and w
+    [channels, k] with float32 scales per token and channel; exact integer sums, rounded once
+    to `dtype` (bfloat16, float16 or float32; out's type where out is given).  Any sizes, k up to
+    131,000; fastest where k and the strides of x and w are multiples of 16.
+    """
+    op = "int8_matmul"
+    device = _device(op, x)
+    _check(op, device, "x", x, torch.int8, (None, None))
+    m, k = x.shape
+    _check(op, device, "w", w, torch.int8, (None, k))
+    n = w.shape[0]
+    _check(op, device, "x_scales", x_scales, torch.float32, (m,))
+    _check(op, device, "w_scales", w_scales, torch.float32, (n,))
+    if bias is not None:
+        _check(op, device, "bias", bias, torch.float32, (n,))
+    for name, t in (("x_scales", x_scales), ("w_scales", w_scales), ("bias", bias)):
+        if t is not None and not t.is_contiguous():
+            _refuse(f"{op}: {name} is not contiguous")
+    if out is None:
+        if dtype not in DTYPES:
+            _refuse(f"{op}: dtype is bfloat16, float16 or float32")
+        out = torch.empty((m, n), dtype=dtype, device=device)
+    else:
+        if out.dtype not in DTYPES:
+            _refuse(f"{op}: out is bfloat16, float16 or float32")
+        _check(op, device, "out", out, out.dtype, (m, n))
+    a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x), x_scales.data_ptr(), w.data_ptr(),
+                   _row_stride(op, "w", w), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                   out.data_ptr(), _row_stride(op, "out", out))
+    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), _stream(stream, device)), op)
+    return out

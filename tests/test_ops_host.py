@@ -1,0 +1,153 @@
+"""The operators on caller tensors without a GPU: the header and its Python mirror, and what is refused
+before anything is launched."""
+import ctypes
+import os
+import re
+import subprocess
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from redukt_amd import ffi, ops  # noqa: E402
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "redukt_ops.h")
+BAD, OK = int(ffi.BackendResult.INVALID_ARGUMENT), int(ffi.BackendResult.OK)
+P = 1 << 20        # an aligned address that no call may reach
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return ops._load()
+
+
+def test_every_declared_operator_is_exported(lib):
+    names = set(re.findall(r"\b(redukt_op_\w+)\s*\(", open(HEADER).read()))
+    assert len(names) >= 5 and all(hasattr(lib, n) for n in names)
+
+
+def test_the_structs_are_the_headers(tmp_path):
+    structs = {"redukt_delta_rows": ops.DeltaRows, "redukt_quantize_rows": ops.QuantizeRows, "redukt_int8_matmul": ops.Int8Matmul}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "redukt_ops.h"', "int main(void) {"]
+    want = []
+    for name, cls in structs.items():
+        lines.append('printf("%%zu\\n", sizeof(%s));' % name)
+        want.append(ctypes.sizeof(cls))
+        for f, _ in cls._fields_:
+            lines.append('printf("%%zu\\n", offsetof(%s, %s));' % (name, f))
+            want.append(getattr(cls, f).offset)
+    src = tmp_path / "s.c"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    exe = str(tmp_path / "s")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe], check=True)
+    assert [int(v) for v in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()] == want
+
+
+def rows(**over):
+    v = dict(dtype=0, rows=4, hk=2, hv=4, dk=64, dv=64, flags=0, scale=1.0, q=P, k=P, v=P, out=P, q_stride=128, k_stride=128,
+             v_stride=256, out_stride=256, g=P, beta=P, g_stride=4, beta_stride=4)
+    v.update(over)
+    return ops.DeltaRows(**v)
+
+
+BAD_ROWS = [dict(dtype=3), dict(hk=0), dict(hv=0), dict(hk=3), dict(hv=4100, hk=1), dict(dk=32), dict(dk=96), dict(dk=0), dict(dv=0),
+            dict(dv=16), dict(dv=288), dict(flags=2), dict(rows=1 << 31), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
+            dict(g=None), dict(beta=None), dict(q=P + 8), dict(k=P + 2), dict(v=P + 4), dict(out=P + 8), dict(g=P + 2),
+            dict(beta=P + 1), dict(q_stride=132), dict(k_stride=127), dict(v_stride=128), dict(out_stride=0), dict(out_stride=128),
+            dict(q_stride=-128), dict(g_stride=-1)]
+
+
+@pytest.mark.parametrize("over", BAD_ROWS, ids=str)
+def test_delta_rows_refused(lib, over):
+    a = rows(**over)
+    assert lib.redukt_op_delta_step(ctypes.byref(a), P, 8, P, None) == BAD
+    assert lib.redukt_op_delta_chunk(ctypes.byref(a), P, 2, P, P, 8, P, P, 1 << 40, None) == BAD
+
+
+def test_delta_step_refused(lib):
+    a = ctypes.byref(rows())
+    assert lib.redukt_op_delta_step(None, P, 8, P, None) == BAD
+    assert lib.redukt_op_delta_step(a, None, 8, P, None) == BAD
+    assert lib.redukt_op_delta_step(a, P + 4, 8, P, None) == BAD          # states unaligned
+    assert lib.redukt_op_delta_step(a, P, 8, P + 2, None) == BAD          # slots unaligned
+    assert lib.redukt_op_delta_step(a, P, 3, None, None) == BAD           # four entries, three slots
+    assert lib.redukt_op_delta_step(a, P, 1 << 31, P, None) == BAD
+    assert lib.redukt_op_delta_step(ctypes.byref(rows(rows=65537)), P, 1 << 20, P, None) == BAD
+    assert lib.redukt_op_delta_step(ctypes.byref(rows(rows=0, q=None)), None, 0, None, None) == OK
+    # sizes are right, but no device owns the address
+    assert lib.redukt_op_delta_step(a, P, 8, P, None) == BAD
+
+
+def test_delta_chunk_refused(lib):
+    a = ctypes.byref(rows())
+    big = 1 << 40
+    call = lib.redukt_op_delta_chunk
+    assert call(None, P, 2, P, P, 8, P, P, big, None) == BAD
+    assert call(a, None, 2, P, P, 8, P, P, big, None) == BAD
+    assert call(a, P + 2, 2, P, P, 8, P, P, big, None) == BAD
+    assert call(a, P, 65537, P, P, 1 << 20, P, P, big, None) == BAD
+    assert call(a, P, 2, P + 4, P, 8, P, P, big, None) == BAD
+    assert call(a, P, 2, P, P + 8, 8, P, P, big, None) == BAD
+    assert call(a, P, 2, P, P + 1024, 8, P, P, big, None) == BAD         # pools that overlap in part
+    assert call(a, P, 9, P, P, 8, None, P, big, None) == BAD             # nine sequences, eight slots
+    assert call(a, P, 2, None, None, 0, P, P, big, None) == BAD          # slots of no pool
+    assert call(a, P, 0, None, None, 0, None, None, 0, None) == OK
+    need = lib.redukt_op_delta_chunk_workspace(a, 2)
+    if need:
+        assert call(a, P, 2, P, P, 8, P, None, big, None) == BAD
+        assert call(a, P, 2, P, P, 8, P, P + 4, big, None) == BAD
+        assert call(a, P, 2, P, P, 8, P, P, need - 1, None) == BAD
+    assert call(a, P, 2, P, P, 8, P, P, big, None) == BAD                # no device owns the address
+
+
+def test_workspace_of_sizes_that_are_not_taken(lib):
+    for over in BAD_ROWS[:12]:
+        assert lib.redukt_op_delta_chunk_workspace(ctypes.byref(rows(**over)), 2) == 0
+    assert lib.redukt_op_delta_chunk_workspace(None, 2) == 0
+    assert lib.redukt_op_delta_chunk_workspace(ctypes.byref(rows()), 65537) == 0
+
+
+def quantize_args(**over):
+    v = dict(dtype=0, rows=4, cols=100, x=P, x_stride=100, codes=P, codes_stride=100, scales=P)
+    v.update(over)
+    return ctypes.byref(ops.QuantizeRows(**v))
+
+
+def test_quantize_rows_refused(lib):
+    call = lib.redukt_op_quantize_rows
+    assert call(None, None) == BAD
+    for over in (dict(dtype=3), dict(rows=1 << 31), dict(cols=1 << 31), dict(x=None), dict(codes=None), dict(scales=None), dict(x=P + 1),
+                 dict(scales=P + 2), dict(x_stride=99), dict(codes_stride=99), dict(codes_stride=0), dict(x_stride=-100), {}):
+        assert call(quantize_args(**over), None) == BAD, over
+    assert call(quantize_args(rows=0, x=None), None) == OK
+
+
+def matmul_args(**over):
+    v = dict(dtype=0, m=4, n=6, k=100, x=P, x_stride=100, x_scales=P, w=P, w_stride=100, w_scales=P, bias=P, out=P, out_stride=6)
+    v.update(over)
+    return ctypes.byref(ops.Int8Matmul(**v))
+
+
+def test_int8_matmul_refused(lib):
+    call = lib.redukt_op_int8_matmul
+    assert call(None, None) == BAD
+    for over in (dict(dtype=3), dict(m=1 << 31), dict(n=1 << 31), dict(k=131001), dict(x=None), dict(w=None), dict(x_scales=None),
+                 dict(w_scales=None), dict(out=None), dict(x_scales=P + 2), dict(w_scales=P + 1), dict(bias=P + 2), dict(out=P + 1),
+                 dict(out_stride=5), dict(x_stride=99), dict(w_stride=99), dict(x_stride=-100), {}):
+        assert call(matmul_args(**over), None) == BAD, over
+    assert call(matmul_args(m=0, out=None), None) == OK
+    assert call(matmul_args(n=0, out=None), None) == OK
+
+
+def test_tensors_off_the_gpu_are_refused():
+    x = torch.zeros(2, 2, 64)
+    g = torch.zeros(2, 2)
+    pool = torch.zeros(2, 2, 64, 64)
+    codes, s = torch.zeros(2, 16, dtype=torch.int8), torch.ones(2)
+    for call in (lambda: ops.delta_step(x, x, x, g, g, pool), lambda: ops.delta_chunk(x, x, x, g, g, torch.zeros(2, dtype=torch.int32)),
+                 lambda: ops.quantize_rows(x[0]), lambda: ops.int8_matmul(codes, s, codes, s), lambda: ops.quantize_rows(None),
+                 lambda: ops.delta_chunk_workspace(1, 1, 1, 1, 64, 64, torch.int32)):
+        with pytest.raises(ffi.BackendError) as e:
+            call()
+        assert e.value.result == ffi.BackendResult.INVALID_ARGUMENT
