@@ -5,12 +5,15 @@
 // Columns of S do not meet, so any split over dv is free; S^T k and S^T q sum over dk.
 #include <hip/hip_runtime.h>
 
+#include "mfma_common.h"
 #include "op_common.h"
+
+// (mfma_common.h turns contraction off for the step kernels' bit-exact arithmetic)
+#pragma clang fp contract(fast)
 
 namespace rdk {
 namespace {
 
-constexpr int kWave = 64;
 constexpr float kUnitEps = 1e-6f;      // added to the sum of squares that k and q are divided by
 
 struct DeltaArgs {
@@ -133,6 +136,513 @@ const void* delta_rows_fn(uint32_t dtype, uint32_t dk) {
     return fns[dtype][dk == 128];
 }
 
+// ---------------------------------------------------------------- sequences in chunks
+//
+// C = 64 tokens at a time, with G the running sum of g within the chunk, c = C - 1 its last
+// token, u_i and p_i the factors that normalize k_i and q_i (the scale in p_i):
+//     A_ij = beta_i u_i u_j e^(G_i - G_j) k_i.k_j (j < i),      T = (I + A)^-1
+//     X = V - diag(u_i e^G_i) K S,      D = T diag(beta) X
+//     O = diag(p_i e^G_i) Q S + P D,    P_ij = p_i u_j e^(G_i - G_j) q_i.k_j (j <= i)
+//     S <- e^G_c S + K^T diag(u_i e^(G_c - G_i)) D
+// T diag(beta), P and the three diagonals need no state: k_delta_prep makes them for all chunks
+// side by side.  k_delta_chunks goes through a sequence's chunks in order with the state in
+// registers, 16 columns a wave.
+//
+// Arithmetic.  The products run on the bf16 matrix cores.  Keys and queries in bf16 are their
+// own operand (f16: two limbs, f32: three, exact); S, X, D and T are f32 split into three limbs
+// of 8 bits, and products of limbs are kept down to 2^-24 of the whole, so the state is as
+// exact as f32 sums are (two limbs leave about 4e-6).  P, and S and D where only a 16-bit output
+// comes of them, are two limbs (2^-17 against an output's half step of 2^-8 or 2^-11).  G is
+// summed in 64 bits: the decays are e to small differences of sums that may be large.
+//
+// Layout.  The 16 x 16 result tile of an MFMA has column l % 16, rows 4 (l / 16) + r in lane l;
+// its right operand wants column l % 16 and eight consecutive inner indices 8 (l / 16) + j.
+// Rows of a pair of result tiles (2 s, 2 s + 1) stand for the indices
+//     32 s + 8 (row / 4) + 4 (tile % 2) + row % 4,                                      (*)
+// so a lane's eight results of the pair are eight consecutive inner indices of the next product:
+// S, X and D go from result to right operand within a lane, without LDS and without an exchange.
+// Left operands take their rows in the same order.
+
+constexpr int kChunk = 64;
+constexpr int kTri = 6;                    // 16 x 32 fragments of a lower triangle of 64
+constexpr int kFrag = 1024;                // bytes of one fragment's limb: 64 lanes of 8 bf16
+
+template <typename T> struct Limbs;
+template <> struct Limbs<__bf16> { static constexpr int in = 1, out = 2; };
+template <> struct Limbs<_Float16> { static constexpr int in = 2, out = 2; };
+template <> struct Limbs<float> { static constexpr int in = 3, out = 3; };
+
+constexpr int unit_bytes(int out_limbs) { return kTri * (3 + out_limbs) * kFrag + 4 * kChunk * 4; }
+
+// The index that row `row` of result tile `tile` stands for (*).
+__device__ __forceinline__ int tile_index(int tile, int row) {
+    return 32 * (tile / 2) + 8 * (row / 4) + 4 * (tile % 2) + row % 4;
+}
+
+template <int N>
+struct Split {
+    bf16x8 l[N];
+};
+
+// Eight f32 as N bf16 limbs: each the rounded rest of those before it.
+template <int N>
+__device__ __forceinline__ Split<N> split8(const float (&v)[8]) {
+    Split<N> o;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        float r = v[j];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            o.l[n][j] = (__bf16)r;
+            if (n + 1 < N) r -= (float)o.l[n][j];
+        }
+    }
+    return o;
+}
+
+template <int N>
+__device__ __forceinline__ Split<N> split_pair(const f32x4& a, const f32x4& b) {
+    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return split8<N>(v);
+}
+
+// Eight elements of an operand in memory as limbs (exactly).
+template <typename T>
+__device__ __forceinline__ Split<Limbs<T>::in> load_limbs(const T* p) {
+    if constexpr (sizeof(T) == 2 && Limbs<T>::in == 1) {
+        return {{*(const bf16x8*)p}};
+    } else {
+        float v[8];
+        op_load(p, v);
+        return split8<Limbs<T>::in>(v);
+    }
+}
+
+// c += a b, with the products of limbs i and j kept for i + j < K.
+template <int K, int NA, int NB>
+__device__ __forceinline__ f32x4 mma_limbs(const Split<NA>& a, const Split<NB>& b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+            if (i + j < K) c = mma(a.l[i], b.l[j], c);
+    return c;
+}
+
+struct ChunkArgs {
+    DeltaArgs d;
+    unsigned char* ws;         // unit (chunk slot, value head): unit_bytes
+};
+
+// Sequence i's rows, within [0, rows].
+__device__ __forceinline__ uint32_t row_of(const ChunkArgs& a, uint32_t i) {
+    return min((uint32_t)max(a.d.cu[i], 0), a.d.r.rows);
+}
+
+// Chunk c of the sequence that starts at row b and is the i-th has slot b / 64 + i + c: slots of one sequence
+// are consecutive, those of the next begin after them, and rows / 64 + n slots are enough.
+__device__ __forceinline__ uint32_t first_chunk(uint32_t b, uint32_t i) { return b / kChunk + i; }
+
+__device__ __forceinline__ f32x4 mma4(float a, float b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+constexpr int kPitchA = kChunk + 4;        // f32 rows of the 64 x 64 matrices in LDS
+
+// Fragments of the lower triangle at m (f32 [64][kPitchA], natural order) with N limbs to ws: fragment f is tile
+// 0, 1, 2, 2, 3, 3 and inner indices 32 s + [0, 32) with s = 0, 0, 0, 1, 0, 1.
+template <int N>
+__device__ __forceinline__ void store_triangle(const float* m, unsigned char* to, int wave, int lane) {
+    for (int f = wave; f < kTri; f += 4) {
+        const int tile = f < 2 ? f : 2 + (f - 2) / 2, s = f < 2 ? 0 : (f - 2) % 2;
+        const float* row = m + tile_index(tile, lane % 16) * kPitchA + 32 * s + 8 * (lane / 16);
+        float v[8];
+        op_load(row, v);
+        const Split<N> x = split8<N>(v);
+#pragma unroll
+        for (int n = 0; n < N; n++) *(bf16x8*)(to + (f * N + n) * kFrag + lane * 16) = x.l[n];
+    }
+}
+
+// One workgroup a chunk and key head: k.k and q.k of the chunk once, then T diag(beta), P and the diagonals of
+// each value head of the group.
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
+    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32;
+    __shared__ __attribute__((aligned(16))) float sA[kChunk * kPitchA], sT[kChunk * kPitchA];
+    __shared__ double sG[kChunk];
+    __shared__ float sB[kChunk], sU[kChunk], sP[kChunk];
+    const redukt_delta_rows& r = a.d.r;
+    const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
+    const uint32_t slot = blockIdx.x / r.hk, hq = blockIdx.x % r.hk, group = r.hv / r.hk;
+    uint32_t lo = 0, hi = a.d.n - 1;       // the last sequence that starts at this slot or before
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (first_chunk(row_of(a, mid), mid) <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    const uint32_t b = row_of(a, lo), e = row_of(a, lo + 1), first = first_chunk(b, lo);
+    if (slot < first) return;
+    const uint64_t t0_ = (uint64_t)b + (uint64_t)(slot - first) * kChunk;
+    if (t0_ >= e) return;
+    const uint32_t t0 = (uint32_t)t0_, len = min(e - t0, (uint32_t)kChunk);
+
+    // k.k and q.k: wave w the tiles (w, 0 .. w)
+    f32x4 kk[4] = {}, qk[4] = {};
+    float k2[4] = {}, q2 = 0.0f;           // this lane's part of the sums of squares: rows l16 of the column tiles, of the query tile
+    const T* kp = (const T*)r.k + (size_t)hq * DK;
+    const T* qp = (const T*)r.q + (size_t)hq * DK;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const int col = 32 * s + 8 * g4;
+        Split<LI> kf[4], qf;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > wave) break;
+            const uint32_t t = 16 * j + l16;
+            float v[8] = {};
+            if (t < len) op_load(kp + (int64_t)(t0 + t) * r.k_stride + col, v);
+            kf[j] = split8<LI>(v);
+#pragma unroll
+            for (int x = 0; x < 8; x++) k2[j] += v[x] * v[x];
+        }
+        {
+            const uint32_t t = 16 * wave + l16;
+            float v[8] = {};
+            if (t < len) op_load(qp + (int64_t)(t0 + t) * r.q_stride + col, v);
+            qf = split8<LI>(v);
+#pragma unroll
+            for (int x = 0; x < 8; x++) q2 += v[x] * v[x];
+        }
+        Split<LI> own = kf[0];
+#pragma unroll
+        for (int j = 1; j < 4; j++)
+            if (j == wave) own = kf[j];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > wave) break;
+            kk[j] = mma_limbs<3>(own, kf[j], kk[j]);
+            qk[j] = mma_limbs<3>(qf, kf[j], qk[j]);
+        }
+    }
+    const bool norm = (r.flags & REDUKT_DELTA_NORMALIZE) != 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (j > wave) break;
+        float v = k2[j];
+        v += __shfl_xor(v, 16, kWave);
+        v += __shfl_xor(v, 32, kWave);
+        if (j == wave && g4 == 0) sU[16 * wave + l16] = norm ? rsqrtf(v + kUnitEps) : 1.0f;
+    }
+    q2 += __shfl_xor(q2, 16, kWave);
+    q2 += __shfl_xor(q2, 32, kWave);
+    if (g4 == 0) sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
+
+    for (uint32_t h = hq * group; h < (hq + 1) * group; h++) {
+        unsigned char* unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
+        float* vec = (float*)(unit + kTri * (3 + LO) * kFrag);
+        __syncthreads();                   // sU, sP are written; the last head's reads are done
+        if (wave == 0) {
+            const bool in = (uint32_t)lane < len;
+            double g = in ? (double)fmaxf(r.g[(int64_t)(t0 + lane) * r.g_stride + h], -1e5f) : 0.0;
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) {
+                const double v = __shfl_up(g, o, kWave);
+                if (lane >= o) g += v;
+            }
+            const double last = __shfl(g, kWave - 1, kWave);
+            sG[lane] = g;
+            sB[lane] = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f;
+            const float eg = expf((float)g), u = sU[lane];
+            vec[lane] = u * eg;
+            vec[kChunk + lane] = sP[lane] * eg;
+            vec[2 * kChunk + lane] = in ? u * expf((float)(last - g)) : 0.0f;
+            vec[3 * kChunk + lane] = expf((float)last);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int tj = 16 * j + l16;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int ti = 16 * wave + 4 * g4 + x;
+                float va = 0.0f, vp = 0.0f;
+                if (tj <= ti) {
+                    const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
+                    va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
+                    vp = sP[ti] * w * qk[j][x];
+                }
+                sA[ti * kPitchA + tj] = va;
+                sT[ti * kPitchA + tj] = vp;
+            }
+        }
+        __syncthreads();
+        store_triangle<LO>(sT, unit + kTri * 3 * kFrag, wave, lane);
+        __syncthreads();
+        {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
+            const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
+            float t[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float v0 = i == l16 ? 1.0f : 0.0f, v1 = 0.0f;
+#pragma unroll
+                for (int j = 0; j < i; j++) {
+                    if (j % 2) v1 -= A[i * kPitchA + j] * t[j];
+                    else v0 -= A[i * kPitchA + j] * t[j];
+                }
+                t[i] = v0 + v1;
+            }
+            float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
+            if (g4 == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
+            }
+        }
+        __syncthreads();
+        // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
+        auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
+        if (wave < 2) {
+            const int i = 2 * wave + 1, j = 2 * wave;
+            f32x4 m = {}, y = {};
+#pragma unroll
+            for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
+#pragma unroll
+            for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+        } else {   // the upper blocks within 32, which the fragments cover
+            const int i = 2 * (wave - 2);
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
+        }
+        __syncthreads();
+        {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
+            const int i = wave / 2, j = wave % 2;
+            f32x4 y = {};
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                if (p > i) break;
+                f32x4 m = {};
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    if (q < j) continue;
+#pragma unroll
+                    for (int s = 0; s < 4; s++)
+                        m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+                }
+#pragma unroll
+                for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+        }
+        __syncthreads();
+        // T diag(beta)
+        for (int f = wave; f < kTri; f += 4) {
+            const int tile = f < 2 ? f : 2 + (f - 2) / 2, s = f < 2 ? 0 : (f - 2) % 2, c0 = 32 * s + 8 * g4;
+            float v[8];
+            op_load(sT + tile_index(tile, l16) * kPitchA + c0, v);
+#pragma unroll
+            for (int x = 0; x < 8; x++) v[x] *= sB[c0 + x];
+            const Split<3> y = split8<3>(v);
+#pragma unroll
+            for (int n = 0; n < 3; n++) *(bf16x8*)(unit + (f * 3 + n) * kFrag + lane * 16) = y.l[n];
+        }
+    }
+}
+
+// Elements a row of an LDS operand takes: odd multiples of 16 bytes, so that 16 lanes that read 16 bytes of 16
+// neighbouring rows meet no bank twice.
+template <typename T> constexpr int pitch_of(int n) { return n + 16 / (int)sizeof(T); }
+
+// One workgroup of W waves takes 16 W columns of one head's state through a sequence.  The chunk's keys and queries
+// stand in LDS (keys in both orders), T, P and the diagonals come from the workspace.
+template <typename T, int DK, int W>
+__global__ __launch_bounds__(64 * W) void k_delta_chunks(ChunkArgs a) {
+    constexpr int LO = Limbs<T>::out, KS = DK / 32, NT = DK / 16;
+    constexpr int PK = pitch_of<T>(DK), PT = pitch_of<T>(kChunk);
+    constexpr int kBytes = (2 * kChunk * PK + DK * PT) * (int)sizeof(T);
+    constexpr int kUnits = 32 * (DK / 8) / (64 * W);       // (pair of tokens, eight columns) a thread
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kBytes];
+    T* const sK = (T*)lds;                 // row: token in the order (*)
+    T* const sQ = sK + kChunk * PK;
+    T* const sKT = sQ + kChunk * PK;       // row: column of k in the order (*); the tokens in their own
+    const redukt_delta_rows& r = a.d.r;
+    const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
+    // the workgroups that read one key head's chunks are neighbours of one XCD
+    const uint32_t group = r.hv / r.hk, cols = (r.dv / 16 + W - 1) / W;
+    const XcdTile w = xcd_tile(blockIdx.x, group * cols, a.d.n * r.hk);
+    if (!w.live) return;
+    const uint32_t i = w.unit / r.hk, hq = w.unit % r.hk, h = hq * group + w.part / cols;
+    const uint32_t col16 = (w.part % cols) * W + wave;
+    const bool mine = col16 < r.dv / 16;   // (the last workgroup of a head may have a wave too many, which helps loading)
+    const uint32_t col = mine ? 16 * col16 + l16 : l16;
+    const int slot = entry_slot(a.d.slots, a.d.n_slots, i, a.d.states != nullptr, lane);
+    if (slot == kSkip) return;
+    const uint32_t b = row_of(a, i), e = max(row_of(a, i + 1), b);
+    T* const out = (T*)r.out + (size_t)h * r.dv + col;
+    if (slot == kBad) {
+        if (mine)
+            for (uint32_t t = b + g4; t < e; t += 4) out[(int64_t)t * r.out_stride] = (T)__builtin_nanf("");
+        return;
+    }
+    const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv + col;
+    f32x4 S[NT];
+#pragma unroll
+    for (int p = 0; p < NT; p++)
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+            S[p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] : 0.0f;
+    const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
+    typedef T vec8 __attribute__((ext_vector_type(8)));
+    for (uint32_t c = 0; c < chunks; c++) {
+        const uint32_t t0 = b + c * kChunk, len = min(e - t0, (uint32_t)kChunk);
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            const int id = u * 64 * W + threadIdx.x, tp = id / (DK / 8), o = id % (DK / 8);
+            vec8 kv[2] = {}, qv[2] = {};
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const uint32_t t = 2 * tp + y;
+                if (t < len) {
+                    kv[y] = *(const vec8*)((const T*)r.k + (int64_t)(t0 + t) * r.k_stride + hq * DK + 8 * o);
+                    qv[y] = *(const vec8*)((const T*)r.q + (int64_t)(t0 + t) * r.q_stride + hq * DK + 8 * o);
+                }
+                const int row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
+                *(vec8*)(sK + row * PK + 8 * o) = kv[y];
+                *(vec8*)(sQ + row * PK + 8 * o) = qv[y];
+            }
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                typedef T vec2 __attribute__((ext_vector_type(2)));
+                const int d = 8 * o + x, row = 32 * (d / 32) + 16 * (d / 4 % 2) + 4 * (d / 8 % 4) + d % 4;
+                *(vec2*)(sKT + row * PT + 2 * tp) = vec2{kv[0][x], kv[1][x]};
+            }
+        }
+        __syncthreads();
+        const unsigned char* unit = a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO);
+        const float* vec = (const float*)(unit + kTri * (3 + LO) * kFrag);
+        f32x4 X[4] = {}, O[4] = {};
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const Split<3> x = split_pair<3>(S[2 * s], S[2 * s + 1]);
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                X[m] = mma_limbs<3>(load_limbs(sK + (16 * m + l16) * PK + 32 * s + 8 * g4), x, X[m]);
+                O[m] = mma_limbs<LO>(load_limbs(sQ + (16 * m + l16) * PK + 32 * s + 8 * g4), x, O[m]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const int t = tile_index(m, 4 * g4);
+            const f32x4 kd = *(const f32x4*)(vec + t), qd = *(const f32x4*)(vec + kChunk + t);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const float v = mine && (uint32_t)(t + x) < len
+                                    ? (float)((const T*)r.v)[(int64_t)(t0 + t + x) * r.v_stride + (size_t)h * r.dv + col]
+                                    : 0.0f;
+                X[m][x] = v - kd[x] * X[m][x];
+                O[m][x] *= qd[x];
+            }
+        }
+        f32x4 D[4] = {};
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const Split<3> x = split_pair<3>(X[2 * s], X[2 * s + 1]);
+#pragma unroll
+            for (int m = 2 * s; m < 4; m++) {
+                const int f = m < 2 ? m : 2 + 2 * (m - 2) + s;
+                Split<3> tf;
+#pragma unroll
+                for (int n = 0; n < 3; n++) tf.l[n] = *(const bf16x8*)(unit + (f * 3 + n) * kFrag + lane * 16);
+                D[m] = mma_limbs<3>(tf, x, D[m]);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const Split<LO> x = split_pair<LO>(D[2 * s], D[2 * s + 1]);
+#pragma unroll
+            for (int m = 2 * s; m < 4; m++) {
+                const int f = m < 2 ? m : 2 + 2 * (m - 2) + s;
+                Split<LO> pf;
+#pragma unroll
+                for (int n = 0; n < LO; n++)
+                    pf.l[n] = *(const bf16x8*)(unit + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
+                O[m] = mma_limbs<LO>(pf, x, O[m]);
+            }
+        }
+        if (mine) {
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int t = tile_index(m, 4 * g4) + x;
+                    if ((uint32_t)t < len) out[(int64_t)(t0 + t) * r.out_stride] = (T)O[m][x];
+                }
+        }
+        const float keep = vec[3 * kChunk];
+#pragma unroll
+        for (int m = 0; m < 4; m++) {
+            const f32x4 wd = *(const f32x4*)(vec + 2 * kChunk + tile_index(m, 4 * g4));
+#pragma unroll
+            for (int x = 0; x < 4; x++) D[m][x] *= wd[x];
+        }
+#pragma unroll
+        for (int p = 0; p < NT; p++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) S[p][x] *= keep;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const Split<3> x = split_pair<3>(D[2 * s], D[2 * s + 1]);
+#pragma unroll
+            for (int p = 0; p < NT; p++)
+                S[p] = mma_limbs<3>(load_limbs(sKT + (16 * p + l16) * PT + 32 * s + 8 * g4), x, S[p]);
+        }
+    }
+    if (a.d.states && mine) {
+#pragma unroll
+        for (int p = 0; p < NT; p++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) a.d.states[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] = S[p][x];
+    }
+}
+
+const void* delta_prep_fn(uint32_t dtype, uint32_t dk) {
+    static const void* const fns[3][2] = {
+        {(const void*)k_delta_prep<__bf16, 64>, (const void*)k_delta_prep<__bf16, 128>},
+        {(const void*)k_delta_prep<_Float16, 64>, (const void*)k_delta_prep<_Float16, 128>},
+        {(const void*)k_delta_prep<float, 64>, (const void*)k_delta_prep<float, 128>},
+    };
+    return fns[dtype][dk == 128];
+}
+
+template <int W>
+const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
+    static const void* const fns[3][2] = {
+        {(const void*)k_delta_chunks<__bf16, 64, W>, (const void*)k_delta_chunks<__bf16, 128, W>},
+        {(const void*)k_delta_chunks<_Float16, 64, W>, (const void*)k_delta_chunks<_Float16, 128, W>},
+        {(const void*)k_delta_chunks<float, 64, W>, (const void*)k_delta_chunks<float, 128, W>},
+    };
+    return fns[dtype][dk == 128];
+}
+
+uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
+
+int32_t launch_chunks(ChunkArgs& k, void* stream) {
+    const redukt_delta_rows& r = k.d.r;
+    const uint64_t prep = chunk_slots(r, k.d.n) * r.hk;
+    constexpr int W = 2;
+    const uint64_t cols = (r.dv / 16 + W - 1) / W, units = (uint64_t)k.d.n * r.hk;
+    const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
+    if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    if (r.rows) {
+        const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
+        if (rc != BACKEND_OK) return rc;
+    }
+    return op_launch(delta_chunks_fn<W>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(64 * W), 0, stream, k);
+}
+
 bool sizes_ok(const redukt_delta_rows* a) {
     return a && a->dtype <= REDUKT_OP_F32 && a->hk > 0 && a->hv > 0 && a->hv <= 4096 && a->hv % a->hk == 0 &&
            (a->dk == 64 || a->dk == 128) && a->dv > 0 && a->dv % 32 == 0 && a->dv <= 256 && a->rows < (1u << 31) &&
@@ -185,8 +695,8 @@ int32_t redukt_op_delta_step(const redukt_delta_rows* a, float* states, uint32_t
 }
 
 uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_seq) {
-    (void)a, (void)n_seq;
-    return 0;
+    if (!sizes_ok(a) || n_seq > kMaxOpRows) return 0;
+    return chunk_slots(*a, n_seq) * a->hv * unit_bytes(a->dtype == REDUKT_OP_F32 ? 3 : 2);
 }
 
 int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uint32_t n_seq, const float* state_in,
@@ -209,8 +719,8 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    DeltaArgs k{*a, state_in, state_out, n_slots, slots, cu, n_seq};
-    return launch_rows(k, stream);
+    ChunkArgs k{{*a, state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace};
+    return launch_chunks(k, stream);
 }
 
 }  // extern "C"
