@@ -229,6 +229,29 @@ __device__ __forceinline__ f32x4 mma_limbs(const Split<NA>& a, const Split<NB>& 
     return c;
 }
 
+// c[m] += a(m) b for four row tiles m, limb by limb so that the tiles' sums overlap.
+template <int K, int NB, typename A, typename C>
+__device__ __forceinline__ void mma_rows(A&& a, const Split<NB>& b, C&& c) {
+    const decltype(a(0)) x[4] = {a(0), a(1), a(2), a(3)};
+    constexpr int NA = sizeof(x[0]) / sizeof(bf16x8);
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+            if (i + j < K) {
+#pragma unroll
+                for (int m = 0; m < 4; m++) c[m] = mma(x[m].l[i], b.l[j], c[m]);
+            }
+}
+
+template <int N>
+__device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
+    Split<N> o;
+#pragma unroll
+    for (int n = 0; n < N; n++) o.l[n] = v[n];
+    return o;
+}
+
 struct ChunkArgs {
     DeltaArgs d;
     unsigned char* ws;         // unit (chunk slot, value head): unit_bytes
@@ -455,15 +478,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
 // neighbouring rows meet no bank twice.
 template <typename T> constexpr int pitch_of(int n) { return n + 16 / (int)sizeof(T); }
 
-// One workgroup of W waves takes 16 W columns of one head's state through a sequence.  The chunk's keys and queries
-// stand in LDS (keys in both orders), T, P and the diagonals come from the workspace.
+// One workgroup of W waves takes 16 W columns of one head's state through a sequence.  A chunk's keys (in both
+// orders) and queries stand in LDS; T, P, the values and the diagonals are each wave's own registers.  All of
+// them are requested a chunk ahead: behind barrier A(c), when every wave is done with the state's products, the
+// keys and queries of chunk c + 1 replace those of c in LDS (k^T has two buffers, since chunk c still reads its
+// own) and those of c + 2 are requested; barrier B(c) ends the chunk.
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W) void k_delta_chunks(ChunkArgs a) {
+__global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
     constexpr int LO = Limbs<T>::out, KS = DK / 32, NT = DK / 16;
     constexpr int PK = pitch_of<T>(DK), PT = pitch_of<T>(kChunk);
-    constexpr int kBytes = (2 * kChunk * PK + DK * PT) * (int)sizeof(T);
     constexpr int kUnits = 32 * (DK / 8) / (64 * W);       // (pair of tokens, eight columns) a thread
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kBytes];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * (kChunk * PK + DK * PT) * sizeof(T)];
+    __shared__ __attribute__((aligned(16))) float sV[2][4 * kChunk];
     T* const sK = (T*)lds;                 // row: token in the order (*)
     T* const sQ = sK + kChunk * PK;
     T* const sKT = sQ + kChunk * PK;       // row: column of k in the order (*); the tokens in their own
@@ -493,45 +519,101 @@ __global__ __launch_bounds__(64 * W) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
         for (int x = 0; x < 4; x++)
             S[p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] : 0.0f;
-    const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
+    const uint32_t chunks = (e - b + kChunk - 1) / kChunk;
+    const unsigned char* const units = a.ws + ((size_t)first_chunk(b, i) * r.hv + h) * unit_bytes(LO);
+    const size_t unit_step = (size_t)r.hv * unit_bytes(LO);
     typedef T vec8 __attribute__((ext_vector_type(8)));
-    for (uint32_t c = 0; c < chunks; c++) {
-        const uint32_t t0 = b + c * kChunk, len = min(e - t0, (uint32_t)kChunk);
-        __syncthreads();
+    typedef T vec2 __attribute__((ext_vector_type(2)));
+    vec8 kv[kUnits][2], qv[kUnits][2];
+    bf16x8 tf[kTri][3], pf[kTri][LO];
+    T vv[4][4];
+    float4 dv = make_float4(0, 0, 0, 0);
+
+    const auto rows_in = [&](uint32_t c) { return min(e - b - c * kChunk, (uint32_t)kChunk); };
+    // Requests of chunk c, rows past its end the last one (they are replaced by zeros where they are used).
+    const auto load_kq = [&](uint32_t c) {
+        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            const uint32_t id = u * 64 * W + threadIdx.x, tp = id / (DK / 8), o = id % (DK / 8);
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const uint32_t t = t0 + min(2 * tp + y, len - 1);
+                kv[u][y] = *(const vec8*)((const T*)r.k + (int64_t)t * r.k_stride + hq * DK + 8 * o);
+                qv[u][y] = *(const vec8*)((const T*)r.q + (int64_t)t * r.q_stride + hq * DK + 8 * o);
+            }
+        }
+        if (wave == 0) dv = ((const float4*)(units + c * unit_step + kTri * (3 + LO) * kFrag))[lane];
+    };
+    const auto store_kq = [&](uint32_t c) {
+        const uint32_t len = rows_in(c);
+        T* const kt = sKT + c % 2 * (DK * PT);
 #pragma unroll
         for (int u = 0; u < kUnits; u++) {
             const int id = u * 64 * W + threadIdx.x, tp = id / (DK / 8), o = id % (DK / 8);
-            vec8 kv[2] = {}, qv[2] = {};
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                const uint32_t t = 2 * tp + y;
-                if (t < len) {
-                    kv[y] = *(const vec8*)((const T*)r.k + (int64_t)(t0 + t) * r.k_stride + hq * DK + 8 * o);
-                    qv[y] = *(const vec8*)((const T*)r.q + (int64_t)(t0 + t) * r.q_stride + hq * DK + 8 * o);
-                }
-                const int row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
-                *(vec8*)(sK + row * PK + 8 * o) = kv[y];
-                *(vec8*)(sQ + row * PK + 8 * o) = qv[y];
+                const int t = 2 * tp + y, row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
+                if ((uint32_t)t >= len) kv[u][y] = qv[u][y] = vec8{};
+                *(vec8*)(sK + row * PK + 8 * o) = kv[u][y];
+                *(vec8*)(sQ + row * PK + 8 * o) = qv[u][y];
             }
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                typedef T vec2 __attribute__((ext_vector_type(2)));
                 const int d = 8 * o + x, row = 32 * (d / 32) + 16 * (d / 4 % 2) + 4 * (d / 8 % 4) + d % 4;
-                *(vec2*)(sKT + row * PT + 2 * tp) = vec2{kv[0][x], kv[1][x]};
+                *(vec2*)(kt + row * PT + 2 * tp) = vec2{kv[u][0][x], kv[u][1][x]};
             }
         }
-        __syncthreads();
-        const unsigned char* unit = a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO);
-        const float* vec = (const float*)(unit + kTri * (3 + LO) * kFrag);
+        if (wave == 0) ((float4*)sV[c % 2])[lane] = dv;
+    };
+    const auto load_v = [&](uint32_t c) {
+        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
+#pragma unroll
+        for (int m = 0; m < 4; m++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                vv[m][x] = ((const T*)r.v)[(int64_t)(t0 + min((uint32_t)tile_index(m, 4 * g4) + x, len - 1)) * r.v_stride +
+                                           (size_t)h * r.dv + col];
+    };
+    const auto load_t = [&](uint32_t c) {
+#pragma unroll
+        for (int f = 0; f < kTri; f++)
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                tf[f][n] = *(const bf16x8*)(units + c * unit_step + (f * 3 + n) * kFrag + lane * 16);
+    };
+    const auto load_p = [&](uint32_t c) {
+#pragma unroll
+        for (int f = 0; f < kTri; f++)
+#pragma unroll
+            for (int n = 0; n < LO; n++)
+                pf[f][n] = *(const bf16x8*)(units + c * unit_step + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
+    };
+    if (chunks) {
+        load_kq(0);
+        load_t(0);
+        load_v(0);
+        load_p(0);
+        store_kq(0);
+        if (chunks > 1) load_kq(1);
+    }
+    __syncthreads();
+    for (uint32_t c = 0; c < chunks; c++) {
+        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
+        const bool more = c + 1 < chunks;
+        const float* const vec = sV[c % 2];
+        const T* const kt = sKT + c % 2 * (DK * PT);
         f32x4 X[4] = {}, O[4] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
             const Split<3> x = split_pair<3>(S[2 * s], S[2 * s + 1]);
-#pragma unroll
-            for (int m = 0; m < 4; m++) {
-                X[m] = mma_limbs<3>(load_limbs(sK + (16 * m + l16) * PK + 32 * s + 8 * g4), x, X[m]);
-                O[m] = mma_limbs<LO>(load_limbs(sQ + (16 * m + l16) * PK + 32 * s + 8 * g4), x, O[m]);
-            }
+            mma_rows<3>([&](int m) { return load_limbs(sK + (16 * m + l16) * PK + 32 * s + 8 * g4); }, x, X);
+            mma_rows<LO>([&](int m) { return load_limbs(sQ + (16 * m + l16) * PK + 32 * s + 8 * g4); }, x, O);
+        }
+        __syncthreads();                   // A
+        if (more) {
+            store_kq(c + 1);
+            if (c + 2 < chunks) load_kq(c + 2);
         }
 #pragma unroll
         for (int m = 0; m < 4; m++) {
@@ -539,48 +621,28 @@ __global__ __launch_bounds__(64 * W) void k_delta_chunks(ChunkArgs a) {
             const f32x4 kd = *(const f32x4*)(vec + t), qd = *(const f32x4*)(vec + kChunk + t);
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                const float v = mine && (uint32_t)(t + x) < len
-                                    ? (float)((const T*)r.v)[(int64_t)(t0 + t + x) * r.v_stride + (size_t)h * r.dv + col]
-                                    : 0.0f;
-                X[m][x] = v - kd[x] * X[m][x];
+                X[m][x] = ((uint32_t)(t + x) < len ? (float)vv[m][x] : 0.0f) - kd[x] * X[m][x];
                 O[m][x] *= qd[x];
             }
         }
+        if (more) load_v(c + 1);
         f32x4 D[4] = {};
+        {
+            const Split<3> x0 = split_pair<3>(X[0], X[1]);
+            mma_rows<3>([&](int m) { return as_split<3>(tf[m < 2 ? m : 2 * m - 2]); }, x0, D);
+            const Split<3> x1 = split_pair<3>(X[2], X[3]);
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const Split<3> x = split_pair<3>(X[2 * s], X[2 * s + 1]);
-#pragma unroll
-            for (int m = 2 * s; m < 4; m++) {
-                const int f = m < 2 ? m : 2 + 2 * (m - 2) + s;
-                Split<3> tf;
-#pragma unroll
-                for (int n = 0; n < 3; n++) tf.l[n] = *(const bf16x8*)(unit + (f * 3 + n) * kFrag + lane * 16);
-                D[m] = mma_limbs<3>(tf, x, D[m]);
-            }
+            for (int m = 2; m < 4; m++) D[m] = mma_limbs<3>(as_split<3>(tf[2 * m - 1]), x1, D[m]);
         }
+        if (more) load_t(c + 1);
+        {
+            const Split<LO> x0 = split_pair<LO>(D[0], D[1]);
+            mma_rows<LO>([&](int m) { return as_split<LO>(pf[m < 2 ? m : 2 * m - 2]); }, x0, O);
+            const Split<LO> x1 = split_pair<LO>(D[2], D[3]);
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const Split<LO> x = split_pair<LO>(D[2 * s], D[2 * s + 1]);
-#pragma unroll
-            for (int m = 2 * s; m < 4; m++) {
-                const int f = m < 2 ? m : 2 + 2 * (m - 2) + s;
-                Split<LO> pf;
-#pragma unroll
-                for (int n = 0; n < LO; n++)
-                    pf.l[n] = *(const bf16x8*)(unit + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
-                O[m] = mma_limbs<LO>(pf, x, O[m]);
-            }
+            for (int m = 2; m < 4; m++) O[m] = mma_limbs<LO>(as_split<LO>(pf[2 * m - 1]), x1, O[m]);
         }
-        if (mine) {
-#pragma unroll
-            for (int m = 0; m < 4; m++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int t = tile_index(m, 4 * g4) + x;
-                    if ((uint32_t)t < len) out[(int64_t)(t0 + t) * r.out_stride] = (T)O[m][x];
-                }
-        }
+        if (more) load_p(c + 1);
         const float keep = vec[3 * kChunk];
 #pragma unroll
         for (int m = 0; m < 4; m++) {
@@ -596,9 +658,19 @@ __global__ __launch_bounds__(64 * W) void k_delta_chunks(ChunkArgs a) {
         for (int s = 0; s < 2; s++) {
             const Split<3> x = split_pair<3>(D[2 * s], D[2 * s + 1]);
 #pragma unroll
-            for (int p = 0; p < NT; p++)
-                S[p] = mma_limbs<3>(load_limbs(sKT + (16 * p + l16) * PT + 32 * s + 8 * g4), x, S[p]);
+            for (int p = 0; p < NT; p += 4)
+                mma_rows<3>([&](int m) { return load_limbs(kt + (16 * (p + m) + l16) * PT + 32 * s + 8 * g4); }, x, &S[p]);
         }
+        if (mine) {
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int t = tile_index(m, 4 * g4) + x;
+                    if ((uint32_t)t < len) out[(int64_t)(t0 + t) * r.out_stride] = (T)O[m][x];
+                }
+        }
+        __syncthreads();                   // B
     }
     if (a.d.states && mine) {
 #pragma unroll
@@ -629,10 +701,14 @@ const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
 
 uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
 
+#ifndef KW
+#define KW 4
+#endif
+constexpr int kW = KW;
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
     const uint64_t prep = chunk_slots(r, k.d.n) * r.hk;
-    constexpr int W = 2;
+    constexpr int W = kW;
     const uint64_t cols = (r.dv / 16 + W - 1) / W, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
