@@ -54,7 +54,7 @@ typedef struct {
     const void* k;          /* hk * dk */
     const void* v;          /* hv * dv */
     void* out;              /* hv * dv */
-    int64_t q_stride, k_stride, v_stride, out_stride;   /* elements from a row to the next */
+    int64_t q_stride, k_stride, v_stride, out_stride;   /* elements from a row to the next, at most 2^22 */
     const float* g;         /* row t: hv values at g + t * g_stride */
     const float* beta;
     int64_t g_stride, beta_stride;

@@ -140,20 +140,26 @@ const void* delta_rows_fn(uint32_t dtype, uint32_t dk) {
 //
 // C = 64 tokens at a time, with G the running sum of g within the chunk, c = C - 1 its last
 // token, u_i and p_i the factors that normalize k_i and q_i (the scale in p_i):
-//     A_ij = beta_i u_i u_j e^(G_i - G_j) k_i.k_j (j < i),      T = (I + A)^-1
-//     X = V - diag(u_i e^G_i) K S,      D = T diag(beta) X
-//     O = diag(p_i e^G_i) Q S + P D,    P_ij = p_i u_j e^(G_i - G_j) q_i.k_j (j <= i)
-//     S <- e^G_c S + K^T diag(u_i e^(G_c - G_i)) D
-// T diag(beta), P and the three diagonals need no state: k_delta_prep makes them for all chunks
-// side by side.  k_delta_chunks goes through a sequence's chunks in order with the state in
-// registers, 16 columns a wave.
+//     A_ij = beta_i u_i u_j e^(G_i - G_j) k_i.k_j (j < i),      T = (I + A)^-1 diag(beta)
+//     P_ij = p_i u_j e^(G_i - G_j) q_i.k_j (j <= i)
+//     X = V - diag(u_i e^G_i) K S
+//     O = diag(p_i e^G_i) Q S + (P T) X
+//     S <- e^G_c S + K^T (diag(u_i e^(G_c - G_i)) T) X
+// P T, diag() T and the diagonals need no state: k_delta_prep makes them for all chunks side by
+// side.  k_delta_chunks goes through a sequence's chunks in order with the state in registers, 16
+// columns a wave.
 //
 // Arithmetic.  The products run on the bf16 matrix cores.  Keys and queries in bf16 are their
-// own operand (f16: two limbs, f32: three, exact); S, X, D and T are f32 split into three limbs
-// of 8 bits, and products of limbs are kept down to 2^-24 of the whole, so the state is as
-// exact as f32 sums are (two limbs leave about 4e-6).  P, and S and D where only a 16-bit output
+// own operand (f16: two limbs, f32: three, exact); S, X and diag() T are f32 split into three
+// limbs of 8 bits, and products of limbs are kept down to 2^-24 of the whole, so the state is as
+// exact as f32 sums are (two limbs leave about 4e-6).  P T, and S and X where only a 16-bit output
 // comes of them, are two limbs (2^-17 against an output's half step of 2^-8 or 2^-11).  G is
 // summed in 64 bits: the decays are e to small differences of sums that may be large.
+//
+// What is not finite.  A matrix product would spread one over rows it does not reach by the rule
+// (0 times it), so rows of X from a column's first such value on are taken as zeros, and the column's
+// outputs from there on and its state become NaN; k_delta_prep marks the tokens from the first whose
+// key, g or beta is not finite (g = -inf is).
 //
 // Layout.  The 16 x 16 result tile of an MFMA has column l % 16, rows 4 (l / 16) + r in lane l;
 // its right operand wants column l % 16 and eight consecutive inner indices 8 (l / 16) + j.
@@ -172,7 +178,10 @@ template <> struct Limbs<__bf16> { static constexpr int in = 1, out = 2; };
 template <> struct Limbs<_Float16> { static constexpr int in = 2, out = 2; };
 template <> struct Limbs<float> { static constexpr int in = 3, out = 3; };
 
-constexpr int unit_bytes(int out_limbs) { return kTri * (3 + out_limbs) * kFrag + 4 * kChunk * 4; }
+// What k_delta_prep leaves of a chunk and value head: the fragments of diag() T in three limbs, of P T in LO, and
+// f32 vectors [64]: u_i e^G_i, p_i e^G_i, and e^G_c in every place.
+constexpr int kVecs = 3;
+constexpr int unit_bytes(int out_limbs) { return kTri * (3 + out_limbs) * kFrag + kVecs * kChunk * 4; }
 
 // The index that row `row` of result tile `tile` stands for (*).
 __device__ __forceinline__ int tile_index(int tile, int row) {
@@ -244,14 +253,6 @@ __device__ __forceinline__ void mma_rows(A&& a, const Split<NB>& b, C&& c) {
             }
 }
 
-template <int N>
-__device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
-    Split<N> o;
-#pragma unroll
-    for (int n = 0; n < N; n++) o.l[n] = v[n];
-    return o;
-}
-
 struct ChunkArgs {
     DeltaArgs d;
     unsigned char* ws;         // unit (chunk slot, value head): unit_bytes
@@ -272,29 +273,30 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, const f32x4& c) {
 
 constexpr int kPitchA = kChunk + 4;        // f32 rows of the 64 x 64 matrices in LDS
 
-// Fragments of the lower triangle at m (f32 [64][kPitchA], natural order) with N limbs to ws: fragment f is tile
-// 0, 1, 2, 2, 3, 3 and inner indices 32 s + [0, 32) with s = 0, 0, 0, 1, 0, 1.
+// Fragments of the lower triangle at m (f32 [64][kPitchA], natural order), its rows times f, with N limbs to `to`: fragment
+// x is tile 0, 1, 2, 2, 3, 3 and inner indices 32 s + [0, 32) with s = 0, 0, 0, 1, 0, 1.
 template <int N>
-__device__ __forceinline__ void store_triangle(const float* m, unsigned char* to, int wave, int lane) {
-    for (int f = wave; f < kTri; f += 4) {
-        const int tile = f < 2 ? f : 2 + (f - 2) / 2, s = f < 2 ? 0 : (f - 2) % 2;
-        const float* row = m + tile_index(tile, lane % 16) * kPitchA + 32 * s + 8 * (lane / 16);
+__device__ __forceinline__ void store_triangle(const float* m, const float* f, unsigned char* to, int wave, int lane) {
+    for (int x = wave; x < kTri; x += 4) {
+        const int tile = x < 2 ? x : 2 + (x - 2) / 2, s = x < 2 ? 0 : (x - 2) % 2, row = tile_index(tile, lane % 16);
         float v[8];
-        op_load(row, v);
-        const Split<N> x = split8<N>(v);
+        op_load(m + row * kPitchA + 32 * s + 8 * (lane / 16), v);
+        const float scale = f ? f[row] : 1.0f;
 #pragma unroll
-        for (int n = 0; n < N; n++) *(bf16x8*)(to + (f * N + n) * kFrag + lane * 16) = x.l[n];
+        for (int j = 0; j < 8; j++) v[j] *= scale;
+        const Split<N> y = split8<N>(v);
+#pragma unroll
+        for (int n = 0; n < N; n++) *(bf16x8*)(to + (x * N + n) * kFrag + lane * 16) = y.l[n];
     }
 }
 
-// One workgroup a chunk and key head: k.k and q.k of the chunk once, then T diag(beta), P and the diagonals of
-// each value head of the group.
+// One workgroup a chunk and key head: k.k and q.k of the chunk once, then the unit of each value head of the group.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32;
     __shared__ __attribute__((aligned(16))) float sA[kChunk * kPitchA], sT[kChunk * kPitchA];
     __shared__ double sG[kChunk];
-    __shared__ float sB[kChunk], sU[kChunk], sP[kChunk];
+    __shared__ float sB[kChunk], sU[kChunk], sP[kChunk], sW[kChunk];
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
     const uint32_t slot = blockIdx.x / r.hk, hq = blockIdx.x % r.hk, group = r.hv / r.hk;
@@ -355,7 +357,8 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
         float v = k2[j];
         v += __shfl_xor(v, 16, kWave);
         v += __shfl_xor(v, 32, kWave);
-        if (j == wave && g4 == 0) sU[16 * wave + l16] = norm ? rsqrtf(v + kUnitEps) : 1.0f;
+        // (a sum that is not finite stays one: 0 x it is NaN)
+        if (j == wave && g4 == 0) sU[16 * wave + l16] = norm ? rsqrtf(v + kUnitEps) + 0.0f * v : 1.0f + 0.0f * v;
     }
     q2 += __shfl_xor(q2, 16, kWave);
     q2 += __shfl_xor(q2, 32, kWave);
@@ -367,7 +370,12 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
         __syncthreads();                   // sU, sP are written; the last head's reads are done
         if (wave == 0) {
             const bool in = (uint32_t)lane < len;
-            double g = in ? (double)fmaxf(r.g[(int64_t)(t0 + lane) * r.g_stride + h], -1e5f) : 0.0;
+            const float g0 = in ? r.g[(int64_t)(t0 + lane) * r.g_stride + h] : 0.0f;
+            const float beta = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f, u = sU[lane];
+            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff()) || u != u;
+            const uint64_t bads = __ballot(bad);
+            const bool past = bads && lane >= __builtin_ctzll(bads);       // from the first such token on
+            double g = past ? 0.0 : (double)fmaxf(g0, -1e5f);
 #pragma unroll
             for (int o = 1; o < kWave; o <<= 1) {
                 const double v = __shfl_up(g, o, kWave);
@@ -375,32 +383,31 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
             }
             const double last = __shfl(g, kWave - 1, kWave);
             sG[lane] = g;
-            sB[lane] = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f;
-            const float eg = expf((float)g), u = sU[lane];
-            vec[lane] = u * eg;
+            sB[lane] = past ? __builtin_nanf("") : beta;
+            const float eg = expf((float)g);
+            sW[lane] = in && !past ? u * expf((float)(last - g)) : 0.0f;
+            vec[lane] = past ? __builtin_nanf("") : u * eg;
             vec[kChunk + lane] = sP[lane] * eg;
-            vec[2 * kChunk + lane] = in ? u * expf((float)(last - g)) : 0.0f;
-            vec[3 * kChunk + lane] = expf((float)last);
+            vec[2 * kChunk + lane] = expf((float)last);
         }
         __syncthreads();
+        f32x4 vp[4] = {};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int tj = 16 * j + l16;
+            const float bj = sB[tj];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int ti = 16 * wave + 4 * g4 + x;
-                float va = 0.0f, vp = 0.0f;
-                if (tj <= ti) {
+                float va = 0.0f;
+                if (j <= wave && tj <= ti && bj == bj && sB[ti] == sB[ti]) {
                     const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
                     va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
-                    vp = sP[ti] * w * qk[j][x];
+                    vp[j][x] = sP[ti] * w * qk[j][x];
                 }
                 sA[ti * kPitchA + tj] = va;
-                sT[ti * kPitchA + tj] = vp;
             }
         }
-        __syncthreads();
-        store_triangle<LO>(sT, unit + kTri * 3 * kFrag, wave, lane);
         __syncthreads();
         {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
             const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
@@ -456,21 +463,42 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
 #pragma unroll
                 for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
             }
+            __syncthreads();               // A is done with: P takes its place, and its columns take beta with T's
 #pragma unroll
             for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
         }
         __syncthreads();
-        // T diag(beta)
-        for (int f = wave; f < kTri; f += 4) {
-            const int tile = f < 2 ? f : 2 + (f - 2) / 2, s = f < 2 ? 0 : (f - 2) % 2, c0 = 32 * s + 8 * g4;
-            float v[8];
-            op_load(sT + tile_index(tile, l16) * kPitchA + c0, v);
+        f32x4 y[4] = {};                   // rows 16 wave of P (I + A)^-1
 #pragma unroll
-            for (int x = 0; x < 8; x++) v[x] *= sB[c0 + x];
-            const Split<3> y = split8<3>(v);
+        for (int j = 0; j < 4; j++) {
+            if (j > wave) break;
 #pragma unroll
-            for (int n = 0; n < 3; n++) *(bf16x8*)(unit + (f * 3 + n) * kFrag + lane * 16) = y.l[n];
+            for (int k = j; k < 4; k++) {
+                if (k > wave) break;
+#pragma unroll
+                for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
+            }
         }
+        // diag() T, and P T once every wave has read P: columns times beta (0 from a token that is not finite on)
+        const auto beta_of = [&](int t) { const float v = sB[t]; return v == v ? v : 0.0f; };
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float bj = beta_of(16 * j + l16);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
+                sA[at_] = y[j][x] * bj;
+                sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
+            }
+        }
+        __syncthreads();
+        store_triangle<3>(sT, sW, unit, wave, lane);
+        store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
     }
 }
 
@@ -478,18 +506,36 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
 // neighbouring rows meet no bank twice.
 template <typename T> constexpr int pitch_of(int n) { return n + 16 / (int)sizeof(T); }
 
+// A buffer descriptor: loads past `bytes` give zeros, stores there are dropped.
+__device__ __forceinline__ auto rows_rsrc(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+template <typename T, typename R>
+__device__ __forceinline__ float buffer_elem(R rsrc, uint32_t at) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0));
+    else
+        return (float)__builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0));
+}
+
 // One workgroup of W waves takes 16 W columns of one head's state through a sequence.  A chunk's keys (in both
-// orders) and queries stand in LDS; T, P, the values and the diagonals are each wave's own registers.  All of
-// them are requested a chunk ahead: behind barrier A(c), when every wave is done with the state's products, the
-// keys and queries of chunk c + 1 replace those of c in LDS (k^T has two buffers, since chunk c still reads its
-// own) and those of c + 2 are requested; barrier B(c) ends the chunk.
+// orders), queries and its unit of the workspace stand in LDS; its values are each wave's own.  All of them are
+// requested a chunk ahead of their use.  A chunk has two halves: up to barrier A the products with the state
+// (keys, queries) while the unit of this chunk is put in place; up to barrier B those with X (the unit, k^T) while
+// the next chunk's keys and queries are.  k^T has two buffers where they fit and is written with the keys; where
+// they do not (f32, dk 128) it is written from the same registers in the first half, and the next
+// request of keys waits for that.
 template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
-    constexpr int LO = Limbs<T>::out, KS = DK / 32, NT = DK / 16;
+__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkArgs a) {
+    constexpr int LO = Limbs<T>::out, KS = DK / 32, NT = DK / 16, SZ = sizeof(T);
     constexpr int PK = pitch_of<T>(DK), PT = pitch_of<T>(kChunk);
     constexpr int kUnits = 32 * (DK / 8) / (64 * W);       // (pair of tokens, eight columns) a thread
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * (kChunk * PK + DK * PT) * sizeof(T)];
-    __shared__ __attribute__((aligned(16))) float sV[2][4 * kChunk];
+    constexpr int kImage = unit_bytes(LO), kImageLoads = (kImage / 16 + 64 * W - 1) / (64 * W);
+    constexpr bool kTwo = DK * SZ <= 256;
+    static_assert(kUnits >= 1 && 32 * (DK / 8) % (64 * W) == 0, "");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[(2 * kChunk * PK + (kTwo ? 2 : 1) * DK * PT) * SZ];
+    __shared__ __attribute__((aligned(16))) unsigned char image[kImageLoads * 64 * W * 16];
     T* const sK = (T*)lds;                 // row: token in the order (*)
     T* const sQ = sK + kChunk * PK;
     T* const sKT = sQ + kChunk * PK;       // row: column of k in the order (*); the tokens in their own
@@ -501,13 +547,13 @@ __global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
     if (!w.live) return;
     const uint32_t i = w.unit / r.hk, hq = w.unit % r.hk, h = hq * group + w.part / cols;
     const uint32_t col16 = (w.part % cols) * W + wave;
-    const bool mine = col16 < r.dv / 16;   // (the last workgroup of a head may have a wave too many, which helps loading)
+    const bool mine = col16 < r.dv / 16;   // (the last workgroup of a head may have waves too many, which help loading)
     const uint32_t col = mine ? 16 * col16 + l16 : l16;
     const int slot = entry_slot(a.d.slots, a.d.n_slots, i, a.d.states != nullptr, lane);
     if (slot == kSkip) return;
     const uint32_t b = row_of(a, i), e = max(row_of(a, i + 1), b);
-    T* const out = (T*)r.out + (size_t)h * r.dv + col;
     if (slot == kBad) {
+        T* const out = (T*)r.out + (size_t)h * r.dv + col;
         if (mine)
             for (uint32_t t = b + g4; t < e; t += 4) out[(int64_t)t * r.out_stride] = (T)__builtin_nanf("");
         return;
@@ -520,89 +566,122 @@ __global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
         for (int x = 0; x < 4; x++)
             S[p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] : 0.0f;
     const uint32_t chunks = (e - b + kChunk - 1) / kChunk;
-    const unsigned char* const units = a.ws + ((size_t)first_chunk(b, i) * r.hv + h) * unit_bytes(LO);
-    const size_t unit_step = (size_t)r.hv * unit_bytes(LO);
-    typedef T vec8 __attribute__((ext_vector_type(8)));
+    const unsigned char* const units = a.ws + ((size_t)first_chunk(b, i) * r.hv + h) * kImage;
+    const size_t unit_step = (size_t)r.hv * kImage;
+    typedef T vec8 __attribute__((ext_vector_type(8), aligned(16)));      // (rows in LDS are odd multiples of 16 bytes)
     typedef T vec2 __attribute__((ext_vector_type(2)));
+    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
     vec8 kv[kUnits][2], qv[kUnits][2];
-    bf16x8 tf[kTri][3], pf[kTri][LO];
-    T vv[4][4];
-    float4 dv = make_float4(0, 0, 0, 0);
+    u32x4 iv[kImageLoads];
+    float vv[4][4];
+    // A row's place within a chunk is a part of the lane's and a uniform one; buffer accesses end the chunk by their bounds
+    // (which count the vector offset only, so the scalar one stays 0).
+    const uint32_t tp0 = threadIdx.x / (DK / 8), o8 = threadIdx.x % (DK / 8) * 8;
+    const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ, vs = (uint32_t)r.v_stride * SZ,
+                   os = (uint32_t)r.out_stride * SZ;
+    const uint32_t k_at = 2 * tp0 * ks + o8 * SZ, q_at = 2 * tp0 * qs + o8 * SZ, v_at = 8 * g4 * vs + (h * r.dv + col) * SZ,
+                   o_at = mine ? 8 * g4 * os + (h * r.dv + col) * SZ : 0x80000000u;
 
     const auto rows_in = [&](uint32_t c) { return min(e - b - c * kChunk, (uint32_t)kChunk); };
-    // Requests of chunk c, rows past its end the last one (they are replaced by zeros where they are used).
-    const auto load_kq = [&](uint32_t c) {
-        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
-#pragma unroll
-        for (int u = 0; u < kUnits; u++) {
-            const uint32_t id = u * 64 * W + threadIdx.x, tp = id / (DK / 8), o = id % (DK / 8);
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const uint32_t t = t0 + min(2 * tp + y, len - 1);
-                kv[u][y] = *(const vec8*)((const T*)r.k + (int64_t)t * r.k_stride + hq * DK + 8 * o);
-                qv[u][y] = *(const vec8*)((const T*)r.q + (int64_t)t * r.q_stride + hq * DK + 8 * o);
-            }
-        }
-        if (wave == 0) dv = ((const float4*)(units + c * unit_step + kTri * (3 + LO) * kFrag))[lane];
+    const auto rsrc_of = [&](const void* p, uint32_t c, uint32_t stride, uint32_t first_col, uint32_t width) {
+        return rows_rsrc((const unsigned char*)p + (size_t)(b + c * kChunk) * stride + (size_t)first_col * SZ,
+                         (rows_in(c) - 1) * stride + width * SZ);
     };
-    const auto store_kq = [&](uint32_t c) {
-        const uint32_t len = rows_in(c);
-        T* const kt = sKT + c % 2 * (DK * PT);
+    const auto load16 = [&](auto rsrc, uint32_t off) {
+        if constexpr (SZ == 2) {
+            return __builtin_bit_cast(vec8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
+        } else {
+            struct { u32x4 v[2]; } x = {{__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0),
+                                        __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off + 16, 0, 0)}};
+            return __builtin_bit_cast(vec8, x);
+        }
+    };
+    const auto load_kq = [&](uint32_t c) {
+        const auto rk = rsrc_of(r.k, c, ks, hq * DK, DK);
+        const auto rq = rsrc_of(r.q, c, qs, hq * DK, DK);
 #pragma unroll
-        for (int u = 0; u < kUnits; u++) {
-            const int id = u * 64 * W + threadIdx.x, tp = id / (DK / 8), o = id % (DK / 8);
+        for (int u = 0; u < kUnits; u++)
 #pragma unroll
             for (int y = 0; y < 2; y++) {
-                const int t = 2 * tp + y, row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
-                if ((uint32_t)t >= len) kv[u][y] = qv[u][y] = vec8{};
-                *(vec8*)(sK + row * PK + 8 * o) = kv[u][y];
-                *(vec8*)(sQ + row * PK + 8 * o) = qv[u][y];
+                const uint32_t t = 2 * u * (64 * W / (DK / 8)) + y;
+                kv[u][y] = load16(rk, k_at + t * ks);
+                qv[u][y] = load16(rq, q_at + t * qs);
             }
+    };
+    const auto store_kt = [&](uint32_t c) {
+        T* const kt = sKT + (kTwo ? c % 2 * (DK * PT) : 0);
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            const int tp = u * (64 * W / (DK / 8)) + tp0;
 #pragma unroll
             for (int x = 0; x < 8; x++) {
-                const int d = 8 * o + x, row = 32 * (d / 32) + 16 * (d / 4 % 2) + 4 * (d / 8 % 4) + d % 4;
+                const int d = o8 + x, row = 32 * (d / 32) + 16 * (d / 4 % 2) + 4 * (d / 8 % 4) + d % 4;
                 *(vec2*)(kt + row * PT + 2 * tp) = vec2{kv[u][0][x], kv[u][1][x]};
             }
         }
-        if (wave == 0) ((float4*)sV[c % 2])[lane] = dv;
+    };
+    const auto store_kq = [&](uint32_t c) {
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            const int tp = u * (64 * W / (DK / 8)) + tp0;
+#pragma unroll
+            for (int y = 0; y < 2; y++) {
+                const int t = 2 * tp + y, row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
+                *(vec8*)(sK + row * PK + o8) = kv[u][y];
+                *(vec8*)(sQ + row * PK + o8) = qv[u][y];
+            }
+        }
+        if (kTwo) store_kt(c);
+    };
+    const auto load_image = [&](uint32_t c) {
+        const auto ri = rows_rsrc(units + c * unit_step, kImage);
+#pragma unroll
+        for (int x = 0; x < kImageLoads; x++)
+            iv[x] = __builtin_amdgcn_raw_buffer_load_b128(ri, (int)(threadIdx.x * 16 + x * 64 * W * 16), 0, 0);
+    };
+    const auto store_image = [&]() {
+#pragma unroll
+        for (int x = 0; x < kImageLoads; x++) *(u32x4*)(image + (x * 64 * W + threadIdx.x) * 16) = iv[x];
     };
     const auto load_v = [&](uint32_t c) {
-        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
+        const auto rv = rsrc_of(r.v, c, vs, 0, r.hv * r.dv);
 #pragma unroll
         for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int x = 0; x < 4; x++)
-                vv[m][x] = ((const T*)r.v)[(int64_t)(t0 + min((uint32_t)tile_index(m, 4 * g4) + x, len - 1)) * r.v_stride +
-                                           (size_t)h * r.dv + col];
-    };
-    const auto load_t = [&](uint32_t c) {
-#pragma unroll
-        for (int f = 0; f < kTri; f++)
-#pragma unroll
-            for (int n = 0; n < 3; n++)
-                tf[f][n] = *(const bf16x8*)(units + c * unit_step + (f * 3 + n) * kFrag + lane * 16);
-    };
-    const auto load_p = [&](uint32_t c) {
-#pragma unroll
-        for (int f = 0; f < kTri; f++)
-#pragma unroll
-            for (int n = 0; n < LO; n++)
-                pf[f][n] = *(const bf16x8*)(units + c * unit_step + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
+            for (int x = 0; x < 4; x++) vv[m][x] = buffer_elem<T>(rv, v_at + (tile_index(m, 0) + x) * vs);
     };
     if (chunks) {
         load_kq(0);
-        load_t(0);
+        load_image(0);
         load_v(0);
-        load_p(0);
         store_kq(0);
-        if (chunks > 1) load_kq(1);
+        if (kTwo && chunks > 1) load_kq(1);
     }
     __syncthreads();
+    const float* const vec = (const float*)(image + kTri * (3 + LO) * kFrag);
+    const auto frag = [&](int f, int limb, int first, int limbs) {
+        return *(const bf16x8*)(image + (first + f * limbs + limb) * kFrag + lane * 16);
+    };
+    const auto tfrag = [&](int f) {
+        Split<3> o;
+#pragma unroll
+        for (int n = 0; n < 3; n++) o.l[n] = frag(f, n, 0, 3);
+        return o;
+    };
+    const auto pfrag = [&](int f) {
+        Split<LO> o;
+#pragma unroll
+        for (int n = 0; n < LO; n++) o.l[n] = frag(f, n, kTri * 3, LO);
+        return o;
+    };
     for (uint32_t c = 0; c < chunks; c++) {
-        const uint32_t t0 = b + c * kChunk, len = rows_in(c);
         const bool more = c + 1 < chunks;
-        const float* const vec = sV[c % 2];
-        const T* const kt = sKT + c % 2 * (DK * PT);
+        store_image();
+        if (more) load_image(c + 1);
+        if (!kTwo) {
+            store_kt(c);
+            if (more) load_kq(c + 1);
+        }
         f32x4 X[4] = {}, O[4] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
@@ -613,47 +692,74 @@ __global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
         __syncthreads();                   // A
         if (more) {
             store_kq(c + 1);
-            if (c + 2 < chunks) load_kq(c + 2);
+            if (kTwo && c + 2 < chunks) load_kq(c + 2);
         }
+        uint32_t top = 0;
 #pragma unroll
         for (int m = 0; m < 4; m++) {
             const int t = tile_index(m, 4 * g4);
             const f32x4 kd = *(const f32x4*)(vec + t), qd = *(const f32x4*)(vec + kChunk + t);
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                X[m][x] = ((uint32_t)(t + x) < len ? (float)vv[m][x] : 0.0f) - kd[x] * X[m][x];
+                const float v = vv[m][x] - kd[x] * X[m][x];
+                X[m][x] = v;
                 O[m][x] *= qd[x];
+                top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
             }
         }
         if (more) load_v(c + 1);
+        int bad = kChunk;                  // this column's first token that is not finite
+        const bool any_bad = __any(top >= 0x7f800000u);
+        if (any_bad) {
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (!(fabsf(X[m][x]) < __builtin_inff())) bad = min(bad, tile_index(m, 4 * g4) + x);
+            bad = min(bad, __shfl_xor(bad, 16, kWave));
+            bad = min(bad, __shfl_xor(bad, 32, kWave));
+#pragma unroll
+            for (int m = 0; m < 4; m++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (tile_index(m, 4 * g4) + x >= bad) X[m][x] = 0.0f;
+        }
         f32x4 D[4] = {};
         {
-            const Split<3> x0 = split_pair<3>(X[0], X[1]);
-            mma_rows<3>([&](int m) { return as_split<3>(tf[m < 2 ? m : 2 * m - 2]); }, x0, D);
-            const Split<3> x1 = split_pair<3>(X[2], X[3]);
-#pragma unroll
-            for (int m = 2; m < 4; m++) D[m] = mma_limbs<3>(as_split<3>(tf[2 * m - 1]), x1, D[m]);
+            const Split<3> x = split_pair<3>(X[0], X[1]);
+            mma_rows<3>([&](int m) { return tfrag(m < 2 ? m : 2 * m - 2); }, x, D);
+            mma_rows<LO>([&](int m) { return pfrag(m < 2 ? m : 2 * m - 2); }, x, O);
         }
-        if (more) load_t(c + 1);
         {
-            const Split<LO> x0 = split_pair<LO>(D[0], D[1]);
-            mma_rows<LO>([&](int m) { return as_split<LO>(pf[m < 2 ? m : 2 * m - 2]); }, x0, O);
-            const Split<LO> x1 = split_pair<LO>(D[2], D[3]);
+            const Split<3> x = split_pair<3>(X[2], X[3]);
+            const Split<3> t2 = tfrag(3), t3 = tfrag(5);
+            const Split<LO> p2 = pfrag(3), p3 = pfrag(5);
 #pragma unroll
-            for (int m = 2; m < 4; m++) O[m] = mma_limbs<LO>(as_split<LO>(pf[2 * m - 1]), x1, O[m]);
+            for (int n = 0; n < 3; n++)
+#pragma unroll
+                for (int j = 0; j < 3 - n; j++) {
+                    D[2] = mma(t2.l[n], x.l[j], D[2]);
+                    D[3] = mma(t3.l[n], x.l[j], D[3]);
+                    if (n + j < LO) {
+                        O[2] = mma(p2.l[n], x.l[j], O[2]);
+                        O[3] = mma(p3.l[n], x.l[j], O[3]);
+                    }
+                }
         }
-        if (more) load_p(c + 1);
-        const float keep = vec[3 * kChunk];
+        if (any_bad) {
+            const float nan = __builtin_nanf("");
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const f32x4 wd = *(const f32x4*)(vec + 2 * kChunk + tile_index(m, 4 * g4));
+            for (int m = 0; m < 4; m++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) D[m][x] *= wd[x];
+                for (int x = 0; x < 4; x++)
+                    if (tile_index(m, 4 * g4) + x >= bad) O[m][x] = D[m][x] = nan;
         }
+        const float keep = vec[2 * kChunk];
 #pragma unroll
         for (int p = 0; p < NT; p++)
 #pragma unroll
             for (int x = 0; x < 4; x++) S[p][x] *= keep;
+        const T* const kt = sKT + (kTwo ? c % 2 * (DK * PT) : 0);
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const Split<3> x = split_pair<3>(D[2 * s], D[2 * s + 1]);
@@ -661,15 +767,16 @@ __global__ __launch_bounds__(64 * W, 1) void k_delta_chunks(ChunkArgs a) {
             for (int p = 0; p < NT; p += 4)
                 mma_rows<3>([&](int m) { return load_limbs(kt + (16 * (p + m) + l16) * PT + 32 * s + 8 * g4); }, x, &S[p]);
         }
-        if (mine) {
+        const auto ro = rsrc_of(r.out, c, os, 0, r.hv * r.dv);
 #pragma unroll
-            for (int m = 0; m < 4; m++)
+        for (int m = 0; m < 4; m++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    const int t = tile_index(m, 4 * g4) + x;
-                    if ((uint32_t)t < len) out[(int64_t)(t0 + t) * r.out_stride] = (T)O[m][x];
-                }
-        }
+            for (int x = 0; x < 4; x++) {
+                const int o = (int)(o_at + (tile_index(m, 0) + x) * os);
+                const T y = (T)(float)O[m][x];
+                if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, y), ro, o, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, y), ro, o, 0, 0);
+            }
         __syncthreads();                   // B
     }
     if (a.d.states && mine) {
@@ -689,12 +796,16 @@ const void* delta_prep_fn(uint32_t dtype, uint32_t dk) {
     return fns[dtype][dk == 128];
 }
 
+// Waves of a workgroup: at dk 64 the loads of a chunk keep four waves busy.
+constexpr int waves_of(int dk, int w) { return dk == 64 && w > 4 ? 4 : w; }
+
 template <int W>
 const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
+    constexpr int W64 = waves_of(64, W);
     static const void* const fns[3][2] = {
-        {(const void*)k_delta_chunks<__bf16, 64, W>, (const void*)k_delta_chunks<__bf16, 128, W>},
-        {(const void*)k_delta_chunks<_Float16, 64, W>, (const void*)k_delta_chunks<_Float16, 128, W>},
-        {(const void*)k_delta_chunks<float, 64, W>, (const void*)k_delta_chunks<float, 128, W>},
+        {(const void*)k_delta_chunks<__bf16, 64, W64>, (const void*)k_delta_chunks<__bf16, 128, W>},
+        {(const void*)k_delta_chunks<_Float16, 64, W64>, (const void*)k_delta_chunks<_Float16, 128, W>},
+        {(const void*)k_delta_chunks<float, 64, W64>, (const void*)k_delta_chunks<float, 128, W>},
     };
     return fns[dtype][dk == 128];
 }
@@ -702,13 +813,13 @@ const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
 uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
 
 #ifndef KW
-#define KW 4
+#define KW 2
 #endif
 constexpr int kW = KW;
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
     const uint64_t prep = chunk_slots(r, k.d.n) * r.hk;
-    constexpr int W = kW;
+    const uint32_t W = waves_of(r.dk, kW);
     const uint64_t cols = (r.dv / 16 + W - 1) / W, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
@@ -716,7 +827,7 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    return op_launch(delta_chunks_fn<W>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(64 * W), 0, stream, k);
+    return op_launch(delta_chunks_fn<kW>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(64 * W), 0, stream, k);
 }
 
 bool sizes_ok(const redukt_delta_rows* a) {
@@ -724,6 +835,8 @@ bool sizes_ok(const redukt_delta_rows* a) {
            (a->dk == 64 || a->dk == 128) && a->dv > 0 && a->dv % 32 == 0 && a->dv <= 256 && a->rows < (1u << 31) &&
            (a->flags & ~REDUKT_DELTA_NORMALIZE) == 0;
 }
+
+constexpr int64_t kMaxStride = 1 << 22;      // a chunk's 64 rows stay within 32-bit offsets
 
 bool rows_ok(const redukt_delta_rows* a) {
     const int64_t per = 16 / op_elem_bytes(a->dtype);
@@ -733,7 +846,7 @@ bool rows_ok(const redukt_delta_rows* a) {
                              (int64_t)a->hv * a->dv};
     for (int i = 0; i < 4; i++) {
         if (!ptrs[i] || !op_aligned(ptrs[i], 16) || strides[i] % per) return false;
-        if (a->rows > 1 && strides[i] < width[i] && (i == 3 || strides[i] != 0)) return false;
+        if (a->rows > 1 && (strides[i] < width[i] || strides[i] > kMaxStride)) return false;
     }
     return a->g && a->beta && op_aligned(a->g, 4) && op_aligned(a->beta, 4) &&
            (a->rows <= 1 || (a->g_stride >= 0 && a->beta_stride >= 0));
@@ -743,6 +856,15 @@ bool rows_ok(const redukt_delta_rows* a) {
 bool apart(const void* a, const void* b, size_t n) {
     const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
     return x == y || (x < y ? y - x : x - y) >= n;
+}
+
+// The rows with a step from one to the next that is a row's width where there is one row only.
+redukt_delta_rows stepped(redukt_delta_rows a) {
+    if (a.rows == 1) {
+        a.q_stride = a.k_stride = (int64_t)a.hk * a.dk;
+        a.v_stride = a.out_stride = (int64_t)a.hv * a.dv;
+    }
+    return a;
 }
 
 int32_t launch_rows(DeltaArgs& k, void* stream) {
@@ -766,7 +888,7 @@ int32_t redukt_op_delta_step(const redukt_delta_rows* a, float* states, uint32_t
     if (n_slots >= (1u << 31) || (!slots && a->rows > n_slots)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(a->out);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    DeltaArgs k{*a, states, states, n_slots, slots, nullptr, a->rows};
+    DeltaArgs k{stepped(*a), states, states, n_slots, slots, nullptr, a->rows};
     return launch_rows(k, stream);
 }
 
@@ -795,7 +917,7 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ChunkArgs k{{*a, state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace};
+    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace};
     return launch_chunks(k, stream);
 }
 

@@ -268,6 +268,43 @@ def test_delta_chunk_of_values_of_many_sizes():
     check(S[0], S64, S_tol, "state")
 
 
+@types
+@pytest.mark.parametrize("which", ["v", "k", "q", "g", "beta", "g_inf", "state"])
+@pytest.mark.parametrize("at", [0, 29, 64, 99])
+def test_delta_chunk_what_is_not_finite_reaches_no_earlier_token(which, at, dtype):
+    """A value that is not finite at one token leaves every earlier token's output as it was, and other columns, heads
+    and sequences where the rule does not carry it to them."""
+    lens, dk, dv = [130, 70], 64, 64
+    x = rule_inputs(200, 2, 2, dk, dv, dtype, seed=2, normalize=True)
+    cu = torch.tensor([0, 130, 200], dtype=torch.int32, device="cuda")
+    before = pool_of(2, 2, dk, dv)
+    S = torch.empty_like(before)
+    want = ops.delta_chunk(*x, cu, state_in=before, state_out=S, normalize=True)
+    y, start = [t.clone() for t in x], before.clone()
+    cols = slice(None)
+    if which == "v":
+        y[2][at, 1, 5] = float("nan")
+        cols = slice(5, 6)
+    elif which == "state":
+        start[0, 1, 3, 5] = float("inf")
+        cols, at = slice(5, 6), 0
+    elif which == "g_inf":
+        y[3][at, 1] = float("inf")
+    else:
+        y[{"q": 0, "k": 1, "g": 3, "beta": 4}[which]][at, 1] = float("nan")
+    S2 = torch.empty_like(before)
+    got = ops.delta_chunk(*y, cu, state_in=start, state_out=S2, normalize=True)
+    bad = torch.zeros(200, 2, dv, dtype=torch.bool, device="cuda")
+    if which == "q":
+        bad[at, 1] = True
+    else:
+        bad[at:130, 1, cols] = True
+        assert S2[0, 1, :, cols].isnan().all()
+        S2[0, 1, :, cols] = S[0, 1, :, cols]
+    assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
+    assert torch.equal(S2, S)
+
+
 def test_delta_chunk_in_place_shared_and_bad_slots():
     hv, dk, dv = 2, 64, 64
     lens = [40, 70, 3, 5, 9]

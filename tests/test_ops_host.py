@@ -55,7 +55,8 @@ BAD_ROWS = [dict(dtype=3), dict(hk=0), dict(hv=0), dict(hk=3), dict(hv=4100, hk=
             dict(dv=16), dict(dv=288), dict(flags=2), dict(rows=1 << 31), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
             dict(g=None), dict(beta=None), dict(q=P + 8), dict(k=P + 2), dict(v=P + 4), dict(out=P + 8), dict(g=P + 2),
             dict(beta=P + 1), dict(q_stride=132), dict(k_stride=127), dict(v_stride=128), dict(out_stride=0), dict(out_stride=128),
-            dict(q_stride=-128), dict(g_stride=-1)]
+            dict(q_stride=-128), dict(g_stride=-1),
+            dict(q_stride=0), dict(v_stride=0), dict(k_stride=(1 << 22) + 8), dict(out_stride=1 << 30)]
 
 
 @pytest.mark.parametrize("over", BAD_ROWS, ids=str)
