@@ -512,11 +512,11 @@ __device__ __forceinline__ auto rows_rsrc(const void* p, uint32_t bytes) {
 }
 
 template <typename T, typename R>
-__device__ __forceinline__ float buffer_elem(R rsrc, uint32_t at) {
+__device__ __forceinline__ T buffer_elem(R rsrc, uint32_t at) {
     if constexpr (sizeof(T) == 4)
-        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0));
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0));
     else
-        return (float)__builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0));
+        return __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0));
 }
 
 // One workgroup of W waves takes 16 W columns of one head's state through a sequence.  A chunk's keys (in both
@@ -573,7 +573,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
     typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
     vec8 kv[kUnits][2], qv[kUnits][2];
     u32x4 iv[kImageLoads];
-    float vv[4][4];
+    T vv[4][4];                            // (as they are: a conversion would wait for them)
     // A row's place within a chunk is a part of the lane's and a uniform one; buffer accesses end the chunk by their bounds
     // (which count the vector offset only, so the scalar one stays 0).
     const uint32_t tp0 = threadIdx.x / (DK / 8), o8 = threadIdx.x % (DK / 8) * 8;
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
         load_image(0);
         load_v(0);
         store_kq(0);
-        if (kTwo && chunks > 1) load_kq(1);
+        if (kTwo) load_kq(min(1u, chunks - 1));
     }
     __syncthreads();
     const float* const vec = (const float*)(image + kTri * (3 + LO) * kFrag);
@@ -675,12 +675,13 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
         return o;
     };
     for (uint32_t c = 0; c < chunks; c++) {
-        const bool more = c + 1 < chunks;
+        // (the last chunk requests itself again instead of one past the end)
+        const uint32_t next = min(c + 1, chunks - 1);
         store_image();
-        if (more) load_image(c + 1);
+        load_image(next);
         if (!kTwo) {
             store_kt(c);
-            if (more) load_kq(c + 1);
+            load_kq(next);
         }
         f32x4 X[4] = {}, O[4] = {};
 #pragma unroll
@@ -690,10 +691,8 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
             mma_rows<LO>([&](int m) { return load_limbs(sQ + (16 * m + l16) * PK + 32 * s + 8 * g4); }, x, O);
         }
         __syncthreads();                   // A
-        if (more) {
-            store_kq(c + 1);
-            if (kTwo && c + 2 < chunks) load_kq(c + 2);
-        }
+        store_kq(c + 1);
+        if (kTwo) load_kq(min(c + 2, chunks - 1));
         uint32_t top = 0;
 #pragma unroll
         for (int m = 0; m < 4; m++) {
@@ -701,13 +700,13 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
             const f32x4 kd = *(const f32x4*)(vec + t), qd = *(const f32x4*)(vec + kChunk + t);
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                const float v = vv[m][x] - kd[x] * X[m][x];
+                const float v = (float)vv[m][x] - kd[x] * X[m][x];
                 X[m][x] = v;
                 O[m][x] *= qd[x];
                 top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
             }
         }
-        if (more) load_v(c + 1);
+        load_v(next);
         int bad = kChunk;                  // this column's first token that is not finite
         const bool any_bad = __any(top >= 0x7f800000u);
         if (any_bad) {
