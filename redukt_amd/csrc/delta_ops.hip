@@ -193,19 +193,36 @@ struct Split {
     bf16x8 l[N];
 };
 
-// Eight f32 as N bf16 limbs: each the rounded rest of those before it.
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// a and b rounded to bf16, in the low and the high half of a word.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+}
+
+// Eight f32 as N bf16 limbs: each the rounded rest of those before it (the differences are exact).
 template <int N>
 __device__ __forceinline__ Split<N> split8(const float (&v)[8]) {
-    Split<N> o;
+    u32x4 w[N];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        float r = v[j];
+    for (int j = 0; j < 4; j++) {
+        float a = v[2 * j], b = v[2 * j + 1];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            o.l[n][j] = (__bf16)r;
-            if (n + 1 < N) r -= (float)o.l[n][j];
+            const uint32_t p = pack_bf16(a, b);
+            w[n][j] = p;
+            if (n + 1 < N) {
+                a -= __builtin_bit_cast(float, p << 16);
+                b -= __builtin_bit_cast(float, p & 0xffff0000u);
+            }
         }
     }
+    Split<N> o;
+#pragma unroll
+    for (int n = 0; n < N; n++) o.l[n] = __builtin_bit_cast(bf16x8, w[n]);
     return o;
 }
 
@@ -253,9 +270,20 @@ __device__ __forceinline__ void mma_rows(A&& a, const Split<NB>& b, C&& c) {
             }
 }
 
+constexpr int kt_bytes(int dk, int in_limbs) { return dk / 16 * 2 * in_limbs * kFrag; }
+
+template <int N>
+__device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
+    Split<N> o;
+#pragma unroll
+    for (int n = 0; n < N; n++) o.l[n] = v[n];
+    return o;
+}
+
 struct ChunkArgs {
     DeltaArgs d;
-    unsigned char* ws;         // unit (chunk slot, value head): unit_bytes
+    unsigned char* ws;         // units: (chunk slot, value head)
+    unsigned char* kt;         // fragments of k^T: (chunk slot, key head)
 };
 
 // Sequence i's rows, within [0, rows].
@@ -290,16 +318,16 @@ __device__ __forceinline__ void store_triangle(const float* m, const float* f, u
     }
 }
 
-// One workgroup a chunk and key head: k.k and q.k of the chunk once, then the unit of each value head of the group.
+// One workgroup a chunk and value head: its unit, and with a key head's first value head the fragments of k^T.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32;
     __shared__ __attribute__((aligned(16))) float sA[kChunk * kPitchA], sT[kChunk * kPitchA];
     __shared__ double sG[kChunk];
     __shared__ float sB[kChunk], sU[kChunk], sP[kChunk], sW[kChunk];
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
-    const uint32_t slot = blockIdx.x / r.hk, hq = blockIdx.x % r.hk, group = r.hv / r.hk;
+    const uint32_t slot = blockIdx.x / r.hv, h = blockIdx.x % r.hv, group = r.hv / r.hk, hq = h / group;
     uint32_t lo = 0, hi = a.d.n - 1;       // the last sequence that starts at this slot or before
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1) / 2;
@@ -364,230 +392,232 @@ __global__ __launch_bounds__(256) void k_delta_prep(ChunkArgs a) {
     q2 += __shfl_xor(q2, 32, kWave);
     if (g4 == 0) sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
 
-    for (uint32_t h = hq * group; h < (hq + 1) * group; h++) {
-        unsigned char* unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
-        float* vec = (float*)(unit + kTri * (3 + LO) * kFrag);
-        __syncthreads();                   // sU, sP are written; the last head's reads are done
-        if (wave == 0) {
-            const bool in = (uint32_t)lane < len;
-            const float g0 = in ? r.g[(int64_t)(t0 + lane) * r.g_stride + h] : 0.0f;
-            const float beta = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f, u = sU[lane];
-            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff()) || u != u;
-            const uint64_t bads = __ballot(bad);
-            const bool past = bads && lane >= __builtin_ctzll(bads);       // from the first such token on
-            double g = past ? 0.0 : (double)fmaxf(g0, -1e5f);
+    unsigned char* unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
+    float* vec = (float*)(unit + kTri * (3 + LO) * kFrag);
+    if (h % group == 0) {
+        // row (*) of k^T's tile p, the tokens 32 s + 8 g + [0, 8)
+        unsigned char* const kt = a.kt + ((size_t)slot * r.hk + hq) * kt_bytes(DK, LI);
+        for (int f = wave; f < DK / 16 * 2; f += 4) {
+            const T* const col = kp + tile_index(f / 2, l16);
+            float v[8];
 #pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const double v = __shfl_up(g, o, kWave);
-                if (lane >= o) g += v;
+            for (int x = 0; x < 8; x++) {
+                const uint32_t t = 32 * (f % 2) + 8 * g4 + x;
+                v[x] = t < len ? (float)col[(int64_t)(t0 + t) * r.k_stride] : 0.0f;
             }
-            const double last = __shfl(g, kWave - 1, kWave);
-            sG[lane] = g;
-            sB[lane] = past ? __builtin_nanf("") : beta;
-            const float eg = expf((float)g);
-            sW[lane] = in && !past ? u * expf((float)(last - g)) : 0.0f;
-            vec[lane] = past ? __builtin_nanf("") : u * eg;
-            vec[kChunk + lane] = sP[lane] * eg;
-            vec[2 * kChunk + lane] = expf((float)last);
+            const Split<LI> y = split8<LI>(v);
+#pragma unroll
+            for (int n = 0; n < LI; n++) *(bf16x8*)(kt + (f * LI + n) * kFrag + lane * 16) = y.l[n];
         }
-        __syncthreads();
-        f32x4 vp[4] = {};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int tj = 16 * j + l16;
-            const float bj = sB[tj];
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int ti = 16 * wave + 4 * g4 + x;
-                float va = 0.0f;
-                if (j <= wave && tj <= ti && bj == bj && sB[ti] == sB[ti]) {
-                    const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
-                    va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
-                    vp[j][x] = sP[ti] * w * qk[j][x];
-                }
-                sA[ti * kPitchA + tj] = va;
-            }
-        }
-        __syncthreads();
-        {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
-            const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
-            float t[16];
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float v0 = i == l16 ? 1.0f : 0.0f, v1 = 0.0f;
-#pragma unroll
-                for (int j = 0; j < i; j++) {
-                    if (j % 2) v1 -= A[i * kPitchA + j] * t[j];
-                    else v0 -= A[i * kPitchA + j] * t[j];
-                }
-                t[i] = v0 + v1;
-            }
-            float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
-            if (g4 == 0) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
-            }
-        }
-        __syncthreads();
-        // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
-        auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
-        if (wave < 2) {
-            const int i = 2 * wave + 1, j = 2 * wave;
-            f32x4 m = {}, y = {};
-#pragma unroll
-            for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
-#pragma unroll
-            for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
-#pragma unroll
-            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
-        } else {   // the upper blocks within 32, which the fragments cover
-            const int i = 2 * (wave - 2);
-#pragma unroll
-            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
-        }
-        __syncthreads();
-        {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
-            const int i = wave / 2, j = wave % 2;
-            f32x4 y = {};
-#pragma unroll
-            for (int p = 0; p < 2; p++) {
-                if (p > i) break;
-                f32x4 m = {};
-#pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    if (q < j) continue;
-#pragma unroll
-                    for (int s = 0; s < 4; s++)
-                        m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
-            }
-            __syncthreads();               // A is done with: P takes its place, and its columns take beta with T's
-#pragma unroll
-            for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-#pragma unroll
-                for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
-        }
-        __syncthreads();
-        f32x4 y[4] = {};                   // rows 16 wave of P (I + A)^-1
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j > wave) break;
-#pragma unroll
-            for (int k = j; k < 4; k++) {
-                if (k > wave) break;
-#pragma unroll
-                for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
-            }
-        }
-        // diag() T, and P T once every wave has read P: columns times beta (0 from a token that is not finite on)
-        const auto beta_of = [&](int t) { const float v = sB[t]; return v == v ? v : 0.0f; };
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float bj = beta_of(16 * j + l16);
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
-                sA[at_] = y[j][x] * bj;
-                sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
-            }
-        }
-        __syncthreads();
-        store_triangle<3>(sT, sW, unit, wave, lane);
-        store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
     }
+    __syncthreads();                       // sU and sP are written
+    if (wave == 0) {
+        const bool in = (uint32_t)lane < len;
+        const float g0 = in ? r.g[(int64_t)(t0 + lane) * r.g_stride + h] : 0.0f;
+        const float beta = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f, u = sU[lane];
+        const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff()) || u != u;
+        const uint64_t bads = __ballot(bad);
+        const bool past = bads && lane >= __builtin_ctzll(bads);       // from the first such token on
+        double g = past ? 0.0 : (double)fmaxf(g0, -1e5f);
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const double v = __shfl_up(g, o, kWave);
+            if (lane >= o) g += v;
+        }
+        const double last = __shfl(g, kWave - 1, kWave);
+        sG[lane] = g;
+        sB[lane] = past ? __builtin_nanf("") : beta;
+        const float eg = expf((float)g);
+        sW[lane] = in && !past ? u * expf((float)(last - g)) : 0.0f;
+        vec[lane] = past ? __builtin_nanf("") : u * eg;
+        vec[kChunk + lane] = sP[lane] * eg;
+        vec[2 * kChunk + lane] = expf((float)last);
+    }
+    __syncthreads();
+    f32x4 vp[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int tj = 16 * j + l16;
+        const float bj = sB[tj];
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int ti = 16 * wave + 4 * g4 + x;
+            float va = 0.0f;
+            if (j <= wave && tj <= ti && bj == bj && sB[ti] == sB[ti]) {
+                const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
+                va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
+                vp[j][x] = sP[ti] * w * qk[j][x];
+            }
+            sA[ti * kPitchA + tj] = va;
+        }
+    }
+    __syncthreads();
+    {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
+        const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
+        float t[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v0 = i == l16 ? 1.0f : 0.0f, v1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; j++) {
+                if (j % 2) v1 -= A[i * kPitchA + j] * t[j];
+                else v0 -= A[i * kPitchA + j] * t[j];
+            }
+            t[i] = v0 + v1;
+        }
+        float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
+        if (g4 == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
+        }
+    }
+    __syncthreads();
+    // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
+    auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
+    if (wave < 2) {
+        const int i = 2 * wave + 1, j = 2 * wave;
+        f32x4 m = {}, y = {};
+#pragma unroll
+        for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
+#pragma unroll
+        for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
+#pragma unroll
+        for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+    } else {   // the upper blocks within 32, which the fragments cover
+        const int i = 2 * (wave - 2);
+#pragma unroll
+        for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
+    }
+    __syncthreads();
+    {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
+        const int i = wave / 2, j = wave % 2;
+        f32x4 y = {};
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            if (p > i) break;
+            f32x4 m = {};
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                if (q < j) continue;
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+                    m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+            }
+#pragma unroll
+            for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
+        }
+        __syncthreads();               // A is done with: P takes its place, and its columns take beta with T's
+#pragma unroll
+        for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
+    }
+    __syncthreads();
+    f32x4 y[4] = {};                   // rows 16 wave of P (I + A)^-1
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (j > wave) break;
+#pragma unroll
+        for (int k = j; k < 4; k++) {
+            if (k > wave) break;
+#pragma unroll
+            for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
+        }
+    }
+    // diag() T, and P T once every wave has read P: columns times beta (0 from a token that is not finite on)
+    const auto beta_of = [&](int t) { const float v = sB[t]; return v == v ? v : 0.0f; };
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float bj = beta_of(16 * j + l16);
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+            const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
+            sA[at_] = y[j][x] * bj;
+            sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
+        }
+    }
+    __syncthreads();
+    store_triangle<3>(sT, sW, unit, wave, lane);
+    store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
 }
-
-// Elements a row of an LDS operand takes: odd multiples of 16 bytes, so that 16 lanes that read 16 bytes of 16
-// neighbouring rows meet no bank twice.
-template <typename T> constexpr int pitch_of(int n) { return n + 16 / (int)sizeof(T); }
 
 // A buffer descriptor: loads past `bytes` give zeros, stores there are dropped.
 __device__ __forceinline__ auto rows_rsrc(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
 
+// One element as its bits, a register each (a conversion, or a packing, would wait for the load), and its value.
 template <typename T, typename R>
-__device__ __forceinline__ T buffer_elem(R rsrc, uint32_t at) {
-    if constexpr (sizeof(T) == 4)
-        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0));
-    else
-        return __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0));
+__device__ __forceinline__ uint32_t buffer_bits(R rsrc, uint32_t at) {
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ float of_bits(uint32_t v) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, v);
+    else return (float)__builtin_bit_cast(T, (unsigned short)v);
 }
 
-// One workgroup of W waves takes 16 W columns of one head's state through a sequence.  A chunk's keys (in both
-// orders), queries and its unit of the workspace stand in LDS; its values are each wave's own.  All of them are
-// requested a chunk ahead of their use.  A chunk has two halves: up to barrier A the products with the state
-// (keys, queries) while the unit of this chunk is put in place; up to barrier B those with X (the unit, k^T) while
-// the next chunk's keys and queries are.  k^T has two buffers where they fit and is written with the keys; where
-// they do not (f32, dk 128) it is written from the same registers in the first half, and the next
-// request of keys waits for that.
-template <typename T, int DK, int W>
-__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkArgs a) {
-    constexpr int LO = Limbs<T>::out, KS = DK / 32, NT = DK / 16, SZ = sizeof(T);
-    constexpr int PK = pitch_of<T>(DK), PT = pitch_of<T>(kChunk);
-    constexpr int kUnits = 32 * (DK / 8) / (64 * W);       // (pair of tokens, eight columns) a thread
-    constexpr int kImage = unit_bytes(LO), kImageLoads = (kImage / 16 + 64 * W - 1) / (64 * W);
-    constexpr bool kTwo = DK * SZ <= 256;
-    static_assert(kUnits >= 1 && 32 * (DK / 8) % (64 * W) == 0, "");
-    __shared__ __attribute__((aligned(16))) unsigned char lds[(2 * kChunk * PK + (kTwo ? 2 : 1) * DK * PT) * SZ];
-    __shared__ __attribute__((aligned(16))) unsigned char image[kImageLoads * 64 * W * 16];
-    T* const sK = (T*)lds;                 // row: token in the order (*)
-    T* const sQ = sK + kChunk * PK;
-    T* const sKT = sQ + kChunk * PK;       // row: column of k in the order (*); the tokens in their own
+// One workgroup of four waves takes 16 NC columns of one head's state through a sequence.  A wave owns a quarter of the
+// state's rows and of a chunk's tokens, so the chain of a chunk (S -> X -> D -> S) is a quarter as long as one
+// wave's would be; S, X and D pass between the waves as limbs through LDS, three barriers a chunk.  Every left operand is read
+// by one wave only, straight from memory into registers, a chunk ahead of its use.
+template <typename T, int DK, int NC>
+__global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs a) {
+    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, NW = DK / 64, SZ = sizeof(T);
+    __shared__ __attribute__((aligned(16))) unsigned char sS[NC][KS][3][kFrag], sX[NC][2][3][kFrag], sD[NC][2][3][kFrag];
+    __shared__ __attribute__((aligned(16))) int sBad[NC][16][4];
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
     // the workgroups that read one key head's chunks are neighbours of one XCD
-    const uint32_t group = r.hv / r.hk, cols = (r.dv / 16 + W - 1) / W;
+    const uint32_t group = r.hv / r.hk, cols = (r.dv / 16 + NC - 1) / NC;
     const XcdTile w = xcd_tile(blockIdx.x, group * cols, a.d.n * r.hk);
     if (!w.live) return;
     const uint32_t i = w.unit / r.hk, hq = w.unit % r.hk, h = hq * group + w.part / cols;
-    const uint32_t col16 = (w.part % cols) * W + wave;
-    const bool mine = col16 < r.dv / 16;   // (the last workgroup of a head may have waves too many, which help loading)
-    const uint32_t col = mine ? 16 * col16 + l16 : l16;
+    const uint32_t col0 = w.part % cols * (16 * NC) + l16;
     const int slot = entry_slot(a.d.slots, a.d.n_slots, i, a.d.states != nullptr, lane);
     if (slot == kSkip) return;
     const uint32_t b = row_of(a, i), e = max(row_of(a, i + 1), b);
     if (slot == kBad) {
-        T* const out = (T*)r.out + (size_t)h * r.dv + col;
-        if (mine)
-            for (uint32_t t = b + g4; t < e; t += 4) out[(int64_t)t * r.out_stride] = (T)__builtin_nanf("");
+        T* const out = (T*)r.out + (size_t)h * r.dv;
+        for (uint32_t t = b + threadIdx.x / 16; t < e; t += 16)
+            for (uint32_t col = col0; col < min(col0 - l16 + 16 * NC, r.dv); col += 16)
+                out[(int64_t)t * r.out_stride + col] = (T)__builtin_nanf("");
         return;
     }
-    const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv + col;
-    f32x4 S[NT];
+    // (of a head's last workgroup a column tile may be past dv: it takes column l16 along and stores nothing)
+    const auto live = [&](int nc) { return col0 + 16 * nc < r.dv; };
+    const auto col_of = [&](int nc) { return live(nc) ? col0 + 16 * nc : (uint32_t)l16; };
+    const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv;
+    f32x4 S[NC][NW];
 #pragma unroll
-    for (int p = 0; p < NT; p++)
+    for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-        for (int x = 0; x < 4; x++)
-            S[p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] : 0.0f;
-    const uint32_t chunks = (e - b + kChunk - 1) / kChunk;
-    const unsigned char* const units = a.ws + ((size_t)first_chunk(b, i) * r.hv + h) * kImage;
-    const size_t unit_step = (size_t)r.hv * kImage;
-    typedef T vec8 __attribute__((ext_vector_type(8), aligned(16)));      // (rows in LDS are odd multiples of 16 bytes)
-    typedef T vec2 __attribute__((ext_vector_type(2)));
-    typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-    vec8 kv[kUnits][2], qv[kUnits][2];
-    u32x4 iv[kImageLoads];
-    T vv[4][4];                            // (as they are: a conversion would wait for them)
-    // A row's place within a chunk is a part of the lane's and a uniform one; buffer accesses end the chunk by their bounds
-    // (which count the vector offset only, so the scalar one stays 0).
-    const uint32_t tp0 = threadIdx.x / (DK / 8), o8 = threadIdx.x % (DK / 8) * 8;
+        for (int p = 0; p < NW; p++)
+#pragma unroll
+            for (int x = 0; x < 4; x++)
+                S[nc][p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(NW * wave + p, 4 * g4 + x) * r.dv + col_of(nc)] : 0.0f;
+    const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
+    typedef T vec8 __attribute__((ext_vector_type(8), aligned(16)));
+    vec8 kf[KS], qf[KS];
+    bf16x8 tf[2][3], pf[2][LO], ktf[NW][2][LI];
+    uint32_t vv[NC][4];
+    f32x4 kd, qd;
+    float keep;
+    // Rows of a chunk by buffer accesses, whose bounds end the chunk (they count the vector offset only, so the
+    // scalar one stays 0).
     const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ, vs = (uint32_t)r.v_stride * SZ,
                    os = (uint32_t)r.out_stride * SZ;
-    const uint32_t k_at = 2 * tp0 * ks + o8 * SZ, q_at = 2 * tp0 * qs + o8 * SZ, v_at = 8 * g4 * vs + (h * r.dv + col) * SZ,
-                   o_at = mine ? 8 * g4 * os + (h * r.dv + col) * SZ : 0x80000000u;
-
+    const uint32_t row = tile_index(wave, l16), row4 = tile_index(wave, 4 * g4);
     const auto rows_in = [&](uint32_t c) { return min(e - b - c * kChunk, (uint32_t)kChunk); };
     const auto rsrc_of = [&](const void* p, uint32_t c, uint32_t stride, uint32_t first_col, uint32_t width) {
         return rows_rsrc((const unsigned char*)p + (size_t)(b + c * kChunk) * stride + (size_t)first_col * SZ,
                          (rows_in(c) - 1) * stride + width * SZ);
     };
-    const auto load16 = [&](auto rsrc, uint32_t off) {
+    const auto load8 = [&](auto rsrc, uint32_t off) {
         if constexpr (SZ == 2) {
             return __builtin_bit_cast(vec8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
         } else {
@@ -596,193 +626,193 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_delta_chunks(ChunkAr
             return __builtin_bit_cast(vec8, x);
         }
     };
+    const auto unit_of = [&](uint32_t c) { return a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO); };
     const auto load_kq = [&](uint32_t c) {
         const auto rk = rsrc_of(r.k, c, ks, hq * DK, DK);
         const auto rq = rsrc_of(r.q, c, qs, hq * DK, DK);
 #pragma unroll
-        for (int u = 0; u < kUnits; u++)
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const uint32_t t = 2 * u * (64 * W / (DK / 8)) + y;
-                kv[u][y] = load16(rk, k_at + t * ks);
-                qv[u][y] = load16(rq, q_at + t * qs);
-            }
-    };
-    const auto store_kt = [&](uint32_t c) {
-        T* const kt = sKT + (kTwo ? c % 2 * (DK * PT) : 0);
-#pragma unroll
-        for (int u = 0; u < kUnits; u++) {
-            const int tp = u * (64 * W / (DK / 8)) + tp0;
-#pragma unroll
-            for (int x = 0; x < 8; x++) {
-                const int d = o8 + x, row = 32 * (d / 32) + 16 * (d / 4 % 2) + 4 * (d / 8 % 4) + d % 4;
-                *(vec2*)(kt + row * PT + 2 * tp) = vec2{kv[u][0][x], kv[u][1][x]};
-            }
+        for (int s = 0; s < KS; s++) {
+            kf[s] = load8(rk, row * ks + (32 * s + 8 * g4) * SZ);
+            qf[s] = load8(rq, row * qs + (32 * s + 8 * g4) * SZ);
         }
-    };
-    const auto store_kq = [&](uint32_t c) {
-#pragma unroll
-        for (int u = 0; u < kUnits; u++) {
-            const int tp = u * (64 * W / (DK / 8)) + tp0;
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-                const int t = 2 * tp + y, row = 32 * (t / 32) + 16 * (t / 4 % 2) + 4 * (t / 8 % 4) + t % 4;
-                *(vec8*)(sK + row * PK + o8) = kv[u][y];
-                *(vec8*)(sQ + row * PK + o8) = qv[u][y];
-            }
-        }
-        if (kTwo) store_kt(c);
-    };
-    const auto load_image = [&](uint32_t c) {
-        const auto ri = rows_rsrc(units + c * unit_step, kImage);
-#pragma unroll
-        for (int x = 0; x < kImageLoads; x++)
-            iv[x] = __builtin_amdgcn_raw_buffer_load_b128(ri, (int)(threadIdx.x * 16 + x * 64 * W * 16), 0, 0);
-    };
-    const auto store_image = [&]() {
-#pragma unroll
-        for (int x = 0; x < kImageLoads; x++) *(u32x4*)(image + (x * 64 * W + threadIdx.x) * 16) = iv[x];
     };
     const auto load_v = [&](uint32_t c) {
-        const auto rv = rsrc_of(r.v, c, vs, 0, r.hv * r.dv);
+        const auto rv = rsrc_of(r.v, c, vs, h * r.dv, r.dv);
 #pragma unroll
-        for (int m = 0; m < 4; m++)
+        for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) vv[m][x] = buffer_elem<T>(rv, v_at + (tile_index(m, 0) + x) * vs);
+            for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rv, (row4 + x) * vs + col_of(nc) * SZ);
+        const float* const vec = (const float*)(unit_of(c) + kTri * (3 + LO) * kFrag);
+        kd = *(const f32x4*)(vec + row4);
+        qd = *(const f32x4*)(vec + kChunk + row4);
+    };
+    // fragment 0 is this wave's tile and tokens [0, 32), 1 tokens [32, 64) (waves 2 and 3 only)
+    const int f0 = wave < 2 ? wave : 2 * wave - 2, f1 = wave < 2 ? wave : f0 + 1;
+    const auto load_tp = [&](uint32_t c) {
+        const unsigned char* const u = unit_of(c);
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int f = s ? f1 : f0;
+#pragma unroll
+            for (int n = 0; n < 3; n++) tf[s][n] = *(const bf16x8*)(u + (f * 3 + n) * kFrag + lane * 16);
+#pragma unroll
+            for (int n = 0; n < LO; n++) pf[s][n] = *(const bf16x8*)(u + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
+        }
+    };
+    const auto load_kt = [&](uint32_t c) {
+        const unsigned char* const u = a.kt + ((size_t)(first + c) * r.hk + hq) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
+#pragma unroll
+        for (int f = 0; f < NW * 2; f++)
+#pragma unroll
+            for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(u + (f * LI + n) * kFrag + lane * 16);
+        keep = ((const float*)(unit_of(c) + kTri * (3 + LO) * kFrag))[2 * kChunk];
+    };
+    // The four rows of tile `tile` that this lane holds, as half of a right operand's fragment.
+    const auto put = [&](unsigned char (*to)[3][kFrag], int tile, const f32x4& v) {
+        float a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
+#pragma unroll
+        for (int n = 0; n < 3; n++) {
+            const uint32_t p = pack_bf16(a0, a1), q = pack_bf16(a2, a3);
+            *(uint2*)(to[tile / 2][n] + lane * 16 + tile % 2 * 8) = make_uint2(p, q);
+            a0 -= __builtin_bit_cast(float, p << 16), a1 -= __builtin_bit_cast(float, p & 0xffff0000u);
+            a2 -= __builtin_bit_cast(float, q << 16), a3 -= __builtin_bit_cast(float, q & 0xffff0000u);
+        }
+    };
+    const auto get = [&](const unsigned char (&from)[3][kFrag]) {
+        Split<3> o;
+#pragma unroll
+        for (int n = 0; n < 3; n++) o.l[n] = *(const bf16x8*)(from[n] + lane * 16);
+        return o;
+    };
+    const auto limbs = [&](const vec8& x) {
+        if constexpr (LI == 1) {
+            return Split<1>{{__builtin_bit_cast(bf16x8, x)}};
+        } else {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = (float)x[j];
+            return split8<LI>(v);
+        }
+    };
+    const auto put_state = [&]() {
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+            for (int p = 0; p < NW; p++) put(sS[nc], NW * wave + p, S[nc][p]);
     };
     if (chunks) {
         load_kq(0);
-        load_image(0);
         load_v(0);
-        store_kq(0);
-        if (kTwo) load_kq(min(1u, chunks - 1));
+        load_tp(0);
+        load_kt(0);
+        put_state();
     }
-    __syncthreads();
-    const float* const vec = (const float*)(image + kTri * (3 + LO) * kFrag);
-    const auto frag = [&](int f, int limb, int first, int limbs) {
-        return *(const bf16x8*)(image + (first + f * limbs + limb) * kFrag + lane * 16);
-    };
-    const auto tfrag = [&](int f) {
-        Split<3> o;
-#pragma unroll
-        for (int n = 0; n < 3; n++) o.l[n] = frag(f, n, 0, 3);
-        return o;
-    };
-    const auto pfrag = [&](int f) {
-        Split<LO> o;
-#pragma unroll
-        for (int n = 0; n < LO; n++) o.l[n] = frag(f, n, kTri * 3, LO);
-        return o;
-    };
     for (uint32_t c = 0; c < chunks; c++) {
         // (the last chunk requests itself again instead of one past the end)
         const uint32_t next = min(c + 1, chunks - 1);
-        store_image();
-        load_image(next);
-        if (!kTwo) {
-            store_kt(c);
-            load_kq(next);
-        }
-        f32x4 X[4] = {}, O[4] = {};
+        __syncthreads();                   // S is there
+        f32x4 X[NC][2] = {}, O[NC][2] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            const Split<3> x = split_pair<3>(S[2 * s], S[2 * s + 1]);
-            mma_rows<3>([&](int m) { return load_limbs(sK + (16 * m + l16) * PK + 32 * s + 8 * g4); }, x, X);
-            mma_rows<LO>([&](int m) { return load_limbs(sQ + (16 * m + l16) * PK + 32 * s + 8 * g4); }, x, O);
+            const Split<LI> kl = limbs(kf[s]), ql = limbs(qf[s]);
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++) {
+                const Split<3> x = get(sS[nc][s]);
+                X[nc][s % 2] = mma_limbs<3>(kl, x, X[nc][s % 2]);
+                O[nc][s % 2] = mma_limbs<LO>(ql, x, O[nc][s % 2]);
+            }
         }
-        __syncthreads();                   // A
-        store_kq(c + 1);
-        if (kTwo) load_kq(min(c + 2, chunks - 1));
-        uint32_t top = 0;
+        load_kq(next);
+        bool any_bad = false;
 #pragma unroll
-        for (int m = 0; m < 4; m++) {
-            const int t = tile_index(m, 4 * g4);
-            const f32x4 kd = *(const f32x4*)(vec + t), qd = *(const f32x4*)(vec + kChunk + t);
+        for (int nc = 0; nc < NC; nc++) {
+            uint32_t top = 0;
+            f32x4 x;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const float v = (float)vv[m][x] - kd[x] * X[m][x];
-                X[m][x] = v;
-                O[m][x] *= qd[x];
+            for (int y = 0; y < 4; y++) {
+                const float v = of_bits<T>(vv[nc][y]) - kd[y] * (X[nc][0][y] + X[nc][1][y]);
+                x[y] = v;
+                O[nc][0][y] = qd[y] * (O[nc][0][y] + O[nc][1][y]);
                 top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
             }
+            int bad = kChunk;              // this tile's first token in this column that is not finite
+            if (__any(top >= 0x7f800000u)) {
+#pragma unroll
+                for (int y = 3; y >= 0; y--)
+                    if (!(fabsf(x[y]) < __builtin_inff())) bad = row4 + y, x[y] = 0.0f;
+                bad = min(bad, __shfl_xor(bad, 16, kWave));
+                bad = min(bad, __shfl_xor(bad, 32, kWave));
+            }
+            if (lane < 16) sBad[nc][l16][wave] = bad;
+            put(sX[nc], wave, x);
         }
         load_v(next);
-        int bad = kChunk;                  // this column's first token that is not finite
-        const bool any_bad = __any(top >= 0x7f800000u);
-        if (any_bad) {
+        __syncthreads();                   // X is there
+        f32x4 D[NC] = {};
+        int bad[NC];
 #pragma unroll
-            for (int m = 0; m < 4; m++)
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (!(fabsf(X[m][x]) < __builtin_inff())) bad = min(bad, tile_index(m, 4 * g4) + x);
-            bad = min(bad, __shfl_xor(bad, 16, kWave));
-            bad = min(bad, __shfl_xor(bad, 32, kWave));
-#pragma unroll
-            for (int m = 0; m < 4; m++)
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (tile_index(m, 4 * g4) + x >= bad) X[m][x] = 0.0f;
+        for (int nc = 0; nc < NC; nc++) {
+            const int4 v = *(const int4*)sBad[nc][l16];
+            bad[nc] = min(min(v.x, v.y), min(v.z, v.w));
+            any_bad |= bad[nc] < kChunk;
+            const Split<3> x = get(sX[nc][0]);
+            D[nc] = mma_limbs<3>(as_split<3>(tf[0]), x, D[nc]);
+            O[nc][0] = mma_limbs<LO>(as_split<LO>(pf[0]), x, O[nc][0]);
         }
-        f32x4 D[4] = {};
-        {
-            const Split<3> x = split_pair<3>(X[0], X[1]);
-            mma_rows<3>([&](int m) { return tfrag(m < 2 ? m : 2 * m - 2); }, x, D);
-            mma_rows<LO>([&](int m) { return pfrag(m < 2 ? m : 2 * m - 2); }, x, O);
-        }
-        {
-            const Split<3> x = split_pair<3>(X[2], X[3]);
-            const Split<3> t2 = tfrag(3), t3 = tfrag(5);
-            const Split<LO> p2 = pfrag(3), p3 = pfrag(5);
+        if (wave >= 2) {
 #pragma unroll
-            for (int n = 0; n < 3; n++)
-#pragma unroll
-                for (int j = 0; j < 3 - n; j++) {
-                    D[2] = mma(t2.l[n], x.l[j], D[2]);
-                    D[3] = mma(t3.l[n], x.l[j], D[3]);
-                    if (n + j < LO) {
-                        O[2] = mma(p2.l[n], x.l[j], O[2]);
-                        O[3] = mma(p3.l[n], x.l[j], O[3]);
-                    }
-                }
-        }
-        if (any_bad) {
-            const float nan = __builtin_nanf("");
-#pragma unroll
-            for (int m = 0; m < 4; m++)
-#pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (tile_index(m, 4 * g4) + x >= bad) O[m][x] = D[m][x] = nan;
-        }
-        const float keep = vec[2 * kChunk];
-#pragma unroll
-        for (int p = 0; p < NT; p++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) S[p][x] *= keep;
-        const T* const kt = sKT + (kTwo ? c % 2 * (DK * PT) : 0);
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const Split<3> x = split_pair<3>(D[2 * s], D[2 * s + 1]);
-#pragma unroll
-            for (int p = 0; p < NT; p += 4)
-                mma_rows<3>([&](int m) { return load_limbs(kt + (16 * (p + m) + l16) * PT + 32 * s + 8 * g4); }, x, &S[p]);
-        }
-        const auto ro = rsrc_of(r.out, c, os, 0, r.hv * r.dv);
-#pragma unroll
-        for (int m = 0; m < 4; m++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int o = (int)(o_at + (tile_index(m, 0) + x) * os);
-                const T y = (T)(float)O[m][x];
-                if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, y), ro, o, 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, y), ro, o, 0, 0);
+            for (int nc = 0; nc < NC; nc++) {
+                const Split<3> x = get(sX[nc][1]);
+                D[nc] = mma_limbs<3>(as_split<3>(tf[1]), x, D[nc]);
+                O[nc][0] = mma_limbs<LO>(as_split<LO>(pf[1]), x, O[nc][0]);
             }
-        __syncthreads();                   // B
+        }
+        load_tp(next);
+        if (__any(any_bad)) {
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    if ((int)row4 + y >= bad[nc]) O[nc][0][y] = D[nc][y] = __builtin_nanf("");
+        }
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++) put(sD[nc], wave, D[nc]);
+        __syncthreads();                   // D is there
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++) {
+#pragma unroll
+            for (int p = 0; p < NW; p++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) S[nc][p][y] *= keep;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const Split<3> x = get(sD[nc][s]);
+#pragma unroll
+                for (int p = 0; p < NW; p++) S[nc][p] = mma_limbs<3>(as_split<LI>(ktf[p][s]), x, S[nc][p]);
+            }
+        }
+        load_kt(next);
+        put_state();
+        const auto ro = rsrc_of(r.out, c, os, h * r.dv, r.dv);
+#pragma unroll
+        for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int o = (int)((row4 + y) * os + (live(nc) ? (col0 + 16 * nc) * SZ : 0x80000000u));
+                const T v = (T)(float)O[nc][0][y];
+                if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), ro, o, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), ro, o, 0, 0);
+            }
     }
-    if (a.d.states && mine) {
+    if (a.d.states) {
 #pragma unroll
-        for (int p = 0; p < NT; p++)
+        for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-            for (int x = 0; x < 4; x++) a.d.states[at + (size_t)tile_index(p, 4 * g4 + x) * r.dv] = S[p][x];
+            for (int p = 0; p < NW; p++)
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    if (live(nc))
+                        a.d.states[at + (size_t)tile_index(NW * wave + p, 4 * g4 + x) * r.dv + col0 + 16 * nc] = S[nc][p][x];
     }
 }
 
@@ -795,38 +825,38 @@ const void* delta_prep_fn(uint32_t dtype, uint32_t dk) {
     return fns[dtype][dk == 128];
 }
 
-// Waves of a workgroup: at dk 64 the loads of a chunk keep four waves busy.
-constexpr int waves_of(int dk, int w) { return dk == 64 && w > 4 ? 4 : w; }
-
-template <int W>
+template <int NC>
 const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
-    constexpr int W64 = waves_of(64, W);
     static const void* const fns[3][2] = {
-        {(const void*)k_delta_chunks<__bf16, 64, W64>, (const void*)k_delta_chunks<__bf16, 128, W>},
-        {(const void*)k_delta_chunks<_Float16, 64, W64>, (const void*)k_delta_chunks<_Float16, 128, W>},
-        {(const void*)k_delta_chunks<float, 64, W64>, (const void*)k_delta_chunks<float, 128, W>},
+        {(const void*)k_delta_chunks<__bf16, 64, NC>, (const void*)k_delta_chunks<__bf16, 128, NC>},
+        {(const void*)k_delta_chunks<_Float16, 64, NC>, (const void*)k_delta_chunks<_Float16, 128, NC>},
+        {(const void*)k_delta_chunks<float, 64, NC>, (const void*)k_delta_chunks<float, 128, NC>},
     };
     return fns[dtype][dk == 128];
 }
 
 uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
 
-#ifndef KW
-#define KW 2
+#ifndef KNC
+#define KNC 1
 #endif
-constexpr int kW = KW;
+uint64_t units_bytes(const redukt_delta_rows& a, uint32_t n_seq) {
+    return chunk_slots(a, n_seq) * a.hv * unit_bytes(a.dtype == REDUKT_OP_F32 ? 3 : 2);
+}
+
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
-    const uint64_t prep = chunk_slots(r, k.d.n) * r.hk;
-    const uint32_t W = waves_of(r.dk, kW);
-    const uint64_t cols = (r.dv / 16 + W - 1) / W, units = (uint64_t)k.d.n * r.hk;
+    const uint64_t prep = chunk_slots(r, k.d.n) * r.hv;
+    constexpr uint32_t NC = KNC;
+    const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    k.kt = k.ws + units_bytes(r, k.d.n);
     if (r.rows) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    return op_launch(delta_chunks_fn<kW>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(64 * W), 0, stream, k);
+    return op_launch(delta_chunks_fn<NC>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(256), 0, stream, k);
 }
 
 bool sizes_ok(const redukt_delta_rows* a) {
@@ -893,7 +923,8 @@ int32_t redukt_op_delta_step(const redukt_delta_rows* a, float* states, uint32_t
 
 uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_seq) {
     if (!sizes_ok(a) || n_seq > kMaxOpRows) return 0;
-    return chunk_slots(*a, n_seq) * a->hv * unit_bytes(a->dtype == REDUKT_OP_F32 ? 3 : 2);
+    const int limbs = a->dtype == REDUKT_OP_F32 ? 3 : a->dtype == REDUKT_OP_F16 ? 2 : 1;
+    return units_bytes(*a, n_seq) + chunk_slots(*a, n_seq) * a->hk * kt_bytes(a->dk, limbs);
 }
 
 int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uint32_t n_seq, const float* state_in,
@@ -916,7 +947,7 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace};
+    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr};
     return launch_chunks(k, stream);
 }
 
