@@ -166,8 +166,9 @@ const void* delta_rows_fn(uint32_t dtype, uint32_t dk) {
 // Rows of a pair of result tiles (2 s, 2 s + 1) stand for the indices
 //     32 s + 8 (row / 4) + 4 (tile % 2) + row % 4,                                      (*)
 // so a lane's eight results of the pair are eight consecutive inner indices of the next product:
-// S, X and D go from result to right operand within a lane, without LDS and without an exchange.
-// Left operands take their rows in the same order.
+// S, X and D go from result to right operand without an exchange between lanes.  Left operands
+// take their rows in the same order.  (At dk 64 a wave has one tile of S, 16 indices in their own
+// order, and multiplies it 16 inner indices at a time.)
 
 constexpr int kChunk = 64;
 constexpr int kTri = 6;                    // 16 x 32 fragments of a lower triangle of 64
@@ -226,12 +227,6 @@ __device__ __forceinline__ Split<N> split8(const float (&v)[8]) {
     return o;
 }
 
-template <int N>
-__device__ __forceinline__ Split<N> split_pair(const f32x4& a, const f32x4& b) {
-    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-    return split8<N>(v);
-}
-
 // Eight elements of an operand in memory as limbs (exactly).
 template <typename T>
 __device__ __forceinline__ Split<Limbs<T>::in> load_limbs(const T* p) {
@@ -255,23 +250,6 @@ __device__ __forceinline__ f32x4 mma_limbs(const Split<NA>& a, const Split<NB>& 
     return c;
 }
 
-// c[m] += a(m) b for four row tiles m, limb by limb so that the tiles' sums overlap.
-template <int K, int NB, typename A, typename C>
-__device__ __forceinline__ void mma_rows(A&& a, const Split<NB>& b, C&& c) {
-    const decltype(a(0)) x[4] = {a(0), a(1), a(2), a(3)};
-    constexpr int NA = sizeof(x[0]) / sizeof(bf16x8);
-#pragma unroll
-    for (int i = 0; i < NA; i++)
-#pragma unroll
-        for (int j = 0; j < NB; j++)
-            if (i + j < K) {
-#pragma unroll
-                for (int m = 0; m < 4; m++) c[m] = mma(x[m].l[i], b.l[j], c[m]);
-            }
-}
-
-constexpr int kt_bytes(int dk, int in_limbs) { return dk / 16 * 2 * in_limbs * kFrag; }
-
 template <int N>
 __device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
     Split<N> o;
@@ -279,6 +257,8 @@ __device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
     for (int n = 0; n < N; n++) o.l[n] = v[n];
     return o;
 }
+
+constexpr int kt_bytes(int dk, int in_limbs) { return dk / 16 * 2 * in_limbs * kFrag; }
 
 struct ChunkArgs {
     DeltaArgs d;
@@ -301,6 +281,69 @@ __device__ __forceinline__ f32x4 mma4(float a, float b, const f32x4& c) {
 
 constexpr int kPitchA = kChunk + 4;        // f32 rows of the 64 x 64 matrices in LDS
 
+// A buffer descriptor: loads past `bytes` give zeros, stores there are dropped.
+__device__ __forceinline__ auto rows_rsrc(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
+}
+
+// One element as its bits, a register each (a conversion, or a packing, would wait for the load), and its value.
+template <typename T, typename R>
+__device__ __forceinline__ uint32_t buffer_bits(R rsrc, uint32_t at) {
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ float of_bits(uint32_t v) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, v);
+    else return (float)__builtin_bit_cast(T, (unsigned short)v);
+}
+
+// The index of row `row` of tile `tile` of the state: (*) where a wave has a pair of tiles.
+template <int DK>
+__device__ __forceinline__ int state_index(int tile, int row) {
+    return DK == 128 ? tile_index(tile, row) : 16 * tile + row;
+}
+
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
+
+// 4 NW f32 of a lane (16 NW inner indices of a product) as N limbs.
+template <int NW, int N>
+struct Part {
+    typedef __bf16 vec __attribute__((ext_vector_type(4 * NW)));
+    vec l[N];
+};
+
+template <int NW, int N>
+__device__ __forceinline__ Part<NW, N> split_part(const float (&v)[4 * NW]) {
+    typedef uint32_t words __attribute__((ext_vector_type(2 * NW)));
+    words w[N];
+#pragma unroll
+    for (int j = 0; j < 2 * NW; j++) {
+        float a = v[2 * j], b = v[2 * j + 1];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const uint32_t p = pack_bf16(a, b);
+            w[n][j] = p;
+            a -= __builtin_bit_cast(float, p << 16);
+            b -= __builtin_bit_cast(float, p & 0xffff0000u);
+        }
+    }
+    Part<NW, N> o;
+#pragma unroll
+    for (int n = 0; n < N; n++) o.l[n] = __builtin_bit_cast(typename Part<NW, N>::vec, w[n]);
+    return o;
+}
+
+__device__ __forceinline__ f32x4 mma_part(const bf16x8& a, const bf16x8& b, const f32x4& c) { return mma(a, b, c); }
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mma_part(const bf16x4& a, const bf16x4& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
+}
+
 // Fragments of the lower triangle at m (f32 [64][kPitchA], natural order), its rows times f, with N limbs to `to`: fragment
 // x is tile 0, 1, 2, 2, 3, 3 and inner indices 32 s + [0, 32) with s = 0, 0, 0, 1, 0, 1.
 template <int N>
@@ -319,16 +362,25 @@ __device__ __forceinline__ void store_triangle(const float* m, const float* f, u
 }
 
 // One workgroup a chunk and value head: its unit, and with a key head's first value head the fragments of k^T.
+// Bound by the chain of its steps (a read from memory, the products, the solve by blocks of 16, 32 and 64), so it
+// asks for all of its inputs at once, and several workgroups share a CU.
 template <typename T, int DK>
-__global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(ChunkArgs a) {
-    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32;
-    __shared__ __attribute__((aligned(16))) float sA[kChunk * kPitchA], sT[kChunk * kPitchA];
+__global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 : 2) void k_delta_prep(ChunkArgs a) {
+    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, SZ = sizeof(T);
+    constexpr int PK = DK + 16 / SZ;           // rows of odd multiples of 16 bytes: 16 neighbouring ones meet no bank twice
+    constexpr int kLoads = kChunk * DK * SZ / 16 / 256;
+    constexpr int kBytes = 2 * kChunk * PK * SZ > 2 * kChunk * kPitchA * 4 ? 2 * kChunk * PK * SZ : 2 * kChunk * kPitchA * 4;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kBytes];       // k and q, then A and T
     __shared__ double sG[kChunk];
     __shared__ float sB[kChunk], sU[kChunk], sP[kChunk], sW[kChunk];
+    T* const sK = (T*)lds;
+    T* const sQ = sK + kChunk * PK;
+    float* const sA = (float*)lds;
+    float* const sT = sA + kChunk * kPitchA;
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
     const uint32_t slot = blockIdx.x / r.hv, h = blockIdx.x % r.hv, group = r.hv / r.hk, hq = h / group;
-    uint32_t lo = 0, hi = a.d.n - 1;       // the last sequence that starts at this slot or before
+    uint32_t lo = 0, hi = a.d.n - 1;           // the last sequence that starts at this slot or before
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1) / 2;
         if (first_chunk(row_of(a, mid), mid) <= slot) lo = mid;
@@ -340,110 +392,109 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
     if (t0_ >= e) return;
     const uint32_t t0 = (uint32_t)t0_, len = min(e - t0, (uint32_t)kChunk);
 
+    {   // rows past the chunk's end as zeros
+        const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ;
+        const auto rk = rows_rsrc((const unsigned char*)r.k + (size_t)t0 * ks + (size_t)hq * DK * SZ, (len - 1) * ks + DK * SZ);
+        const auto rq = rows_rsrc((const unsigned char*)r.q + (size_t)t0 * qs + (size_t)hq * DK * SZ, (len - 1) * qs + DK * SZ);
+        u32x4 kv[kLoads], qv[kLoads];
+        constexpr int kPer = DK * SZ / 16;     // 16 bytes each
+#pragma unroll
+        for (int u = 0; u < kLoads; u++) {
+            const int id = u * 256 + threadIdx.x;
+            kv[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(id / kPer * ks + id % kPer * 16), 0, 0);
+            qv[u] = __builtin_amdgcn_raw_buffer_load_b128(rq, (int)(id / kPer * qs + id % kPer * 16), 0, 0);
+        }
+        float g0 = 0.0f, beta = 0.0f;
+        if (wave == 0 && (uint32_t)lane < len) {
+            g0 = r.g[(int64_t)(t0 + lane) * r.g_stride + h];
+            beta = r.beta[(int64_t)(t0 + lane) * r.beta_stride + h];
+        }
+#pragma unroll
+        for (int u = 0; u < kLoads; u++) {
+            const int id = u * 256 + threadIdx.x;
+            *(u32x4*)((unsigned char*)sK + id / kPer * (PK * SZ) + id % kPer * 16) = kv[u];
+            *(u32x4*)((unsigned char*)sQ + id / kPer * (PK * SZ) + id % kPer * 16) = qv[u];
+        }
+        if (wave == 0) {
+            // (a token whose g or beta is not finite is marked by a NaN beta)
+            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff());
+            double g = bad ? 0.0 : (double)fmaxf(g0, -1e5f);
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) {
+                const double v = __shfl_up(g, o, kWave);
+                if (lane >= o) g += v;
+            }
+            sG[lane] = g;
+            sB[lane] = bad ? __builtin_nanf("") : beta;
+        }
+    }
+    __syncthreads();
+
     // k.k and q.k: wave w the tiles (w, 0 .. w)
     f32x4 kk[4] = {}, qk[4] = {};
-    float k2[4] = {}, q2 = 0.0f;           // this lane's part of the sums of squares: rows l16 of the column tiles, of the query tile
-    const T* kp = (const T*)r.k + (size_t)hq * DK;
-    const T* qp = (const T*)r.q + (size_t)hq * DK;
+    float k2 = 0.0f, q2 = 0.0f;                // this lane's part of the sums of squares of row 16 w + l16
+    const bool norm = (r.flags & REDUKT_DELTA_NORMALIZE) != 0;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
         const int col = 32 * s + 8 * g4;
-        Split<LI> kf[4], qf;
+        float kr[8], qr[8];
+        op_load(sK + (16 * wave + l16) * PK + col, kr);
+        op_load(sQ + (16 * wave + l16) * PK + col, qr);
+#pragma unroll
+        for (int x = 0; x < 8; x++) k2 += kr[x] * kr[x], q2 += qr[x] * qr[x];
+        const Split<LI> kl = split8<LI>(kr), ql = split8<LI>(qr);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j > wave) break;
-            const uint32_t t = 16 * j + l16;
-            float v[8] = {};
-            if (t < len) op_load(kp + (int64_t)(t0 + t) * r.k_stride + col, v);
-            kf[j] = split8<LI>(v);
-#pragma unroll
-            for (int x = 0; x < 8; x++) k2[j] += v[x] * v[x];
-        }
-        {
-            const uint32_t t = 16 * wave + l16;
-            float v[8] = {};
-            if (t < len) op_load(qp + (int64_t)(t0 + t) * r.q_stride + col, v);
-            qf = split8<LI>(v);
-#pragma unroll
-            for (int x = 0; x < 8; x++) q2 += v[x] * v[x];
-        }
-        Split<LI> own = kf[0];
-#pragma unroll
-        for (int j = 1; j < 4; j++)
-            if (j == wave) own = kf[j];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j > wave) break;
-            kk[j] = mma_limbs<3>(own, kf[j], kk[j]);
-            qk[j] = mma_limbs<3>(qf, kf[j], qk[j]);
+            const Split<LI> kj = load_limbs(sK + (16 * j + l16) * PK + col);
+            kk[j] = mma_limbs<3>(kl, kj, kk[j]);
+            qk[j] = mma_limbs<3>(ql, kj, qk[j]);
         }
     }
-    const bool norm = (r.flags & REDUKT_DELTA_NORMALIZE) != 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (j > wave) break;
-        float v = k2[j];
-        v += __shfl_xor(v, 16, kWave);
-        v += __shfl_xor(v, 32, kWave);
+    k2 += __shfl_xor(k2, 16, kWave), q2 += __shfl_xor(q2, 16, kWave);
+    k2 += __shfl_xor(k2, 32, kWave), q2 += __shfl_xor(q2, 32, kWave);
+    if (g4 == 0) {
         // (a sum that is not finite stays one: 0 x it is NaN)
-        if (j == wave && g4 == 0) sU[16 * wave + l16] = norm ? rsqrtf(v + kUnitEps) + 0.0f * v : 1.0f + 0.0f * v;
+        sU[16 * wave + l16] = norm ? rsqrtf(k2 + kUnitEps) + 0.0f * k2 : 1.0f + 0.0f * k2;
+        sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
     }
-    q2 += __shfl_xor(q2, 16, kWave);
-    q2 += __shfl_xor(q2, 32, kWave);
-    if (g4 == 0) sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
-
-    unsigned char* unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
-    float* vec = (float*)(unit + kTri * (3 + LO) * kFrag);
     if (h % group == 0) {
-        // row (*) of k^T's tile p, the tokens 32 s + 8 g + [0, 8)
+        // row l16 of k^T's tile p (as the state's rows), the tokens 32 s + 8 g + [0, 8)
         unsigned char* const kt = a.kt + ((size_t)slot * r.hk + hq) * kt_bytes(DK, LI);
         for (int f = wave; f < DK / 16 * 2; f += 4) {
-            const T* const col = kp + tile_index(f / 2, l16);
+            const T* const col = sK + state_index<DK>(f / 2, l16);
             float v[8];
 #pragma unroll
-            for (int x = 0; x < 8; x++) {
-                const uint32_t t = 32 * (f % 2) + 8 * g4 + x;
-                v[x] = t < len ? (float)col[(int64_t)(t0 + t) * r.k_stride] : 0.0f;
-            }
+            for (int x = 0; x < 8; x++) v[x] = (float)col[(32 * (f % 2) + 8 * g4 + x) * PK];
             const Split<LI> y = split8<LI>(v);
 #pragma unroll
             for (int n = 0; n < LI; n++) *(bf16x8*)(kt + (f * LI + n) * kFrag + lane * 16) = y.l[n];
         }
     }
-    __syncthreads();                       // sU and sP are written
+    __syncthreads();                           // k and q are done with; sU, sP are written
+
+    unsigned char* const unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
+    // from the first token `past` whose key, g or beta is not finite on there are no rows
+    const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
+    const int past = bads ? __builtin_ctzll(bads) : kChunk;
     if (wave == 0) {
-        const bool in = (uint32_t)lane < len;
-        const float g0 = in ? r.g[(int64_t)(t0 + lane) * r.g_stride + h] : 0.0f;
-        const float beta = in ? r.beta[(int64_t)(t0 + lane) * r.beta_stride + h] : 0.0f, u = sU[lane];
-        const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff()) || u != u;
-        const uint64_t bads = __ballot(bad);
-        const bool past = bads && lane >= __builtin_ctzll(bads);       // from the first such token on
-        double g = past ? 0.0 : (double)fmaxf(g0, -1e5f);
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const double v = __shfl_up(g, o, kWave);
-            if (lane >= o) g += v;
-        }
-        const double last = __shfl(g, kWave - 1, kWave);
-        sG[lane] = g;
-        sB[lane] = past ? __builtin_nanf("") : beta;
-        const float eg = expf((float)g);
-        sW[lane] = in && !past ? u * expf((float)(last - g)) : 0.0f;
-        vec[lane] = past ? __builtin_nanf("") : u * eg;
+        float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
+        const double last = sG[kChunk - 1];
+        const float eg = expf((float)sG[lane]), u = sU[lane];
+        sW[lane] = lane < past ? u * expf((float)(last - sG[lane])) : 0.0f;
+        vec[lane] = lane < past ? u * eg : __builtin_nanf("");
         vec[kChunk + lane] = sP[lane] * eg;
         vec[2 * kChunk + lane] = expf((float)last);
     }
-    __syncthreads();
     f32x4 vp[4] = {};
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int tj = 16 * j + l16;
-        const float bj = sB[tj];
 #pragma unroll
         for (int x = 0; x < 4; x++) {
             const int ti = 16 * wave + 4 * g4 + x;
             float va = 0.0f;
-            if (j <= wave && tj <= ti && bj == bj && sB[ti] == sB[ti]) {
+            if (j <= wave && tj <= ti && ti < past) {
                 const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
                 va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
                 vp[j][x] = sP[ti] * w * qk[j][x];
@@ -473,7 +524,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
     }
     __syncthreads();
     // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
-    auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
+    const auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
     if (wave < 2) {
         const int i = 2 * wave + 1, j = 2 * wave;
         f32x4 m = {}, y = {};
@@ -500,13 +551,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
             for (int q = 0; q < 2; q++) {
                 if (q < j) continue;
 #pragma unroll
-                for (int s = 0; s < 4; s++)
-                    m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+                for (int s = 0; s < 4; s++) m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
             }
 #pragma unroll
             for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
         }
-        __syncthreads();               // A is done with: P takes its place, and its columns take beta with T's
+        __syncthreads();                       // A is done with: P takes its place
 #pragma unroll
         for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
 #pragma unroll
@@ -515,7 +565,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
             for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
     }
     __syncthreads();
-    f32x4 y[4] = {};                   // rows 16 wave of P (I + A)^-1
+    f32x4 y[4] = {};                           // rows 16 wave of P (I + A)^-1
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         if (j > wave) break;
@@ -526,12 +576,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
             for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
         }
     }
-    // diag() T, and P T once every wave has read P: columns times beta (0 from a token that is not finite on)
-    const auto beta_of = [&](int t) { const float v = sB[t]; return v == v ? v : 0.0f; };
-    __syncthreads();
+    __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const float bj = beta_of(16 * j + l16);
+        const float bj = 16 * j + l16 < past ? sB[16 * j + l16] : 0.0f;
 #pragma unroll
         for (int x = 0; x < 4; x++) {
             const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
@@ -544,34 +592,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 2 : 3) void k_delta_prep(Chun
     store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
 }
 
-// A buffer descriptor: loads past `bytes` give zeros, stores there are dropped.
-__device__ __forceinline__ auto rows_rsrc(const void* p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
-}
-
-// One element as its bits, a register each (a conversion, or a packing, would wait for the load), and its value.
-template <typename T, typename R>
-__device__ __forceinline__ uint32_t buffer_bits(R rsrc, uint32_t at) {
-    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(rsrc, (int)at, 0, 0);
-    else return __builtin_amdgcn_raw_buffer_load_b16(rsrc, (int)at, 0, 0);
-}
-template <typename T>
-__device__ __forceinline__ float of_bits(uint32_t v) {
-    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, v);
-    else return (float)__builtin_bit_cast(T, (unsigned short)v);
-}
-
-// One workgroup of four waves takes 16 NC columns of one head's state through a sequence.  A wave owns a quarter of the
-// state's rows and of a chunk's tokens, so the chain of a chunk (S -> X -> D -> S) is a quarter as long as one
-// wave's would be; S, X and D pass between the waves as limbs through LDS, three barriers a chunk.  Every left operand is read
-// by one wave only, straight from memory into registers, a chunk ahead of its use.
+// One workgroup takes 16 NC columns of one head's state through a sequence.  Waves 0 to 3 carry the state: each owns a
+// quarter of its rows and of a chunk's tokens, so the chain of a chunk (S -> X -> D -> S) is a quarter as long as one
+// wave's would be; partial sums of K S, and X and D as limbs, pass between them through LDS, three barriers a chunk.
+// Waves 4 to 7 make the outputs of the same tokens from the limbs of S and X that they find there, beside the chain
+// instead of in it.  Every left operand is read by one wave only, straight from memory into registers, a chunk
+// ahead of its use.
 template <typename T, int DK, int NC>
-__global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs a) {
-    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, NW = DK / 64, SZ = sizeof(T);
-    __shared__ __attribute__((aligned(16))) unsigned char sS[NC][KS][3][kFrag], sX[NC][2][3][kFrag], sD[NC][2][3][kFrag];
+__global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
+    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, NW = DK / 64, SZ = sizeof(T);
+    constexpr int KF = 4 * NW;                 // a lane's inner indices of one wave's rows of the state
+    __shared__ __attribute__((aligned(16))) f32x4 sR[NC][4][4][kWave];       // partial K S: [tile of tokens][wave]
+    __shared__ __attribute__((aligned(16))) unsigned char sS[NC][4][LO][kWave * KF * 2], sX[NC][2][3][kFrag], sD[NC][2][3][kFrag];
     __shared__ __attribute__((aligned(16))) int sBad[NC][16][4];
     const redukt_delta_rows& r = a.d.r;
-    const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
+    const int lane = threadIdx.x % kWave, wave = wave_index() % 4, g4 = lane / 16, l16 = lane % 16;
     // the workgroups that read one key head's chunks are neighbours of one XCD
     const uint32_t group = r.hv / r.hk, cols = (r.dv / 16 + NC - 1) / NC;
     const XcdTile w = xcd_tile(blockIdx.x, group * cols, a.d.n * r.hk);
@@ -583,7 +618,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs a) {
     const uint32_t b = row_of(a, i), e = max(row_of(a, i + 1), b);
     if (slot == kBad) {
         T* const out = (T*)r.out + (size_t)h * r.dv;
-        for (uint32_t t = b + threadIdx.x / 16; t < e; t += 16)
+        for (uint32_t t = b + threadIdx.x / 16; t < e; t += 32)
             for (uint32_t col = col0; col < min(col0 - l16 + 16 * NC, r.dv); col += 16)
                 out[(int64_t)t * r.out_stride + col] = (T)__builtin_nanf("");
         return;
@@ -591,228 +626,286 @@ __global__ __launch_bounds__(256, 2) void k_delta_chunks(ChunkArgs a) {
     // (of a head's last workgroup a column tile may be past dv: it takes column l16 along and stores nothing)
     const auto live = [&](int nc) { return col0 + 16 * nc < r.dv; };
     const auto col_of = [&](int nc) { return live(nc) ? col0 + 16 * nc : (uint32_t)l16; };
-    const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv;
-    f32x4 S[NC][NW];
-#pragma unroll
-    for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-        for (int p = 0; p < NW; p++)
-#pragma unroll
-            for (int x = 0; x < 4; x++)
-                S[nc][p][x] = a.d.in ? a.d.in[at + (size_t)tile_index(NW * wave + p, 4 * g4 + x) * r.dv + col_of(nc)] : 0.0f;
     const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
-    typedef T vec8 __attribute__((ext_vector_type(8), aligned(16)));
-    vec8 kf[KS], qf[KS];
-    bf16x8 tf[2][3], pf[2][LO], ktf[NW][2][LI];
-    uint32_t vv[NC][4];
-    f32x4 kd, qd;
-    float keep;
+    typedef T vecK __attribute__((ext_vector_type(KF)));
     // Rows of a chunk by buffer accesses, whose bounds end the chunk (they count the vector offset only, so the
     // scalar one stays 0).
-    const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ, vs = (uint32_t)r.v_stride * SZ,
-                   os = (uint32_t)r.out_stride * SZ;
-    const uint32_t row = tile_index(wave, l16), row4 = tile_index(wave, 4 * g4);
     const auto rows_in = [&](uint32_t c) { return min(e - b - c * kChunk, (uint32_t)kChunk); };
     const auto rsrc_of = [&](const void* p, uint32_t c, uint32_t stride, uint32_t first_col, uint32_t width) {
         return rows_rsrc((const unsigned char*)p + (size_t)(b + c * kChunk) * stride + (size_t)first_col * SZ,
                          (rows_in(c) - 1) * stride + width * SZ);
     };
-    const auto load8 = [&](auto rsrc, uint32_t off) {
-        if constexpr (SZ == 2) {
-            return __builtin_bit_cast(vec8, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
+    const auto loadK = [&](auto rsrc, uint32_t off) {
+        if constexpr (KF * SZ == 8) {
+            return __builtin_bit_cast(vecK, __builtin_amdgcn_raw_buffer_load_b64(rsrc, (int)off, 0, 0));
+        } else if constexpr (KF * SZ == 16) {
+            return __builtin_bit_cast(vecK, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0));
         } else {
             struct { u32x4 v[2]; } x = {{__builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off, 0, 0),
                                         __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)off + 16, 0, 0)}};
-            return __builtin_bit_cast(vec8, x);
+            return __builtin_bit_cast(vecK, x);
         }
     };
-    const auto unit_of = [&](uint32_t c) { return a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO); };
-    const auto load_kq = [&](uint32_t c) {
-        const auto rk = rsrc_of(r.k, c, ks, hq * DK, DK);
-        const auto rq = rsrc_of(r.q, c, qs, hq * DK, DK);
+    const auto limbs = [&](const vecK& x) {
+        Part<NW, LI> o;
+        if constexpr (LI == 1) {
+            o.l[0] = __builtin_bit_cast(typename Part<NW, LI>::vec, x);
+        } else {
+            float v[KF];
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            kf[s] = load8(rk, row * ks + (32 * s + 8 * g4) * SZ);
-            qf[s] = load8(rq, row * qs + (32 * s + 8 * g4) * SZ);
+            for (int j = 0; j < KF; j++) v[j] = (float)x[j];
+            o = split_part<NW, LI>(v);
         }
-    };
-    const auto load_v = [&](uint32_t c) {
-        const auto rv = rsrc_of(r.v, c, vs, h * r.dv, r.dv);
-#pragma unroll
-        for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-            for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rv, (row4 + x) * vs + col_of(nc) * SZ);
-        const float* const vec = (const float*)(unit_of(c) + kTri * (3 + LO) * kFrag);
-        kd = *(const f32x4*)(vec + row4);
-        qd = *(const f32x4*)(vec + kChunk + row4);
-    };
-    // fragment 0 is this wave's tile and tokens [0, 32), 1 tokens [32, 64) (waves 2 and 3 only)
-    const int f0 = wave < 2 ? wave : 2 * wave - 2, f1 = wave < 2 ? wave : f0 + 1;
-    const auto load_tp = [&](uint32_t c) {
-        const unsigned char* const u = unit_of(c);
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int f = s ? f1 : f0;
-#pragma unroll
-            for (int n = 0; n < 3; n++) tf[s][n] = *(const bf16x8*)(u + (f * 3 + n) * kFrag + lane * 16);
-#pragma unroll
-            for (int n = 0; n < LO; n++) pf[s][n] = *(const bf16x8*)(u + (kTri * 3 + f * LO + n) * kFrag + lane * 16);
-        }
-    };
-    const auto load_kt = [&](uint32_t c) {
-        const unsigned char* const u = a.kt + ((size_t)(first + c) * r.hk + hq) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
-#pragma unroll
-        for (int f = 0; f < NW * 2; f++)
-#pragma unroll
-            for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(u + (f * LI + n) * kFrag + lane * 16);
-        keep = ((const float*)(unit_of(c) + kTri * (3 + LO) * kFrag))[2 * kChunk];
-    };
-    // The four rows of tile `tile` that this lane holds, as half of a right operand's fragment.
-    const auto put = [&](unsigned char (*to)[3][kFrag], int tile, const f32x4& v) {
-        float a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
-#pragma unroll
-        for (int n = 0; n < 3; n++) {
-            const uint32_t p = pack_bf16(a0, a1), q = pack_bf16(a2, a3);
-            *(uint2*)(to[tile / 2][n] + lane * 16 + tile % 2 * 8) = make_uint2(p, q);
-            a0 -= __builtin_bit_cast(float, p << 16), a1 -= __builtin_bit_cast(float, p & 0xffff0000u);
-            a2 -= __builtin_bit_cast(float, q << 16), a3 -= __builtin_bit_cast(float, q & 0xffff0000u);
-        }
-    };
-    const auto get = [&](const unsigned char (&from)[3][kFrag]) {
-        Split<3> o;
-#pragma unroll
-        for (int n = 0; n < 3; n++) o.l[n] = *(const bf16x8*)(from[n] + lane * 16);
         return o;
     };
-    const auto limbs = [&](const vec8& x) {
-        if constexpr (LI == 1) {
-            return Split<1>{{__builtin_bit_cast(bf16x8, x)}};
-        } else {
-            float v[8];
+    const auto unit_of = [&](uint32_t c) { return a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO); };
+    const auto get = [&](const unsigned char (&from)[3][kFrag], auto n_) {
+        constexpr int N = decltype(n_)::value;
+        Split<N> o;
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = (float)x[j];
-            return split8<LI>(v);
-        }
+        for (int n = 0; n < N; n++) o.l[n] = *(const bf16x8*)(from[n] + lane * 16);
+        return o;
     };
-    const auto put_state = [&]() {
+    // fragment 0 of a triangle is this wave's tile and tokens [0, 32), 1 tokens [32, 64) (waves 2 and 3 only)
+    const int f0 = wave < 2 ? wave : 2 * wave - 2, f1 = wave < 2 ? wave : f0 + 1;
+    const uint32_t row4 = tile_index(wave, 4 * g4);        // the first of a lane's four tokens
+    const auto bad_of = [&](int nc) {                      // the column's first token that is not finite
+        const int4 v = *(const int4*)sBad[nc][l16];
+        return min(min(v.x, v.y), min(v.z, v.w));
+    };
+
+    if (wave_index() < 4) {
+        __builtin_amdgcn_s_setprio(3);
+        const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv;
+        const auto state_at = [&](int nc, int p, int x) {
+            return at + (size_t)state_index<DK>(NW * wave + p, 4 * g4 + x) * r.dv + col_of(nc);
+        };
+        f32x4 S[NC][NW];
 #pragma unroll
         for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-            for (int p = 0; p < NW; p++) put(sS[nc], NW * wave + p, S[nc][p]);
-    };
-    if (chunks) {
-        load_kq(0);
-        load_v(0);
-        load_tp(0);
-        load_kt(0);
-        put_state();
-    }
-    for (uint32_t c = 0; c < chunks; c++) {
-        // (the last chunk requests itself again instead of one past the end)
-        const uint32_t next = min(c + 1, chunks - 1);
-        __syncthreads();                   // S is there
-        f32x4 X[NC][2] = {}, O[NC][2] = {};
+            for (int p = 0; p < NW; p++)
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const Split<LI> kl = limbs(kf[s]), ql = limbs(qf[s]);
+                for (int x = 0; x < 4; x++) S[nc][p][x] = a.d.in ? a.d.in[state_at(nc, p, x)] : 0.0f;
+        const uint32_t ks = (uint32_t)r.k_stride * SZ, vs = (uint32_t)r.v_stride * SZ;
+        vecK kf[4];
+        bf16x8 tf[2][3], ktf[NW][2][LI];
+        uint32_t vv[NC][4];
+        f32x4 kd;
+        float keep;
+        const auto load_k = [&](uint32_t c) {              // all tokens, the columns of this wave's rows of the state
+            const auto rk = rsrc_of(r.k, c, ks, hq * DK, DK);
 #pragma unroll
-            for (int nc = 0; nc < NC; nc++) {
-                const Split<3> x = get(sS[nc][s]);
-                X[nc][s % 2] = mma_limbs<3>(kl, x, X[nc][s % 2]);
-                O[nc][s % 2] = mma_limbs<LO>(ql, x, O[nc][s % 2]);
-            }
-        }
-        load_kq(next);
-        bool any_bad = false;
-#pragma unroll
-        for (int nc = 0; nc < NC; nc++) {
-            uint32_t top = 0;
-            f32x4 x;
-#pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const float v = of_bits<T>(vv[nc][y]) - kd[y] * (X[nc][0][y] + X[nc][1][y]);
-                x[y] = v;
-                O[nc][0][y] = qd[y] * (O[nc][0][y] + O[nc][1][y]);
-                top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
-            }
-            int bad = kChunk;              // this tile's first token in this column that is not finite
-            if (__any(top >= 0x7f800000u)) {
-#pragma unroll
-                for (int y = 3; y >= 0; y--)
-                    if (!(fabsf(x[y]) < __builtin_inff())) bad = row4 + y, x[y] = 0.0f;
-                bad = min(bad, __shfl_xor(bad, 16, kWave));
-                bad = min(bad, __shfl_xor(bad, 32, kWave));
-            }
-            if (lane < 16) sBad[nc][l16][wave] = bad;
-            put(sX[nc], wave, x);
-        }
-        load_v(next);
-        __syncthreads();                   // X is there
-        f32x4 D[NC] = {};
-        int bad[NC];
-#pragma unroll
-        for (int nc = 0; nc < NC; nc++) {
-            const int4 v = *(const int4*)sBad[nc][l16];
-            bad[nc] = min(min(v.x, v.y), min(v.z, v.w));
-            any_bad |= bad[nc] < kChunk;
-            const Split<3> x = get(sX[nc][0]);
-            D[nc] = mma_limbs<3>(as_split<3>(tf[0]), x, D[nc]);
-            O[nc][0] = mma_limbs<LO>(as_split<LO>(pf[0]), x, O[nc][0]);
-        }
-        if (wave >= 2) {
-#pragma unroll
-            for (int nc = 0; nc < NC; nc++) {
-                const Split<3> x = get(sX[nc][1]);
-                D[nc] = mma_limbs<3>(as_split<3>(tf[1]), x, D[nc]);
-                O[nc][0] = mma_limbs<LO>(as_split<LO>(pf[1]), x, O[nc][0]);
-            }
-        }
-        load_tp(next);
-        if (__any(any_bad)) {
+            for (int m = 0; m < 4; m++) kf[m] = loadK(rk, tile_index(m, l16) * ks + (4 * KF * wave + KF * g4) * SZ);
+        };
+        const auto load_v = [&](uint32_t c) {
+            const auto rv = rsrc_of(r.v, c, vs, h * r.dv, r.dv);
 #pragma unroll
             for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-                for (int y = 0; y < 4; y++)
-                    if ((int)row4 + y >= bad[nc]) O[nc][0][y] = D[nc][y] = __builtin_nanf("");
-        }
+                for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rv, (row4 + x) * vs + col_of(nc) * SZ);
+            kd = *(const f32x4*)(unit_of(c) + kTri * (3 + LO) * kFrag + row4 * 4);
+        };
+        const auto load_t = [&](uint32_t c) {
+            const unsigned char* const u = unit_of(c);
 #pragma unroll
-        for (int nc = 0; nc < NC; nc++) put(sD[nc], wave, D[nc]);
-        __syncthreads();                   // D is there
+            for (int n = 0; n < 3; n++) tf[0][n] = *(const bf16x8*)(u + (f0 * 3 + n) * kFrag + lane * 16);
+            if (wave >= 2) {
 #pragma unroll
-        for (int nc = 0; nc < NC; nc++) {
-#pragma unroll
-            for (int p = 0; p < NW; p++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) S[nc][p][y] *= keep;
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                const Split<3> x = get(sD[nc][s]);
-#pragma unroll
-                for (int p = 0; p < NW; p++) S[nc][p] = mma_limbs<3>(as_split<LI>(ktf[p][s]), x, S[nc][p]);
+                for (int n = 0; n < 3; n++) tf[1][n] = *(const bf16x8*)(u + (f1 * 3 + n) * kFrag + lane * 16);
             }
+        };
+        const auto load_kt = [&](uint32_t c) {
+            const unsigned char* const u = a.kt + ((size_t)(first + c) * r.hk + hq) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
+#pragma unroll
+            for (int f = 0; f < NW * 2; f++)
+#pragma unroll
+                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(u + (f * LI + n) * kFrag + lane * 16);
+            keep = ((const float*)(unit_of(c) + kTri * (3 + LO) * kFrag))[2 * kChunk];
+        };
+        // The four rows of this wave's tile that a lane holds, as half of a right operand's fragment.
+        const auto put = [&](unsigned char (*to)[3][kFrag], const f32x4& v) {
+            const float x[4] = {v[0], v[1], v[2], v[3]};
+            const Part<1, 3> y = split_part<1, 3>(x);
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                *(typename Part<1, 3>::vec*)(to[wave / 2][n] + lane * 16 + wave % 2 * 8) = y.l[n];
+        };
+        if (chunks) {
+            load_k(0);
+            load_v(0);
+            load_t(0);
+            load_kt(0);
         }
-        load_kt(next);
-        put_state();
-        const auto ro = rsrc_of(r.out, c, os, h * r.dv, r.dv);
+        for (uint32_t c = 0; c < chunks; c++) {
+            // (the last chunk requests itself again instead of one past the end)
+            const uint32_t next = min(c + 1, chunks - 1);
+            f32x4 X[NC];
 #pragma unroll
-        for (int nc = 0; nc < NC; nc++)
+            for (int nc = 0; nc < NC; nc++) {
+                float v[KF];
 #pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const int o = (int)((row4 + y) * os + (live(nc) ? (col0 + 16 * nc) * SZ : 0x80000000u));
-                const T v = (T)(float)O[nc][0][y];
-                if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), ro, o, 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), ro, o, 0, 0);
+                for (int j = 0; j < KF; j++) v[j] = S[nc][j / 4][j % 4];
+                const Part<NW, 3> x = split_part<NW, 3>(v);
+#pragma unroll
+                for (int n = 0; n < LO; n++) *(typename Part<NW, 3>::vec*)(sS[nc][wave][n] + lane * (KF * 2)) = x.l[n];
+                f32x4 y[4] = {};
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+#pragma unroll
+                    for (int n = 0; n < LI; n++)
+                        if (n + j < 3) {
+#pragma unroll
+                            for (int m = 0; m < 4; m++) y[m] = mma_part(limbs(kf[m]).l[n], x.l[j], y[m]);
+                        }
+#pragma unroll
+                for (int m = 0; m < 4; m++) {
+                    if (m == wave) X[nc] = y[m];
+                    else sR[nc][m][wave][lane] = y[m];
+                }
             }
-    }
-    if (a.d.states) {
+            load_k(next);
+            __syncthreads();                   // A: S and partial sums are there
 #pragma unroll
-        for (int nc = 0; nc < NC; nc++)
+            for (int nc = 0; nc < NC; nc++) {
 #pragma unroll
-            for (int p = 0; p < NW; p++)
+                for (int o = 1; o < 4; o++) X[nc] += sR[nc][wave][(wave + o) % 4][lane];
+                uint32_t top = 0;
+                f32x4 x;
 #pragma unroll
-                for (int x = 0; x < 4; x++)
-                    if (live(nc))
-                        a.d.states[at + (size_t)tile_index(NW * wave + p, 4 * g4 + x) * r.dv + col0 + 16 * nc] = S[nc][p][x];
+                for (int y = 0; y < 4; y++) {
+                    const float v = of_bits<T>(vv[nc][y]) - kd[y] * X[nc][y];
+                    x[y] = v;
+                    top = max(top, __builtin_bit_cast(uint32_t, v) & 0x7fffffffu);
+                }
+                int bad = kChunk;              // this tile's first token in this column that is not finite
+                if (__any(top >= 0x7f800000u)) {
+#pragma unroll
+                    for (int y = 3; y >= 0; y--)
+                        if (!(fabsf(x[y]) < __builtin_inff())) bad = row4 + y, x[y] = 0.0f;
+                    bad = min(bad, __shfl_xor(bad, 16, kWave));
+                    bad = min(bad, __shfl_xor(bad, 32, kWave));
+                }
+                if (lane < 16) sBad[nc][l16][wave] = bad;
+                put(sX[nc], x);
+            }
+            load_v(next);
+            __syncthreads();                   // B: X is there
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++) {
+                const int bad = bad_of(nc);
+                f32x4 D = mma_limbs<3>(as_split<3>(tf[0]), get(sX[nc][0], Int<3>()), f32x4{});
+                if (wave >= 2) D = mma_limbs<3>(as_split<3>(tf[1]), get(sX[nc][1], Int<3>()), D);
+                if (__any(bad < kChunk)) {
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if ((int)row4 + y >= bad) D[y] = __builtin_nanf("");
+                }
+                put(sD[nc], D);
+            }
+            load_t(next);
+            __syncthreads();                   // C: D is there
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++) {
+                const Split<3> x0 = get(sD[nc][0], Int<3>()), x1 = get(sD[nc][1], Int<3>());
+#pragma unroll
+                for (int p = 0; p < NW; p++) {
+#pragma unroll
+                    for (int y = 0; y < 4; y++) S[nc][p][y] *= keep;
+                }
+#pragma unroll
+                for (int n = 0; n < LI; n++)
+#pragma unroll
+                    for (int j = 0; j < 3 - n; j++)
+#pragma unroll
+                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][0][n], x0.l[j], S[nc][p]);
+#pragma unroll
+                for (int n = 0; n < LI; n++)
+#pragma unroll
+                    for (int j = 0; j < 3 - n; j++)
+#pragma unroll
+                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][1][n], x1.l[j], S[nc][p]);
+            }
+            load_kt(next);
+        }
+        if (a.d.states) {
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+                for (int p = 0; p < NW; p++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (live(nc)) a.d.states[state_at(nc, p, x)] = S[nc][p][x];
+        }
+    } else {
+        const uint32_t qs = (uint32_t)r.q_stride * SZ, os = (uint32_t)r.out_stride * SZ;
+        vecK qf[4];
+        bf16x8 pf[2][LO];
+        f32x4 qd;
+        const auto load_q = [&](uint32_t c) {              // this wave's tokens, all columns
+            const auto rq = rsrc_of(r.q, c, qs, hq * DK, DK);
+#pragma unroll
+            for (int s = 0; s < 4; s++) qf[s] = loadK(rq, tile_index(wave, l16) * qs + (4 * KF * s + KF * g4) * SZ);
+            qd = *(const f32x4*)(unit_of(c) + kTri * (3 + LO) * kFrag + (kChunk + row4) * 4);
+        };
+        const auto load_p = [&](uint32_t c) {
+            const unsigned char* const u = unit_of(c) + kTri * 3 * kFrag;
+#pragma unroll
+            for (int n = 0; n < LO; n++) pf[0][n] = *(const bf16x8*)(u + (f0 * LO + n) * kFrag + lane * 16);
+            if (wave >= 2) {
+#pragma unroll
+                for (int n = 0; n < LO; n++) pf[1][n] = *(const bf16x8*)(u + (f1 * LO + n) * kFrag + lane * 16);
+            }
+        };
+        if (chunks) {
+            load_q(0);
+            load_p(0);
+        }
+        for (uint32_t c = 0; c < chunks; c++) {
+            const uint32_t next = min(c + 1, chunks - 1);
+            f32x4 O[NC] = {};
+            __syncthreads();                   // A
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const Part<NW, LI> q = limbs(qf[s]);
+#pragma unroll
+                for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+                    for (int j = 0; j < LO; j++) {
+                        const auto x = *(const typename Part<NW, LI>::vec*)(sS[nc][s][j] + lane * (KF * 2));
+#pragma unroll
+                        for (int n = 0; n < LI; n++)
+                            if (n + j < LO) O[nc] = mma_part(q.l[n], x, O[nc]);
+                    }
+            }
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++)
+#pragma unroll
+                for (int y = 0; y < 4; y++) O[nc][y] *= qd[y];
+            load_q(next);
+            __syncthreads();                   // B
+            const auto ro = rsrc_of(r.out, c, os, h * r.dv, r.dv);
+#pragma unroll
+            for (int nc = 0; nc < NC; nc++) {
+                const int bad = bad_of(nc);
+                O[nc] = mma_limbs<LO>(as_split<LO>(pf[0]), get(sX[nc][0], Int<LO>()), O[nc]);
+                if (wave >= 2) O[nc] = mma_limbs<LO>(as_split<LO>(pf[1]), get(sX[nc][1], Int<LO>()), O[nc]);
+                if (__any(bad < kChunk)) {
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        if ((int)row4 + y >= bad) O[nc][y] = __builtin_nanf("");
+                }
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const int o = (int)((row4 + y) * os + (live(nc) ? (col0 + 16 * nc) * SZ : 0x80000000u));
+                    const T v = (T)(float)O[nc][y];
+                    if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), ro, o, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), ro, o, 0, 0);
+                }
+            }
+            load_p(next);
+            __syncthreads();                   // C
+        }
     }
 }
 
@@ -856,7 +949,7 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    return op_launch(delta_chunks_fn<NC>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(256), 0, stream, k);
+    return op_launch(delta_chunks_fn<NC>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(512), 0, stream, k);
 }
 
 bool sizes_ok(const redukt_delta_rows* a) {
