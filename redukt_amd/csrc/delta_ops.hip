@@ -262,8 +262,9 @@ constexpr int kt_bytes(int dk, int in_limbs) { return dk / 16 * 2 * in_limbs * k
 
 struct ChunkArgs {
     DeltaArgs d;
-    unsigned char* ws;         // units: (chunk slot, value head)
-    unsigned char* kt;         // fragments of k^T: (chunk slot, key head)
+    unsigned char* ws;         // units: (value head, chunk slot)
+    unsigned char* kt;         // fragments of k^T: (key head, chunk slot)
+    uint32_t slots;
 };
 
 // Sequence i's rows, within [0, rows].
@@ -302,6 +303,17 @@ __device__ __forceinline__ float of_bits(uint32_t v) {
 template <int DK>
 __device__ __forceinline__ int state_index(int tile, int row) {
     return DK == 128 ? tile_index(tile, row) : 16 * tile + row;
+}
+
+// a[0] b0 + a[1] b1 with three limbs each, as four chains of sums.
+__device__ __forceinline__ f32x4 mma_four(const bf16x8 (&a)[2][3], const Split<3>& b0, const Split<3>& b1) {
+    f32x4 x = mma(a[0][0], b0.l[0], f32x4{}), z = mma(a[1][0], b1.l[0], f32x4{});
+    f32x4 y = mma(a[0][1], b0.l[0], f32x4{}), w = mma(a[1][1], b1.l[0], f32x4{});
+    x = mma(a[0][0], b0.l[1], x), z = mma(a[1][0], b1.l[1], z);
+    y = mma(a[0][1], b0.l[1], y), w = mma(a[1][1], b1.l[1], w);
+    x = mma(a[0][0], b0.l[2], x), z = mma(a[1][0], b1.l[2], z);
+    y = mma(a[0][2], b0.l[0], y), w = mma(a[1][2], b1.l[0], w);
+    return (x + z) + (y + w);
 }
 
 template <int V>
@@ -460,7 +472,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     }
     if (h % group == 0) {
         // row l16 of k^T's tile p (as the state's rows), the tokens 32 s + 8 g + [0, 8)
-        unsigned char* const kt = a.kt + ((size_t)slot * r.hk + hq) * kt_bytes(DK, LI);
+        unsigned char* const kt = a.kt + ((size_t)hq * a.slots + slot) * kt_bytes(DK, LI);
         for (int f = wave; f < DK / 16 * 2; f += 4) {
             const T* const col = sK + state_index<DK>(f / 2, l16);
             float v[8];
@@ -473,7 +485,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     }
     __syncthreads();                           // k and q are done with; sU, sP are written
 
-    unsigned char* const unit = a.ws + ((size_t)slot * r.hv + h) * unit_bytes(LO);
+    unsigned char* const unit = a.ws + ((size_t)h * a.slots + slot) * unit_bytes(LO);
     // from the first token `past` whose key, g or beta is not finite on there are no rows
     const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
     const int past = bads ? __builtin_ctzll(bads) : kChunk;
@@ -629,11 +641,15 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
     typedef T vecK __attribute__((ext_vector_type(KF)));
     // Rows of a chunk by buffer accesses, whose bounds end the chunk (they count the vector offset only, so the
-    // scalar one stays 0).
-    const auto rows_in = [&](uint32_t c) { return min(e - b - c * kChunk, (uint32_t)kChunk); };
-    const auto rsrc_of = [&](const void* p, uint32_t c, uint32_t stride, uint32_t first_col, uint32_t width) {
-        return rows_rsrc((const unsigned char*)p + (size_t)(b + c * kChunk) * stride + (size_t)first_col * SZ,
-                         (rows_in(c) - 1) * stride + width * SZ);
+    // scalar one stays 0): a pointer that moves on by a chunk, and the bytes of the chunk's rows.
+    struct Rows {
+        const unsigned char* p;
+        uint32_t stride, width;
+        __device__ __forceinline__ auto rsrc(uint32_t rows) const { return rows_rsrc(p, (rows - 1) * stride + width); }
+        __device__ __forceinline__ void step(uint32_t chunks) { p += (size_t)(chunks * kChunk) * stride; }
+    };
+    const auto rows_of = [&](const void* p, int64_t stride, uint32_t first_col, uint32_t width) {
+        return Rows{(const unsigned char*)p + ((size_t)b * (uint32_t)stride + first_col) * SZ, (uint32_t)stride * SZ, width * SZ};
     };
     const auto loadK = [&](auto rsrc, uint32_t off) {
         if constexpr (KF * SZ == 8) {
@@ -658,7 +674,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         }
         return o;
     };
-    const auto unit_of = [&](uint32_t c) { return a.ws + ((size_t)(first + c) * r.hv + h) * unit_bytes(LO); };
+    const unsigned char* unit = a.ws + ((size_t)h * a.slots + first) * unit_bytes(LO);
+    const unsigned char* kt = a.kt + ((size_t)hq * a.slots + first) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
     const auto get = [&](const unsigned char (&from)[3][kFrag], auto n_) {
         constexpr int N = decltype(n_)::value;
         Split<N> o;
@@ -666,8 +683,12 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         for (int n = 0; n < N; n++) o.l[n] = *(const bf16x8*)(from[n] + lane * 16);
         return o;
     };
-    // fragment 0 of a triangle is this wave's tile and tokens [0, 32), 1 tokens [32, 64) (waves 2 and 3 only)
-    const int f0 = wave < 2 ? wave : 2 * wave - 2, f1 = wave < 2 ? wave : f0 + 1;
+    // Fragment 0 of a triangle is this wave's tile and tokens [0, 32), 1 tokens [32, 64): zeros for waves 0 and 1, by a
+    // buffer without bytes.
+    const int f0 = wave < 2 ? wave : 2 * wave - 2;
+    const auto frag1 = [&](const unsigned char* p) {
+        return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(p, wave < 2 ? 0 : kFrag), lane * 16, 0, 0));
+    };
     const uint32_t row4 = tile_index(wave, 4 * g4);        // the first of a lane's four tokens
     const auto bad_of = [&](int nc) {                      // the column's first token that is not finite
         const int4 v = *(const int4*)sBad[nc][l16];
@@ -687,41 +708,40 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             for (int p = 0; p < NW; p++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) S[nc][p][x] = a.d.in ? a.d.in[state_at(nc, p, x)] : 0.0f;
-        const uint32_t ks = (uint32_t)r.k_stride * SZ, vs = (uint32_t)r.v_stride * SZ;
-        vecK kf[4];
+        Rows rk = rows_of(r.k, r.k_stride, hq * DK, DK), rv = rows_of(r.v, r.v_stride, h * r.dv, r.dv);
+        vecK kf[4];                            // tiles wave, wave + 1, .. (mod 4)
         bf16x8 tf[2][3], ktf[NW][2][LI];
         uint32_t vv[NC][4];
         f32x4 kd;
         float keep;
-        const auto load_k = [&](uint32_t c) {              // all tokens, the columns of this wave's rows of the state
-            const auto rk = rsrc_of(r.k, c, ks, hq * DK, DK);
+        uint32_t k_at[4];
 #pragma unroll
-            for (int m = 0; m < 4; m++) kf[m] = loadK(rk, tile_index(m, l16) * ks + (4 * KF * wave + KF * g4) * SZ);
+        for (int o = 0; o < 4; o++) k_at[o] = tile_index((wave + o) % 4, l16) * rk.stride + (4 * KF * wave + KF * g4) * SZ;
+        const auto load_k = [&](uint32_t rows) {           // all tokens, the columns of this wave's rows of the state
+            const auto rsrc = rk.rsrc(rows);
+#pragma unroll
+            for (int o = 0; o < 4; o++) kf[o] = loadK(rsrc, k_at[o]);
         };
-        const auto load_v = [&](uint32_t c) {
-            const auto rv = rsrc_of(r.v, c, vs, h * r.dv, r.dv);
+        const auto load_v = [&](uint32_t rows) {
+            const auto rsrc = rv.rsrc(rows);
 #pragma unroll
             for (int nc = 0; nc < NC; nc++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rv, (row4 + x) * vs + col_of(nc) * SZ);
-            kd = *(const f32x4*)(unit_of(c) + kTri * (3 + LO) * kFrag + row4 * 4);
+                for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rsrc, (row4 + x) * rv.stride + col_of(nc) * SZ);
+            kd = *(const f32x4*)(unit + kTri * (3 + LO) * kFrag + row4 * 4);
         };
-        const auto load_t = [&](uint32_t c) {
-            const unsigned char* const u = unit_of(c);
+        const auto load_t = [&]() {
 #pragma unroll
-            for (int n = 0; n < 3; n++) tf[0][n] = *(const bf16x8*)(u + (f0 * 3 + n) * kFrag + lane * 16);
-            if (wave >= 2) {
+            for (int n = 0; n < 3; n++) tf[0][n] = *(const bf16x8*)(unit + (f0 * 3 + n) * kFrag + lane * 16);
 #pragma unroll
-                for (int n = 0; n < 3; n++) tf[1][n] = *(const bf16x8*)(u + (f1 * 3 + n) * kFrag + lane * 16);
-            }
+            for (int n = 0; n < 3; n++) tf[1][n] = frag1(unit + (f0 * 3 + 3 + n) * kFrag);
         };
-        const auto load_kt = [&](uint32_t c) {
-            const unsigned char* const u = a.kt + ((size_t)(first + c) * r.hk + hq) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
+        const auto load_kt = [&]() {
 #pragma unroll
             for (int f = 0; f < NW * 2; f++)
 #pragma unroll
-                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(u + (f * LI + n) * kFrag + lane * 16);
-            keep = ((const float*)(unit_of(c) + kTri * (3 + LO) * kFrag))[2 * kChunk];
+                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(kt + (f * LI + n) * kFrag + lane * 16);
+            keep = ((const float*)(unit + kTri * (3 + LO) * kFrag))[2 * kChunk];
         };
         // The four rows of this wave's tile that a lane holds, as half of a right operand's fragment.
         const auto put = [&](unsigned char (*to)[3][kFrag], const f32x4& v) {
@@ -731,15 +751,21 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             for (int n = 0; n < 3; n++)
                 *(typename Part<1, 3>::vec*)(to[wave / 2][n] + lane * 16 + wave % 2 * 8) = y.l[n];
         };
+        uint32_t left = e - b;                 // rows from this chunk's first on
         if (chunks) {
-            load_k(0);
-            load_v(0);
-            load_t(0);
-            load_kt(0);
+            const uint32_t rows = min(left, (uint32_t)kChunk);
+            load_k(rows);
+            load_v(rows);
+            load_t();
+            load_kt();
         }
         for (uint32_t c = 0; c < chunks; c++) {
             // (the last chunk requests itself again instead of one past the end)
-            const uint32_t next = min(c + 1, chunks - 1);
+            const uint32_t on = left > kChunk ? 1 : 0;
+            left -= on * kChunk;
+            const uint32_t rows = min(left, (uint32_t)kChunk);
+            rk.step(on), rv.step(on);
+            unit += on * unit_bytes(LO), kt += on * kt_bytes(DK, LI);
             f32x4 X[NC];
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -756,15 +782,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                     for (int n = 0; n < LI; n++)
                         if (n + j < 3) {
 #pragma unroll
-                            for (int m = 0; m < 4; m++) y[m] = mma_part(limbs(kf[m]).l[n], x.l[j], y[m]);
+                            for (int o = 0; o < 4; o++) y[o] = mma_part(limbs(kf[o]).l[n], x.l[j], y[o]);
                         }
+                X[nc] = y[0];
 #pragma unroll
-                for (int m = 0; m < 4; m++) {
-                    if (m == wave) X[nc] = y[m];
-                    else sR[nc][m][wave][lane] = y[m];
-                }
+                for (int o = 1; o < 4; o++) sR[nc][(wave + o) % 4][wave][lane] = y[o];
             }
-            load_k(next);
+            load_k(rows);
             __syncthreads();                   // A: S and partial sums are there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -786,16 +810,15 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                     bad = min(bad, __shfl_xor(bad, 16, kWave));
                     bad = min(bad, __shfl_xor(bad, 32, kWave));
                 }
-                if (lane < 16) sBad[nc][l16][wave] = bad;
+                sBad[nc][l16][wave] = bad;     // (the same from all four lanes of a column)
                 put(sX[nc], x);
             }
-            load_v(next);
+            load_v(rows);
             __syncthreads();                   // B: X is there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 const int bad = bad_of(nc);
-                f32x4 D = mma_limbs<3>(as_split<3>(tf[0]), get(sX[nc][0], Int<3>()), f32x4{});
-                if (wave >= 2) D = mma_limbs<3>(as_split<3>(tf[1]), get(sX[nc][1], Int<3>()), D);
+                f32x4 D = mma_four(tf, get(sX[nc][0], Int<3>()), get(sX[nc][1], Int<3>()));
                 if (__any(bad < kChunk)) {
 #pragma unroll
                     for (int y = 0; y < 4; y++)
@@ -803,7 +826,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 }
                 put(sD[nc], D);
             }
-            load_t(next);
+            load_t();
             __syncthreads();                   // C: D is there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -826,7 +849,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
                         for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][1][n], x1.l[j], S[nc][p]);
             }
-            load_kt(next);
+            load_kt();
         }
         if (a.d.states) {
 #pragma unroll
@@ -838,31 +861,35 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                         if (live(nc)) a.d.states[state_at(nc, p, x)] = S[nc][p][x];
         }
     } else {
-        const uint32_t qs = (uint32_t)r.q_stride * SZ, os = (uint32_t)r.out_stride * SZ;
+        Rows rq = rows_of(r.q, r.q_stride, hq * DK, DK), ro = rows_of(r.out, r.out_stride, h * r.dv, r.dv);
         vecK qf[4];
         bf16x8 pf[2][LO];
         f32x4 qd;
-        const auto load_q = [&](uint32_t c) {              // this wave's tokens, all columns
-            const auto rq = rsrc_of(r.q, c, qs, hq * DK, DK);
+        const uint32_t q_at = tile_index(wave, l16) * rq.stride + KF * g4 * SZ;
+        const auto load_q = [&](uint32_t rows) {           // this wave's tokens, all columns
+            const auto rsrc = rq.rsrc(rows);
 #pragma unroll
-            for (int s = 0; s < 4; s++) qf[s] = loadK(rq, tile_index(wave, l16) * qs + (4 * KF * s + KF * g4) * SZ);
-            qd = *(const f32x4*)(unit_of(c) + kTri * (3 + LO) * kFrag + (kChunk + row4) * 4);
+            for (int s = 0; s < 4; s++) qf[s] = loadK(rsrc, q_at + 4 * KF * s * SZ);
+            qd = *(const f32x4*)(unit + kTri * (3 + LO) * kFrag + (kChunk + row4) * 4);
         };
-        const auto load_p = [&](uint32_t c) {
-            const unsigned char* const u = unit_of(c) + kTri * 3 * kFrag;
+        const auto load_p = [&]() {
+            const unsigned char* const u = unit + kTri * 3 * kFrag;
 #pragma unroll
             for (int n = 0; n < LO; n++) pf[0][n] = *(const bf16x8*)(u + (f0 * LO + n) * kFrag + lane * 16);
-            if (wave >= 2) {
 #pragma unroll
-                for (int n = 0; n < LO; n++) pf[1][n] = *(const bf16x8*)(u + (f1 * LO + n) * kFrag + lane * 16);
-            }
+            for (int n = 0; n < LO; n++) pf[1][n] = frag1(u + (f0 * LO + LO + n) * kFrag);
         };
+        uint32_t left = e - b;
         if (chunks) {
-            load_q(0);
-            load_p(0);
+            load_q(min(left, (uint32_t)kChunk));
+            load_p();
         }
         for (uint32_t c = 0; c < chunks; c++) {
-            const uint32_t next = min(c + 1, chunks - 1);
+            const auto to = ro.rsrc(min(left, (uint32_t)kChunk));
+            const uint32_t on = left > kChunk ? 1 : 0;
+            left -= on * kChunk;
+            rq.step(on), ro.step(1);
+            unit += on * unit_bytes(LO);
             f32x4 O[NC] = {};
             __syncthreads();                   // A
 #pragma unroll
@@ -882,14 +909,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             for (int nc = 0; nc < NC; nc++)
 #pragma unroll
                 for (int y = 0; y < 4; y++) O[nc][y] *= qd[y];
-            load_q(next);
+            load_q(min(left, (uint32_t)kChunk));
             __syncthreads();                   // B
-            const auto ro = rsrc_of(r.out, c, os, h * r.dv, r.dv);
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 const int bad = bad_of(nc);
                 O[nc] = mma_limbs<LO>(as_split<LO>(pf[0]), get(sX[nc][0], Int<LO>()), O[nc]);
-                if (wave >= 2) O[nc] = mma_limbs<LO>(as_split<LO>(pf[1]), get(sX[nc][1], Int<LO>()), O[nc]);
+                O[nc] = mma_limbs<LO>(as_split<LO>(pf[1]), get(sX[nc][1], Int<LO>()), O[nc]);
                 if (__any(bad < kChunk)) {
 #pragma unroll
                     for (int y = 0; y < 4; y++)
@@ -897,13 +923,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 }
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const int o = (int)((row4 + y) * os + (live(nc) ? (col0 + 16 * nc) * SZ : 0x80000000u));
+                    const int o = (int)((row4 + y) * ro.stride + (live(nc) ? (col0 + 16 * nc) * SZ : 0x80000000u));
                     const T v = (T)(float)O[nc][y];
-                    if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), ro, o, 0, 0);
-                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), ro, o, 0, 0);
+                    if constexpr (SZ == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, v), to, o, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), to, o, 0, 0);
                 }
             }
-            load_p(next);
+            load_p();
             __syncthreads();                   // C
         }
     }
@@ -930,26 +956,28 @@ const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
 
 uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
 
-#ifndef KNC
-#define KNC 1
-#endif
 uint64_t units_bytes(const redukt_delta_rows& a, uint32_t n_seq) {
     return chunk_slots(a, n_seq) * a.hv * unit_bytes(a.dtype == REDUKT_OP_F32 ? 3 : 2);
 }
 
+constexpr uint64_t kManyTiles = 1024;
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
     const uint64_t prep = chunk_slots(r, k.d.n) * r.hv;
-    constexpr uint32_t NC = KNC;
+    // Two column tiles a workgroup read a chunk's operands once for both, but a chunk then takes them 1.3 times as long: worth
+    // it once there are workgroups waiting for a CU (37 ragged sequences of 16 heads of 128 columns 283 -> 231 us; one of
+    // 32 heads, 256 tiles, 310 -> 369).
+    const uint32_t NC = (uint64_t)k.d.n * r.hv * (r.dv / 16) >= kManyTiles ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
     k.kt = k.ws + units_bytes(r, k.d.n);
+    k.slots = (uint32_t)chunk_slots(r, k.d.n);
     if (r.rows) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    return op_launch(delta_chunks_fn<NC>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(512), 0, stream, k);
+    return op_launch(NC == 2 ? delta_chunks_fn<2>(r.dtype, r.dk) : delta_chunks_fn<1>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(512), 0, stream, k);
 }
 
 bool sizes_ok(const redukt_delta_rows* a) {
@@ -1040,7 +1068,7 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr};
+    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr, 0};
     return launch_chunks(k, stream);
 }
 
