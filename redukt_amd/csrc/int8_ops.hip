@@ -52,11 +52,20 @@ __global__ __launch_bounds__(kBlock) void k_quantize_rows(redukt_quantize_rows a
 }
 
 // ---------------------------------------------------------------- product
+//
+// out[i][j] = (sum_c x[i][c] w[j][c]) (x_scales[i] w_scales[j]) + bias[j].  Sums of codes are exact, so the order of the
+// columns is free and every kernel gives the same bits.  The channels are the matrix instructions' left operand, so a lane
+// holds neighbouring channels of one token.
 
 // v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive codes of row l % 16, the columns 16 (l / 16)
 // + [0, 16); of the result, column l % 16 of rows 4 (l / 16) + [0, 4).
 __device__ __forceinline__ i32x4 mma8(const i32x4& a, const i32x4& b, const i32x4& c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float scaled(const redukt_int8_matmul& a, int sum, uint32_t i, uint32_t j) {
+    const float y = (float)sum * (a.x_scales[i] * a.w_scales[j]);
+    return a.bias ? y + a.bias[j] : y;
 }
 
 // Codes of any alignment: 64 x 64 outputs a workgroup, 64 columns at a time staged byte by byte
@@ -66,7 +75,7 @@ template <typename T>
 __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
     __shared__ __attribute__((aligned(16))) int8_t sx[kTile * kPitch], sw[kTile * kPitch];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const uint32_t i0 = blockIdx.y * kTile, j0 = blockIdx.x * kTile;
+    const uint32_t tiles = (a.n + kTile - 1) / kTile, i0 = blockIdx.x / tiles * kTile, j0 = blockIdx.x % tiles * kTile;
     i32x4 acc[4] = {};
     for (uint32_t c0 = 0; c0 < a.k; c0 += kTile) {
         for (int e = threadIdx.x; e < kTile * kTile; e += kBlock) {
@@ -75,29 +84,253 @@ __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
             sw[r * kPitch + e % kTile] = j0 + r < a.n && c < a.k ? a.w[(int64_t)(j0 + r) * a.w_stride + c] : 0;
         }
         __syncthreads();
-        const i32x4 fx = *(const i32x4*)(sx + (16 * wave + lane % 16) * kPitch + 16 * (lane / 16));
+        const i32x4 fw = *(const i32x4*)(sw + (16 * wave + lane % 16) * kPitch + 16 * (lane / 16));
 #pragma unroll
         for (int t = 0; t < 4; t++)
-            acc[t] = mma8(fx, *(const i32x4*)(sw + (16 * t + lane % 16) * kPitch + 16 * (lane / 16)), acc[t]);
+            acc[t] = mma8(fw, *(const i32x4*)(sx + (16 * t + lane % 16) * kPitch + 16 * (lane / 16)), acc[t]);
         __syncthreads();
     }
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-        const uint32_t j = j0 + 16 * t + lane % 16;
-        if (j >= a.n) continue;
-        const float ws = a.w_scales[j], bias = a.bias ? a.bias[j] : 0.0f;
+        const uint32_t i = i0 + 16 * t + lane % 16;
+        if (i >= a.m) continue;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const uint32_t i = i0 + 16 * wave + 4 * (lane / 16) + e;
-            if (i >= a.m) continue;
-            const float y = (float)acc[t][e] * (a.x_scales[i] * ws);
-            ((T*)a.out)[(int64_t)i * a.out_stride + j] = (T)(a.bias ? y + bias : y);
+            const uint32_t j = j0 + 16 * wave + 4 * (lane / 16) + e;
+            if (j < a.n) ((T*)a.out)[(int64_t)i * a.out_stride + j] = (T)scaled(a, acc[t][e], i, j);
         }
     }
 }
 
-const void* by_type(uint32_t dtype, const void* bf16, const void* f16, const void* f32) {
-    return dtype == REDUKT_OP_BF16 ? bf16 : dtype == REDUKT_OP_F16 ? f16 : f32;
+// Few tokens: the weights are read once, straight into registers, and nothing else costs much.  Of a workgroup's eight waves
+// `split` share 16 channels, each taking every split-th line of 128 columns; their sums meet in LDS.  MT: tiles of 16 tokens.
+struct Int8Few {
+    redukt_int8_matmul a;
+    uint32_t split;
+};
+
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void k_int8_few(Int8Few f) {
+    __shared__ i32x4 part[8][MT][kWave];
+    const redukt_int8_matmul& a = f.a;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l16 = lane % 16, g4 = lane / 16;
+    const uint32_t split = f.split, j0 = (blockIdx.x * (8 / split) + wave / split) * 16;
+    const uint32_t lines = (a.k + 127) / 128;
+    const int8_t* const w = a.w + (int64_t)min(j0 + l16, a.n - 1) * a.w_stride;
+    const int8_t* x[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) x[t] = a.x + (int64_t)min((uint32_t)(16 * t + l16), a.m - 1) * a.x_stride;
+    i32x4 acc[MT] = {};
+    if (j0 < a.n) {
+        for (uint32_t c = wave % split; c < lines; c += split) {
+            // (columns past k: the last ones again, against zeros)
+            uint32_t at[2];
+            i32x4 fw[2], fx[2][MT];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                at[s] = 128 * c + 64 * s + 16 * g4;
+                fw[s] = *(const i32x4*)(w + min(at[s], a.k - 16));
+#pragma unroll
+                for (int t = 0; t < MT; t++) fx[s][t] = *(const i32x4*)(x[t] + min(at[s], a.k - 16));
+            }
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const i32x4 z = {};
+                const i32x4 v = at[s] < a.k ? fw[s] : z;
+#pragma unroll
+                for (int t = 0; t < MT; t++) acc[t] = mma8(v, fx[s][t], acc[t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // (of the waves that share channels, each finishes every split-th tile of tokens)
+    for (int t = wave % split; t < MT; t += split) {
+        i32x4 sum = part[wave / split * split][t][lane];
+        for (uint32_t s = 1; s < split; s++) sum += part[wave / split * split + s][t][lane];
+        const uint32_t i = 16 * t + l16;
+        if (i >= a.m) continue;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t j = j0 + 4 * g4 + e;
+            if (j < a.n) ((T*)a.out)[(int64_t)i * a.out_stride + j] = (T)scaled(a, sum[e], i, j);
+        }
+    }
+}
+
+// Many tokens: tiles of TN channels by TM tokens, 128 columns at a time from memory straight into one of two LDS buffers while
+// the matrix cores work on the other.  A wave takes (TN / WN) x (TM / WM) outputs in 32 x 32 tiles.
+//
+// A row of 128 codes is eight pieces of 16 bytes; piece c of row r stands at place c ^ (r / 2 % 8), so that the 16 rows that 16
+// lanes read a piece of meet no bank twice.  The loads write LDS in lane order, so the lane picks the piece that belongs
+// to its place.
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+typedef __attribute__((address_space(3))) void lds_void;
+constexpr int kCols = 128;
+
+__device__ __forceinline__ i32x16 mma32(const i32x4& a, const i32x4& b, const i32x16& c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+}
+
+// ROWS rows of a tile into `to`, 8 rows a wave and request; `at` is the lane's place in the operand, rows8 the bytes of 8 rows.
+template <int ROWS, int WAVES>
+__device__ __forceinline__ void stage_rows(__amdgpu_buffer_rsrc_t from, lds_u8* __restrict__ to, uint32_t at, uint32_t rows8, int wave) {
+#pragma unroll
+    for (int u = 0; u < ROWS / 8 / WAVES; u++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(to + (u * WAVES + wave) * 1024), 16, (int)(at + u * WAVES * rows8), 0, 0, 0);
+}
+
+__device__ __forceinline__ i32x4 piece(const lds_u8* rows, int row, int c) {
+    return *(const __attribute__((address_space(3))) i32x4*)(rows + row * kCols + ((c ^ (row / 2 % 8)) * 16));
+}
+
+template <int NI, int NJ>
+__device__ __forceinline__ void multiply(const lds_u8* __restrict__ w, const lds_u8* __restrict__ x, i32x16 (&acc)[NI][NJ], int rw, int rx, int lane) {
+#pragma unroll
+    for (int s = 0; s < kCols / 32; s++) {
+        i32x4 fw[NI], fx[NJ];
+#pragma unroll
+        for (int i = 0; i < NI; i++) fw[i] = piece(w, rw + 32 * i + lane % 32, 2 * s + lane / 32);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) fx[j] = piece(x, rx + 32 * j + lane % 32, 2 * s + lane / 32);
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) acc[i][j] = mma32(fw[i], fx[j], acc[i][j]);
+    }
+}
+
+struct Int8Tiles {
+    redukt_int8_matmul a;
+    uint32_t tiles_m, tiles_n;
+    uint32_t wide;             // rows of out take 16-byte stores
+};
+
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tiles(Int8Tiles f) {
+    constexpr int W = WM * WN, NI = TN / WN / 32, NJ = TM / WM / 32, kHalf = (TM + TN) * kCols;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds0[kHalf], lds1[kHalf];
+    const redukt_int8_matmul& a = f.a;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    // Workgroups go round the eight XCDs in turn: an XCD takes neighbouring tiles, eight of the tokens' by four of the
+    // channels' at a time, whose rows its L2 then holds once.
+    const uint32_t total = f.tiles_m * f.tiles_n, per = (total + 7) / 8, t = blockIdx.x % 8 * per + blockIdx.x / 8;
+    if (blockIdx.x / 8 >= per || t >= total) return;
+    const uint32_t band = 8 * f.tiles_n, m0 = t / band * 8, high = min(f.tiles_m - m0, 8u);
+    const uint32_t i0 = (m0 + t % band % high) * TM, j0 = t % band / high * TN;
+
+    const uint32_t xs = (uint32_t)a.x_stride, ws = (uint32_t)a.w_stride;
+    const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x + (size_t)i0 * xs), (short)0,
+                                                      (int)((min(a.m - i0, (uint32_t)TM) - 1) * xs + a.k), 0x00020000);
+    const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (size_t)j0 * ws), (short)0,
+                                                      (int)((min(a.n - j0, (uint32_t)TN) - 1) * ws + a.k), 0x00020000);
+    const int row = wave * 8 + lane / 8;
+    const uint32_t col = ((lane % 8) ^ (row / 2 % 8)) * 16;
+    static_assert(W * 8 % 16 == 0, "a lane's rows have one order of pieces");
+    // (rows past the tile and columns past k are out of the buffers' bounds and come as zeros)
+    const auto stage = [&](lds_u8* __restrict__ to, uint32_t c) {
+        const bool in = c + col < a.k;
+        stage_rows<TN, W>(rw, to, in ? row * ws + col + c : 0x80000000u, 8 * ws, wave);
+        stage_rows<TM, W>(rx, to + TN * kCols, in ? row * xs + col + c : 0x80000000u, 8 * xs, wave);
+    };
+    const int rj = wave / WN * (TM / WM), ri = wave % WN * (TN / WN);
+    i32x16 acc[NI][NJ] = {};
+    const auto step = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ now, uint32_t c) {
+        if (c + kCols < a.k) stage(next, c + kCols);
+        multiply<NI, NJ>(now, now + TN * kCols, acc, ri, rj, lane);
+        __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0): the next columns are in LDS
+        __syncthreads();
+    };
+    stage((lds_u8*)lds0, 0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __syncthreads();
+    for (uint32_t c = 0; c < a.k; c += 2 * kCols) {
+        step((lds_u8*)lds1, (const lds_u8*)lds0, c);
+        if (c + kCols < a.k) step((lds_u8*)lds0, (const lds_u8*)lds1, c + kCols);
+    }
+
+    // 32 tokens of a wave's channels at a time through LDS, so that a row of them is stored as whole lines.
+    constexpr int CH = TN / WN, kRow = CH * sizeof(T), kPieces = kRow / 16, kPer = 16 / sizeof(T);
+    static_assert(32 * kRow * W <= 2 * kHalf, "");
+    unsigned char* const mine = (32 * kRow * W <= kHalf || wave < W / 2 ? lds0 : lds1) + (32 * kRow * W <= kHalf ? wave : wave % (W / 2)) * 32 * kRow;
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    typedef T out16 __attribute__((ext_vector_type(kPer)));
+    float sw[NI][4][4], bias[NI][4][4];
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t j = min(j0 + ri + 32 * i + 8 * g + 4 * (lane / 32) + e, a.n - 1);
+                sw[i][g][e] = a.w_scales[j];
+                bias[i][g][e] = a.bias ? a.bias[j] : 0.0f;
+            }
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const uint32_t i_row = i0 + rj + 32 * j;
+        const float sx = a.x_scales[min(i_row + lane % 32, a.m - 1)];
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                out4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y = (float)acc[i][j][4 * g + e] * (sx * sw[i][g][e]);
+                    v[e] = (T)(a.bias ? y + bias[i][g][e] : y);
+                }
+                const int at = (32 * i + 8 * g + 4 * (lane / 32)) * (int)sizeof(T), r = lane % 32;
+                *(out4*)(mine + r * kRow + ((at / 16 ^ r % kPieces) * 16) + at % 16) = v;
+            }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+        for (int u = 0; u < 32 * kPieces / kWave; u++) {
+            const int id = u * kWave + lane, r = id / kPieces, p = id % kPieces;
+            const out16 v = *(const out16*)(mine + r * kRow + ((p ^ r % kPieces) * 16));
+            const uint32_t i = i_row + r, c = j0 + ri + p * kPer;
+            if (i >= a.m || c >= a.n) continue;
+            T* const o = (T*)a.out + (int64_t)i * a.out_stride + c;
+            if (f.wide && c + kPer <= a.n) {
+                *(out16*)o = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; e++)
+                    if (c + e < a.n) o[e] = v[e];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+#define OP_BY_TYPE(dtype, fn, ...) \
+    ((dtype) == REDUKT_OP_BF16 ? (const void*)fn<__bf16 __VA_OPT__(, ) __VA_ARGS__> \
+     : (dtype) == REDUKT_OP_F16 ? (const void*)fn<_Float16 __VA_OPT__(, ) __VA_ARGS__> \
+                                : (const void*)fn<float __VA_OPT__(, ) __VA_ARGS__>)
+
+constexpr int64_t kMaxStride = 1 << 22;      // 256 rows stay within 32-bit offsets
+
+int32_t few(const redukt_int8_matmul& a, void* stream) {
+    const uint32_t groups = (a.n + 15) / 16, lines = (a.k + 127) / 128;
+    uint32_t split = 1;
+    while (split < 8 && split * 2 <= lines && groups * split < 2048) split *= 2;
+    Int8Few k{a, split};
+    const uint32_t per = 8 / split, grid = (groups + per - 1) / per;
+    const void* fn = a.m <= 16 ? OP_BY_TYPE(a.dtype, k_int8_few, 1) : a.m <= 32 ? OP_BY_TYPE(a.dtype, k_int8_few, 2)
+                                                                                : OP_BY_TYPE(a.dtype, k_int8_few, 4);
+    return op_launch(fn, dim3(grid), dim3(512), 0, stream, k);
+}
+
+template <int TM, int TN, int WM, int WN>
+int32_t tiles(const redukt_int8_matmul& a, void* stream) {
+    const bool wide = op_aligned(a.out, 16) && a.out_stride * op_elem_bytes(a.dtype) % 16 == 0;
+    Int8Tiles k{a, (a.m + TM - 1) / TM, (a.n + TN - 1) / TN, wide};
+    const uint64_t total = (uint64_t)k.tiles_m * k.tiles_n, grid = (total + 7) / 8 * 8;
+    if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    return op_launch(OP_BY_TYPE(a.dtype, k_int8_tiles, TM, TN, WM, WN), dim3((uint32_t)grid), dim3(64 * WM * WN), 0, stream, k);
 }
 
 }  // namespace
@@ -117,9 +350,7 @@ int32_t redukt_op_quantize_rows(const redukt_quantize_rows* a, void* stream) {
     OpDevice dev(a->scales);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     redukt_quantize_rows k = *a;
-    const void* fn = by_type(a->dtype, (const void*)k_quantize_rows<__bf16>, (const void*)k_quantize_rows<_Float16>,
-                             (const void*)k_quantize_rows<float>);
-    return op_launch(fn, dim3(a->rows), dim3(kBlock), 0, stream, k);
+    return op_launch(OP_BY_TYPE(a->dtype, k_quantize_rows), dim3(a->rows), dim3(kBlock), 0, stream, k);
 }
 
 int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
@@ -136,12 +367,17 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
         return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(a->out);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    redukt_int8_matmul k = *a;
-    const void* fn = by_type(a->dtype, (const void*)k_int8_bytes<__bf16>, (const void*)k_int8_bytes<_Float16>,
-                             (const void*)k_int8_bytes<float>);
-    const dim3 grid((a->n + kTile - 1) / kTile, (a->m + kTile - 1) / kTile);
-    if (grid.y > 65535) return BACKEND_INVALID_ARGUMENT;
-    return op_launch(fn, grid, dim3(kBlock), 0, stream, k);
+    const bool aligned = op_aligned(a->x, 16) && op_aligned(a->w, 16) && a->x_stride % 16 == 0 && a->w_stride % 16 == 0 &&
+                         a->k % 16 == 0 && a->k > 0 && a->x_stride <= kMaxStride && a->w_stride <= kMaxStride;
+    if (!aligned) {
+        redukt_int8_matmul k = *a;
+        const uint64_t grid = (uint64_t)((a->n + kTile - 1) / kTile) * ((a->m + kTile - 1) / kTile);
+        if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+        return op_launch(OP_BY_TYPE(a->dtype, k_int8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
+    }
+    if (a->m <= 64) return few(*a, stream);
+    return (uint64_t)((a->m + 255) / 256) * ((a->n + 255) / 256) >= 128 ? tiles<256, 256, 2, 4>(*a, stream)
+                                                                        : tiles<128, 128, 2, 2>(*a, stream);
 }
 
 }  // extern "C"
