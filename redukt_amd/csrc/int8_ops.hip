@@ -102,99 +102,96 @@ __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
     }
 }
 
-// Few tokens: the weights are read once, straight into registers, and nothing else costs much.  Of a workgroup's eight waves
-// `split` share 16 channels, each taking every split-th line of 128 columns; their sums meet in LDS.  MT: tiles of 16 tokens.
+// Up to 16 tokens: the weights are read once, straight into registers, and nothing else costs much (one token of 50,280 x 768:
+// 38.6 MB at 3.4 TB/s with the launch).  Of a workgroup's eight waves `split` share 16 channels, each taking every split-th line
+// of 128 columns; their sums meet in LDS.
 struct Int8Few {
     redukt_int8_matmul a;
     uint32_t split;
 };
 
-template <typename T, int MT>
+template <typename T>
 __global__ __launch_bounds__(512) void k_int8_few(Int8Few f) {
-    __shared__ i32x4 part[8][MT][kWave];
+    __shared__ i32x4 part[8][kWave];
     const redukt_int8_matmul& a = f.a;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l16 = lane % 16, g4 = lane / 16;
     const uint32_t split = f.split, j0 = (blockIdx.x * (8 / split) + wave / split) * 16;
     const uint32_t lines = (a.k + 127) / 128;
     const int8_t* const w = a.w + (int64_t)min(j0 + l16, a.n - 1) * a.w_stride;
-    const int8_t* x[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) x[t] = a.x + (int64_t)min((uint32_t)(16 * t + l16), a.m - 1) * a.x_stride;
-    i32x4 acc[MT] = {};
+    const int8_t* const x = a.x + (int64_t)min((uint32_t)l16, a.m - 1) * a.x_stride;
+    i32x4 acc = {};
     if (j0 < a.n) {
         for (uint32_t c = wave % split; c < lines; c += split) {
             // (columns past k: the last ones again, against zeros)
             uint32_t at[2];
-            i32x4 fw[2], fx[2][MT];
+            i32x4 fw[2], fx[2];
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 at[s] = 128 * c + 64 * s + 16 * g4;
                 fw[s] = *(const i32x4*)(w + min(at[s], a.k - 16));
-#pragma unroll
-                for (int t = 0; t < MT; t++) fx[s][t] = *(const i32x4*)(x[t] + min(at[s], a.k - 16));
+                fx[s] = *(const i32x4*)(x + min(at[s], a.k - 16));
             }
 #pragma unroll
             for (int s = 0; s < 2; s++) {
                 const i32x4 z = {};
-                const i32x4 v = at[s] < a.k ? fw[s] : z;
-#pragma unroll
-                for (int t = 0; t < MT; t++) acc[t] = mma8(v, fx[s][t], acc[t]);
+                acc = mma8(at[s] < a.k ? fw[s] : z, fx[s], acc);
             }
         }
     }
-#pragma unroll
-    for (int t = 0; t < MT; t++) part[wave][t][lane] = acc[t];
+    part[wave][lane] = acc;
     __syncthreads();
-    // (of the waves that share channels, each finishes every split-th tile of tokens)
-    for (int t = wave % split; t < MT; t += split) {
-        i32x4 sum = part[wave / split * split][t][lane];
-        for (uint32_t s = 1; s < split; s++) sum += part[wave / split * split + s][t][lane];
-        const uint32_t i = 16 * t + l16;
-        if (i >= a.m) continue;
+    if (wave % split) return;
+    for (uint32_t s = 1; s < split; s++) acc += part[wave + s][lane];
+    if ((uint32_t)l16 >= a.m) return;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t j = j0 + 4 * g4 + e;
-            if (j < a.n) ((T*)a.out)[(int64_t)i * a.out_stride + j] = (T)scaled(a, sum[e], i, j);
-        }
+    for (int e = 0; e < 4; e++) {
+        const uint32_t j = j0 + 4 * g4 + e;
+        if (j < a.n) ((T*)a.out)[(int64_t)l16 * a.out_stride + j] = (T)scaled(a, acc[e], l16, j);
     }
 }
 
-// Many tokens: tiles of TN channels by TM tokens, 128 columns at a time from memory straight into one of two LDS buffers while
-// the matrix cores work on the other.  A wave takes (TN / WN) x (TM / WM) outputs in 32 x 32 tiles.
+// Many tokens: tiles of TN channels by TM tokens, KC columns at a time from memory straight into one of STAGES LDS buffers while
+// the matrix cores work on another.  A wave takes (TN / WN) x (TM / WM) outputs in 32 x 32 tiles.
 //
-// A row of 128 codes is eight pieces of 16 bytes; piece c of row r stands at place c ^ (r / 2 % 8), so that the 16 rows that 16
-// lanes read a piece of meet no bank twice.  The loads write LDS in lane order, so the lane picks the piece that belongs
-// to its place.
+// A row of KC codes is KC / 16 pieces of 16 bytes; piece c of row r stands at place c ^ (r / 2 % 8) (KC 128) or c ^ (r % 16)
+// (KC 256), so that the 16 rows that 16 lanes read a piece of meet no bank twice.  The loads write LDS in lane order, so the
+// lane picks the piece that belongs to its place.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 typedef __attribute__((address_space(3))) void lds_void;
-constexpr int kCols = 128;
 
 __device__ __forceinline__ i32x16 mma32(const i32x4& a, const i32x4& b, const i32x16& c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
-// ROWS rows of a tile into `to`, 8 rows a wave and request; `at` is the lane's place in the operand, rows8 the bytes of 8 rows.
-template <int ROWS, int WAVES>
-__device__ __forceinline__ void stage_rows(__amdgpu_buffer_rsrc_t from, lds_u8* __restrict__ to, uint32_t at, uint32_t rows8, int wave) {
+template <int KC>
+__device__ __forceinline__ int place_of(int row, int c) {
+    return KC == 128 ? c ^ (row / 2 % 8) : c ^ (row % 16);
+}
+
+// ROWS rows of a tile into `to`, 1 KB a wave and request; `at` is the lane's place in the operand, stride the bytes of a row.
+template <int KC, int ROWS, int WAVES>
+__device__ __forceinline__ void stage_rows(__amdgpu_buffer_rsrc_t from, lds_u8* __restrict__ to, uint32_t at, uint32_t stride, int wave) {
 #pragma unroll
-    for (int u = 0; u < ROWS / 8 / WAVES; u++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(to + (u * WAVES + wave) * 1024), 16, (int)(at + u * WAVES * rows8), 0, 0, 0);
+    for (int u = 0; u < ROWS * KC / 1024 / WAVES; u++)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(to + (u * WAVES + wave) * 1024), 16,
+                                                 (int)(at + u * (WAVES * 1024 / KC) * stride), 0, 0, 0);
 }
 
+template <int KC>
 __device__ __forceinline__ i32x4 piece(const lds_u8* rows, int row, int c) {
-    return *(const __attribute__((address_space(3))) i32x4*)(rows + row * kCols + ((c ^ (row / 2 % 8)) * 16));
+    return *(const __attribute__((address_space(3))) i32x4*)(rows + row * KC + place_of<KC>(row, c) * 16);
 }
 
-template <int NI, int NJ>
+template <int KC, int NI, int NJ>
 __device__ __forceinline__ void multiply(const lds_u8* __restrict__ w, const lds_u8* __restrict__ x, i32x16 (&acc)[NI][NJ], int rw, int rx, int lane) {
 #pragma unroll
-    for (int s = 0; s < kCols / 32; s++) {
+    for (int s = 0; s < KC / 32; s++) {
         i32x4 fw[NI], fx[NJ];
 #pragma unroll
-        for (int i = 0; i < NI; i++) fw[i] = piece(w, rw + 32 * i + lane % 32, 2 * s + lane / 32);
+        for (int i = 0; i < NI; i++) fw[i] = piece<KC>(w, rw + 32 * i + lane % 32, 2 * s + lane / 32);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) fx[j] = piece(x, rx + 32 * j + lane % 32, 2 * s + lane / 32);
+        for (int j = 0; j < NJ; j++) fx[j] = piece<KC>(x, rx + 32 * j + lane % 32, 2 * s + lane / 32);
 #pragma unroll
         for (int i = 0; i < NI; i++)
 #pragma unroll
@@ -208,10 +205,18 @@ struct Int8Tiles {
     uint32_t wide;             // rows of out take 16-byte stores
 };
 
-template <typename T, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tiles(Int8Tiles f) {
-    constexpr int W = WM * WN, NI = TN / WN / 32, NJ = TM / WM / 32, kHalf = (TM + TN) * kCols;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds0[kHalf], lds1[kHalf];
+// s_waitcnt vmcnt(N), the other counters as they are.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+}
+
+template <typename T, int TM, int TN, int WM, int WN, int KC, int STAGES>
+__global__ __launch_bounds__(64 * WM * WN) void k_int8_tiles(Int8Tiles f) {
+    constexpr int W = WM * WN, NI = TN / WN / 32, NJ = TM / WM / 32, kStage = (TM + TN) * KC;
+    constexpr int kPending = (STAGES - 2) * kStage / 1024 / W;     // requests of the stages behind the next one
+    static_assert(kPending < 64 && TM * KC / 1024 % W == 0 && TN * KC / 1024 % W == 0, "");
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES][kStage];
     const redukt_int8_matmul& a = f.a;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     // Workgroups go round the eight XCDs in turn: an XCD takes neighbouring tiles, eight of the tokens' by four of the
@@ -226,35 +231,39 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tiles(Int8Tiles f) {
                                                       (int)((min(a.m - i0, (uint32_t)TM) - 1) * xs + a.k), 0x00020000);
     const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)(a.w + (size_t)j0 * ws), (short)0,
                                                       (int)((min(a.n - j0, (uint32_t)TN) - 1) * ws + a.k), 0x00020000);
-    const int row = wave * 8 + lane / 8;
-    const uint32_t col = ((lane % 8) ^ (row / 2 % 8)) * 16;
-    static_assert(W * 8 % 16 == 0, "a lane's rows have one order of pieces");
+    constexpr int kPieces = KC / 16, kRows = 64 / kPieces;         // rows of one request
+    const int row = wave * kRows + lane / kPieces;
+    const uint32_t col = place_of<KC>(row, lane % kPieces) * 16;
+    static_assert(W * kRows % 16 == 0, "a lane's rows have one order of pieces");
     // (rows past the tile and columns past k are out of the buffers' bounds and come as zeros)
     const auto stage = [&](lds_u8* __restrict__ to, uint32_t c) {
         const bool in = c + col < a.k;
-        stage_rows<TN, W>(rw, to, in ? row * ws + col + c : 0x80000000u, 8 * ws, wave);
-        stage_rows<TM, W>(rx, to + TN * kCols, in ? row * xs + col + c : 0x80000000u, 8 * xs, wave);
+        stage_rows<KC, TN, W>(rw, to, in ? row * ws + col + c : 0x80000000u, ws, wave);
+        stage_rows<KC, TM, W>(rx, to + TN * KC, in ? row * xs + col + c : 0x80000000u, xs, wave);
     };
     const int rj = wave / WN * (TM / WM), ri = wave % WN * (TN / WN);
     i32x16 acc[NI][NJ] = {};
-    const auto step = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ now, uint32_t c) {
-        if (c + kCols < a.k) stage(next, c + kCols);
-        multiply<NI, NJ>(now, now + TN * kCols, acc, ri, rj, lane);
-        __builtin_amdgcn_s_waitcnt(0x0f70);    // vmcnt(0): the next columns are in LDS
-        __syncthreads();
-    };
-    stage((lds_u8*)lds0, 0);
-    __builtin_amdgcn_s_waitcnt(0x0f70);
-    __syncthreads();
-    for (uint32_t c = 0; c < a.k; c += 2 * kCols) {
-        step((lds_u8*)lds1, (const lds_u8*)lds0, c);
-        if (c + kCols < a.k) step((lds_u8*)lds0, (const lds_u8*)lds1, c + kCols);
+    // A step's columns are waited for (with those behind them still under way); then every wave is done with the buffer of the
+    // columns before them, which takes the ones STAGES - 1 further on (past k: zeros, without a request to memory).
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) stage((lds_u8*)lds[s], s * KC);
+    for (uint32_t c = 0; c < a.k; c += STAGES * KC) {
+#pragma unroll
+        for (int s = 0; s < STAGES; s++) {
+            if (c + s * KC >= a.k) break;
+            wait_loads<kPending>();
+            __syncthreads();
+            stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * KC);
+            multiply<KC, NI, NJ>((const lds_u8*)lds[s], (const lds_u8*)lds[s] + TN * KC, acc, ri, rj, lane);
+        }
     }
+    wait_loads<0>();                           // (zeros may still be on their way)
+    __syncthreads();
 
     // 32 tokens of a wave's channels at a time through LDS, so that a row of them is stored as whole lines.
-    constexpr int CH = TN / WN, kRow = CH * sizeof(T), kPieces = kRow / 16, kPer = 16 / sizeof(T);
-    static_assert(32 * kRow * W <= 2 * kHalf, "");
-    unsigned char* const mine = (32 * kRow * W <= kHalf || wave < W / 2 ? lds0 : lds1) + (32 * kRow * W <= kHalf ? wave : wave % (W / 2)) * 32 * kRow;
+    constexpr int CH = TN / WN, kRow = CH * sizeof(T), kOuts = kRow / 16, kPer = 16 / sizeof(T);
+    static_assert(32 * kRow * W <= STAGES * kStage, "");
+    unsigned char* const mine = &lds[0][0] + wave * 32 * kRow;
     typedef T out4 __attribute__((ext_vector_type(4)));
     typedef T out16 __attribute__((ext_vector_type(kPer)));
     float sw[NI][4][4], bias[NI][4][4];
@@ -283,14 +292,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tiles(Int8Tiles f) {
                     v[e] = (T)(a.bias ? y + bias[i][g][e] : y);
                 }
                 const int at = (32 * i + 8 * g + 4 * (lane / 32)) * (int)sizeof(T), r = lane % 32;
-                *(out4*)(mine + r * kRow + ((at / 16 ^ r % kPieces) * 16) + at % 16) = v;
+                *(out4*)(mine + r * kRow + ((at / 16 ^ r % kOuts) * 16) + at % 16) = v;
             }
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 #pragma unroll
-        for (int u = 0; u < 32 * kPieces / kWave; u++) {
-            const int id = u * kWave + lane, r = id / kPieces, p = id % kPieces;
-            const out16 v = *(const out16*)(mine + r * kRow + ((p ^ r % kPieces) * 16));
+        for (int u = 0; u < 32 * kOuts / kWave; u++) {
+            const int id = u * kWave + lane, r = id / kOuts, p = id % kOuts;
+            const out16 v = *(const out16*)(mine + r * kRow + ((p ^ r % kOuts) * 16));
             const uint32_t i = i_row + r, c = j0 + ri + p * kPer;
             if (i >= a.m || c >= a.n) continue;
             T* const o = (T*)a.out + (int64_t)i * a.out_stride + c;
@@ -311,6 +320,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_int8_tiles(Int8Tiles f) {
      : (dtype) == REDUKT_OP_F16 ? (const void*)fn<_Float16 __VA_OPT__(, ) __VA_ARGS__> \
                                 : (const void*)fn<float __VA_OPT__(, ) __VA_ARGS__>)
 
+#ifndef KF
+#define KF 64
+#endif
 constexpr int64_t kMaxStride = 1 << 22;      // 256 rows stay within 32-bit offsets
 
 int32_t few(const redukt_int8_matmul& a, void* stream) {
@@ -319,18 +331,16 @@ int32_t few(const redukt_int8_matmul& a, void* stream) {
     while (split < 8 && split * 2 <= lines && groups * split < 2048) split *= 2;
     Int8Few k{a, split};
     const uint32_t per = 8 / split, grid = (groups + per - 1) / per;
-    const void* fn = a.m <= 16 ? OP_BY_TYPE(a.dtype, k_int8_few, 1) : a.m <= 32 ? OP_BY_TYPE(a.dtype, k_int8_few, 2)
-                                                                                : OP_BY_TYPE(a.dtype, k_int8_few, 4);
-    return op_launch(fn, dim3(grid), dim3(512), 0, stream, k);
+    return op_launch(OP_BY_TYPE(a.dtype, k_int8_few), dim3(grid), dim3(512), 0, stream, k);
 }
 
-template <int TM, int TN, int WM, int WN>
+template <int TM, int TN, int WM, int WN, int KC, int STAGES>
 int32_t tiles(const redukt_int8_matmul& a, void* stream) {
     const bool wide = op_aligned(a.out, 16) && a.out_stride * op_elem_bytes(a.dtype) % 16 == 0;
     Int8Tiles k{a, (a.m + TM - 1) / TM, (a.n + TN - 1) / TN, wide};
     const uint64_t total = (uint64_t)k.tiles_m * k.tiles_n, grid = (total + 7) / 8 * 8;
     if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
-    return op_launch(OP_BY_TYPE(a.dtype, k_int8_tiles, TM, TN, WM, WN), dim3((uint32_t)grid), dim3(64 * WM * WN), 0, stream, k);
+    return op_launch(OP_BY_TYPE(a.dtype, k_int8_tiles, TM, TN, WM, WN, KC, STAGES), dim3((uint32_t)grid), dim3(64 * WM * WN), 0, stream, k);
 }
 
 }  // namespace
@@ -375,9 +385,16 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
         if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
         return op_launch(OP_BY_TYPE(a->dtype, k_int8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
-    if (a->m <= 64) return few(*a, stream);
-    return (uint64_t)((a->m + 255) / 256) * ((a->n + 255) / 256) >= 128 ? tiles<256, 256, 2, 4>(*a, stream)
-                                                                        : tiles<128, 128, 2, 2>(*a, stream);
+    // Every kernel gives the same bits, so the choice is by time alone (us, on either side of each edge; n and k after m).  Up to
+    // 16 tokens: weights straight into registers (16 of 8,192 x 8,192: 19.0, tiles 22.9; 33: 22.9 at two row tiles and 24.6).
+    if (a->m <= 16) return few(*a, stream);
+    // Tiles of 256 once they fill the CUs (8,192 of 8,192 x 4,096: 249, tiles of 128: 291; 2,048 of 4,096 x 1,536, 128 tiles: 27.8 and
+    // 20.9), of 128 once they nearly do (4,096 of 768 x 768, 192 tiles: 10.3, tiles of 64: 10.8; 1,000 of 1,536 x 768, 96 tiles:
+    // 9.4 and 7.0), else of 64 by 256 columns (128 of 8,192 x 8,192: 26.8, by 128 columns 32.2).
+    const auto count = [&](uint32_t t) { return (uint64_t)((a->m + t - 1) / t) * ((a->n + t - 1) / t); };
+    if (count(256) >= 256) return tiles<256, 256, 2, 4, 128, 2>(*a, stream);
+    if (count(128) >= 192) return tiles<128, 128, 2, 2, 128, 2>(*a, stream);
+    return tiles<64, 64, 2, 2, 256, 2>(*a, stream);
 }
 
 }  // extern "C"
