@@ -17,11 +17,15 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // ---------------------------------------------------------------- codes
 
-__device__ __forceinline__ int8_t code_of(float v, float inv) {
-    float t = roundf(v * inv);
-    if (t < -127.0f) t = -127.0f;
-    if (t > 127.0f) t = 127.0f;
-    return t != t ? (int8_t)0 : (int8_t)(int)t;
+// v / scale to the nearest whole number, halves away from zero, as an int in [-127, 127]; NaN gives 0.  Adding the largest f32
+// below 1/2 with v's sign and dropping the fraction rounds so: the sum of a half and it is a tie, which goes up to the even 1 (and
+// so on up to 2^22), and that of the largest value below a half stays below 1.  The conversion saturates, and takes NaN to 0.
+__device__ __forceinline__ int code_of(float v, float inv) {
+    const float t = v * inv;
+    const float h = t + __builtin_copysignf(0x1.fffffep-2f, t);
+    int q;
+    asm("v_cvt_i32_f32 %0, %1" : "=v"(q) : "v"(h));
+    return min(max(q, -127), 127);
 }
 
 // |v| into a running maximum that a NaN never enters.
@@ -30,25 +34,59 @@ __device__ __forceinline__ float fold_abs(float m, float v) {
     return a > m ? a : m;
 }
 
-// One workgroup a row: the row's maximum, then its codes from a second read.
-template <typename T>
+// WAVES waves a row (one: a row each).  V elements a load: 16 bytes where the rows are aligned, else one.  Of a row, kHeld loads a
+// lane stay in registers between the maximum and the codes, so it is read once; what is longer is read again.
+template <typename T, int V, int WAVES>
 __global__ __launch_bounds__(kBlock) void k_quantize_rows(redukt_quantize_rows a) {
+    constexpr int kHeld = 4, kLanes = WAVES * kWave, kSpan = kLanes * V;
     __shared__ float wm[kWaves];
-    const uint32_t r = blockIdx.x;
-    const T* x = (const T*)a.x + (int64_t)r * a.x_stride;
+    const int lane = threadIdx.x % kLanes;
+    const uint32_t r = WAVES == 1 ? blockIdx.x * kWaves + threadIdx.x / kWave : blockIdx.x;
+    if (r >= a.rows) return;                   // (whole waves, and none of a shared row)
+    const T* const x = (const T*)a.x + (int64_t)r * a.x_stride;
+    int8_t* const q = a.codes + (int64_t)r * a.codes_stride;
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef int8_t codes __attribute__((ext_vector_type(V)));
+    const uint32_t whole = a.cols / V * V, c0 = lane * V;
+    vec held[kHeld];
     float m = 0.0f;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += kBlock) m = fold_abs(m, (float)x[c]);
+#pragma unroll
+    for (int u = 0; u < kHeld; u++) {
+        held[u] = vec{};
+        if (c0 + u * kSpan < whole) held[u] = *(const vec*)(x + c0 + u * kSpan);
+    }
+#pragma unroll
+    for (int u = 0; u < kHeld; u++)
+#pragma unroll
+        for (int e = 0; e < V; e++) m = fold_abs(m, (float)held[u][e]);
+    for (uint32_t c = c0 + kHeld * kSpan; c < whole; c += kSpan) {
+        const vec v = *(const vec*)(x + c);
+#pragma unroll
+        for (int e = 0; e < V; e++) m = fold_abs(m, (float)v[e]);
+    }
+    if (V > 1 && whole + lane < a.cols) m = fold_abs(m, (float)x[whole + lane]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fold_abs(m, __shfl_xor(m, o, kWave));
-    if (threadIdx.x % kWave == 0) wm[threadIdx.x / kWave] = m;
-    __syncthreads();
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % kWave == 0) wm[threadIdx.x / kWave] = m;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) m = fold_abs(m, wm[w]);
+        for (int w = 0; w < WAVES; w++) m = fold_abs(m, wm[w]);
+    }
     const float scale = m > 0.0f ? m / 127.0f : 1.0f;
     const float inv = 1.0f / scale;
-    int8_t* q = a.codes + (int64_t)r * a.codes_stride;
-    for (uint32_t c = threadIdx.x; c < a.cols; c += kBlock) q[c] = code_of((float)x[c], inv);
-    if (threadIdx.x == 0) a.scales[r] = scale;
+    const auto store = [&](uint32_t c, const vec& v) {
+        codes y;
+#pragma unroll
+        for (int e = 0; e < V; e++) y[e] = (int8_t)code_of((float)v[e], inv);
+        *(codes*)(q + c) = y;
+    };
+#pragma unroll
+    for (int u = 0; u < kHeld; u++)
+        if (c0 + u * kSpan < whole) store(c0 + u * kSpan, held[u]);
+    for (uint32_t c = c0 + kHeld * kSpan; c < whole; c += kSpan) store(c, *(const vec*)(x + c));
+    if (V > 1 && whole + lane < a.cols) q[whole + lane] = (int8_t)code_of((float)x[whole + lane], inv);
+    if (lane == 0) a.scales[r] = scale;
 }
 
 // ---------------------------------------------------------------- product
@@ -320,9 +358,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_int8_tiles(Int8Tiles f) {
      : (dtype) == REDUKT_OP_F16 ? (const void*)fn<_Float16 __VA_OPT__(, ) __VA_ARGS__> \
                                 : (const void*)fn<float __VA_OPT__(, ) __VA_ARGS__>)
 
-#ifndef KF
-#define KF 64
-#endif
+template <int WAVES>
+const void* quantize_wide_fn(uint32_t dtype) {
+    return dtype == REDUKT_OP_BF16  ? (const void*)k_quantize_rows<__bf16, 8, WAVES>
+           : dtype == REDUKT_OP_F16 ? (const void*)k_quantize_rows<_Float16, 8, WAVES>
+                                    : (const void*)k_quantize_rows<float, 4, WAVES>;
+}
+
 constexpr int64_t kMaxStride = 1 << 22;      // 256 rows stay within 32-bit offsets
 
 int32_t few(const redukt_int8_matmul& a, void* stream) {
@@ -360,7 +402,13 @@ int32_t redukt_op_quantize_rows(const redukt_quantize_rows* a, void* stream) {
     OpDevice dev(a->scales);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     redukt_quantize_rows k = *a;
-    return op_launch(OP_BY_TYPE(a->dtype, k_quantize_rows), dim3(a->rows), dim3(kBlock), 0, stream, k);
+    const int size = (int)op_elem_bytes(a->dtype), v = 16 / size;
+    const bool wide = op_aligned(a->x, 16) && op_aligned(a->codes, v) && (a->rows == 1 || (a->x_stride * size % 16 == 0 && a->codes_stride % v == 0));
+    // A row that four loads a lane of one wave cover is that wave's; longer ones take four waves.
+    const bool one = a->cols <= 4u * kWave * (wide ? v : 1);
+    const void* fn = !wide ? (one ? OP_BY_TYPE(a->dtype, k_quantize_rows, 1, 1) : OP_BY_TYPE(a->dtype, k_quantize_rows, 1, 4))
+                     : one ? quantize_wide_fn<1>(a->dtype) : quantize_wide_fn<4>(a->dtype);
+    return op_launch(fn, dim3(one ? (a->rows + kWaves - 1) / kWaves : a->rows), dim3(kBlock), 0, stream, k);
 }
 
 int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {

@@ -75,30 +75,32 @@ def _done(code: int, what: str) -> None:
         raise ffi.BackendError(ffi.BackendResult.from_code(code), what)
 
 
-def _check(op: str, device, name: str, t, dtype, shape) -> None:
-    """t is a tensor on `device` of this type and shape (None: any size)."""
+def _check(op: str, device: int, name: str, t, dtype, shape) -> None:
+    """t is a tensor on GPU `device` of this type and shape (None: any size)."""
     if not isinstance(t, torch.Tensor):
         _refuse(f"{op}: {name} is not a tensor")
-    if t.device != device:
-        _refuse(f"{op}: {name} is on {t.device}, not on {device}")
-    if t.dtype != dtype:
+    if t.get_device() != device:
+        _refuse(f"{op}: {name} is on {t.device}, not on GPU {device}")
+    if t.dtype is not dtype:
         _refuse(f"{op}: {name} is {t.dtype}, not {dtype}")
-    if len(t.shape) != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape)):
+    if t.shape != shape and (len(t.shape) != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape))):
         _refuse(f"{op}: {name} has shape {tuple(t.shape)}, not {tuple('*' if w is None else w for w in shape)}")
 
 
-def _device(op: str, t):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+def _device(op: str, t) -> int:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _refuse(f"{op}: tensors on a GPU are needed")
-    return t.device
+    return t.get_device()
 
 
-def _stream(stream: Optional[int], device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+def _stream(stream: Optional[int], device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
 
 
-def _row_stride(op: str, name: str, t) -> int:
-    """Elements from a row of t [rows, ..., width] to the next, whose rows are contiguous."""
+def _row_stride(op: str, name: str, t, width: int) -> int:
+    """Elements from a row of t [rows, ...] to the next, whose rows are contiguous and of `width` elements."""
+    if t.is_contiguous():
+        return width
     shape, strides = t.shape, t.stride()
     want = 1
     for i in range(len(shape) - 1, 0, -1):
@@ -108,35 +110,38 @@ def _row_stride(op: str, name: str, t) -> int:
     return strides[0] if shape[0] > 1 else want
 
 
-def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, torch.Tensor]:
+def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, torch.Tensor, int]:
     device = _device(op, q)
     if q.dtype not in DTYPES or q.dim() != 3:
         _refuse(f"{op}: q [rows, key heads, dk] is bfloat16, float16 or float32")
-    T, hk, dk = q.shape
-    _check(op, device, "k", k, q.dtype, (T, hk, dk))
-    _check(op, device, "v", v, q.dtype, (T, None, None))
-    hv, dv = v.shape[1:]
+    dtype = q.dtype
+    T, hk, dk = shape = q.shape
+    _check(op, device, "k", k, dtype, shape)
+    _check(op, device, "v", v, dtype, (T, None, None))
+    _, hv, dv = shape = v.shape
     _check(op, device, "g", g, torch.float32, (T, hv))
     _check(op, device, "beta", beta, torch.float32, (T, hv))
     if out is None:
-        out = torch.empty((T, hv, dv), dtype=q.dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=q.device)
     else:
-        _check(op, device, "out", out, q.dtype, (T, hv, dv))
-    a = DeltaRows(DTYPES[q.dtype], T, hk, hv, dk, dv, NORMALIZE if normalize else 0,
-                  dk ** -0.5 if scale is None and dk else scale or 0.0, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  out.data_ptr(), _row_stride(op, "q", q), _row_stride(op, "k", k), _row_stride(op, "v", v),
-                  _row_stride(op, "out", out), g.data_ptr(), beta.data_ptr(), _row_stride(op, "g", g),
-                  _row_stride(op, "beta", beta))
-    return a, out
+        _check(op, device, "out", out, dtype, shape)
+    wk, wv = hk * dk, hv * dv
+    if scale is None:
+        scale = dk ** -0.5 if dk else 0.0
+    a = DeltaRows(DTYPES[dtype], T, hk, hv, dk, dv, NORMALIZE if normalize else 0, scale, q.data_ptr(), k.data_ptr(),
+                  v.data_ptr(), out.data_ptr(), _row_stride(op, "q", q, wk), _row_stride(op, "k", k, wk),
+                  _row_stride(op, "v", v, wv), _row_stride(op, "out", out, wv), g.data_ptr(), beta.data_ptr(),
+                  _row_stride(op, "g", g, hv), _row_stride(op, "beta", beta, hv))
+    return a, out, device
 
 
-def _pool(op: str, device, name: str, t, a: DeltaRows) -> None:
+def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
     _check(op, device, name, t, torch.float32, (None, a.hv, a.dk, a.dv))
     if not t.is_contiguous():
         _refuse(f"{op}: {name} is not contiguous")
 
 
-def _slots(op: str, device, slots, n: int) -> Optional[int]:
+def _slots(op: str, device: int, slots, n: int) -> Optional[int]:
     if slots is None:
         return None
     _check(op, device, "slots", slots, torch.int32, (n,))
@@ -159,8 +164,7 @@ def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[f
     one projection's output), by whole 16 bytes.
     """
     op = "delta_step"
-    a, out = _rows(op, q, k, v, g, beta, out, scale, normalize)
-    device = q.device
+    a, out, device = _rows(op, q, k, v, g, beta, out, scale, normalize)
     _pool(op, device, "states", states, a)
     code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
                                         _slots(op, device, slots, a.rows), _stream(stream, device))
@@ -187,8 +191,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     meanwhile (allocated if None).
     """
     op = "delta_chunk"
-    a, out = _rows(op, q, k, v, g, beta, out, scale, normalize)
-    device = q.device
+    a, out, device = _rows(op, q, k, v, g, beta, out, scale, normalize)
     _check(op, device, "cu_seqlens", cu_seqlens, torch.int32, (None,))
     n = cu_seqlens.shape[0] - 1
     if n < 0 or not cu_seqlens.is_contiguous():
@@ -203,7 +206,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     L = _load()
     need = L.redukt_op_delta_chunk_workspace(ctypes.byref(a), n)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     else:
         _check(op, device, "workspace", workspace, torch.uint8, (None,))
     code = L.redukt_op_delta_chunk(ctypes.byref(a), cu_seqlens.data_ptr(), n,
@@ -227,17 +230,17 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
     rows, cols = x.shape
     if codes is None:
-        codes = torch.empty((rows, cols), dtype=torch.int8, device=device)
+        codes = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
     else:
         _check(op, device, "codes", codes, torch.int8, (rows, cols))
     if scales is None:
-        scales = torch.empty((rows,), dtype=torch.float32, device=device)
+        scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
     else:
         _check(op, device, "scales", scales, torch.float32, (rows,))
         if not scales.is_contiguous():
             _refuse(f"{op}: scales is not contiguous")
-    a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x), codes.data_ptr(),
-                     _row_stride(op, "codes", codes), scales.data_ptr())
+    a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
+                     _row_stride(op, "codes", codes, cols), scales.data_ptr())
     _done(_load().redukt_op_quantize_rows(ctypes.byref(a), _stream(stream, device)), op)
     return codes, scales
 
@@ -264,13 +267,13 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
     if out is None:
         if dtype not in DTYPES:
             _refuse(f"{op}: dtype is bfloat16, float16 or float32")
-        out = torch.empty((m, n), dtype=dtype, device=device)
+        out = torch.empty((m, n), dtype=dtype, device=x.device)
     else:
         if out.dtype not in DTYPES:
             _refuse(f"{op}: out is bfloat16, float16 or float32")
         _check(op, device, "out", out, out.dtype, (m, n))
-    a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x), x_scales.data_ptr(), w.data_ptr(),
-                   _row_stride(op, "w", w), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
-                   out.data_ptr(), _row_stride(op, "out", out))
+    a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
+                   _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                   out.data_ptr(), _row_stride(op, "out", out, n))
     _done(_load().redukt_op_int8_matmul(ctypes.byref(a), _stream(stream, device)), op)
     return out
