@@ -373,6 +373,28 @@ __device__ __forceinline__ void store_triangle(const float* m, const float* f, u
     }
 }
 
+// v moved between lanes by the DPP control CTRL, 0 where a lane has no source or its row is not in ROWS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// The sum of the lanes up to each one: within rows of 16, then the rows' last lanes into those behind them.
+__device__ __forceinline__ double prefix_sum(double v) {
+    v = dpp_add<0x111, 0xF>(v);                // row_shr 1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);                // row_bcast 15 into rows 1 and 3
+    return dpp_add<0x143, 0xC>(v);             // row_bcast 31 into rows 2 and 3
+}
+
+// 2^x by the hardware (1 ulp; what is below 2^-126 becomes 0).
+__device__ __forceinline__ float exp2_hw(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
 // One workgroup a chunk and value head: its unit, and with a key head's first value head the fragments of k^T.
 // Bound by the chain of its steps (a read from memory, the products, the solve by blocks of 16, 32 and 64), so it
 // asks for all of its inputs at once, and several workgroups share a CU.
@@ -408,6 +430,11 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
         const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ;
         const auto rk = rows_rsrc((const unsigned char*)r.k + (size_t)t0 * ks + (size_t)hq * DK * SZ, (len - 1) * ks + DK * SZ);
         const auto rq = rows_rsrc((const unsigned char*)r.q + (size_t)t0 * qs + (size_t)hq * DK * SZ, (len - 1) * qs + DK * SZ);
+        float g0 = 0.0f, beta = 0.0f;
+        if (wave == 0 && (uint32_t)lane < len) {
+            g0 = r.g[(int64_t)(t0 + lane) * r.g_stride + h];
+            beta = r.beta[(int64_t)(t0 + lane) * r.beta_stride + h];
+        }
         u32x4 kv[kLoads], qv[kLoads];
         constexpr int kPer = DK * SZ / 16;     // 16 bytes each
 #pragma unroll
@@ -416,28 +443,17 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
             kv[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(id / kPer * ks + id % kPer * 16), 0, 0);
             qv[u] = __builtin_amdgcn_raw_buffer_load_b128(rq, (int)(id / kPer * qs + id % kPer * 16), 0, 0);
         }
-        float g0 = 0.0f, beta = 0.0f;
-        if (wave == 0 && (uint32_t)lane < len) {
-            g0 = r.g[(int64_t)(t0 + lane) * r.g_stride + h];
-            beta = r.beta[(int64_t)(t0 + lane) * r.beta_stride + h];
+        if (wave == 0) {
+            // (a token whose g or beta is not finite is marked by a NaN beta; decays are kept as logarithms to base 2)
+            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff());
+            sG[lane] = prefix_sum(bad ? 0.0 : (double)fmaxf(g0, -1e5f) * 1.4426950408889634);
+            sB[lane] = bad ? __builtin_nanf("") : beta;
         }
 #pragma unroll
         for (int u = 0; u < kLoads; u++) {
             const int id = u * 256 + threadIdx.x;
             *(u32x4*)((unsigned char*)sK + id / kPer * (PK * SZ) + id % kPer * 16) = kv[u];
             *(u32x4*)((unsigned char*)sQ + id / kPer * (PK * SZ) + id % kPer * 16) = qv[u];
-        }
-        if (wave == 0) {
-            // (a token whose g or beta is not finite is marked by a NaN beta)
-            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff());
-            double g = bad ? 0.0 : (double)fmaxf(g0, -1e5f);
-#pragma unroll
-            for (int o = 1; o < kWave; o <<= 1) {
-                const double v = __shfl_up(g, o, kWave);
-                if (lane >= o) g += v;
-            }
-            sG[lane] = g;
-            sB[lane] = bad ? __builtin_nanf("") : beta;
         }
     }
     __syncthreads();
@@ -492,26 +508,42 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     if (wave == 0) {
         float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
         const double last = sG[kChunk - 1];
-        const float eg = expf((float)sG[lane]), u = sU[lane];
-        sW[lane] = lane < past ? u * expf((float)(last - sG[lane])) : 0.0f;
+        const float eg = exp2_hw(sG[lane]), u = sU[lane];
+        sW[lane] = lane < past ? u * exp2_hw(last - sG[lane]) : 0.0f;
         vec[lane] = lane < past ? u * eg : __builtin_nanf("");
         vec[kChunk + lane] = sP[lane] * eg;
-        vec[2 * kChunk + lane] = expf((float)last);
+        vec[2 * kChunk + lane] = exp2_hw(last);
     }
     f32x4 vp[4] = {};
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int tj = 16 * j + l16;
+    {
+        double gi[4];
+        float bi[4], pi[4];
 #pragma unroll
         for (int x = 0; x < 4; x++) {
             const int ti = 16 * wave + 4 * g4 + x;
-            float va = 0.0f;
-            if (j <= wave && tj <= ti && ti < past) {
-                const float w = expf((float)(sG[ti] - sG[tj])) * sU[tj];
-                va = tj < ti ? sB[ti] * sU[ti] * w * kk[j][x] : 0.0f;
-                vp[j][x] = sP[ti] * w * qk[j][x];
+            gi[x] = sG[ti];
+            bi[x] = ti < past ? sB[ti] * sU[ti] : 0.0f;
+            pi[x] = ti < past ? sP[ti] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int tj = 16 * j + l16;
+            if (j > wave) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + tj] = 0.0f;
+                continue;
             }
-            sA[ti * kPitchA + tj] = va;
+            const double gj = sG[tj];
+            const float uj = tj < past ? sU[tj] : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                // (from a token that is not finite on the products are not looked at, and nothing before it is reached)
+                const int ti = 16 * wave + 4 * g4 + x;
+                const float w = exp2_hw(gi[x] - gj) * uj;
+                const bool in = tj <= ti && ti < past;
+                sA[ti * kPitchA + tj] = in && tj < ti ? bi[x] * w * kk[j][x] : 0.0f;
+                vp[j][x] = in ? pi[x] * w * qk[j][x] : 0.0f;
+            }
         }
     }
     __syncthreads();
