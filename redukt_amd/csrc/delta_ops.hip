@@ -264,7 +264,8 @@ struct ChunkArgs {
     DeltaArgs d;
     unsigned char* ws;         // units: (value head, chunk slot)
     unsigned char* kt;         // fragments of k^T: (key head, chunk slot)
-    uint32_t slots;
+    uint32_t slots;            // chunk slots
+    uint32_t per;              // value heads of a workgroup of k_delta_prep
 };
 
 // Sequence i's rows, within [0, rows].
@@ -395,7 +396,8 @@ __device__ __forceinline__ double prefix_sum(double v) {
 // 2^x by the hardware (1 ulp; what is below 2^-126 becomes 0).
 __device__ __forceinline__ float exp2_hw(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// One workgroup a chunk and value head: its unit, and with a key head's first value head the fragments of k^T.
+// One workgroup a chunk and `per` value heads of one key head: their units, and with a key head's first value head the
+// fragments of k^T.
 // Bound by the chain of its steps (a read from memory, the products, the solve by blocks of 16, 32 and 64), so it
 // asks for all of its inputs at once, and several workgroups share a CU.
 template <typename T, int DK>
@@ -413,7 +415,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     float* const sT = sA + kChunk * kPitchA;
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
-    const uint32_t slot = blockIdx.x / r.hv, h = blockIdx.x % r.hv, group = r.hv / r.hk, hq = h / group;
+    const uint32_t slots_h = r.hv / a.per, slot = blockIdx.x / slots_h, h0 = blockIdx.x % slots_h * a.per, group = r.hv / r.hk, hq = h0 / group;
     uint32_t lo = 0, hi = a.d.n - 1;           // the last sequence that starts at this slot or before
     while (lo < hi) {
         const uint32_t mid = (lo + hi + 1) / 2;
@@ -426,15 +428,26 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     if (t0_ >= e) return;
     const uint32_t t0 = (uint32_t)t0_, len = min(e - t0, (uint32_t)kChunk);
 
-    {   // rows past the chunk's end as zeros
-        const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ;
-        const auto rk = rows_rsrc((const unsigned char*)r.k + (size_t)t0 * ks + (size_t)hq * DK * SZ, (len - 1) * ks + DK * SZ);
-        const auto rq = rows_rsrc((const unsigned char*)r.q + (size_t)t0 * qs + (size_t)hq * DK * SZ, (len - 1) * qs + DK * SZ);
-        float g0 = 0.0f, beta = 0.0f;
+    float g0 = 0.0f, beta = 0.0f;              // of token `lane` and one value head, in wave 0
+    const auto load_gates = [&](uint32_t h) {
         if (wave == 0 && (uint32_t)lane < len) {
             g0 = r.g[(int64_t)(t0 + lane) * r.g_stride + h];
             beta = r.beta[(int64_t)(t0 + lane) * r.beta_stride + h];
         }
+    };
+    const auto put_gates = [&]() {
+        if (wave == 0) {
+            // (a token whose g or beta is not finite is marked by a NaN beta; decays are kept as logarithms to base 2)
+            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff());
+            sG[lane] = prefix_sum(bad ? 0.0 : (double)fmaxf(g0, -1e5f) * 1.4426950408889634);
+            sB[lane] = bad ? __builtin_nanf("") : beta;
+        }
+    };
+    {   // rows past the chunk's end as zeros
+        const uint32_t ks = (uint32_t)r.k_stride * SZ, qs = (uint32_t)r.q_stride * SZ;
+        const auto rk = rows_rsrc((const unsigned char*)r.k + (size_t)t0 * ks + (size_t)hq * DK * SZ, (len - 1) * ks + DK * SZ);
+        const auto rq = rows_rsrc((const unsigned char*)r.q + (size_t)t0 * qs + (size_t)hq * DK * SZ, (len - 1) * qs + DK * SZ);
+        load_gates(h0);
         u32x4 kv[kLoads], qv[kLoads];
         constexpr int kPer = DK * SZ / 16;     // 16 bytes each
 #pragma unroll
@@ -443,12 +456,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
             kv[u] = __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(id / kPer * ks + id % kPer * 16), 0, 0);
             qv[u] = __builtin_amdgcn_raw_buffer_load_b128(rq, (int)(id / kPer * qs + id % kPer * 16), 0, 0);
         }
-        if (wave == 0) {
-            // (a token whose g or beta is not finite is marked by a NaN beta; decays are kept as logarithms to base 2)
-            const bool bad = !(g0 < __builtin_inff()) || !(fabsf(beta) < __builtin_inff());
-            sG[lane] = prefix_sum(bad ? 0.0 : (double)fmaxf(g0, -1e5f) * 1.4426950408889634);
-            sB[lane] = bad ? __builtin_nanf("") : beta;
-        }
+        put_gates();
 #pragma unroll
         for (int u = 0; u < kLoads; u++) {
             const int id = u * 256 + threadIdx.x;
@@ -486,7 +494,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
         sU[16 * wave + l16] = norm ? rsqrtf(k2 + kUnitEps) + 0.0f * k2 : 1.0f + 0.0f * k2;
         sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
     }
-    if (h % group == 0) {
+    if (h0 % group == 0) {
         // row l16 of k^T's tile p (as the state's rows), the tokens 32 s + 8 g + [0, 8)
         unsigned char* const kt = a.kt + ((size_t)hq * a.slots + slot) * kt_bytes(DK, LI);
         for (int f = wave; f < DK / 16 * 2; f += 4) {
@@ -501,139 +509,150 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     }
     __syncthreads();                           // k and q are done with; sU, sP are written
 
-    unsigned char* const unit = a.ws + ((size_t)h * a.slots + slot) * unit_bytes(LO);
-    // from the first token `past` whose key, g or beta is not finite on there are no rows
-    const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
-    const int past = bads ? __builtin_ctzll(bads) : kChunk;
-    if (wave == 0) {
-        float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
-        const double last = sG[kChunk - 1];
-        const float eg = exp2_hw(sG[lane]), u = sU[lane];
-        sW[lane] = lane < past ? u * exp2_hw(last - sG[lane]) : 0.0f;
-        vec[lane] = lane < past ? u * eg : __builtin_nanf("");
-        vec[kChunk + lane] = sP[lane] * eg;
-        vec[2 * kChunk + lane] = exp2_hw(last);
-    }
-    f32x4 vp[4] = {};
-    {
-        double gi[4];
-        float bi[4], pi[4];
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const int ti = 16 * wave + 4 * g4 + x;
-            gi[x] = sG[ti];
-            bi[x] = ti < past ? sB[ti] * sU[ti] : 0.0f;
-            pi[x] = ti < past ? sP[ti] : 0.0f;
+    int here = threadIdx.x;
+    for (uint32_t h = h0; h < h0 + a.per; h++) {
+        asm volatile("" : "+v"(here));          // (addresses are made anew for each head: kept, they would take 80 registers)
+        const int lane = here % kWave, g4 = lane / 16, l16 = lane % 16;
+        if (h > h0) {
+            __syncthreads();                   // the last head's fragments have been read
+            put_gates();
+            __syncthreads();
         }
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int tj = 16 * j + l16;
-            if (j > wave) {
-#pragma unroll
-                for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + tj] = 0.0f;
-                continue;
-            }
-            const double gj = sG[tj];
-            const float uj = tj < past ? sU[tj] : 0.0f;
+        if (h + 1 < h0 + a.per) load_gates(h + 1);
+        unsigned char* const unit = a.ws + ((size_t)h * a.slots + slot) * unit_bytes(LO);
+        // from the first token `past` whose key, g or beta is not finite on there are no rows
+        const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
+        const int past = bads ? __builtin_ctzll(bads) : kChunk;
+        if (wave == 0) {
+            float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
+            const double last = sG[kChunk - 1];
+            const float eg = exp2_hw(sG[lane]), u = sU[lane];
+            sW[lane] = lane < past ? u * exp2_hw(last - sG[lane]) : 0.0f;
+            vec[lane] = lane < past ? u * eg : __builtin_nanf("");
+            vec[kChunk + lane] = sP[lane] * eg;
+            vec[2 * kChunk + lane] = exp2_hw(last);
+        }
+        f32x4 vp[4] = {};
+        {
+            double gi[4];
+            float bi[4], pi[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                // (from a token that is not finite on the products are not looked at, and nothing before it is reached)
                 const int ti = 16 * wave + 4 * g4 + x;
-                const float w = exp2_hw(gi[x] - gj) * uj;
-                const bool in = tj <= ti && ti < past;
-                sA[ti * kPitchA + tj] = in && tj < ti ? bi[x] * w * kk[j][x] : 0.0f;
-                vp[j][x] = in ? pi[x] * w * qk[j][x] : 0.0f;
-            }
-        }
-    }
-    __syncthreads();
-    {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
-        const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
-        float t[16];
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v0 = i == l16 ? 1.0f : 0.0f, v1 = 0.0f;
-#pragma unroll
-            for (int j = 0; j < i; j++) {
-                if (j % 2) v1 -= A[i * kPitchA + j] * t[j];
-                else v0 -= A[i * kPitchA + j] * t[j];
-            }
-            t[i] = v0 + v1;
-        }
-        float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
-        if (g4 == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
-        }
-    }
-    __syncthreads();
-    // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
-    const auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
-    if (wave < 2) {
-        const int i = 2 * wave + 1, j = 2 * wave;
-        f32x4 m = {}, y = {};
-#pragma unroll
-        for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
-#pragma unroll
-        for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
-#pragma unroll
-        for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
-    } else {   // the upper blocks within 32, which the fragments cover
-        const int i = 2 * (wave - 2);
-#pragma unroll
-        for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
-    }
-    __syncthreads();
-    {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
-        const int i = wave / 2, j = wave % 2;
-        f32x4 y = {};
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-            if (p > i) break;
-            f32x4 m = {};
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                if (q < j) continue;
-#pragma unroll
-                for (int s = 0; s < 4; s++) m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+                gi[x] = sG[ti];
+                bi[x] = ti < past ? sB[ti] * sU[ti] : 0.0f;
+                pi[x] = ti < past ? sP[ti] : 0.0f;
             }
 #pragma unroll
-            for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
+            for (int j = 0; j < 4; j++) {
+                const int tj = 16 * j + l16;
+                if (j > wave) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + tj] = 0.0f;
+                    continue;
+                }
+                const double gj = sG[tj];
+                const float uj = tj < past ? sU[tj] : 0.0f;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    // (from a token that is not finite on the products are not looked at, and nothing before it is reached)
+                    const int ti = 16 * wave + 4 * g4 + x;
+                    const float w = exp2_hw(gi[x] - gj) * uj;
+                    const bool in = tj <= ti && ti < past;
+                    sA[ti * kPitchA + tj] = in && tj < ti ? bi[x] * w * kk[j][x] : 0.0f;
+                    vp[j][x] = in ? pi[x] * w * qk[j][x] : 0.0f;
+                }
+            }
         }
-        __syncthreads();                       // A is done with: P takes its place
+        __syncthreads();
+        {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
+            const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
+            float t[16];
 #pragma unroll
-        for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+            for (int i = 0; i < 16; i++) {
+                float v0 = i == l16 ? 1.0f : 0.0f, v1 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+                for (int j = 0; j < i; j++) {
+                    if (j % 2) v1 -= A[i * kPitchA + j] * t[j];
+                    else v0 -= A[i * kPitchA + j] * t[j];
+                }
+                t[i] = v0 + v1;
+            }
+            float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
+            if (g4 == 0) {
 #pragma unroll
-            for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
-    }
-    __syncthreads();
-    f32x4 y[4] = {};                           // rows 16 wave of P (I + A)^-1
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (j > wave) break;
-#pragma unroll
-        for (int k = j; k < 4; k++) {
-            if (k > wave) break;
-#pragma unroll
-            for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
+                for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
+            }
         }
-    }
-    __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
+        __syncthreads();
+        // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
+        const auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
+        if (wave < 2) {
+            const int i = 2 * wave + 1, j = 2 * wave;
+            f32x4 m = {}, y = {};
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float bj = 16 * j + l16 < past ? sB[16 * j + l16] : 0.0f;
+            for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-            const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
-            sA[at_] = y[j][x] * bj;
-            sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
+            for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+        } else {   // the upper blocks within 32, which the fragments cover
+            const int i = 2 * (wave - 2);
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
         }
+        __syncthreads();
+        {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
+            const int i = wave / 2, j = wave % 2;
+            f32x4 y = {};
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                if (p > i) break;
+                f32x4 m = {};
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    if (q < j) continue;
+#pragma unroll
+                    for (int s = 0; s < 4; s++) m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+                }
+#pragma unroll
+                for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
+            }
+            __syncthreads();                       // A is done with: P takes its place
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
+        }
+        __syncthreads();
+        f32x4 y[4] = {};                           // rows 16 wave of P (I + A)^-1
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > wave) break;
+#pragma unroll
+            for (int k = j; k < 4; k++) {
+                if (k > wave) break;
+#pragma unroll
+                for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
+            }
+        }
+        __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float bj = 16 * j + l16 < past ? sB[16 * j + l16] : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
+                sA[at_] = y[j][x] * bj;
+                sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
+            }
+        }
+        __syncthreads();
+        store_triangle<3>(sT, sW, unit, wave, lane);
+        store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
     }
-    __syncthreads();
-    store_triangle<3>(sT, sW, unit, wave, lane);
-    store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
 }
 
 // One workgroup takes 16 NC columns of one head's state through a sequence.  Waves 0 to 3 carry the state: each owns a
@@ -995,7 +1014,10 @@ uint64_t units_bytes(const redukt_delta_rows& a, uint32_t n_seq) {
 constexpr uint64_t kManyTiles = 1024;
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
-    const uint64_t prep = chunk_slots(r, k.d.n) * r.hv;
+    // Two value heads of one key head share its products where workgroups still fill the CUs twice over (129 chunks of 32 heads,
+    // two to a key head: 304 -> 289 us with k_delta_chunks).
+    if (r.hv / r.hk % 2 == 0 && chunk_slots(r, k.d.n) * r.hv >= 1024) k.per = 2;
+    const uint64_t prep = chunk_slots(r, k.d.n) * (r.hv / k.per);
     // Two column tiles a workgroup read a chunk's operands once for both, but a chunk then takes them 1.3 times as long: worth
     // it once there are workgroups waiting for a CU (37 ragged sequences of 16 heads of 128 columns 283 -> 231 us; one of
     // 32 heads, 256 tiles, 310 -> 369).
@@ -1100,7 +1122,7 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr, 0};
+    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr, 0, 1};
     return launch_chunks(k, stream);
 }
 
