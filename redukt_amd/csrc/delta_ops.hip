@@ -53,7 +53,7 @@ __device__ __forceinline__ float rows_sum(float v) {
 // Both sums over dk are formed from the state as it is read (S'^T q = a S^T q + (k.q) d), in one
 // exchange between the eight row groups.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a) {
+__global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
     constexpr int R = DK / 8;
     const redukt_delta_rows& r = a.r;
     const int lane = threadIdx.x % kWave, rg = lane / 8, c4 = (lane % 8) * 4;
@@ -63,75 +63,62 @@ __global__ __launch_bounds__(256) void k_delta_rows(DeltaArgs a) {
     if (i >= a.n) return;
     const uint32_t hb = (uint32_t)(id % (r.hv * blocks)), h = hb / blocks, col = hb % blocks * 32 + c4;
     const uint32_t hq = h / (r.hv / r.hk);
-    uint32_t t0 = i, t1 = i + 1;
-    if (a.cu) {
-        t0 = min((uint32_t)max(a.cu[i], 0), r.rows);
-        t1 = min((uint32_t)max(a.cu[i + 1], 0), r.rows);
-    }
-    const int slot = entry_slot(a.slots, a.n_slots, i, a.states != nullptr, lane);
+    const int slot = entry_slot(a.slots, a.n_slots, i, true, lane);
     if (slot == kSkip) return;
-    T* out = (T*)r.out + (size_t)h * r.dv + col;
+    T* const out = (T*)r.out + (int64_t)i * r.out_stride + (size_t)h * r.dv + col;
     if (slot == kBad) {
-        for (uint32_t t = t0 + rg; t < t1; t += 8)
-            for (int j = 0; j < 4; j++) out[(int64_t)t * r.out_stride + j] = (T)__builtin_nanf("");
+        for (int j = 0; j < 4; j++) out[j] = (T)__builtin_nanf("");
         return;
     }
-    const size_t at = (((size_t)slot * r.hv + h) * DK + rg * R) * r.dv + col;
+    float* const state = a.states + (((size_t)slot * r.hv + h) * DK + rg * R) * r.dv + col;
     float4 S[R];
 #pragma unroll
-    for (int e = 0; e < R; e++) S[e] = a.in ? *(const float4*)(a.in + at + (size_t)e * r.dv) : make_float4(0, 0, 0, 0);
-    for (uint32_t t = t0; t < t1; t++) {
-        float k[R], q[R], v[4];
-        op_load((const T*)r.k + (int64_t)t * r.k_stride + hq * DK + rg * R, k);
-        op_load((const T*)r.q + (int64_t)t * r.q_stride + hq * DK + rg * R, q);
-        op_load((const T*)r.v + (int64_t)t * r.v_stride + h * r.dv + col, v);
-        const float decay = expf(r.g[(int64_t)t * r.g_stride + h]), beta = r.beta[(int64_t)t * r.beta_stride + h];
-        float4 sk = make_float4(0, 0, 0, 0), sq = make_float4(0, 0, 0, 0);
-        float kk = 0, qq = 0, kq = 0;
+    for (int e = 0; e < R; e++) S[e] = *(const float4*)(state + (size_t)e * r.dv);
+    float k[R], q[R], v[4];
+    op_load((const T*)r.k + (int64_t)i * r.k_stride + hq * DK + rg * R, k);
+    op_load((const T*)r.q + (int64_t)i * r.q_stride + hq * DK + rg * R, q);
+    op_load((const T*)r.v + (int64_t)i * r.v_stride + h * r.dv + col, v);
+    const float decay = expf(r.g[(int64_t)i * r.g_stride + h]), beta = r.beta[(int64_t)i * r.beta_stride + h];
+    float4 sk = make_float4(0, 0, 0, 0), sq = make_float4(0, 0, 0, 0);
+    float kk = 0, qq = 0, kq = 0;
 #pragma unroll
-        for (int e = 0; e < R; e++) {
-            sk.x += k[e] * S[e].x, sk.y += k[e] * S[e].y, sk.z += k[e] * S[e].z, sk.w += k[e] * S[e].w;
-            sq.x += q[e] * S[e].x, sq.y += q[e] * S[e].y, sq.z += q[e] * S[e].z, sq.w += q[e] * S[e].w;
-            kk += k[e] * k[e], qq += q[e] * q[e], kq += k[e] * q[e];
-        }
-        sk.x = rows_sum(sk.x), sk.y = rows_sum(sk.y), sk.z = rows_sum(sk.z), sk.w = rows_sum(sk.w);
-        sq.x = rows_sum(sq.x), sq.y = rows_sum(sq.y), sq.z = rows_sum(sq.z), sq.w = rows_sum(sq.w);
-        kq = rows_sum(kq);
-        float uk = 1.0f, uq = r.scale;
-        if (r.flags & REDUKT_DELTA_NORMALIZE) {
-            uk = rsqrtf(rows_sum(kk) + kUnitEps);
-            uq *= rsqrtf(rows_sum(qq) + kUnitEps);
-        }
-        // d carries the key's factor, so that the rows of k enter as they are
-        const float ak = decay * uk;
-        const float4 d = make_float4(beta * (v[0] - ak * sk.x) * uk, beta * (v[1] - ak * sk.y) * uk,
-                                     beta * (v[2] - ak * sk.z) * uk, beta * (v[3] - ak * sk.w) * uk);
-#pragma unroll
-        for (int e = 0; e < R; e++) {
-            S[e].x = decay * S[e].x + k[e] * d.x;
-            S[e].y = decay * S[e].y + k[e] * d.y;
-            S[e].z = decay * S[e].z + k[e] * d.z;
-            S[e].w = decay * S[e].w + k[e] * d.w;
-        }
-        if (rg == 0) {
-            T* o = out + (int64_t)t * r.out_stride;
-            o[0] = (T)(uq * (decay * sq.x + kq * d.x));
-            o[1] = (T)(uq * (decay * sq.y + kq * d.y));
-            o[2] = (T)(uq * (decay * sq.z + kq * d.z));
-            o[3] = (T)(uq * (decay * sq.w + kq * d.w));
-        }
+    for (int e = 0; e < R; e++) {
+        sk.x += k[e] * S[e].x, sk.y += k[e] * S[e].y, sk.z += k[e] * S[e].z, sk.w += k[e] * S[e].w;
+        sq.x += q[e] * S[e].x, sq.y += q[e] * S[e].y, sq.z += q[e] * S[e].z, sq.w += q[e] * S[e].w;
+        kk += k[e] * k[e], qq += q[e] * q[e], kq += k[e] * q[e];
     }
-    if (a.states) {
+    sk.x = rows_sum(sk.x), sk.y = rows_sum(sk.y), sk.z = rows_sum(sk.z), sk.w = rows_sum(sk.w);
+    sq.x = rows_sum(sq.x), sq.y = rows_sum(sq.y), sq.z = rows_sum(sq.z), sq.w = rows_sum(sq.w);
+    kq = rows_sum(kq);
+    float uk = 1.0f, uq = r.scale;
+    if (r.flags & REDUKT_DELTA_NORMALIZE) {
+        uk = rsqrtf(rows_sum(kk) + kUnitEps);
+        uq *= rsqrtf(rows_sum(qq) + kUnitEps);
+    }
+    // d carries the key's factor, so that the rows of k enter as they are
+    const float ak = decay * uk;
+    const float4 d = make_float4(beta * (v[0] - ak * sk.x) * uk, beta * (v[1] - ak * sk.y) * uk, beta * (v[2] - ak * sk.z) * uk,
+                                 beta * (v[3] - ak * sk.w) * uk);
 #pragma unroll
-        for (int e = 0; e < R; e++) *(float4*)(a.states + at + (size_t)e * r.dv) = S[e];
+    for (int e = 0; e < R; e++) {
+        S[e].x = decay * S[e].x + k[e] * d.x;
+        S[e].y = decay * S[e].y + k[e] * d.y;
+        S[e].z = decay * S[e].z + k[e] * d.z;
+        S[e].w = decay * S[e].w + k[e] * d.w;
+        *(float4*)(state + (size_t)e * r.dv) = S[e];
+    }
+    if (rg == 0) {
+        typedef T out4 __attribute__((ext_vector_type(4)));
+        *(out4*)out = out4{(T)(uq * (decay * sq.x + kq * d.x)), (T)(uq * (decay * sq.y + kq * d.y)),
+                           (T)(uq * (decay * sq.z + kq * d.z)), (T)(uq * (decay * sq.w + kq * d.w))};
     }
 }
 
-const void* delta_rows_fn(uint32_t dtype, uint32_t dk) {
+const void* delta_step_fn(uint32_t dtype, uint32_t dk) {
     static const void* const fns[3][2] = {
-        {(const void*)k_delta_rows<__bf16, 64>, (const void*)k_delta_rows<__bf16, 128>},
-        {(const void*)k_delta_rows<_Float16, 64>, (const void*)k_delta_rows<_Float16, 128>},
-        {(const void*)k_delta_rows<float, 64>, (const void*)k_delta_rows<float, 128>},
+        {(const void*)k_delta_step<__bf16, 64>, (const void*)k_delta_step<__bf16, 128>},
+        {(const void*)k_delta_step<_Float16, 64>, (const void*)k_delta_step<_Float16, 128>},
+        {(const void*)k_delta_step<float, 64>, (const void*)k_delta_step<float, 128>},
     };
     return fns[dtype][dk == 128];
 }
@@ -734,12 +721,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         for (int n = 0; n < N; n++) o.l[n] = *(const bf16x8*)(from[n] + lane * 16);
         return o;
     };
-    // Fragment 0 of a triangle is this wave's tile and tokens [0, 32), 1 tokens [32, 64): zeros for waves 0 and 1, by a
-    // buffer without bytes.
+    // Fragments of the workspace, by their number from p on.  Of a triangle, the first is this wave's tile and tokens [0, 32), the
+    // second tokens [32, 64): zeros for waves 0 and 1, by a buffer without bytes.
     const int f0 = wave < 2 ? wave : 2 * wave - 2;
-    const auto frag1 = [&](const unsigned char* p) {
-        return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(p, wave < 2 ? 0 : kFrag), lane * 16, 0, 0));
+    const auto frag = [&](const unsigned char* p, uint32_t bytes, int first) {
+        return __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(p, bytes), lane * 16, first * kFrag, 0));
     };
+    const uint32_t frag1 = wave < 2 ? 0 : unit_bytes(LO);
     const uint32_t row4 = tile_index(wave, 4 * g4);        // the first of a lane's four tokens
     const auto bad_of = [&](int nc) {                      // the column's first token that is not finite
         const int4 v = *(const int4*)sBad[nc][l16];
@@ -749,8 +737,10 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     if (wave_index() < 4) {
         __builtin_amdgcn_s_setprio(3);
         const size_t at = ((size_t)slot * r.hv + h) * DK * r.dv;
+        int here = lane;
         const auto state_at = [&](int nc, int p, int x) {
-            return at + (size_t)state_index<DK>(NW * wave + p, 4 * g4 + x) * r.dv + col_of(nc);
+            const uint32_t c = col0 - l16 + here % 16 + 16 * nc;
+            return at + (size_t)state_index<DK>(NW * wave + p, 4 * (here / 16) + x) * r.dv + (c < r.dv ? c : here % 16);
         };
         f32x4 S[NC][NW];
 #pragma unroll
@@ -779,19 +769,20 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             for (int nc = 0; nc < NC; nc++)
 #pragma unroll
                 for (int x = 0; x < 4; x++) vv[nc][x] = buffer_bits<T>(rsrc, (row4 + x) * rv.stride + col_of(nc) * SZ);
-            kd = *(const f32x4*)(unit + kTri * (3 + LO) * kFrag + row4 * 4);
+            kd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(unit, unit_bytes(LO)), (int)row4 * 4,
+                                                                                 kTri * (3 + LO) * kFrag, 0));
         };
         const auto load_t = [&]() {
 #pragma unroll
-            for (int n = 0; n < 3; n++) tf[0][n] = *(const bf16x8*)(unit + (f0 * 3 + n) * kFrag + lane * 16);
+            for (int n = 0; n < 3; n++) tf[0][n] = frag(unit, unit_bytes(LO), f0 * 3 + n);
 #pragma unroll
-            for (int n = 0; n < 3; n++) tf[1][n] = frag1(unit + (f0 * 3 + 3 + n) * kFrag);
+            for (int n = 0; n < 3; n++) tf[1][n] = frag(unit, frag1, f0 * 3 + 3 + n);
         };
         const auto load_kt = [&]() {
 #pragma unroll
             for (int f = 0; f < NW * 2; f++)
 #pragma unroll
-                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = *(const bf16x8*)(kt + (f * LI + n) * kFrag + lane * 16);
+                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = frag(kt, NW * 2 * LI * kFrag, f * LI + n);
             keep = ((const float*)(unit + kTri * (3 + LO) * kFrag))[2 * kChunk];
         };
         // The four rows of this wave's tile that a lane holds, as half of a right operand's fragment.
@@ -903,6 +894,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             load_kt();
         }
         if (a.d.states) {
+            asm volatile("" : "+v"(here));     // (the addresses are made anew: kept from the start, they would take 16 registers)
 #pragma unroll
             for (int nc = 0; nc < NC; nc++)
 #pragma unroll
@@ -921,14 +913,14 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             const auto rsrc = rq.rsrc(rows);
 #pragma unroll
             for (int s = 0; s < 4; s++) qf[s] = loadK(rsrc, q_at + 4 * KF * s * SZ);
-            qd = *(const f32x4*)(unit + kTri * (3 + LO) * kFrag + (kChunk + row4) * 4);
+            qd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(unit, unit_bytes(LO)), (int)row4 * 4,
+                                                                                 kTri * (3 + LO) * kFrag + kChunk * 4, 0));
         };
         const auto load_p = [&]() {
-            const unsigned char* const u = unit + kTri * 3 * kFrag;
 #pragma unroll
-            for (int n = 0; n < LO; n++) pf[0][n] = *(const bf16x8*)(u + (f0 * LO + n) * kFrag + lane * 16);
+            for (int n = 0; n < LO; n++) pf[0][n] = frag(unit, unit_bytes(LO), kTri * 3 + f0 * LO + n);
 #pragma unroll
-            for (int n = 0; n < LO; n++) pf[1][n] = frag1(u + (f0 * LO + LO + n) * kFrag);
+            for (int n = 0; n < LO; n++) pf[1][n] = frag(unit, frag1, kTri * 3 + f0 * LO + LO + n);
         };
         uint32_t left = e - b;
         if (chunks) {
@@ -995,14 +987,17 @@ const void* delta_prep_fn(uint32_t dtype, uint32_t dk) {
     return fns[dtype][dk == 128];
 }
 
-template <int NC>
-const void* delta_chunks_fn(uint32_t dtype, uint32_t dk) {
-    static const void* const fns[3][2] = {
-        {(const void*)k_delta_chunks<__bf16, 64, NC>, (const void*)k_delta_chunks<__bf16, 128, NC>},
-        {(const void*)k_delta_chunks<_Float16, 64, NC>, (const void*)k_delta_chunks<_Float16, 128, NC>},
-        {(const void*)k_delta_chunks<float, 64, NC>, (const void*)k_delta_chunks<float, 128, NC>},
-    };
-    return fns[dtype][dk == 128];
+template <typename T, int NC>
+const void* delta_chunks_of(uint32_t dk) {
+    return dk == 128 ? (const void*)k_delta_chunks<T, 128, NC> : (const void*)k_delta_chunks<T, 64, NC>;
+}
+
+// NC 1, 2, or 4, the last with 16-bit elements only (in f32 its limbs do not fit LDS).
+const void* delta_chunks_fn(uint32_t dtype, uint32_t dk, uint32_t nc) {
+    if (dtype == REDUKT_OP_F32) return nc == 1 ? delta_chunks_of<float, 1>(dk) : delta_chunks_of<float, 2>(dk);
+    if (dtype == REDUKT_OP_F16)
+        return nc == 1 ? delta_chunks_of<_Float16, 1>(dk) : nc == 2 ? delta_chunks_of<_Float16, 2>(dk) : delta_chunks_of<_Float16, 4>(dk);
+    return nc == 1 ? delta_chunks_of<__bf16, 1>(dk) : nc == 2 ? delta_chunks_of<__bf16, 2>(dk) : delta_chunks_of<__bf16, 4>(dk);
 }
 
 uint64_t chunk_slots(const redukt_delta_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / kChunk + n_seq; }
@@ -1011,17 +1006,17 @@ uint64_t units_bytes(const redukt_delta_rows& a, uint32_t n_seq) {
     return chunk_slots(a, n_seq) * a.hv * unit_bytes(a.dtype == REDUKT_OP_F32 ? 3 : 2);
 }
 
-constexpr uint64_t kManyTiles = 1024;
 int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const redukt_delta_rows& r = k.d.r;
     // Two value heads of one key head share its products where workgroups still fill the CUs twice over (129 chunks of 32 heads,
     // two to a key head: 304 -> 289 us with k_delta_chunks).
     if (r.hv / r.hk % 2 == 0 && chunk_slots(r, k.d.n) * r.hv >= 1024) k.per = 2;
     const uint64_t prep = chunk_slots(r, k.d.n) * (r.hv / k.per);
-    // Two column tiles a workgroup read a chunk's operands once for both, but a chunk then takes them 1.3 times as long: worth
-    // it once there are workgroups waiting for a CU (37 ragged sequences of 16 heads of 128 columns 283 -> 231 us; one of
-    // 32 heads, 256 tiles, 310 -> 369).
-    const uint32_t NC = (uint64_t)k.d.n * r.hv * (r.dv / 16) >= kManyTiles ? 2 : 1;
+    // NC column tiles a workgroup read a chunk's operands once for all of them, but a chunk then takes longer (256 tiles of 128
+    // chunks with 1, 2 and 4 tiles: 290, 369 and 516 us): worth it once there are workgroups waiting for a CU (37 ragged sequences
+    // of 16 heads of 128 columns, 4,736 tiles: 281, 225 and 208).
+    const uint64_t all = (uint64_t)k.d.n * r.hv * (r.dv / 16);
+    const uint32_t NC = all >= 4096 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
@@ -1031,7 +1026,7 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    return op_launch(NC == 2 ? delta_chunks_fn<2>(r.dtype, r.dk) : delta_chunks_fn<1>(r.dtype, r.dk), dim3((uint32_t)grid), dim3(512), 0, stream, k);
+    return op_launch(delta_chunks_fn(r.dtype, r.dk, NC), dim3((uint32_t)grid), dim3(512), 0, stream, k);
 }
 
 bool sizes_ok(const redukt_delta_rows* a) {
@@ -1071,10 +1066,10 @@ redukt_delta_rows stepped(redukt_delta_rows a) {
     return a;
 }
 
-int32_t launch_rows(DeltaArgs& k, void* stream) {
+int32_t launch_step(DeltaArgs& k, void* stream) {
     const uint64_t waves = (uint64_t)k.n * k.r.hv * (k.r.dv / 32);
     if ((waves + 3) / 4 > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
-    return op_launch(delta_rows_fn(k.r.dtype, k.r.dk), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, stream, k);
+    return op_launch(delta_step_fn(k.r.dtype, k.r.dk), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, stream, k);
 }
 
 }  // namespace
@@ -1093,7 +1088,7 @@ int32_t redukt_op_delta_step(const redukt_delta_rows* a, float* states, uint32_t
     OpDevice dev(a->out);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     DeltaArgs k{stepped(*a), states, states, n_slots, slots, nullptr, a->rows};
-    return launch_rows(k, stream);
+    return launch_step(k, stream);
 }
 
 uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_seq) {
