@@ -913,14 +913,14 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             const auto rsrc = rq.rsrc(rows);
 #pragma unroll
             for (int s = 0; s < 4; s++) qf[s] = loadK(rsrc, q_at + 4 * KF * s * SZ);
-            qd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(unit, unit_bytes(LO)), (int)row4 * 4,
-                                                                                 kTri * (3 + LO) * kFrag + kChunk * 4, 0));
         };
         const auto load_p = [&]() {
 #pragma unroll
             for (int n = 0; n < LO; n++) pf[0][n] = frag(unit, unit_bytes(LO), kTri * 3 + f0 * LO + n);
 #pragma unroll
             for (int n = 0; n < LO; n++) pf[1][n] = frag(unit, frag1, kTri * 3 + f0 * LO + LO + n);
+            qd = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rows_rsrc(unit, unit_bytes(LO)), (int)row4 * 4,
+                                                                                 kTri * (3 + LO) * kFrag + kChunk * 4, 0));
         };
         uint32_t left = e - b;
         if (chunks) {
@@ -933,7 +933,9 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             left -= on * kChunk;
             rq.step(on), ro.step(1);
             unit += on * unit_bytes(LO);
-            f32x4 O[NC] = {};
+            // What is read here stands still until the next A (X) and until the chain's first step behind C (S), so the work lies where
+            // the chain's own is long: Q S beside the second step, P X beside the fourth and first.
+            f32x4 O[NC], Q[NC][2] = {};
             __syncthreads();                   // A
 #pragma unroll
             for (int s = 0; s < 4; s++) {
@@ -945,20 +947,19 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                         const auto x = *(const typename Part<NW, LI>::vec*)(sS[nc][s][j] + lane * (KF * 2));
 #pragma unroll
                         for (int n = 0; n < LI; n++)
-                            if (n + j < LO) O[nc] = mma_part(q.l[n], x, O[nc]);
+                            if (n + j < LO) Q[nc][s % 2] = mma_part(q.l[n], x, Q[nc][s % 2]);
                     }
             }
-#pragma unroll
-            for (int nc = 0; nc < NC; nc++)
-#pragma unroll
-                for (int y = 0; y < 4; y++) O[nc][y] *= qd[y];
             load_q(min(left, (uint32_t)kChunk));
             __syncthreads();                   // B
+            __syncthreads();                   // C
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 const int bad = bad_of(nc);
-                O[nc] = mma_limbs<LO>(as_split<LO>(pf[0]), get(sX[nc][0], Int<LO>()), O[nc]);
-                O[nc] = mma_limbs<LO>(as_split<LO>(pf[1]), get(sX[nc][1], Int<LO>()), O[nc]);
+                O[nc] = mma_limbs<LO>(as_split<LO>(pf[0]), get(sX[nc][0], Int<LO>()), f32x4{});
+                const f32x4 y = mma_limbs<LO>(as_split<LO>(pf[1]), get(sX[nc][1], Int<LO>()), f32x4{});
+#pragma unroll
+                for (int z = 0; z < 4; z++) O[nc][z] = qd[z] * (Q[nc][0][z] + Q[nc][1][z]) + (O[nc][z] + y[z]);
                 if (__any(bad < kChunk)) {
 #pragma unroll
                     for (int y = 0; y < 4; y++)
@@ -973,7 +974,6 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 }
             }
             load_p();
-            __syncthreads();                   // C
         }
     }
 }

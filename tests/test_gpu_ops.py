@@ -212,6 +212,33 @@ def test_delta_chunk_heads(hk, hv, dk, dv, dtype):
     sequences([70, 1, 130], hk, hv, dk, dv, dtype, normalize=True, initial=False, seed=hv)
 
 
+@types
+@pytest.mark.parametrize("dk,dv", [(64, 128), (128, 160)])
+def test_delta_chunk_many_sequences(dk, dv, dtype):
+    """Enough sequences that a workgroup takes several column tiles, and several heads of the preparation: the same bits as
+    each sequence alone, and the rule's values."""
+    n, hk, hv = 66, 6, 12
+    lens = [(7 * i) % 61 + 70 * (i % 9 == 0) for i in range(n)]
+    T = sum(lens)
+    x = rule_inputs(T, hk, hv, dk, dv, dtype, seed=6, normalize=True)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    at = cu.tolist()
+    before = pool_of(n, hv, dk, dv)
+    after = torch.empty_like(before)
+    out = ops.delta_chunk(*x, cu, state_in=before, state_out=after, normalize=True)
+    for i in (0, 1, 9, 37, n - 1):
+        rows = slice(at[i], at[i + 1])
+        want, S, tol, S_tol = ops_f64.rule(*(t[rows] for t in x), before[i], normalize=True)
+        check(out[rows], want, tol, ("out", i))
+        check(after[i], S, S_tol, ("state", i))
+    for i in range(n):
+        rows = slice(at[i], at[i + 1])
+        one = torch.empty_like(before[:1])
+        alone = ops.delta_chunk(*(t[rows] for t in x), torch.tensor([0, lens[i]], dtype=torch.int32, device="cuda"),
+                                state_in=before[i:i + 1], state_out=one, normalize=True)
+        assert torch.equal(out[rows], alone) and torch.equal(after[i], one[0]), i
+
+
 @pytest.mark.parametrize("dtype,forget", [(BF16, 1.0), (F32, 1.0), (F32, 0.01), (BF16, 30.0)])
 def test_delta_chunk_long(dtype, forget):
     """Long memories and short ones (forget: the decays' factor) over some thousand tokens."""
