@@ -83,7 +83,8 @@ def _check(op: str, device: int, name: str, t, dtype, shape) -> None:
         _refuse(f"{op}: {name} is on {t.device}, not on GPU {device}")
     if t.dtype is not dtype:
         _refuse(f"{op}: {name} is {t.dtype}, not {dtype}")
-    if t.shape != shape and (len(t.shape) != len(shape) or any(w is not None and w != s for w, s in zip(shape, t.shape))):
+    got = t.shape
+    if got != shape and (len(got) != len(shape) or any(w is not None and w != s for w, s in zip(shape, got))):
         _refuse(f"{op}: {name} has shape {tuple(t.shape)}, not {tuple('*' if w is None else w for w in shape)}")
 
 
@@ -114,17 +115,26 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
     device = _device(op, q)
     if q.dtype not in DTYPES or q.dim() != 3:
         _refuse(f"{op}: q [rows, key heads, dk] is bfloat16, float16 or float32")
-    dtype = q.dtype
-    T, hk, dk = shape = q.shape
-    _check(op, device, "k", k, dtype, shape)
-    _check(op, device, "v", v, dtype, (T, None, None))
-    _, hv, dv = shape = v.shape
-    _check(op, device, "g", g, torch.float32, (T, hv))
-    _check(op, device, "beta", beta, torch.float32, (T, hv))
+    dtype, shape = q.dtype, q.shape
+    T, hk, dk = shape
+    try:       # (all at once; what is wrong is looked for only if something is)
+        wide, gates = v.shape, g.shape
+        fine = (k.shape == shape and wide[0] == T and gates == wide[:2] and beta.shape == gates and len(wide) == 3
+                and k.dtype is dtype and v.dtype is dtype and g.dtype is torch.float32 and beta.dtype is torch.float32
+                and k.get_device() == v.get_device() == g.get_device() == beta.get_device() == device)
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _check(op, device, "k", k, dtype, shape)
+        _check(op, device, "v", v, dtype, (T, None, None))
+        _check(op, device, "g", g, torch.float32, tuple(v.shape[:2]))
+        _check(op, device, "beta", beta, torch.float32, tuple(v.shape[:2]))
+        _refuse(f"{op}: tensors do not belong together")
+    _, hv, dv = wide
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
+        out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
     else:
-        _check(op, device, "out", out, dtype, shape)
+        _check(op, device, "out", out, dtype, wide)
     wk, wv = hk * dk, hv * dv
     if scale is None:
         scale = dk ** -0.5 if dk else 0.0
@@ -136,7 +146,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
 
 
 def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
-    _check(op, device, name, t, torch.float32, (None, a.hv, a.dk, a.dv))
+    _check(op, device, name, t, torch.float32, (t.shape[0] if isinstance(t, torch.Tensor) and t.dim() else 0, a.hv, a.dk, a.dv))
     if not t.is_contiguous():
         _refuse(f"{op}: {name} is not contiguous")
 

@@ -423,6 +423,51 @@ def test_a_sequence_alone_is_the_sequence_in_a_batch(dtype):
     assert torch.equal(out[33:223], alone) and torch.equal(S[1], one[0])
 
 
+def test_tensors_that_do_not_belong_together_are_refused():
+    q, k, v, g, beta = x = rule_inputs(4, 2, 4, 64, 64, BF16)
+    pool = pool_of(6, 4, 64, 64)
+    before = pool.clone()
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    slots = torch.zeros(4, dtype=torch.int32, device="cuda")
+    sixth = torch.zeros(4, 6, 64, dtype=BF16, device="cuda")
+    bad = [(q.cpu(), k, v, g, beta), (q.float(), k, v, g, beta), (q, k[:3], v, g, beta), (q, k, v.float(), g, beta), (q, k, v[0], g, beta),
+           (q, k, v, g.double(), beta), (q, k, v, g[:, :3], beta), (q, k, v, g, beta.cpu()), (q, k, None, g, beta), (q.int(), k, v, g, beta),
+           (q, k, v.transpose(1, 2), g, beta), (q[..., ::2], k[..., ::2], v, g, beta), (q, k, sixth[:, :5], torch.zeros(4, 5, device="cuda"), torch.zeros(4, 5, device="cuda")),
+           (q[:1].expand(4, 2, 64), k, v, g, beta)]
+    for y in bad:
+        refused(lambda: ops.delta_step(*y, pool))
+        refused(lambda: ops.delta_chunk(*y, cu))
+    for states in (pool.half(), pool[:3], pool[:, :3], pool.transpose(2, 3), pool.cpu(), None):
+        refused(lambda: ops.delta_step(*x, states))
+        if states is not None:
+            refused(lambda: ops.delta_chunk(*x, torch.zeros(5, dtype=torch.int32, device="cuda"), state_out=states))
+    for s in (slots.long(), slots[:3], slots.cpu(), slots[None]):
+        refused(lambda: ops.delta_step(*x, pool, slots=s))
+    refused(lambda: ops.delta_step(*x, pool, out=torch.empty(4, 4, 64, device="cuda")))
+    refused(lambda: ops.delta_chunk(*x, cu.long()))
+    refused(lambda: ops.delta_chunk(*x, cu[:0]))
+    refused(lambda: ops.delta_chunk(*x, cu, slots=slots[:1]))                                     # slots of no pool
+    refused(lambda: ops.delta_chunk(*x, cu, state_in=pool, state_out=pool[:3]))
+    both = torch.zeros(7, 4, 64, 64, device="cuda")
+    refused(lambda: ops.delta_chunk(*x, cu, state_in=both[:6], state_out=both[1:]))                # overlap in part
+    need = ops.delta_chunk_workspace(4, 1, 2, 4, 64, 64, BF16)
+    refused(lambda: ops.delta_chunk(*x, cu, workspace=torch.empty(need - 1, dtype=torch.uint8, device="cuda")))
+    refused(lambda: ops.delta_chunk(*x, cu, workspace=torch.empty(need + 16, dtype=torch.uint8, device="cuda")[1:]))
+    codes, s = ops.quantize_rows(q.flatten(1))
+    w, sw = codes, s
+    refused(lambda: ops.quantize_rows(q))
+    refused(lambda: ops.quantize_rows(codes))
+    refused(lambda: ops.quantize_rows(q.flatten(1), codes=codes[:, :5]))
+    refused(lambda: ops.quantize_rows(q.flatten(1).t()))
+    for y in [(codes.int(), s, w, sw), (codes, s[:3], w, sw), (codes, s, w[:, :5], sw), (codes, s.double(), w, sw), (codes, s, w, sw.cpu()),
+              (codes[:, ::2], s, w[:, ::2], sw), (codes[0], s, w, sw)]:
+        refused(lambda: ops.int8_matmul(*y))
+    refused(lambda: ops.int8_matmul(codes, s, w, sw, bias=sw[:2]))
+    refused(lambda: ops.int8_matmul(codes, s, w, sw, dtype=torch.float64))
+    refused(lambda: ops.int8_matmul(codes, s, w, sw, out=torch.empty(4, 5, device="cuda")))
+    assert torch.equal(pool, before)
+
+
 # ---------------------------------------------------------------- codes
 
 @types
