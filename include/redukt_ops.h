@@ -8,6 +8,7 @@
  * Contract:
  *   - no model is needed (nothing here touches what redukt_backend_init made), and calls from
  *     several threads do not meet: no entry point keeps or shares anything between calls;
+ *   - INVALID_ARGUMENT also answers sizes whose launch would not fit (2^32 threads or more);
  *   - every pointer but an argument struct's is device memory of ONE device, which need not be
  *     the calling thread's current one (the current device is the same after the call);
  *   - a call enqueues its kernels on `stream`, a hipStream_t of that device as an opaque
@@ -38,9 +39,14 @@ extern "C" {
  * Each of hv value heads keeps a state S [dk][dv] in f32.  A token with key k and query q
  * [dk] (of key head h / (hv / hk)), value v [dv], log decay g and write strength beta makes
  *     S <- e^g S + beta k (v - e^g S^T k)^T        o = scale S^T q
- * in f32 arithmetic.  g may be -inf (the state is dropped).  The rule is stable for |k| <= 1
- * and beta in [0, 2]; with REDUKT_DELTA_NORMALIZE, k and q are divided by
- * sqrt(sum of squares + 1e-6) first. */
+ * in f32 arithmetic.  g may be -inf (the state is dropped).  The rule is stable for |k| <= 1,
+ * g <= 0 and beta in [0, 2]; with REDUKT_DELTA_NORMALIZE, k and q are divided by
+ * sqrt(sum of squares + 1e-6) first.
+ *
+ * A value that is not finite goes where the rule takes it: one of v into its column, one of k,
+ * g or beta into its head, from its token on; one of q into its token.  What it reaches is then
+ * not finite, inf or NaN.  (In delta_chunk, a sum that passes f32's range from finite inputs,
+ * which a stable rule has none of, may also reach up to 63 tokens back.) */
 #define REDUKT_DELTA_NORMALIZE 1u
 
 typedef struct {

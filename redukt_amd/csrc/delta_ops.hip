@@ -1019,7 +1019,7 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
     const uint32_t NC = all >= 4096 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
-    if (prep > 0x7fffffffu || grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    if (!op_grid_ok(prep, 256) || !op_grid_ok(grid, 512)) return BACKEND_INVALID_ARGUMENT;
     k.kt = k.ws + units_bytes(r, k.d.n);
     k.slots = (uint32_t)chunk_slots(r, k.d.n);
     if (r.rows) {
@@ -1068,7 +1068,7 @@ redukt_delta_rows stepped(redukt_delta_rows a) {
 
 int32_t launch_step(DeltaArgs& k, void* stream) {
     const uint64_t waves = (uint64_t)k.n * k.r.hv * (k.r.dv / 32);
-    if ((waves + 3) / 4 > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    if (!op_grid_ok((waves + 3) / 4, 256)) return BACKEND_INVALID_ARGUMENT;
     return op_launch(delta_step_fn(k.r.dtype, k.r.dk), dim3((uint32_t)((waves + 3) / 4)), dim3(256), 0, stream, k);
 }
 

@@ -41,7 +41,7 @@ __global__ __launch_bounds__(kBlock) void k_quantize_rows(redukt_quantize_rows a
     constexpr int kHeld = 4, kLanes = WAVES * kWave, kSpan = kLanes * V;
     __shared__ float wm[kWaves];
     const int lane = threadIdx.x % kLanes;
-    const uint32_t r = WAVES == 1 ? blockIdx.x * kWaves + threadIdx.x / kWave : blockIdx.x;
+    const uint32_t group = blockIdx.y * gridDim.x + blockIdx.x, r = WAVES == 1 ? group * kWaves + threadIdx.x / kWave : group;
     if (r >= a.rows) return;                   // (whole waves, and none of a shared row)
     const T* const x = (const T*)a.x + (int64_t)r * a.x_stride;
     int8_t* const q = a.codes + (int64_t)r * a.codes_stride;
@@ -223,17 +223,24 @@ __device__ __forceinline__ i32x4 piece(const lds_u8* rows, int row, int c) {
 
 template <int KC, int NI, int NJ>
 __device__ __forceinline__ void multiply(const lds_u8* __restrict__ w, const lds_u8* __restrict__ x, i32x16 (&acc)[NI][NJ], int rw, int rx, int lane) {
+    // (the next fragments are asked for before the products of these; 128 of 768 x 4,096: 10.8 -> 9.7 us)
+    i32x4 fw[2][NI], fx[2][NJ];
+    const auto load = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) fw[s % 2][i] = piece<KC>(w, rw + 32 * i + lane % 32, 2 * s + lane / 32);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) fx[s % 2][j] = piece<KC>(x, rx + 32 * j + lane % 32, 2 * s + lane / 32);
+    };
+    load(0);
 #pragma unroll
     for (int s = 0; s < KC / 32; s++) {
-        i32x4 fw[NI], fx[NJ];
-#pragma unroll
-        for (int i = 0; i < NI; i++) fw[i] = piece<KC>(w, rw + 32 * i + lane % 32, 2 * s + lane / 32);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) fx[j] = piece<KC>(x, rx + 32 * j + lane % 32, 2 * s + lane / 32);
+        if (s + 1 < KC / 32) load(s + 1);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < NI; i++)
 #pragma unroll
-            for (int j = 0; j < NJ; j++) acc[i][j] = mma32(fw[i], fx[j], acc[i][j]);
+            for (int j = 0; j < NJ; j++) acc[i][j] = mma32(fw[s % 2][i], fx[s % 2][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -366,6 +373,7 @@ const void* quantize_wide_fn(uint32_t dtype) {
 }
 
 constexpr int64_t kMaxStride = 1 << 22;      // 256 rows stay within 32-bit offsets
+constexpr uint32_t kGridX = 1 << 20;         // workgroups along x; more of them go along y
 
 int32_t few(const redukt_int8_matmul& a, void* stream) {
     const uint32_t groups = (a.n + 15) / 16, lines = (a.k + 127) / 128;
@@ -373,6 +381,7 @@ int32_t few(const redukt_int8_matmul& a, void* stream) {
     while (split < 8 && split * 2 <= lines && groups * split < 2048) split *= 2;
     Int8Few k{a, split};
     const uint32_t per = 8 / split, grid = (groups + per - 1) / per;
+    if (!op_grid_ok(grid, 512)) return BACKEND_INVALID_ARGUMENT;
     return op_launch(OP_BY_TYPE(a.dtype, k_int8_few), dim3(grid), dim3(512), 0, stream, k);
 }
 
@@ -381,7 +390,7 @@ int32_t tiles(const redukt_int8_matmul& a, void* stream) {
     const bool wide = op_aligned(a.out, 16) && a.out_stride * op_elem_bytes(a.dtype) % 16 == 0;
     Int8Tiles k{a, (a.m + TM - 1) / TM, (a.n + TN - 1) / TN, wide};
     const uint64_t total = (uint64_t)k.tiles_m * k.tiles_n, grid = (total + 7) / 8 * 8;
-    if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+    if (!op_grid_ok(grid, 64 * WM * WN)) return BACKEND_INVALID_ARGUMENT;
     return op_launch(OP_BY_TYPE(a.dtype, k_int8_tiles, TM, TN, WM, WN, KC, STAGES), dim3((uint32_t)grid), dim3(64 * WM * WN), 0, stream, k);
 }
 
@@ -408,7 +417,8 @@ int32_t redukt_op_quantize_rows(const redukt_quantize_rows* a, void* stream) {
     const bool one = a->cols <= 4u * kWave * (wide ? v : 1);
     const void* fn = !wide ? (one ? OP_BY_TYPE(a->dtype, k_quantize_rows, 1, 1) : OP_BY_TYPE(a->dtype, k_quantize_rows, 1, 4))
                      : one ? quantize_wide_fn<1>(a->dtype) : quantize_wide_fn<4>(a->dtype);
-    return op_launch(fn, dim3(one ? (a->rows + kWaves - 1) / kWaves : a->rows), dim3(kBlock), 0, stream, k);
+    const uint32_t groups = one ? (a->rows + kWaves - 1) / kWaves : a->rows, x = groups < kGridX ? groups : kGridX;
+    return op_launch(fn, dim3(x, (groups + x - 1) / x), dim3(kBlock), 0, stream, k);
 }
 
 int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
@@ -430,7 +440,7 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
     if (!aligned) {
         redukt_int8_matmul k = *a;
         const uint64_t grid = (uint64_t)((a->n + kTile - 1) / kTile) * ((a->m + kTile - 1) / kTile);
-        if (grid > 0x7fffffffu) return BACKEND_INVALID_ARGUMENT;
+        if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
         return op_launch(OP_BY_TYPE(a->dtype, k_int8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
     // Every kernel gives the same bits, so the choice is by time alone (us, on either side of each edge; n and k after m).  Up to

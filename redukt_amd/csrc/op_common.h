@@ -46,6 +46,9 @@ private:
     bool set_ = false;
 };
 
+// Whether a launch of `groups` workgroups of `threads` is one that the runtime takes (threads along a dimension fit 32 bits).
+inline bool op_grid_ok(uint64_t groups, uint32_t threads) { return groups <= 0xffffffffull / threads; }
+
 template <typename Args>
 inline int32_t op_launch(const void* fn, dim3 grid, dim3 block, size_t lds, void* stream, Args& args) {
     void* p[] = {(void*)&args};

@@ -3,10 +3,12 @@
 The gated delta rule for one token (`delta_step`) and for whole sequences (`delta_chunk`), int8
 codes of activation rows (`quantize_rows`) and the product of codes with a scale per token and
 channel (`int8_matmul`).  Arguments are torch tensors on one GPU; work is queued on torch's
-current stream of that GPU (or on `stream`, a hipStream_t's value: outputs and workspace are
-then best passed in too, since torch frees what it allocates by its own streams).  No model
-needs to be open.  Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch
-nothing; there is no CPU fallback.
+current stream of that GPU, or on `stream`, a hipStream_t's value.  Outputs and workspaces that a
+call allocates belong to torch's current stream, so for another one they are passed in.  Outputs
+overlap no input (but a state pool its own next states).  No model needs to be open.  The
+operators have no gradients: inputs that ask for one are refused while torch records them.
+Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch nothing; there is no CPU
+fallback.
 """
 from __future__ import annotations
 
@@ -94,8 +96,18 @@ def _device(op: str, t) -> int:
     return t.get_device()
 
 
-def _stream(stream: Optional[int], device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream
+def _stream(op: str, stream: Optional[int], device: int, allocates: bool) -> int:
+    current = torch._C._cuda_getCurrentRawStream(device)
+    if stream is None or stream == current:
+        return current
+    if allocates:
+        _refuse(f"{op}: on a stream that is not torch's current one, outputs and workspace are passed in")
+    return stream
+
+
+def _no_gradients(op: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        _refuse(f"{op}: an input asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
 
 
 def _row_stride(op: str, name: str, t, width: int) -> int:
@@ -130,6 +142,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
         _check(op, device, "g", g, torch.float32, tuple(v.shape[:2]))
         _check(op, device, "beta", beta, torch.float32, tuple(v.shape[:2]))
         _refuse(f"{op}: tensors do not belong together")
+    _no_gradients(op, q, k, v, g, beta)
     _, hv, dv = wide
     if out is None:
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
@@ -162,7 +175,7 @@ def _slots(op: str, device: int, slots, n: int) -> Optional[int]:
 
 def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[float] = None, normalize: bool = False,
                stream: Optional[int] = None):
-    """The gated delta rule for one token of each of n entries; states are stepped in place.
+    """The gated delta rule for one token of each of n entries (at most 65,536); states are stepped in place.
 
     q, k [n, key heads, dk] and v [n, value heads, dv] in bfloat16, float16 or float32; g (log
     decay) and beta (write strength) [n, value heads] float32; states [slots, value heads, dk,
@@ -174,10 +187,12 @@ def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[f
     one projection's output), by whole 16 bytes.
     """
     op = "delta_step"
+    allocates = out is None
     a, out, device = _rows(op, q, k, v, g, beta, out, scale, normalize)
+    on = _stream(op, stream, device, allocates)
     _pool(op, device, "states", states, a)
     code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
-                                        _slots(op, device, slots, a.rows), _stream(stream, device))
+                                        _slots(op, device, slots, a.rows), on)
     _done(code, op)
     return out
 
@@ -197,11 +212,13 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     not wanted; state_in itself: in place).  cu_seqlens int32, none decreasing, within the rows.
     A slot of -1 leaves the sequence out; slots out of range, or named before while state_out
     is given, give NaN rows.  Returns out [rows, value heads, dv]; rows of no sequence are not
-    written.  workspace: a uint8 tensor of `delta_chunk_workspace` bytes that nothing else uses
+    written.  At most 65,536 sequences.  workspace: a uint8 tensor of `delta_chunk_workspace` bytes that nothing else uses
     meanwhile (allocated if None).
     """
     op = "delta_chunk"
+    allocates = out is None or workspace is None
     a, out, device = _rows(op, q, k, v, g, beta, out, scale, normalize)
+    on = _stream(op, stream, device, allocates)
     _check(op, device, "cu_seqlens", cu_seqlens, torch.int32, (None,))
     n = cu_seqlens.shape[0] - 1
     if n < 0 or not cu_seqlens.is_contiguous():
@@ -222,8 +239,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     code = L.redukt_op_delta_chunk(ctypes.byref(a), cu_seqlens.data_ptr(), n,
                                    None if state_in is None else state_in.data_ptr(),
                                    None if state_out is None else state_out.data_ptr(), n_slots,
-                                   _slots(op, device, slots, n), workspace.data_ptr(), workspace.numel(),
-                                   _stream(stream, device))
+                                   _slots(op, device, slots, n), workspace.data_ptr(), workspace.numel(), on)
     _done(code, op)
     return out
 
@@ -238,6 +254,8 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     device = _device(op, x)
     if x.dtype not in DTYPES or x.dim() != 2:
         _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
+    _no_gradients(op, x)
+    on = _stream(op, stream, device, codes is None or scales is None)
     rows, cols = x.shape
     if codes is None:
         codes = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
@@ -251,7 +269,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
             _refuse(f"{op}: scales is not contiguous")
     a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
                      _row_stride(op, "codes", codes, cols), scales.data_ptr())
-    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), _stream(stream, device)), op)
+    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), on), op)
     return codes, scales
 
 
@@ -274,6 +292,8 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
     for name, t in (("x_scales", x_scales), ("w_scales", w_scales), ("bias", bias)):
         if t is not None and not t.is_contiguous():
             _refuse(f"{op}: {name} is not contiguous")
+    _no_gradients(op, x_scales, w_scales, bias)
+    on = _stream(op, stream, device, out is None)
     if out is None:
         if dtype not in DTYPES:
             _refuse(f"{op}: dtype is bfloat16, float16 or float32")
@@ -285,5 +305,5 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
     a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))
-    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), _stream(stream, device)), op)
+    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op)
     return out

@@ -1,5 +1,7 @@
 """The operators on caller tensors (redukt_amd.ops, include/redukt_ops.h) on the GPU, against 64-bit
 statements of them (tests/ops_f64.py)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -468,6 +470,49 @@ def test_tensors_that_do_not_belong_together_are_refused():
     assert torch.equal(pool, before)
 
 
+def test_gradients_and_allocations_on_other_streams_are_refused():
+    q, k, v, g, beta = x = rule_inputs(4, 2, 4, 64, 64, BF16)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    codes, s = ops.quantize_rows(q.flatten(1))
+    for i in range(5):
+        y = list(x)
+        y[i] = y[i].clone().requires_grad_()
+        refused(lambda: ops.delta_step(*y, pool_of(4, 4, 64, 64)))
+        refused(lambda: ops.delta_chunk(*y, cu))
+        with torch.no_grad():
+            ops.delta_step(*y, pool_of(4, 4, 64, 64))
+    refused(lambda: ops.quantize_rows(q.flatten(1).clone().requires_grad_()))
+    refused(lambda: ops.int8_matmul(codes, s, codes, s.clone().requires_grad_()))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    work = torch.empty(ops.delta_chunk_workspace(4, 1, 2, 4, 64, 64, BF16), dtype=torch.uint8, device="cuda")
+    raw, out = side.cuda_stream, torch.empty_like(v)
+    refused(lambda: ops.delta_step(*x, pool_of(4, 4, 64, 64), stream=raw))
+    refused(lambda: ops.delta_chunk(*x, cu, out=out, stream=raw))
+    refused(lambda: ops.delta_chunk(*x, cu, workspace=work, stream=raw))
+    refused(lambda: ops.quantize_rows(q.flatten(1), codes=codes, stream=raw))
+    refused(lambda: ops.int8_matmul(codes, s, codes, s, stream=raw))
+    want = ops.delta_chunk(*x, cu)
+    ops.delta_chunk(*x, cu, out=out, workspace=work, stream=raw)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    assert torch.equal(ops.delta_chunk(*x, cu, stream=torch.cuda.current_stream().cuda_stream), want)
+
+
+def test_sizes_whose_launch_does_not_fit_are_refused():
+    q, k, v, g, beta = rule_inputs(1, 1, 4096, 64, 256, BF16)
+    a, out, _ = ops._rows("", q, k, v, g, beta, None, None, False)
+    a.rows, a.q_stride, a.k_stride, a.v_stride, a.out_stride = 65536, 64, 64, 1 << 20, 1 << 20
+    out.zero_()
+    L, here, no = ops._load(), torch.cuda.current_stream().cuda_stream, int(ffi.BackendResult.INVALID_ARGUMENT)
+    assert L.redukt_op_delta_step(ctypes.byref(a), g.data_ptr(), 65536, None, here) == no
+    cu = torch.zeros(2, dtype=torch.int32, device="cuda")
+    work = torch.empty(16, dtype=torch.uint8, device="cuda")
+    assert L.redukt_op_delta_chunk(ctypes.byref(a), cu.data_ptr(), 65536, None, None, 0, None, work.data_ptr(), 1 << 60, here) == no
+    torch.cuda.synchronize()
+    assert not out.any()
+
+
 # ---------------------------------------------------------------- codes
 
 @types
@@ -505,6 +550,17 @@ def test_quantize_rows_strided_and_unaligned(off, pad, dtype):
     want, s = ops_f64.quantize(x.float().cpu().numpy())
     assert np.array_equal(codes[:, off:off + cols].cpu().numpy(), want) and np.array_equal(scales.cpu().numpy(), s)
     assert (codes[:, :off] == 99).all() and (codes[:, off + cols:] == 99).all()
+
+
+@pytest.mark.parametrize("rows, cols", [((1 << 26) + 5, 1), ((1 << 24) + 5, 260)])
+def test_more_rows_than_one_dimension_of_a_launch(rows, cols):
+    x = torch.zeros(rows, cols, dtype=torch.float16, device="cuda")
+    at = torch.tensor([0, 1, (1 << 22) - 1, 1 << 22, (1 << 24) + 1, rows - 1], device="cuda")
+    x[at, cols - 1] = torch.tensor([1.0, -2.0, 3.0, -4.0, 5.0, -6.0], dtype=torch.float16, device="cuda")
+    codes, s = ops.quantize_rows(x)
+    want, ws = ops.quantize_rows(x[at])
+    assert torch.equal(codes[at], want) and torch.equal(s[at], ws)
+    assert int(codes.count_nonzero()) == 6 and int((s == 1.0).sum()) == rows - 6
 
 
 # ---------------------------------------------------------------- product
