@@ -245,12 +245,9 @@ __device__ __forceinline__ Split<N> as_split(const bf16x8 (&v)[N]) {
     return o;
 }
 
-constexpr int kt_bytes(int dk, int in_limbs) { return dk / 16 * 2 * in_limbs * kFrag; }
-
 struct ChunkArgs {
     DeltaArgs d;
     unsigned char* ws;         // units: (value head, chunk slot)
-    unsigned char* kt;         // fragments of k^T: (key head, chunk slot)
     uint32_t slots;            // chunk slots
     uint32_t per;              // value heads of a workgroup of k_delta_prep
 };
@@ -481,19 +478,6 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
         sU[16 * wave + l16] = norm ? rsqrtf(k2 + kUnitEps) + 0.0f * k2 : 1.0f + 0.0f * k2;
         sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
     }
-    if (h0 % group == 0) {
-        // row l16 of k^T's tile p (as the state's rows), the tokens 32 s + 8 g + [0, 8)
-        unsigned char* const kt = a.kt + ((size_t)hq * a.slots + slot) * kt_bytes(DK, LI);
-        for (int f = wave; f < DK / 16 * 2; f += 4) {
-            const T* const col = sK + state_index<DK>(f / 2, l16);
-            float v[8];
-#pragma unroll
-            for (int x = 0; x < 8; x++) v[x] = (float)col[(32 * (f % 2) + 8 * g4 + x) * PK];
-            const Split<LI> y = split8<LI>(v);
-#pragma unroll
-            for (int n = 0; n < LI; n++) *(bf16x8*)(kt + (f * LI + n) * kFrag + lane * 16) = y.l[n];
-        }
-    }
     __syncthreads();                           // k and q are done with; sU, sP are written
 
     int here = threadIdx.x;
@@ -652,7 +636,8 @@ template <typename T, int DK, int NC>
 __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, NW = DK / 64, SZ = sizeof(T);
     constexpr int KF = 4 * NW;                 // a lane's inner indices of one wave's rows of the state
-    __shared__ __attribute__((aligned(16))) f32x4 sR[NC][4][4][kWave];       // partial K S: [tile of tokens][wave]
+    __shared__ __attribute__((aligned(16))) f32x4 sR[NC][4][3][kWave];       // partial K S: [tile of tokens][of the other waves]
+    __shared__ __attribute__((aligned(16))) unsigned char sK[4][LI][kChunk * 16 * NW * 2];     // each wave's columns of K: [token]
     __shared__ __attribute__((aligned(16))) unsigned char sS[NC][4][LO][kWave * KF * 2], sX[NC][2][3][kFrag], sD[NC][2][3][kFrag];
     __shared__ __attribute__((aligned(16))) int sBad[NC][16][4];
     const redukt_delta_rows& r = a.d.r;
@@ -713,7 +698,6 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         return o;
     };
     const unsigned char* unit = a.ws + ((size_t)h * a.slots + first) * unit_bytes(LO);
-    const unsigned char* kt = a.kt + ((size_t)hq * a.slots + first) * kt_bytes(DK, LI) + wave * (NW * 2 * LI * kFrag);
     const auto get = [&](const unsigned char (&from)[3][kFrag], auto n_) {
         constexpr int N = decltype(n_)::value;
         Split<N> o;
@@ -751,7 +735,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 for (int x = 0; x < 4; x++) S[nc][p][x] = a.d.in ? a.d.in[state_at(nc, p, x)] : 0.0f;
         Rows rk = rows_of(r.k, r.k_stride, hq * DK, DK), rv = rows_of(r.v, r.v_stride, h * r.dv, r.dv);
         vecK kf[4];                            // tiles wave, wave + 1, .. (mod 4)
-        bf16x8 tf[2][3], ktf[NW][2][LI];
+        bf16x8 tf[2][3];
         uint32_t vv[NC][4];
         f32x4 kd;
         float keep;
@@ -778,12 +762,24 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
             for (int n = 0; n < 3; n++) tf[1][n] = frag(unit, frag1, f0 * 3 + 3 + n);
         };
-        const auto load_kt = [&]() {
+        const auto load_keep = [&]() {
+            keep = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rows_rsrc(unit, unit_bytes(LO)), lane * 4,
+                                                                                  kTri * (3 + LO) * kFrag + 2 * kChunk * 4, 0));
+        };
+        // K^T for the last step: this wave's columns of K, which it holds as rows, go through LDS and come back transposed, 4 tokens x
+        // 16 columns by 16 lanes.  A row's pieces of KF columns stand at place (piece ^ row / 8 % 4).
+        const auto put_k = [&](int o, const Part<NW, LI>& k) {
+            const int row = tile_index((wave + o) % 4, l16);
 #pragma unroll
-            for (int f = 0; f < NW * 2; f++)
-#pragma unroll
-                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = frag(kt, NW * 2 * LI * kFrag, f * LI + n);
-            keep = ((const float*)(unit + kTri * (3 + LO) * kFrag))[2 * kChunk];
+            for (int n = 0; n < LI; n++)
+                *(typename Part<NW, LI>::vec*)(sK[wave][n] + row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2)) = k.l[n];
+        };
+        const auto get_kt = [&](int p, int s, int n) {       // row l16 of tile p, the tokens 32 s + 8 g4 + [0, 8)
+            typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+            const unsigned char* const at = sK[wave][n] + (32 * s + 8 * g4 + l16 / 4) * (NW * 32) + (l16 % 4 ^ g4) * (KF * 2) + 8 * p;
+            struct { i16x4 v[2]; } x = {{__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)at),
+                                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(at + 4 * NW * 32))}};
+            return __builtin_bit_cast(bf16x8, x);
         };
         // The four rows of this wave's tile that a lane holds, as half of a right operand's fragment.
         const auto put = [&](unsigned char (*to)[3][kFrag], const f32x4& v) {
@@ -799,7 +795,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             load_k(rows);
             load_v(rows);
             load_t();
-            load_kt();
+            load_keep();
         }
         for (uint32_t c = 0; c < chunks; c++) {
             // (the last chunk requests itself again instead of one past the end)
@@ -807,8 +803,10 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             left -= on * kChunk;
             const uint32_t rows = min(left, (uint32_t)kChunk);
             rk.step(on), rv.step(on);
-            unit += on * unit_bytes(LO), kt += on * kt_bytes(DK, LI);
+            unit += on * unit_bytes(LO);
             f32x4 X[NC];
+#pragma unroll
+            for (int o = 0; o < 4; o++) put_k(o, limbs(kf[o]));
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 float v[KF];
@@ -828,14 +826,14 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                         }
                 X[nc] = y[0];
 #pragma unroll
-                for (int o = 1; o < 4; o++) sR[nc][(wave + o) % 4][wave][lane] = y[o];
+                for (int o = 1; o < 4; o++) sR[nc][(wave + o) % 4][3 - o][lane] = y[o];
             }
             load_k(rows);
             __syncthreads();                   // A: S and partial sums are there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
 #pragma unroll
-                for (int o = 1; o < 4; o++) X[nc] += sR[nc][wave][(wave + o) % 4][lane];
+                for (int o = 1; o < 4; o++) X[nc] += sR[nc][wave][o - 1][lane];
                 uint32_t top = 0;
                 f32x4 x;
 #pragma unroll
@@ -869,6 +867,11 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 put(sD[nc], D);
             }
             load_t();
+            bf16x8 ktf[NW][2][LI];
+#pragma unroll
+            for (int f = 0; f < NW * 2; f++)
+#pragma unroll
+                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = get_kt(f / 2, f % 2, n);
             __syncthreads();                   // C: D is there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -891,7 +894,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
                         for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][1][n], x1.l[j], S[nc][p]);
             }
-            load_kt();
+            load_keep();
         }
         if (a.d.states) {
             asm volatile("" : "+v"(here));     // (the addresses are made anew: kept from the start, they would take 16 registers)
@@ -992,11 +995,10 @@ const void* delta_chunks_of(uint32_t dk) {
     return dk == 128 ? (const void*)k_delta_chunks<T, 128, NC> : (const void*)k_delta_chunks<T, 64, NC>;
 }
 
-// NC 1, 2, or 4, the last with 16-bit elements only (in f32 its limbs do not fit LDS).
+// NC 1, 2, or 4, the last in bf16 only (the limbs of the others do not fit LDS).
 const void* delta_chunks_fn(uint32_t dtype, uint32_t dk, uint32_t nc) {
     if (dtype == REDUKT_OP_F32) return nc == 1 ? delta_chunks_of<float, 1>(dk) : delta_chunks_of<float, 2>(dk);
-    if (dtype == REDUKT_OP_F16)
-        return nc == 1 ? delta_chunks_of<_Float16, 1>(dk) : nc == 2 ? delta_chunks_of<_Float16, 2>(dk) : delta_chunks_of<_Float16, 4>(dk);
+    if (dtype == REDUKT_OP_F16) return nc == 1 ? delta_chunks_of<_Float16, 1>(dk) : delta_chunks_of<_Float16, 2>(dk);
     return nc == 1 ? delta_chunks_of<__bf16, 1>(dk) : nc == 2 ? delta_chunks_of<__bf16, 2>(dk) : delta_chunks_of<__bf16, 4>(dk);
 }
 
@@ -1016,11 +1018,10 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
     // chunks with 1, 2 and 4 tiles: 290, 369 and 516 us): worth it once there are workgroups waiting for a CU (37 ragged sequences
     // of 16 heads of 128 columns, 4,736 tiles: 281, 225 and 208).
     const uint64_t all = (uint64_t)k.d.n * r.hv * (r.dv / 16);
-    const uint32_t NC = all >= 4096 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
+    const uint32_t NC = all >= 4096 && r.dtype == REDUKT_OP_BF16 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (!op_grid_ok(prep, 256) || !op_grid_ok(grid, 512)) return BACKEND_INVALID_ARGUMENT;
-    k.kt = k.ws + units_bytes(r, k.d.n);
     k.slots = (uint32_t)chunk_slots(r, k.d.n);
     if (r.rows) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
@@ -1093,8 +1094,7 @@ int32_t redukt_op_delta_step(const redukt_delta_rows* a, float* states, uint32_t
 
 uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_seq) {
     if (!sizes_ok(a) || n_seq > kMaxOpRows) return 0;
-    const int limbs = a->dtype == REDUKT_OP_F32 ? 3 : a->dtype == REDUKT_OP_F16 ? 2 : 1;
-    return units_bytes(*a, n_seq) + chunk_slots(*a, n_seq) * a->hk * kt_bytes(a->dk, limbs);
+    return units_bytes(*a, n_seq);
 }
 
 int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uint32_t n_seq, const float* state_in,
@@ -1117,7 +1117,7 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, nullptr, 0, 1};
+    ChunkArgs k{{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq}, (unsigned char*)workspace, 0, 1};
     return launch_chunks(k, stream);
 }
 
