@@ -257,6 +257,19 @@ __device__ __forceinline__ uint32_t row_of(const ChunkArgs& a, uint32_t i) {
     return min((uint32_t)max(a.d.cu[i], 0), a.d.r.rows);
 }
 
+// The sequence that is the pos-th by length, longest first (n <= 64; every lane of the wave takes part).  Workgroups that wait for a
+// CU start in this order, so that no long sequence begins last (37 of 3 to 932 tokens: 203 -> 194 us).
+__device__ __forceinline__ uint32_t by_length(const ChunkArgs& a, uint32_t pos, int lane) {
+    const bool in = (uint32_t)lane < a.d.n;
+    const uint32_t b = in ? row_of(a, lane) : 0, len = in ? max(row_of(a, lane + 1), b) - b : 0;
+    uint32_t rank = 0;
+    for (uint32_t j = 0; j < a.d.n; j++) {
+        const uint32_t x = __builtin_amdgcn_readlane(len, j);
+        rank += x > len || (x == len && (int)j < lane);
+    }
+    return __builtin_ctzll(__ballot(in && rank == pos));
+}
+
 // Chunk c of the sequence that starts at row b and is the i-th has slot b / 64 + i + c: slots of one sequence
 // are consecutive, those of the next begin after them, and rows / 64 + n slots are enough.
 __device__ __forceinline__ uint32_t first_chunk(uint32_t b, uint32_t i) { return b / kChunk + i; }
@@ -637,7 +650,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, NW = DK / 64, SZ = sizeof(T);
     constexpr int KF = 4 * NW;                 // a lane's inner indices of one wave's rows of the state
     __shared__ __attribute__((aligned(16))) f32x4 sR[NC][4][3][kWave];       // partial K S: [tile of tokens][of the other waves]
-    __shared__ __attribute__((aligned(16))) unsigned char sK[4][LI][kChunk * 16 * NW * 2];     // each wave's columns of K: [token]
+    constexpr bool kRaw = LI == 2 && NC == 4;  // (in f16 two limbs of K would be 1 KB too many beside four column tiles)
+    __shared__ __attribute__((aligned(16))) unsigned char sK[4][kRaw ? 1 : LI][kChunk * 16 * NW * 2];     // each wave's columns of K
     __shared__ __attribute__((aligned(16))) unsigned char sS[NC][4][LO][kWave * KF * 2], sX[NC][2][3][kFrag], sD[NC][2][3][kFrag];
     __shared__ __attribute__((aligned(16))) int sBad[NC][16][4];
     const redukt_delta_rows& r = a.d.r;
@@ -646,7 +660,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     const uint32_t group = r.hv / r.hk, cols = (r.dv / 16 + NC - 1) / NC;
     const XcdTile w = xcd_tile(blockIdx.x, group * cols, a.d.n * r.hk);
     if (!w.live) return;
-    const uint32_t i = w.unit / r.hk, hq = w.unit % r.hk, h = hq * group + w.part / cols;
+    const uint32_t i = a.d.n > 1 && a.d.n <= kWave ? by_length(a, w.unit / r.hk, lane) : w.unit / r.hk;
+    const uint32_t hq = w.unit % r.hk, h = hq * group + w.part / cols;
     const uint32_t col0 = w.part % cols * (16 * NC) + l16;
     const int slot = entry_slot(a.d.slots, a.d.n_slots, i, a.d.states != nullptr, lane);
     if (slot == kSkip) return;
@@ -768,11 +783,15 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         };
         // K^T for the last step: this wave's columns of K, which it holds as rows, go through LDS and come back transposed, 4 tokens x
         // 16 columns by 16 lanes.  A row's pieces of KF columns stand at place (piece ^ row / 8 % 4).
-        const auto put_k = [&](int o, const Part<NW, LI>& k) {
-            const int row = tile_index((wave + o) % 4, l16);
+        const auto put_k = [&](int o) {
+            const int row = tile_index((wave + o) % 4, l16), at = row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2);
+            if constexpr (kRaw) {
+                *(vecK*)(sK[wave][0] + at) = kf[o];
+            } else {
+                const Part<NW, LI> k = limbs(kf[o]);
 #pragma unroll
-            for (int n = 0; n < LI; n++)
-                *(typename Part<NW, LI>::vec*)(sK[wave][n] + row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2)) = k.l[n];
+                for (int n = 0; n < LI; n++) *(typename Part<NW, LI>::vec*)(sK[wave][n] + at) = k.l[n];
+            }
         };
         const auto get_kt = [&](int p, int s, int n) {       // row l16 of tile p, the tokens 32 s + 8 g4 + [0, 8)
             typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
@@ -806,7 +825,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             unit += on * unit_bytes(LO);
             f32x4 X[NC];
 #pragma unroll
-            for (int o = 0; o < 4; o++) put_k(o, limbs(kf[o]));
+            for (int o = 0; o < 4; o++) put_k(o);
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 float v[KF];
@@ -867,11 +886,21 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 put(sD[nc], D);
             }
             load_t();
-            bf16x8 ktf[NW][2][LI];
+            Split<LI> ktf[NW][2];
 #pragma unroll
-            for (int f = 0; f < NW * 2; f++)
+            for (int f = 0; f < NW * 2; f++) {
+                if constexpr (kRaw) {
+                    typedef T eight __attribute__((ext_vector_type(8)));
+                    const eight k = __builtin_bit_cast(eight, get_kt(f / 2, f % 2, 0));
+                    float v[8];
 #pragma unroll
-                for (int n = 0; n < LI; n++) ktf[f / 2][f % 2][n] = get_kt(f / 2, f % 2, n);
+                    for (int j = 0; j < 8; j++) v[j] = (float)k[j];
+                    ktf[f / 2][f % 2] = split8<LI>(v);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < LI; n++) ktf[f / 2][f % 2].l[n] = get_kt(f / 2, f % 2, n);
+                }
+            }
             __syncthreads();                   // C: D is there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -886,13 +915,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
                     for (int j = 0; j < 3 - n; j++)
 #pragma unroll
-                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][0][n], x0.l[j], S[nc][p]);
+                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][0].l[n], x0.l[j], S[nc][p]);
 #pragma unroll
                 for (int n = 0; n < LI; n++)
 #pragma unroll
                     for (int j = 0; j < 3 - n; j++)
 #pragma unroll
-                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][1][n], x1.l[j], S[nc][p]);
+                        for (int p = 0; p < NW; p++) S[nc][p] = mma(ktf[p][1].l[n], x1.l[j], S[nc][p]);
             }
             load_keep();
         }
@@ -995,10 +1024,11 @@ const void* delta_chunks_of(uint32_t dk) {
     return dk == 128 ? (const void*)k_delta_chunks<T, 128, NC> : (const void*)k_delta_chunks<T, 64, NC>;
 }
 
-// NC 1, 2, or 4, the last in bf16 only (the limbs of the others do not fit LDS).
+// NC 1, 2, or 4, the last with 16-bit elements only (in f32 its limbs do not fit LDS).
 const void* delta_chunks_fn(uint32_t dtype, uint32_t dk, uint32_t nc) {
     if (dtype == REDUKT_OP_F32) return nc == 1 ? delta_chunks_of<float, 1>(dk) : delta_chunks_of<float, 2>(dk);
-    if (dtype == REDUKT_OP_F16) return nc == 1 ? delta_chunks_of<_Float16, 1>(dk) : delta_chunks_of<_Float16, 2>(dk);
+    if (dtype == REDUKT_OP_F16)
+        return nc == 1 ? delta_chunks_of<_Float16, 1>(dk) : nc == 2 ? delta_chunks_of<_Float16, 2>(dk) : delta_chunks_of<_Float16, 4>(dk);
     return nc == 1 ? delta_chunks_of<__bf16, 1>(dk) : nc == 2 ? delta_chunks_of<__bf16, 2>(dk) : delta_chunks_of<__bf16, 4>(dk);
 }
 
@@ -1014,11 +1044,11 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
     // two to a key head: 304 -> 289 us with k_delta_chunks).
     if (r.hv / r.hk % 2 == 0 && chunk_slots(r, k.d.n) * r.hv >= 1024) k.per = 2;
     const uint64_t prep = chunk_slots(r, k.d.n) * (r.hv / k.per);
-    // NC column tiles a workgroup read a chunk's operands once for all of them, but a chunk then takes longer (256 tiles of 128
-    // chunks with 1, 2 and 4 tiles: 290, 369 and 516 us): worth it once there are workgroups waiting for a CU (37 ragged sequences
-    // of 16 heads of 128 columns, 4,736 tiles: 281, 225 and 208).
+    // NC column tiles a workgroup read a chunk's operands once for all of them, but a chunk then takes longer: worth it once there are
+    // workgroups waiting for a CU.  Ragged sequences of 16 heads of 128 columns, us with 1, 2 and 4 tiles: 5 of them (640 tiles) 88, 94
+    // and 138; 10 (1,280) 96, 78 and 97; 20 (2,560) 153, 118 and 107; 37 (4,736) 296, 230 and 196.
     const uint64_t all = (uint64_t)k.d.n * r.hv * (r.dv / 16);
-    const uint32_t NC = all >= 4096 && r.dtype == REDUKT_OP_BF16 ? 4 : all >= 1024 ? 2 : 1;
+    const uint32_t NC = all >= 2048 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (!op_grid_ok(prep, 256) || !op_grid_ok(grid, 512)) return BACKEND_INVALID_ARGUMENT;

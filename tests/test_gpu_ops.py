@@ -215,11 +215,12 @@ def test_delta_chunk_heads(hk, hv, dk, dv, dtype):
 
 
 @types
+@pytest.mark.parametrize("n", [12, 23, 66])
 @pytest.mark.parametrize("dk,dv", [(64, 128), (128, 160)])
-def test_delta_chunk_many_sequences(dk, dv, dtype):
-    """Enough sequences that a workgroup takes several column tiles, and several heads of the preparation: the same bits as
-    each sequence alone, and the rule's values."""
-    n, hk, hv = 66, 6, 12
+def test_delta_chunk_many_sequences(dk, dv, n, dtype):
+    """Enough sequences that a workgroup takes several column tiles (two, four), and several heads of the preparation, in the
+    order of their lengths and not: the same bits as each sequence alone, and the rule's values."""
+    hk, hv = 6, 12
     lens = [(7 * i) % 61 + 70 * (i % 9 == 0) for i in range(n)]
     T = sum(lens)
     x = rule_inputs(T, hk, hv, dk, dv, dtype, seed=6, normalize=True)
@@ -228,7 +229,7 @@ def test_delta_chunk_many_sequences(dk, dv, dtype):
     before = pool_of(n, hv, dk, dv)
     after = torch.empty_like(before)
     out = ops.delta_chunk(*x, cu, state_in=before, state_out=after, normalize=True)
-    for i in (0, 1, 9, 37, n - 1):
+    for i in (0, 1, 9, n // 2, n - 1):
         rows = slice(at[i], at[i + 1])
         want, S, tol, S_tol = ops_f64.rule(*(t[rows] for t in x), before[i], normalize=True)
         check(out[rows], want, tol, ("out", i))
