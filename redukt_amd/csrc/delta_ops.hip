@@ -354,21 +354,19 @@ __device__ __forceinline__ f32x4 mma_part(const bf16x4& a, const bf16x4& b, cons
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(i16x4, a), __builtin_bit_cast(i16x4, b), c, 0, 0, 0);
 }
 
-// Fragments of the lower triangle at m (f32 [64][kPitchA], natural order), its rows times f, with N limbs to `to`: fragment
+// Fragment x of the lower triangle at m (f32 [64][kPitchA], natural order), its rows times f, with N limbs to `to`: fragment
 // x is tile 0, 1, 2, 2, 3, 3 and inner indices 32 s + [0, 32) with s = 0, 0, 0, 1, 0, 1.
 template <int N>
-__device__ __forceinline__ void store_triangle(const float* m, const float* f, unsigned char* to, int wave, int lane) {
-    for (int x = wave; x < kTri; x += 4) {
-        const int tile = x < 2 ? x : 2 + (x - 2) / 2, s = x < 2 ? 0 : (x - 2) % 2, row = tile_index(tile, lane % 16);
-        float v[8];
-        op_load(m + row * kPitchA + 32 * s + 8 * (lane / 16), v);
-        const float scale = f ? f[row] : 1.0f;
+__device__ __forceinline__ void store_fragment(const float* m, const float* f, unsigned char* to, int x, int lane) {
+    const int tile = x < 2 ? x : 2 + (x - 2) / 2, s = x < 2 ? 0 : (x - 2) % 2, row = tile_index(tile, lane % 16);
+    float v[8];
+    op_load(m + row * kPitchA + 32 * s + 8 * (lane / 16), v);
+    const float scale = f ? f[row] : 1.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] *= scale;
-        const Split<N> y = split8<N>(v);
+    for (int j = 0; j < 8; j++) v[j] *= scale;
+    const Split<N> y = split8<N>(v);
 #pragma unroll
-        for (int n = 0; n < N; n++) *(bf16x8*)(to + (x * N + n) * kFrag + lane * 16) = y.l[n];
-    }
+    for (int n = 0; n < N; n++) *(bf16x8*)(to + (x * N + n) * kFrag + lane * 16) = y.l[n];
 }
 
 // v moved between lanes by the DPP control CTRL, 0 where a lane has no source or its row is not in ROWS.
@@ -507,15 +505,6 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
         // from the first token `past` whose key, g or beta is not finite on there are no rows
         const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
         const int past = bads ? __builtin_ctzll(bads) : kChunk;
-        if (wave == 0) {
-            float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
-            const double last = sG[kChunk - 1];
-            const float eg = exp2_hw(sG[lane]), u = sU[lane];
-            sW[lane] = lane < past ? u * exp2_hw(last - sG[lane]) : 0.0f;
-            vec[lane] = lane < past ? u * eg : __builtin_nanf("");
-            vec[kChunk + lane] = sP[lane] * eg;
-            vec[2 * kChunk + lane] = exp2_hw(last);
-        }
         f32x4 vp[4] = {};
         {
             double gi[4];
@@ -549,8 +538,8 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
             }
         }
         __syncthreads();
-        {   // the diagonal blocks: column l16 of (I + A)^-1 by substitution
-            const float* A = sA + (16 * wave) * kPitchA + 16 * wave;
+        if (wave == 0) {   // the diagonal blocks: column l16 of block g4 of (I + A)^-1 by substitution
+            const float* A = sA + (16 * g4) * kPitchA + 16 * g4;
             float t[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
@@ -562,11 +551,17 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
                 }
                 t[i] = v0 + v1;
             }
-            float* D = sT + (16 * wave) * kPitchA + 16 * wave + l16;
-            if (g4 == 0) {
+            float* D = sT + (16 * g4) * kPitchA + 16 * g4 + l16;
 #pragma unroll
-                for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
-            }
+            for (int i = 0; i < 16; i++) D[i * kPitchA] = t[i];
+        } else if (wave == 1) {
+            float* const vec = (float*)(unit + kTri * (3 + LO) * kFrag);
+            const double last = sG[kChunk - 1];
+            const float eg = exp2_hw(sG[lane]), u = sU[lane];
+            sW[lane] = lane < past ? u * exp2_hw(last - sG[lane]) : 0.0f;
+            vec[lane] = lane < past ? u * eg : __builtin_nanf("");
+            vec[kChunk + lane] = sP[lane] * eg;
+            vec[2 * kChunk + lane] = exp2_hw(last);
         }
         __syncthreads();
         // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
@@ -611,31 +606,39 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
                 for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
         }
         __syncthreads();
-        f32x4 y[4] = {};                           // rows 16 wave of P (I + A)^-1
+        // P (I + A)^-1 by tiles (row, column), whose products' lengths are row - column + 1: five for each wave
+        const uint32_t tiles = (uint32_t)(0xFA5400E8009D000Cull >> 16 * wave) & 0xFFFF;      // 4 row + column, a nibble each
+        f32x4 y[4] = {};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (j > wave) break;
+        for (int q = 0; q < 4; q++) {
+            if (q > 1 && wave < 3) break;
+            const int i = tiles >> (4 * q + 2) & 3, j = tiles >> 4 * q & 3;
+            for (int k = j; k <= i; k++) {
 #pragma unroll
-            for (int k = j; k < 4; k++) {
-                if (k > wave) break;
-#pragma unroll
-                for (int s = 0; s < 4; s++) y[j] = mma4(at(sA, wave, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[j]);
+                for (int s = 0; s < 4; s++) y[q] = mma4(at(sA, i, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[q]);
             }
         }
         __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int q = 0; q < 4; q++) {
+            if (q > 1 && wave < 3) break;
+            const int i = tiles >> (4 * q + 2) & 3, j = tiles >> 4 * q & 3;
             const float bj = 16 * j + l16 < past ? sB[16 * j + l16] : 0.0f;
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-                const int at_ = (16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16;
-                sA[at_] = y[j][x] * bj;
-                sT[at_] = j <= (wave | 1) ? sT[at_] * bj : 0.0f;
-            }
+            for (int x = 0; x < 4; x++) sA[(16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = y[q][x] * bj;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > (wave | 1)) break;             // (what is above is not looked at, but within 32, where it is zeros)
+            const float bj = 16 * j + l16 < past ? sB[16 * j + l16] : 0.0f;
+#pragma unroll
+            for (int x = 0; x < 4; x++) sT[(16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16] *= bj;
         }
         __syncthreads();
-        store_triangle<3>(sT, sW, unit, wave, lane);
-        store_triangle<LO>(sA, nullptr, unit + kTri * 3 * kFrag, wave, lane);
+        for (int x = wave; x < 2 * kTri; x += 4) {
+            if (x < kTri) store_fragment<3>(sT, sW, unit, x, lane);
+            else store_fragment<LO>(sA, nullptr, unit + kTri * 3 * kFrag, x - kTri, lane);
+        }
     }
 }
 
