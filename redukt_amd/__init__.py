@@ -3,7 +3,8 @@
 The product is the shared library ``libredukt_gpu.so`` built from ``csrc/``: redukt's
 plugin C ABI (include/redukt_backend.h) over hand-written HIP kernels.  This package
 holds the host-side mirror of redukt's plugin loader and backend (``ffi``), the .rbin
-weight format (``rbin``) and the seeded synthetic workloads (``synth``).
+weight format (``rbin``), the seeded synthetic workloads (``synth``) and, on torch tensors,
+the operators of include/redukt_ops.h (``ops``).
 """
 import os
 

@@ -51,7 +51,9 @@ __device__ __forceinline__ float rows_sum(float v) {
 // One wave keeps 32 columns of one head's state in registers: lane 8 rg + c the rows rg DK/8
 // + [0, DK/8) of columns 4 c + [0, 4), so each load of the wave takes whole 128-byte lines.
 // Both sums over dk are formed from the state as it is read (S'^T q = a S^T q + (k.q) d), in one
-// exchange between the eight row groups.
+// exchange between the eight row groups, so the state is read and written once.
+// Bound by those bytes: 500 entries of 32 heads of 128 x 128, 2.1 GB, take 395 us (5.4 TB/s; a large copy moves 5.2, and some of
+// a pool stays in cache); 100 of 16 heads 34 us (6.3, mostly from cache).  One entry of a small model is the launch, 4 us.
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
     constexpr int R = DK / 8;
@@ -391,10 +393,13 @@ __device__ __forceinline__ double prefix_sum(double v) {
 // 2^x by the hardware (1 ulp; what is below 2^-126 becomes 0).
 __device__ __forceinline__ float exp2_hw(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// One workgroup a chunk and `per` value heads of one key head: their units, and with a key head's first value head the
-// fragments of k^T.
-// Bound by the chain of its steps (a read from memory, the products, the solve by blocks of 16, 32 and 64), so it
-// asks for all of its inputs at once, and several workgroups share a CU.
+// One workgroup a chunk and `per` value heads of one key head: their units.  (I + A)^-1 is solved by blocks: 16 by substitution,
+// all four of a chunk side by side in one wave, then 32 and 64 by products, which keeps it as exact as substitution (a product of
+// powers of A would not be, where keys are alike and the powers are large).
+// Bound by the chain of its steps, with four workgroups a CU beside each other: of 128 chunks of 32 heads, two to a key head, 50 us,
+// 12,000 cycles of a workgroup go to the request of its rows and their way to LDS, 4,000 to k.k and q.k, and 25,000 to each head (A and P
+// with their decays 5,000, the substitution 6,000, 32 and 64 5,000, P T and the strengths 5,000, the fragments' stores 4,500).  It
+// moves 200 MB in that time, 4 TB/s.
 template <typename T, int DK>
 __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 : 2) void k_delta_prep(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, SZ = sizeof(T);
@@ -565,12 +570,13 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
         }
         __syncthreads();
         // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
+        // (inner indices in the order 4 g + s: a lane's left elements are neighbours, and no bank is met twice on the right)
         const auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
         if (wave < 2) {
             const int i = 2 * wave + 1, j = 2 * wave;
             f32x4 m = {}, y = {};
 #pragma unroll
-            for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * s + g4), at(sT, j, j, 4 * s + g4, l16), m);
+            for (int s = 0; s < 4; s++) m = mma4(at(sA, i, j, l16, 4 * g4 + s), at(sT, j, j, 4 * g4 + s, l16), m);
 #pragma unroll
             for (int s = 0; s < 4; s++) y = mma4(at(sT, i, i, l16, 4 * g4 + s), m[s], y);
 #pragma unroll
@@ -592,7 +598,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
                 for (int q = 0; q < 2; q++) {
                     if (q < j) continue;
 #pragma unroll
-                    for (int s = 0; s < 4; s++) m = mma4(at(sA, 2 + p, q, l16, 4 * s + g4), at(sT, q, j, 4 * s + g4, l16), m);
+                    for (int s = 0; s < 4; s++) m = mma4(at(sA, 2 + p, q, l16, 4 * g4 + s), at(sT, q, j, 4 * g4 + s, l16), m);
                 }
 #pragma unroll
                 for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
@@ -615,7 +621,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
             const int i = tiles >> (4 * q + 2) & 3, j = tiles >> 4 * q & 3;
             for (int k = j; k <= i; k++) {
 #pragma unroll
-                for (int s = 0; s < 4; s++) y[q] = mma4(at(sA, i, k, l16, 4 * s + g4), at(sT, k, j, 4 * s + g4, l16), y[q]);
+                for (int s = 0; s < 4; s++) y[q] = mma4(at(sA, i, k, l16, 4 * g4 + s), at(sT, k, j, 4 * g4 + s, l16), y[q]);
             }
         }
         __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
@@ -647,7 +653,10 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
 // wave's would be; partial sums of K S, and X and D as limbs, pass between them through LDS, three barriers a chunk.
 // Waves 4 to 7 make the outputs of the same tokens from the limbs of S and X that they find there, beside the chain
 // instead of in it.  Every left operand is read by one wave only, straight from memory into registers, a chunk
-// ahead of its use.
+// ahead of its use; K^T comes from the rows of K by LDS, transposed as it is read.
+// Bound by the chunk's chain and by what a CU's L1 takes in beside it: 64 KB a chunk at dk 128 in bf16 (K, Q, T and P T), 1.7 us.  Of
+// 220 us for 128 chunks of 256 column tiles the chain alone, its operands standing still in registers, is 156; with the fragments of
+// K^T from memory too, 80 KB a chunk, it was 250.
 template <typename T, int DK, int NC>
 __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, NW = DK / 64, SZ = sizeof(T);

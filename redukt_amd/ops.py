@@ -105,8 +105,8 @@ def _stream(op: str, stream: Optional[int], device: int, allocates: bool) -> int
     return stream
 
 
-def _no_gradients(op: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradients(op: str, asked: bool) -> None:
+    if asked and torch.is_grad_enabled():
         _refuse(f"{op}: an input asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
 
 
@@ -142,7 +142,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
         _check(op, device, "g", g, torch.float32, tuple(v.shape[:2]))
         _check(op, device, "beta", beta, torch.float32, tuple(v.shape[:2]))
         _refuse(f"{op}: tensors do not belong together")
-    _no_gradients(op, q, k, v, g, beta)
+    _no_gradients(op, q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad)
     _, hv, dv = wide
     if out is None:
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
@@ -159,9 +159,13 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
 
 
 def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
-    _check(op, device, name, t, torch.float32, (t.shape[0] if isinstance(t, torch.Tensor) and t.dim() else 0, a.hv, a.dk, a.dv))
-    if not t.is_contiguous():
-        _refuse(f"{op}: {name} is not contiguous")
+    try:
+        if (t.dtype is torch.float32 and t.shape[1:] == (a.hv, a.dk, a.dv) and t.is_contiguous() and t.get_device() == device):
+            return
+    except AttributeError:
+        pass
+    _check(op, device, name, t, torch.float32, (None, a.hv, a.dk, a.dv))
+    _refuse(f"{op}: {name} is not contiguous")
 
 
 def _slots(op: str, device: int, slots, n: int) -> Optional[int]:
@@ -254,11 +258,11 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     device = _device(op, x)
     if x.dtype not in DTYPES or x.dim() != 2:
         _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
-    _no_gradients(op, x)
+    _no_gradients(op, x.requires_grad)
     on = _stream(op, stream, device, codes is None or scales is None)
     rows, cols = x.shape
     if codes is None:
-        codes = torch.empty((rows, cols), dtype=torch.int8, device=x.device)
+        codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     else:
         _check(op, device, "codes", codes, torch.int8, (rows, cols))
     if scales is None:
@@ -281,18 +285,25 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
     """
     op = "int8_matmul"
     device = _device(op, x)
-    _check(op, device, "x", x, torch.int8, (None, None))
-    m, k = x.shape
-    _check(op, device, "w", w, torch.int8, (None, k))
-    n = w.shape[0]
-    _check(op, device, "x_scales", x_scales, torch.float32, (m,))
-    _check(op, device, "w_scales", w_scales, torch.float32, (n,))
-    if bias is not None:
-        _check(op, device, "bias", bias, torch.float32, (n,))
-    for name, t in (("x_scales", x_scales), ("w_scales", w_scales), ("bias", bias)):
-        if t is not None and not t.is_contiguous():
-            _refuse(f"{op}: {name} is not contiguous")
-    _no_gradients(op, x_scales, w_scales, bias)
+    f32 = torch.float32
+    try:       # (all at once; what is wrong is looked for only if something is)
+        (m, k), (n, wk) = x.shape, w.shape
+        fine = (x.dtype is torch.int8 and w.dtype is torch.int8 and wk == k and x_scales.dtype is f32 and w_scales.dtype is f32
+                and x_scales.shape == (m,) and w_scales.shape == (n,) and x_scales.is_contiguous() and w_scales.is_contiguous()
+                and w.get_device() == x_scales.get_device() == w_scales.get_device() == device
+                and (bias is None or (bias.dtype is f32 and bias.shape == (n,) and bias.is_contiguous()
+                                      and bias.get_device() == device)))
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:
+        _check(op, device, "x", x, torch.int8, (None, None))
+        _check(op, device, "w", w, torch.int8, (None, x.shape[1]))
+        _check(op, device, "x_scales", x_scales, f32, (x.shape[0],))
+        _check(op, device, "w_scales", w_scales, f32, (w.shape[0],))
+        if bias is not None:
+            _check(op, device, "bias", bias, f32, (w.shape[0],))
+        _refuse(f"{op}: scales and bias are contiguous")
+    _no_gradients(op, x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad))
     on = _stream(op, stream, device, out is None)
     if out is None:
         if dtype not in DTYPES:
