@@ -393,40 +393,33 @@ __device__ __forceinline__ double prefix_sum(double v) {
 // 2^x by the hardware (1 ulp; what is below 2^-126 becomes 0).
 __device__ __forceinline__ float exp2_hw(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// One workgroup a chunk and `per` value heads of one key head: their units.  (I + A)^-1 is solved by blocks: 16 by substitution,
-// all four of a chunk side by side in one wave, then 32 and 64 by products, which keeps it as exact as substitution (a product of
-// powers of A would not be, where keys are alike and the powers are large).
-// Bound by the chain of its steps, with four workgroups a CU beside each other: of 128 chunks of 32 heads, two to a key head, 50 us,
-// 12,000 cycles of a workgroup go to the request of its rows and their way to LDS, 4,000 to k.k and q.k, and 25,000 to each head (A and P
-// with their decays 5,000, the substitution 6,000, 32 and 64 5,000, P T and the strengths 5,000, the fragments' stores 4,500).  It
-// moves 200 MB in that time, 4 TB/s.
 template <typename T, int DK>
-__global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 : 2) void k_delta_prep(ChunkArgs a) {
-    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, SZ = sizeof(T);
-    constexpr int PK = DK + 16 / SZ;           // rows of odd multiples of 16 bytes: 16 neighbouring ones meet no bank twice
+struct PrepLds {
+    static constexpr int PK = DK + 16 / sizeof(T);     // rows of odd multiples of 16 bytes: 16 neighbouring ones meet no bank twice
+    static constexpr int kRows = 2 * kChunk * PK * sizeof(T), kMatrices = 2 * kChunk * kPitchA * 4;
+    __attribute__((aligned(16))) unsigned char m[kRows > kMatrices ? kRows : kMatrices];      // k and q, then A and T
+    double g[kChunk];
+    float b[kChunk], u[kChunk], p[kChunk], w[kChunk];
+};
+
+// Four waves make the units of one chunk, `len` rows from t0 on, and of `per` value heads of one key head.  (I + A)^-1 is solved by
+// blocks: 16 by substitution, all four of a chunk side by side in one wave, then 32 and 64 by products, which keeps it as exact as
+// substitution (a product of powers of A would not be, where keys are alike and the powers are large).
+constexpr int kPrepBarriers = 9;               // that prepare() passes for one head
+template <typename T, int DK>
+__device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds, uint32_t slot, uint32_t t0, uint32_t len, uint32_t h0,
+                                        uint32_t per) {
+    constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, KS = DK / 32, SZ = sizeof(T), PK = PrepLds<T, DK>::PK;
     constexpr int kLoads = kChunk * DK * SZ / 16 / 256;
-    constexpr int kBytes = 2 * kChunk * PK * SZ > 2 * kChunk * kPitchA * 4 ? 2 * kChunk * PK * SZ : 2 * kChunk * kPitchA * 4;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kBytes];       // k and q, then A and T
-    __shared__ double sG[kChunk];
-    __shared__ float sB[kChunk], sU[kChunk], sP[kChunk], sW[kChunk];
-    T* const sK = (T*)lds;
+    double* const sG = lds.g;
+    float *const sB = lds.b, *const sU = lds.u, *const sP = lds.p, *const sW = lds.w;
+    T* const sK = (T*)lds.m;
     T* const sQ = sK + kChunk * PK;
-    float* const sA = (float*)lds;
+    float* const sA = (float*)lds.m;
     float* const sT = sA + kChunk * kPitchA;
     const redukt_delta_rows& r = a.d.r;
     const int lane = threadIdx.x % kWave, wave = wave_index(), g4 = lane / 16, l16 = lane % 16;
-    const uint32_t slots_h = r.hv / a.per, slot = blockIdx.x / slots_h, h0 = blockIdx.x % slots_h * a.per, group = r.hv / r.hk, hq = h0 / group;
-    uint32_t lo = 0, hi = a.d.n - 1;           // the last sequence that starts at this slot or before
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi + 1) / 2;
-        if (first_chunk(row_of(a, mid), mid) <= slot) lo = mid;
-        else hi = mid - 1;
-    }
-    const uint32_t b = row_of(a, lo), e = row_of(a, lo + 1), first = first_chunk(b, lo);
-    if (slot < first) return;
-    const uint64_t t0_ = (uint64_t)b + (uint64_t)(slot - first) * kChunk;
-    if (t0_ >= e) return;
-    const uint32_t t0 = (uint32_t)t0_, len = min(e - t0, (uint32_t)kChunk);
+    const uint32_t hq = h0 / (r.hv / r.hk);
 
     float g0 = 0.0f, beta = 0.0f;              // of token `lane` and one value head, in wave 0
     const auto load_gates = [&](uint32_t h) {
@@ -497,7 +490,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     __syncthreads();                           // k and q are done with; sU, sP are written
 
     int here = threadIdx.x;
-    for (uint32_t h = h0; h < h0 + a.per; h++) {
+    for (uint32_t h = h0; h < h0 + per; h++) {
         asm volatile("" : "+v"(here));          // (addresses are made anew for each head: kept, they would take 80 registers)
         const int lane = here % kWave, g4 = lane / 16, l16 = lane % 16;
         if (h > h0) {
@@ -505,7 +498,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
             put_gates();
             __syncthreads();
         }
-        if (h + 1 < h0 + a.per) load_gates(h + 1);
+        if (h + 1 < h0 + per) load_gates(h + 1);
         unsigned char* const unit = a.ws + ((size_t)h * a.slots + slot) * unit_bytes(LO);
         // from the first token `past` whose key, g or beta is not finite on there are no rows
         const uint64_t bads = __ballot(sU[lane] != sU[lane] || sB[lane] != sB[lane]);
@@ -648,6 +641,27 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
     }
 }
 
+// A workgroup a chunk and `per` value heads, for all chunks and heads side by side.
+// Bound by the chain of its steps, with four workgroups a CU beside each other: of 128 chunks of 32 heads, two to a key head, 50 us,
+// 12,000 cycles of a workgroup go to the request of its rows and their way to LDS, 4,000 to k.k and q.k, and 23,500 to each head (A and P
+// with their decays 6,000, the substitution 5,400, 32 and 64 3,500, P T and the strengths 5,500, the fragments' stores 2,600).  It
+// moves 200 MB in that time, 4 TB/s, three quarters of what a copy moves.
+template <typename T, int DK>
+__global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 : 2) void k_delta_prep(ChunkArgs a) {
+    __shared__ PrepLds<T, DK> lds;
+    const uint32_t slots_h = a.d.r.hv / a.per, slot = blockIdx.x / slots_h, h0 = blockIdx.x % slots_h * a.per;
+    uint32_t lo = 0, hi = a.d.n - 1;           // the last sequence that starts at this slot or before
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi + 1) / 2;
+        if (first_chunk(row_of(a, mid), mid) <= slot) lo = mid;
+        else hi = mid - 1;
+    }
+    const uint32_t b = row_of(a, lo), e = row_of(a, lo + 1), first = first_chunk(b, lo);
+    if (slot < first) return;
+    const uint64_t t0 = (uint64_t)b + (uint64_t)(slot - first) * kChunk;
+    if (t0 < e) prepare<T, DK>(a, lds, slot, (uint32_t)t0, min(e - (uint32_t)t0, (uint32_t)kChunk), h0, a.per);
+}
+
 // One workgroup takes 16 NC columns of one head's state through a sequence.  Waves 0 to 3 carry the state: each owns a
 // quarter of its rows and of a chunk's tokens, so the chain of a chunk (S -> X -> D -> S) is a quarter as long as one
 // wave's would be; partial sums of K S, and X and D as limbs, pass between them through LDS, three barriers a chunk.
@@ -657,7 +671,9 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
 // Bound by the chunk's chain and by what a CU's L1 takes in beside it: 64 KB a chunk at dk 128 in bf16 (K, Q, T and P T), 1.7 us.  Of
 // 220 us for 128 chunks of 256 column tiles the chain alone, its operands standing still in registers, is 156; with the fragments of
 // K^T from memory too, 80 KB a chunk, it was 250.
-template <typename T, int DK, int NC>
+//
+// ALONE: sequences of one chunk at most, whose units waves 0 to 3 make first, each column tile's workgroup the same ones.
+template <typename T, int DK, int NC, bool ALONE>
 __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     constexpr int LI = Limbs<T>::in, LO = Limbs<T>::out, NW = DK / 64, SZ = sizeof(T);
     constexpr int KF = 4 * NW;                 // a lane's inner indices of one wave's rows of the state
@@ -689,6 +705,18 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
     const auto live = [&](int nc) { return col0 + 16 * nc < r.dv; };
     const auto col_of = [&](int nc) { return live(nc) ? col0 + 16 * nc : (uint32_t)l16; };
     const uint32_t chunks = (e - b + kChunk - 1) / kChunk, first = first_chunk(b, i);
+    if constexpr (ALONE) {
+        __shared__ PrepLds<T, DK> lds;
+        if (chunks) {
+            if (wave_index() < 4) {
+                prepare<T, DK>(a, lds, first, b, e - b, h, 1);
+                __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0): the unit is written before it is read
+            } else {
+                for (int x = 0; x < kPrepBarriers; x++) __syncthreads();
+            }
+            __syncthreads();
+        }
+    }
     typedef T vecK __attribute__((ext_vector_type(KF)));
     // Rows of a chunk by buffer accesses, whose bounds end the chunk (they count the vector offset only, so the
     // scalar one stays 0): a pointer that moves on by a chunk, and the bytes of the chunk's rows.
@@ -1031,9 +1059,15 @@ const void* delta_prep_fn(uint32_t dtype, uint32_t dk) {
     return fns[dtype][dk == 128];
 }
 
-template <typename T, int NC>
+template <typename T, int NC, bool ALONE = false>
 const void* delta_chunks_of(uint32_t dk) {
-    return dk == 128 ? (const void*)k_delta_chunks<T, 128, NC> : (const void*)k_delta_chunks<T, 64, NC>;
+    return dk == 128 ? (const void*)k_delta_chunks<T, 128, NC, ALONE> : (const void*)k_delta_chunks<T, 64, NC, ALONE>;
+}
+
+const void* delta_alone_fn(uint32_t dtype, uint32_t dk) {
+    return dtype == REDUKT_OP_BF16  ? delta_chunks_of<__bf16, 1, true>(dk)
+           : dtype == REDUKT_OP_F16 ? delta_chunks_of<_Float16, 1, true>(dk)
+                                    : delta_chunks_of<float, 1, true>(dk);
 }
 
 // NC 1, 2, or 4, the last with 16-bit elements only (in f32 its limbs do not fit LDS).
@@ -1060,11 +1094,16 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
     // workgroups waiting for a CU.  Ragged sequences of 16 heads of 128 columns, us with 1, 2 and 4 tiles: 5 of them (640 tiles) 88, 94
     // and 138; 10 (1,280) 96, 78 and 97; 20 (2,560) 153, 118 and 107; 37 (4,736) 296, 230 and 196.
     const uint64_t all = (uint64_t)k.d.n * r.hv * (r.dv / 16);
+    // No sequence of 64 rows in all has a second chunk: the preparation goes into the same launch, once for each column tile, while every
+    // workgroup has a CU of its own (us in two launches and one: 50 tokens of 12 heads of 64 columns, 48 tiles, 13.5 and 12.2; 64 of 32 heads
+    // of 128, 256 tiles, 16.3 and 14.6; two such sequences, 512 tiles, 20.6 and 25.5).
+    const bool alone = r.rows <= kChunk && all <= 256;
     const uint32_t NC = all >= 2048 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;
     if (!op_grid_ok(prep, 256) || !op_grid_ok(grid, 512)) return BACKEND_INVALID_ARGUMENT;
     k.slots = (uint32_t)chunk_slots(r, k.d.n);
+    if (alone) return op_launch(delta_alone_fn(r.dtype, r.dk), dim3((uint32_t)grid), dim3(512), 0, stream, k);
     if (r.rows) {
         const int32_t rc = op_launch(delta_prep_fn(r.dtype, r.dk), dim3((uint32_t)prep), dim3(256), 0, stream, k);
         if (rc != BACKEND_OK) return rc;

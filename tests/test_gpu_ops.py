@@ -209,6 +209,31 @@ def test_delta_chunk_lengths(lens, dk, dv, dtype):
 
 
 @types
+@pytest.mark.parametrize("lens", [[64], [30, 0, 34], [1] * 16, [5, 0, 0, 50, 3]], ids=lambda v: "-".join(map(str, v)))
+@pytest.mark.parametrize("dk,dv,hk,hv", [(64, 64, 2, 2), (128, 160, 1, 3), (128, 256, 1, 16)])
+def test_delta_chunk_of_64_rows_at_most(dk, dv, hk, hv, lens, dtype):
+    """Few rows in all, with few column tiles and with many."""
+    sequences(lens, hk, hv, dk, dv, dtype, normalize=hk == 1, initial=True, seed=hv)
+
+
+@types
+@pytest.mark.parametrize("which", ["v", "k", "g", "beta"])
+def test_delta_chunk_of_50_rows_what_is_not_finite(which, dtype):
+    x = rule_inputs(50, 2, 2, 64, 64, dtype, seed=2, normalize=True)
+    cu = torch.tensor([0, 20, 50], dtype=torch.int32, device="cuda")
+    S = torch.zeros(2, 2, 64, 64, device="cuda")
+    want = ops.delta_chunk(*x, cu, state_out=S, normalize=True)
+    y = [t.clone() for t in x]
+    y[{"v": 2, "k": 1, "g": 3, "beta": 4}[which]][33, 1] = float("nan")
+    S2 = torch.zeros_like(S)
+    got = ops.delta_chunk(*y, cu, state_out=S2, normalize=True)
+    bad = torch.zeros(50, 2, 64, dtype=torch.bool, device="cuda")
+    bad[33:, 1] = True
+    assert torch.equal(got[~bad], want[~bad]) and not torch.isfinite(got[bad]).any()
+    assert torch.equal(S2[0], S[0]) and torch.equal(S2[1, 0], S[1, 0]) and not torch.isfinite(S2[1, 1]).any()
+
+
+@types
 @pytest.mark.parametrize("hk,hv,dk,dv", [(1, 1, 64, 32), (3, 3, 64, 96), (1, 4, 128, 64), (2, 2, 128, 256), (4, 12, 64, 160)])
 def test_delta_chunk_heads(hk, hv, dk, dv, dtype):
     sequences([70, 1, 130], hk, hv, dk, dv, dtype, normalize=True, initial=False, seed=hv)
