@@ -175,6 +175,25 @@ def test_delta_step_on_another_stream_and_captured():
         assert torch.equal(out, want) and torch.equal(a, b)
 
 
+def test_delta_step_slots_named_twice_among_many():
+    """Entries far apart and neighbouring ones, each side of a thousand."""
+    n = 2500
+    x = rule_inputs(n, 1, 1, 64, 32, BF16)
+    slots = torch.randperm(n, generator=gen(5), device="cuda").to(torch.int32)
+    twice = {2499: 3, 1500: 1499, 1030: 1025, 1024: 1023, 700: 0, 2000: 64}
+    lone = slots.clone()
+    for late, early in twice.items():
+        slots[late] = slots[early]
+        lone[late] = -1
+    pool = pool_of(n, 1, 64, 32)
+    want_pool = pool.clone()
+    got = ops.delta_step(*x, pool, slots=slots)
+    want = ops.delta_step(*x, want_pool, slots=lone)
+    late = torch.zeros(n, dtype=torch.bool, device="cuda")
+    late[list(twice)] = True
+    assert got[late].isnan().all() and torch.equal(got[~late], want[~late]) and torch.equal(pool, want_pool)
+
+
 # ---------------------------------------------------------------- sequences
 
 def sequences(lens, hk, hv, dk, dv, dtype, normalize, initial, behind=0, seed=0, forget=1.0, check_state=True):
