@@ -142,7 +142,8 @@ __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
 }
 
 // Up to 16 tokens: the weights are read once, straight into registers, and nothing else costs much (one token of 50,280 x 768:
-// 38.6 MB in 10.2 us, 3.8 TB/s with the launch; of 8,192 x 8,192 67 MB in 17.6).  Of a workgroup's eight waves `split` share 16 channels, each taking every split-th line
+// 38.6 MB in 10.2 us, 3.8 TB/s with the launch; of 8,192 x 8,192 67 MB in 13.8, 4.9).  Workgroups begin at different columns: rows of a
+// power of two put the same columns into the same channel of a cache, where all would wait at once (8,192 x 8,192: 17.6 -> 13.8 us).  Of a workgroup's eight waves `split` share 16 channels, each taking every split-th line
 // of 128 columns; their sums meet in LDS.
 struct Int8Few {
     redukt_int8_matmul a;
@@ -160,7 +161,9 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Few f) {
     const int8_t* const x = a.x + (int64_t)min((uint32_t)l16, a.m - 1) * a.x_stride;
     i32x4 acc = {};
     if (j0 < a.n) {
-        for (uint32_t c = wave % split; c < lines; c += split) {
+        const uint32_t rot = blockIdx.x * 4 % lines;
+        for (uint32_t turn = wave % split; turn < lines; turn += split) {
+            const uint32_t c = turn + rot - (turn + rot >= lines ? lines : 0);
             // (columns past k: the last ones again, against zeros)
             uint32_t at[2];
             i32x4 fw[2], fx[2];
@@ -448,7 +451,7 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
         return op_launch(OP_BY_TYPE(a->dtype, k_int8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
     // Every kernel gives the same bits, so the choice is by time alone (us, on either side of each edge; n and k after m).  Up to
-    // 16 tokens: weights straight into registers (16 of 8,192 x 8,192: 19.0, tiles 22.9; 33: 22.9 at two row tiles and 24.6).
+    // 16 tokens: weights straight into registers (16 of 8,192 x 8,192: 18.8, tiles 22.9; 33: 22.9 at two row tiles and 24.6).
     if (a->m <= 16) return few(*a, stream);
     // Tiles of 256 once they fill the CUs (8,192 of 8,192 x 4,096: 249, tiles of 128: 291; 2,048 of 4,096 x 1,536, 128 tiles: 27.8 and
     // 20.9), of 128 once they nearly do (4,096 of 768 x 768, 192 tiles: 10.3, tiles of 64: 10.8; 1,000 of 1,536 x 768, 96 tiles:
