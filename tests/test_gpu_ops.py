@@ -457,6 +457,82 @@ def test_delta_chunk_captured_twice_with_a_workspace_each():
             assert torch.equal(out, want) and torch.equal(s, S)
 
 
+def test_delta_chunk_replayed_with_other_lengths_and_slots():
+    """A captured call reads the lengths and slots, like everything else, when it is replayed."""
+    T, n = 300, 5
+    x = rule_inputs(T, 2, 4, 64, 64, BF16, normalize=True)
+    cu, slots = torch.zeros(n + 1, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.int32, device="cuda")
+    pool, eager = pool_of(8, 4, 64, 64), pool_of(8, 4, 64, 64)
+    out = torch.full((T, 4, 64), 7.0, dtype=BF16, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.delta_chunk(*x, cu, state_in=pool, state_out=pool, slots=slots, out=out, normalize=True)
+    for at, to in [([0, 300, 300, 300, 300, 300], [0, 1, 2, 3, 4]), ([7, 20, 21, 150, 150, 299], [5, -1, 0, 7, 5]),
+                   ([0, 0, 64, 128, 129, 300], [4, 3, 2, 1, 0]), ([10, 20, 30, 40, 50, 60], [-1, -1, -1, 8, -2])]:
+        cu.copy_(torch.tensor(at, dtype=torch.int32))
+        slots.copy_(torch.tensor(to, dtype=torch.int32))
+        out.fill_(7.0)
+        want = torch.full_like(out, 7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        ops.delta_chunk(*x, cu, state_in=eager, state_out=eager, slots=slots, out=want, normalize=True)
+        assert torch.equal(out.nan_to_num(9.0), want.nan_to_num(9.0)) and torch.equal(pool, eager)
+        assert (want[:at[0]] == 7.0).all() and (want[at[-1]:] == 7.0).all() and not (want[:at[0]] != want[:at[0]]).any()
+
+
+@types
+def test_delta_chunk_slices_of_a_projection(dtype):
+    n, hk, hv, dk, dv = 200, 2, 4, 128, 64
+    x = rule_inputs(n, hk, hv, dk, dv, dtype, seed=3, normalize=True)
+    fused = torch.cat([torch.full((n, 8), float("nan"), dtype=dtype, device="cuda")] + [t.flatten(1) for t in x[:3]], 1)
+    w, o = hk * dk, 8
+    q, k, v = (fused[:, o:o + w].view(n, hk, dk), fused[:, o + w:o + 2 * w].view(n, hk, dk), fused[:, o + 2 * w:].view(n, hv, dv))
+    gates = torch.cat([x[3], x[4]], 1)
+    wide = torch.full((n, hv * dv + 64), 7.0, dtype=dtype, device="cuda")
+    cu = torch.tensor([0, 3, 131, n], dtype=torch.int32, device="cuda")
+    a, b = torch.empty(3, hv, dk, dv, device="cuda"), torch.empty(3, hv, dk, dv, device="cuda")
+    out = ops.delta_chunk(q, k, v, gates[:, :hv], gates[:, hv:], cu, state_out=a, out=wide[:, :hv * dv].view(n, hv, dv), normalize=True)
+    assert torch.equal(out, ops.delta_chunk(*x, cu, state_out=b, normalize=True)) and torch.equal(a, b)
+    assert (wide[:, hv * dv:] == 7.0).all()
+
+
+def test_delta_chunk_offsets_past_32_bits():
+    """Rows and states beyond 2^32 bytes: the last sequence of many rows is the same as alone."""
+    hk, hv, dk, dv, n = 1, 64, 64, 256, 140000
+    x = rule_inputs(100, hk, hv, dk, dv, BF16, normalize=True)
+    wide = [torch.zeros(n, *t.shape[1:], dtype=t.dtype, device="cuda") for t in x]
+    for t, part in zip(wide, x):
+        t[n - 100:] = part
+    slots = 2 ** 31 // (hv * dk * dv) + 2
+    pool, one = torch.empty(slots, hv, dk, dv, device="cuda"), pool_of(1, hv, dk, dv)
+    pool[slots - 1] = one[0]
+    cu = torch.tensor([n - 100, n], dtype=torch.int32, device="cuda")
+    out = ops.delta_chunk(*wide, cu, state_in=pool, state_out=pool, slots=torch.tensor([slots - 1], dtype=torch.int32, device="cuda"), normalize=True)
+    want = ops.delta_chunk(*x, torch.tensor([0, 100], dtype=torch.int32, device="cuda"), state_in=one, state_out=one, normalize=True)
+    assert torch.equal(out[n - 100:], want) and torch.equal(pool[slots - 1], one[0])
+
+
+def test_the_most_entries_and_sequences():
+    n = 65536
+    x = rule_inputs(n, 1, 1, 64, 32, BF16)
+    pool = pool_of(n, 1, 64, 32)
+    before = pool.clone()
+    out = ops.delta_step(*x, pool)
+    S = before.clone()
+    cu = torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    chunk = ops.delta_chunk(*x, cu, state_in=S, state_out=S)
+    at = [0, 1, 40000, n - 1]
+    for i in at:
+        want, S64, tol, S_tol = ops_f64.rule(*(t[i:i + 1] for t in x), before[i])
+        check(out[i:i + 1], want, tol, i)
+        check(chunk[i:i + 1], want, tol, i)
+        check(pool[i], S64, S_tol, i)
+        check(S[i], S64, S_tol, i)
+    more = [torch.cat([t, t[:1]]) for t in x]
+    refused(lambda: ops.delta_step(*more, torch.empty(n + 1, 1, 64, 32, device="cuda")))
+    refused(lambda: ops.delta_chunk(*more, torch.arange(n + 2, dtype=torch.int32, device="cuda")))
+
+
 @types
 def test_a_sequence_alone_is_the_sequence_in_a_batch(dtype):
     """A sequence's bits do not depend on what else the call holds."""
@@ -657,6 +733,19 @@ def test_int8_matmul_strided_and_unaligned(m, n, k, off, pad, dtype):
     ops.int8_matmul(wide(x), sx, wide(w), sw, bias=bias, out=out[:, off:off + n])
     check(out[:, off:off + n], *ops_f64.matmul(x, sx, w, sw, bias, dtype), "y")
     assert (out[:, :off] == 7.0).all() and (out[:, off + n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("m,n,of", [(45000, 50280, "out"), (4200, 300, "x"), (3, 1100, "w"), (300, 1100, "w")])
+def test_int8_matmul_offsets_past_32_bits(m, n, of):
+    x, sx, w, sw, bias = product(m, n, 64)
+    wx, ww = x, w
+    if of == "x":
+        wx = torch.empty(m, 1 << 20, dtype=torch.int8, device="cuda")[:, :64].copy_(x)
+    if of == "w":
+        ww = torch.empty(n, 1 << 22, dtype=torch.int8, device="cuda")[:, :64].copy_(w)
+    got = ops.int8_matmul(wx, sx, ww, sw, bias=bias)
+    for rows in (slice(0, 3), slice(m - 3, m)):
+        assert torch.equal(got[rows], ops.int8_matmul(x[rows], sx[rows], w, sw, bias=bias))
 
 
 @pytest.mark.parametrize("m,n,k", [(3, 1000, 768), (100, 500, 512), (700, 600, 256)])
