@@ -1099,10 +1099,11 @@ int32_t launch_chunks(ChunkArgs& k, void* stream) {
     // workgroups waiting for a CU.  Ragged sequences of 16 heads of 128 columns, us with 1, 2 and 4 tiles: 5 of them (640 tiles) 88, 94
     // and 138; 10 (1,280) 96, 78 and 97; 20 (2,560) 153, 118 and 107; 37 (4,736) 296, 230 and 196.
     const uint64_t all = (uint64_t)k.d.n * r.hv * (r.dv / 16);
-    // No sequence of 64 rows in all has a second chunk: the preparation goes into the same launch, once for each column tile, while every
-    // workgroup has a CU of its own (us in two launches and one: 50 tokens of 12 heads of 64 columns, 48 tiles, 13.5 and 12.2; 64 of 32 heads
-    // of 128, 256 tiles, 16.3 and 14.6; two such sequences, 512 tiles, 20.6 and 25.5).
-    const bool alone = r.rows <= kChunk && all <= 256;
+    // No sequence of 64 rows in all has a second chunk: the preparation goes into the same launch, once for each column tile, while all
+    // workgroups are on the CUs at once, one on each, or two at dk 64 with 16-bit elements (us in two launches and one, bf16: 12 heads of
+    // 64 columns, 48 tiles, 13.5 and 12.2, ten such sequences, 480 tiles, 17.5 and 16.0, twelve, 576, 20.1 and 25.0; 32 heads of 128,
+    // 256 tiles, 16.3 and 14.6, 40, 320 tiles, 19.6 and 25.2).
+    const bool alone = r.rows <= kChunk && all <= (r.dk == 64 && r.dtype != REDUKT_OP_F32 ? 512 : 256);
     const uint32_t NC = all >= 2048 && r.dtype != REDUKT_OP_F32 ? 4 : all >= 1024 ? 2 : 1;
     const uint64_t cols = (r.dv / 16 + NC - 1) / NC, units = (uint64_t)k.d.n * r.hk;
     const uint64_t grid = (units + kXcds - 1) / kXcds * kXcds * (r.hv / r.hk) * cols;

@@ -533,6 +533,29 @@ def test_the_most_entries_and_sequences():
     refused(lambda: ops.delta_chunk(*more, torch.arange(n + 2, dtype=torch.int32, device="cuda")))
 
 
+def test_two_streams_at_once():
+    """Calls on two streams with nothing in common, workspaces of their own, several times over."""
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for k in range(2):
+        lens = [700 + 300 * k, 64, 130]
+        x = rule_inputs(sum(lens), 4, 8, 128, 128, BF16, seed=k, normalize=True)
+        cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        codes = product(300, 280, 320, seed=k)
+        S = torch.empty(3, 8, 128, 128, device="cuda")
+        jobs.append((x, cu, S, codes, ops.delta_chunk(*x, cu, state_out=S, normalize=True), S.clone(), ops.int8_matmul(*codes)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for side, (x, cu, S, codes, *_) in zip(sides, jobs):
+            with torch.cuda.stream(side):
+                S.zero_()
+                got.append((ops.delta_chunk(*x, cu, state_out=S, normalize=True), ops.int8_matmul(*codes)))
+        torch.cuda.synchronize()
+        for (out, y), (_, _, S, _, want, S_want, y_want) in zip(got, jobs):
+            assert torch.equal(out, want) and torch.equal(S, S_want) and torch.equal(y, y_want)
+
+
 @types
 def test_a_sequence_alone_is_the_sequence_in_a_batch(dtype):
     """A sequence's bits do not depend on what else the call holds."""
