@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256, Limbs<T>::in == 1 ? 4 : Limbs<T>::in == 2 ? 3 
 // instead of in it.  Every left operand is read by one wave only, straight from memory into registers, a chunk
 // ahead of its use; K^T comes from the rows of K by LDS, transposed as it is read.
 // Bound by the chunk's chain and by what a CU's L1 takes in beside it: 64 KB a chunk at dk 128 in bf16 (K, Q, T and P T), 1.7 us.  Of
-// 220 us for 128 chunks of 256 column tiles the chain alone, its operands standing still in registers, is 156; with the fragments of
+// 215 us for 128 chunks of 256 column tiles the chain alone, its operands standing still in registers, is 156; with the fragments of
 // K^T from memory too, 80 KB a chunk, it was 250.
 //
 // ALONE: sequences of one chunk at most, whose units waves 0 to 3 make first, each column tile's workgroup the same ones.
@@ -828,16 +828,24 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         };
         // K^T for the last step: this wave's columns of K, which it holds as rows, go through LDS and come back transposed, 4 tokens x
         // 16 columns by 16 lanes.  A row's pieces of KF columns stand at place (piece ^ row / 8 % 4).
-        const auto put_k = [&](int o) {
-            const int row = tile_index((wave + o) % 4, l16), at = row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2);
-            if constexpr (kRaw) {
-                *(vecK*)(sK[wave][0] + at) = kf[o];
-            } else {
-                const Part<NW, LI> k = limbs(kf[o]);
+        Part<NW, LI> kl[4];                    // the limbs of kf
+        const auto split_k = [&]() {
 #pragma unroll
-                for (int n = 0; n < LI; n++) *(typename Part<NW, LI>::vec*)(sK[wave][n] + at) = k.l[n];
+            for (int o = 0; o < 4; o++) {
+                const int row = tile_index((wave + o) % 4, l16), at = row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2);
+                kl[o] = limbs(kf[o]);
+                if constexpr (kRaw) {
+                    *(vecK*)(sK[wave][0] + at) = kf[o];
+                } else {
+#pragma unroll
+                    for (int n = 0; n < LI; n++) *(typename Part<NW, LI>::vec*)(sK[wave][n] + at) = kl[o].l[n];
+                }
             }
         };
+        // Where the chain's length counts most, a chunk's K is requested as the chunk before begins, and split beside its last products; else
+        // it is split as its own chunk begins (us late and early: 8,192 tokens of 32 heads of 128, 275 and 266; 37 ragged prompts with four
+        // tiles, 192 and 196; 12 sequences of heads of 64, 194 and 198).
+        constexpr bool kEarly = DK == 128 && NC < 4;
         const auto get_kt = [&](int p, int s, int n) {       // row l16 of tile p, the tokens 32 s + 8 g4 + [0, 8)
             typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
             const unsigned char* const at = sK[wave][n] + (32 * s + 8 * g4 + l16 / 4) * (NW * 32) + (l16 % 4 ^ g4) * (KF * 2) + 8 * p;
@@ -860,6 +868,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             load_v(rows);
             load_t();
             load_keep();
+            if (kEarly) split_k();
         }
         for (uint32_t c = 0; c < chunks; c++) {
             // (the last chunk requests itself again instead of one past the end)
@@ -869,8 +878,8 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             rk.step(on), rv.step(on);
             unit += on * unit_bytes(LO);
             f32x4 X[NC];
-#pragma unroll
-            for (int o = 0; o < 4; o++) put_k(o);
+            if (kEarly) load_k(rows);
+            else split_k();
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 float v[KF];
@@ -886,13 +895,13 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                     for (int n = 0; n < LI; n++)
                         if (n + j < 3) {
 #pragma unroll
-                            for (int o = 0; o < 4; o++) y[o] = mma_part(limbs(kf[o]).l[n], x.l[j], y[o]);
+                            for (int o = 0; o < 4; o++) y[o] = mma_part(kl[o].l[n], x.l[j], y[o]);
                         }
                 X[nc] = y[0];
 #pragma unroll
                 for (int o = 1; o < 4; o++) sR[nc][(wave + o) % 4][3 - o][lane] = y[o];
             }
-            load_k(rows);
+            if (!kEarly) load_k(rows);
             __syncthreads();                   // A: S and partial sums are there
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
@@ -950,6 +959,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
             for (int nc = 0; nc < NC; nc++) {
                 const Split<3> x0 = get(sD[nc][0], Int<3>()), x1 = get(sD[nc][1], Int<3>());
+                if (kEarly && nc == 0) split_k();
 #pragma unroll
                 for (int p = 0; p < NW; p++) {
 #pragma unroll
