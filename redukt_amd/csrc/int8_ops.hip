@@ -200,7 +200,8 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Few f) {
 // lane picks the piece that belongs to its place.
 //
 // Tiles of 256 x 256 are bound by the matrix cores and the LDS reads beside them: 8,192 of 8,192 x 4,096 in 249 us, 2.2 POP/s (the
-// library's int8 product 250).  Those of 64 x 64 by their chain of loads: 100 of 4,096 x 1,536 is 6 us, five steps of 256 columns.
+// library's int8 product 250).  The smaller ones by the columns on their way: 64 of 8,192 x 8,192 in 15.2, 67 MB at 4.4 TB/s; 100 of
+// 4,096 x 1,536 in 6.5, the launch and twelve steps.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 typedef __attribute__((address_space(3))) void lds_void;
@@ -257,10 +258,15 @@ struct Int8Tiles {
     uint32_t wide;             // rows of out take 16-byte stores
 };
 
-// s_waitcnt vmcnt(N), the other counters as they are.
+// All but this wave's last N loads into LDS are done, and what it read from LDS is there; then the workgroup meets.  (__syncthreads
+// would wait for every load.)
 template <int N>
-__device__ __forceinline__ void wait_loads() {
-    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0f70);
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x0070);        // vmcnt(N) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
 template <typename T, int TM, int TN, int WM, int WN, int KC, int STAGES>
@@ -303,14 +309,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_int8_tiles(Int8Tiles f) {
 #pragma unroll
         for (int s = 0; s < STAGES; s++) {
             if (c + s * KC >= a.k) break;
-            wait_loads<kPending>();
-            __syncthreads();
+            wait_and_meet<kPending>();
             stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * KC);
             multiply<KC, NI, NJ>((const lds_u8*)lds[s], (const lds_u8*)lds[s] + TN * KC, acc, ri, rj, lane);
         }
     }
-    wait_loads<0>();                           // (zeros may still be on their way)
-    __syncthreads();
+    wait_and_meet<0>();                        // (zeros may still be on their way)
 
     // 32 tokens of a wave's channels at a time through LDS, so that a row of them is stored as whole lines.
     constexpr int CH = TN / WN, kRow = CH * sizeof(T), kOuts = kRow / 16, kPer = 16 / sizeof(T);
@@ -451,14 +455,21 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
         return op_launch(OP_BY_TYPE(a->dtype, k_int8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
     // Every kernel gives the same bits, so the choice is by time alone (us, on either side of each edge; n and k after m).  Up to
-    // 16 tokens: weights straight into registers (16 of 8,192 x 8,192: 18.8, tiles 22.9; 33: 22.9 at two row tiles and 24.6).
-    if (a->m <= 16) return few(*a, stream);
+    // 16 tokens: weights straight into registers (16 of 4,096 x 4,096: 8.3, tiles 9.5; 8 of 768 x 4,096: 6.9 and 9.0), up to 3 where the
+    // channels alone give every CU a tile (2 of 8,192 x 8,192: 14.1, tiles 14.7; 8: 16.0 and 14.5; 8 of 50,280 x 768: 13.4 and 11.9).
+    if (a->m <= (a->n >= 8192 ? 3 : 16)) return few(*a, stream);
     // Tiles of 256 once they fill the CUs (8,192 of 8,192 x 4,096: 249, tiles of 128: 291; 2,048 of 4,096 x 1,536, 128 tiles: 27.8 and
     // 20.9), of 128 once they nearly do (4,096 of 768 x 768, 192 tiles: 10.3, tiles of 64: 10.8; 1,000 of 1,536 x 768, 96 tiles:
-    // 9.4 and 7.0), else of 64 by 256 columns (128 of 8,192 x 8,192: 26.8, by 128 columns 32.2).
+    // 9.4 and 7.0), else of 64, by 32 channels where half of the CUs would have none (64 of 8,192 x 8,192: 15.2, by 64 16.4).  Where no CU has
+    // two workgroups, each keeps more columns on their way (1,024 of 4,096 x 4,096, 256 tiles of 128: 28.2 with two stages, 25.3 with three;
+    // 2,048 of 4,096 x 1,536, 512 tiles: 21.4 and 25.3; 128 of 8,192 x 8,192, 256 of 64: 26.3 with two of 256 columns, 17.6 with four
+    // of 128; 512 of 4,096 x 4,096, 512 of 64: 16.4 and 17.8).
     const auto count = [&](uint32_t t) { return (uint64_t)((a->m + t - 1) / t) * ((a->n + t - 1) / t); };
     if (count(256) >= 256) return tiles<256, 256, 2, 4, 128, 2>(*a, stream);
-    if (count(128) >= 192) return tiles<128, 128, 2, 2, 128, 2>(*a, stream);
+    if (count(128) > 256) return tiles<128, 128, 2, 2, 128, 2>(*a, stream);
+    if (count(128) >= 192) return tiles<128, 128, 2, 2, 128, 3>(*a, stream);
+    if (count(64) <= 128) return tiles<64, 32, 2, 1, 128, 6>(*a, stream);
+    if (count(64) <= 256) return tiles<64, 64, 2, 2, 128, 4>(*a, stream);
     return tiles<64, 64, 2, 2, 256, 2>(*a, stream);
 }
 

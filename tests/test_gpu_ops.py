@@ -719,7 +719,8 @@ def product(m, n, k, seed=0):
 @types
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 16), (1, 1000, 768), (2, 33, 48), (7, 300, 64), (16, 16, 1536), (17, 129, 80),
                                    (33, 64, 128), (64, 250, 192), (65, 512, 256), (100, 100, 100), (128, 128, 64), (200, 300, 336),
-                                   (257, 255, 512), (130, 700, 17), (3, 5, 4099), (1, 40, 16384), (600, 520, 1024)])
+                                   (257, 255, 512), (130, 700, 17), (3, 5, 4099), (1, 40, 16384), (600, 520, 1024), (8, 8200, 256), (3, 8200, 144), (1800, 1800, 160), (2200, 2200, 96),
+                                   (4100, 4100, 80), (20, 96, 1040), (900, 1100, 400)])
 def test_int8_matmul(m, n, k, dtype):
     x, sx, w, sw, bias = product(m, n, k, seed=m + n)
     for b in (None, bias):
