@@ -240,6 +240,8 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     else:
         _check(op, device, "workspace", workspace, torch.uint8, (None,))
+        if not workspace.is_contiguous():      # (its bytes are counted by its elements)
+            _refuse(f"{op}: workspace is not contiguous")
     code = L.redukt_op_delta_chunk(ctypes.byref(a), cu_seqlens.data_ptr(), n,
                                    None if state_in is None else state_in.data_ptr(),
                                    None if state_out is None else state_out.data_ptr(), n_slots,

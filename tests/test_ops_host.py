@@ -152,3 +152,46 @@ def test_tensors_off_the_gpu_are_refused():
         with pytest.raises(ffi.BackendError) as e:
             call()
         assert e.value.result == ffi.BackendResult.INVALID_ARGUMENT
+
+
+# ---------------------------------------------------------------- the Python layer on its own
+
+class Recorded:
+    """Stands for the library: what is called, with which arguments."""
+    def __init__(self, lib):
+        self.calls = []
+        self.redukt_op_delta_chunk_workspace = lib.redukt_op_delta_chunk_workspace
+        for name in ("delta_step", "delta_chunk", "quantize_rows", "int8_matmul"):
+            setattr(self, "redukt_op_" + name, lambda *a: self.calls.append(a) or OK)
+
+
+@pytest.fixture
+def recorded(lib, monkeypatch):
+    """The operators on CPU tensors, with nothing behind the checks of arguments."""
+    r = Recorded(lib)
+    monkeypatch.setattr(ops, "_device", lambda op, t: t.get_device())
+    monkeypatch.setattr(ops, "_stream", lambda *a: None)
+    monkeypatch.setattr(ops, "_load", lambda: r)
+    return r
+
+
+def refused(call):
+    with pytest.raises(ffi.BackendError) as e:
+        call()
+    assert e.value.result == ffi.BackendResult.INVALID_ARGUMENT
+
+
+def rule_tensors(T=3, hk=2, hv=4, dk=64, dv=64, dtype=torch.bfloat16):
+    return (torch.zeros(T, hk, dk, dtype=dtype), torch.zeros(T, hk, dk, dtype=dtype), torch.zeros(T, hv, dv, dtype=dtype),
+            torch.zeros(T, hv), torch.zeros(T, hv))
+
+
+def test_a_workspace_that_is_not_one_block_is_refused(recorded):
+    x, cu = rule_tensors(), torch.tensor([0, 3], dtype=torch.int32)
+    need = ops.delta_chunk_workspace(3, 1, 2, 4, 64, 64, torch.bfloat16)
+    assert need > 0
+    refused(lambda: ops.delta_chunk(*x, cu, workspace=torch.zeros(1, dtype=torch.uint8).expand(need)))
+    refused(lambda: ops.delta_chunk(*x, cu, workspace=torch.zeros(2 * need, dtype=torch.uint8)[::2]))
+    assert not recorded.calls
+    ops.delta_chunk(*x, cu, workspace=torch.zeros(2 * need, dtype=torch.uint8)[need:])
+    assert len(recorded.calls) == 1
