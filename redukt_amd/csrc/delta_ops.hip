@@ -198,8 +198,13 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
 
+// v, or bf16's largest finite value with its sign where v is beyond that: what the first limb of v is rounded from.  (f32's values from
+// 3.3962e38 on would round to infinity, and their rests with them; so the rest is what is beyond, and still exact in two limbs.  Of an
+// infinity the rest is one, of a NaN a NaN.)  For values that may be so large.
+__device__ __forceinline__ float within_bf16(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f); }
+
 // Eight f32 as N bf16 limbs: each the rounded rest of those before it (the differences are exact).
-template <int N>
+template <int N, bool WIDE = false>
 __device__ __forceinline__ Split<N> split8(const float (&v)[8]) {
     u32x4 w[N];
 #pragma unroll
@@ -207,7 +212,7 @@ __device__ __forceinline__ Split<N> split8(const float (&v)[8]) {
         float a = v[2 * j], b = v[2 * j + 1];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            const uint32_t p = pack_bf16(a, b);
+            const uint32_t p = WIDE && n == 0 ? pack_bf16(within_bf16(a), within_bf16(b)) : pack_bf16(a, b);
             w[n][j] = p;
             if (n + 1 < N) {
                 a -= __builtin_bit_cast(float, p << 16);
@@ -333,7 +338,7 @@ struct Part {
     vec l[N];
 };
 
-template <int NW, int N>
+template <int NW, int N, bool WIDE>
 __device__ __forceinline__ Part<NW, N> split_part(const float (&v)[4 * NW]) {
     typedef uint32_t words __attribute__((ext_vector_type(2 * NW)));
     words w[N];
@@ -342,7 +347,7 @@ __device__ __forceinline__ Part<NW, N> split_part(const float (&v)[4 * NW]) {
         float a = v[2 * j], b = v[2 * j + 1];
 #pragma unroll
         for (int n = 0; n < N; n++) {
-            const uint32_t p = pack_bf16(a, b);
+            const uint32_t p = WIDE && n == 0 ? pack_bf16(within_bf16(a), within_bf16(b)) : pack_bf16(a, b);
             w[n][j] = p;
             a -= __builtin_bit_cast(float, p << 16);
             b -= __builtin_bit_cast(float, p & 0xffff0000u);
@@ -371,7 +376,7 @@ __device__ __forceinline__ void store_fragment(const float* m, const float* f, u
     const float scale = f ? f[row] : 1.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] *= scale;
-    const Split<N> y = split8<N>(v);
+    const Split<N> y = split8<N, true>(v);
 #pragma unroll
     for (int n = 0; n < N; n++) *(bf16x8*)(to + (x * N + n) * kFrag + lane * 16) = y.l[n];
 }
@@ -476,7 +481,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
         op_load(sQ + (16 * wave + l16) * PK + col, qr);
 #pragma unroll
         for (int x = 0; x < 8; x++) k2 += kr[x] * kr[x], q2 += qr[x] * qr[x];
-        const Split<LI> kl = split8<LI>(kr), ql = split8<LI>(qr);
+        const Split<LI> kl = split8<LI>(kr), ql = split8<LI, LI == 3>(qr);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (j > wave) break;
@@ -745,7 +750,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             return __builtin_bit_cast(vecK, x);
         }
     };
-    const auto limbs = [&](const vecK& x) {
+    const auto limbs = [&](const vecK& x, auto wide) {
         Part<NW, LI> o;
         if constexpr (LI == 1) {
             o.l[0] = __builtin_bit_cast(typename Part<NW, LI>::vec, x);
@@ -753,7 +758,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             float v[KF];
 #pragma unroll
             for (int j = 0; j < KF; j++) v[j] = (float)x[j];
-            o = split_part<NW, LI>(v);
+            o = split_part<NW, LI, wide.value && LI == 3>(v);
         }
         return o;
     };
@@ -833,7 +838,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
 #pragma unroll
             for (int o = 0; o < 4; o++) {
                 const int row = tile_index((wave + o) % 4, l16), at = row * (NW * 32) + (g4 ^ row / 8 % 4) * (KF * 2);
-                kl[o] = limbs(kf[o]);
+                kl[o] = limbs(kf[o], Int<0>());      // (a key with such an element is not finite: its sum of squares is not)
                 if constexpr (kRaw) {
                     *(vecK*)(sK[wave][0] + at) = kf[o];
                 } else {
@@ -856,7 +861,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
         // The four rows of this wave's tile that a lane holds, as half of a right operand's fragment.
         const auto put = [&](unsigned char (*to)[3][kFrag], const f32x4& v) {
             const float x[4] = {v[0], v[1], v[2], v[3]};
-            const Part<1, 3> y = split_part<1, 3>(x);
+            const Part<1, 3> y = split_part<1, 3, true>(x);
 #pragma unroll
             for (int n = 0; n < 3; n++)
                 *(typename Part<1, 3>::vec*)(to[wave / 2][n] + lane * 16 + wave % 2 * 8) = y.l[n];
@@ -885,7 +890,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 float v[KF];
 #pragma unroll
                 for (int j = 0; j < KF; j++) v[j] = S[nc][j / 4][j % 4];
-                const Part<NW, 3> x = split_part<NW, 3>(v);
+                const Part<NW, 3> x = split_part<NW, 3, true>(v);
 #pragma unroll
                 for (int n = 0; n < LO; n++) *(typename Part<NW, 3>::vec*)(sS[nc][wave][n] + lane * (KF * 2)) = x.l[n];
                 f32x4 y[4] = {};
@@ -1026,7 +1031,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
             __syncthreads();                   // A
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const Part<NW, LI> q = limbs(qf[s]);
+                const Part<NW, LI> q = limbs(qf[s], Int<1>());
 #pragma unroll
                 for (int nc = 0; nc < NC; nc++)
 #pragma unroll

@@ -821,3 +821,75 @@ def test_a_prompt_and_the_tokens_after_it():
         want, S64, tol, S_tol = ops_f64.rule(*seq, torch.zeros(hv, dk, dv, device="cuda"), normalize=True)
         check(torch.cat([outs[0][a:b]] + [o[i:i + 1] for o in outs[1:]]), want, tol, i)
         check(S[i], S64, S_tol, i)
+
+
+# ---------------------------------------------------------------- the ends of f32's range
+
+F32_MAX = torch.finfo(torch.float32).max
+
+
+def one_column(x, cu, before, bad, col, head, normalize, changed, pool=None):
+    """Of a call whose inputs `changed` from x in one column of a head, from row `bad` of the first sequence on: everything else
+    has the bits of the call on x, and that column the rule's values.
+
+    Beside ops_f64's bound stands one for factors that leave f32's range at its other end.  Over the tokens of a chunk a value V is
+    multiplied by decays e^(G_i - G_j), of which what is below 2^-126 is 0: each of the entries of A, at most 1 in size, is off by 2^-126,
+    so T = (I + A)^-1 by |T| |dA| |T| <= 64 * 64 * 2^-126 with |T| <= 1; limbs below 2^-126 add three such steps.  The result is then
+    off by V * 2^-114 at most (|q|, |k| and the scale are at most 1), which is seen only where V is next to f32's end.
+    """
+    floor = 2.0 ** -114 * max(float(changed[2][:, head, col].abs().max()), 0.0 if pool is None else float(pool[0, head, :, col].abs().max()))
+    S, S2 = torch.empty_like(before), torch.empty_like(before)
+    want = ops.delta_chunk(*x, cu, state_in=before, state_out=S, normalize=normalize)
+    start = before if pool is None else pool
+    got = ops.delta_chunk(*changed, cu, state_in=start, state_out=S2, normalize=normalize)
+    end = int(cu[1])
+    exact, S64, tol, S_tol = ops_f64.rule(*(t[:end] for t in changed), start[0], normalize=normalize)
+    check(got[bad:end, head, col], exact[bad:, head, col], tol[bad:, head, col] + floor, "out")
+    check(S2[0, head, :, col], S64[head, :, col], S_tol[head, :, col] + floor, "state")
+    got[bad:end, head, col] = want[bad:end, head, col]
+    S2[0, head, :, col] = S[0, head, :, col]
+    assert torch.equal(got, want) and torch.equal(S2, S)
+
+
+ENDS = [(64, [130, 70]), (128, [130, 70]), (64, [50]), (128, [64]), (64, [101] + [5] * 70)]
+ends = pytest.mark.parametrize("dk,lens", ENDS, ids=["64", "128", "64 rows at most", "64 rows at most, 128", "71 sequences"])
+
+
+@ends
+@pytest.mark.parametrize("size", [F32_MAX, -F32_MAX, 3.3962e38])
+@pytest.mark.parametrize("at", [0, 29, 48])
+def test_delta_chunk_of_a_value_next_to_the_end_of_f32(at, size, dk, lens):
+    """It is finite, and so is what the rule makes of it."""
+    x = rule_inputs(sum(lens), 2, 4, dk, 64, F32, seed=2, normalize=True)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    y = [t.clone() for t in x]
+    y[2][at, 1, 5] = size
+    one_column(x, cu, pool_of(len(lens), 4, dk, 64), at, 5, 1, True, y)
+
+
+@ends
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("size", [F32_MAX, -F32_MAX])
+def test_delta_chunk_of_a_state_next_to_the_end_of_f32(size, dtype, dk, lens):
+    x = rule_inputs(sum(lens), 2, 4, dk, 64, dtype, seed=2)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    before = pool_of(len(lens), 4, dk, 64)
+    pool = before.clone()
+    pool[0, 1, 3, 5] = size
+    one_column(x, cu, before, 0, 5, 1, False, x, pool)
+
+
+@ends
+def test_delta_chunk_of_a_query_next_to_the_end_of_f32(dk, lens):
+    x = rule_inputs(sum(lens), 2, 4, dk, 64, F32, seed=2)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    before = 1e-3 * pool_of(len(lens), 4, dk, 64)
+    x[2] *= 1e-3
+    y = [t.clone() for t in x]
+    at = 33
+    y[0][at, 0, 7] = F32_MAX
+    want, got = (ops.delta_chunk(*t, cu, state_in=before) for t in (x, y))
+    exact, _, tol, _ = ops_f64.rule(*(t[:lens[0]] for t in y), before[0])
+    check(got[at, :2], exact[at, :2], tol[at, :2], "out")
+    got[at, :2] = want[at, :2]
+    assert torch.equal(got, want)
