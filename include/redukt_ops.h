@@ -45,8 +45,9 @@ extern "C" {
  *
  * A value that is not finite goes where the rule takes it: one of v into its column, one of k,
  * g or beta into its head, from its token on; one of q into its token.  What it reaches is then
- * not finite, inf or NaN.  (In delta_chunk, a sum that passes f32's range from finite inputs,
- * which a stable rule has none of, may also reach up to 63 tokens back, and a decay over several
+ * not finite, inf or NaN.  To normalize, a key or query whose sum of squares passes f32's range
+ * (|k| from about 1.8e19 on) counts as one that is not finite.  (In delta_chunk, a sum that passes f32's range from finite inputs,
+ * which a stable rule has none of (the sum of squares of a key is one), may also reach up to 63 tokens back, and a decay over several
  * tokens that is below 2^-126 is 0.) */
 #define REDUKT_DELTA_NORMALIZE 1u
 

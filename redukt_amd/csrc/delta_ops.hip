@@ -16,6 +16,9 @@ namespace {
 
 constexpr float kUnitEps = 1e-6f;      // added to the sum of squares that k and q are divided by
 
+// What normalizes a row of this sum of squares; NaN where the sum is not finite (1 / sqrt(inf) = 0 would make zeros of a finite row).
+__device__ __forceinline__ float unit_factor(float sum) { return rsqrtf(sum + kUnitEps) + 0.0f * sum; }
+
 struct DeltaArgs {
     redukt_delta_rows r;
     const float* in;           // states read (null: zeros)
@@ -99,8 +102,8 @@ __global__ __launch_bounds__(256) void k_delta_step(DeltaArgs a) {
     kq = rows_sum(kq);
     float uk = 1.0f, uq = r.scale;
     if (r.flags & REDUKT_DELTA_NORMALIZE) {
-        uk = rsqrtf(rows_sum(kk) + kUnitEps);
-        uq *= rsqrtf(rows_sum(qq) + kUnitEps);
+        uk = unit_factor(rows_sum(kk));
+        uq *= unit_factor(rows_sum(qq));
     }
     // d carries the key's factor, so that the rows of k enter as they are
     const float ak = decay * uk;
@@ -493,9 +496,9 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
     k2 += __shfl_xor(k2, 16, kWave), q2 += __shfl_xor(q2, 16, kWave);
     k2 += __shfl_xor(k2, 32, kWave), q2 += __shfl_xor(q2, 32, kWave);
     if (g4 == 0) {
-        // (a sum that is not finite stays one: 0 x it is NaN)
-        sU[16 * wave + l16] = norm ? rsqrtf(k2 + kUnitEps) + 0.0f * k2 : 1.0f + 0.0f * k2;
-        sP[16 * wave + l16] = r.scale * (norm ? rsqrtf(q2 + kUnitEps) : 1.0f);
+        // (a key's sum that is not finite marks the token: 0 x it is NaN)
+        sU[16 * wave + l16] = norm ? unit_factor(k2) : 1.0f + 0.0f * k2;
+        sP[16 * wave + l16] = r.scale * (norm ? unit_factor(q2) : 1.0f);
     }
     __syncthreads();                           // k and q are done with; sU, sP are written
 

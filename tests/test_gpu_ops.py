@@ -893,3 +893,50 @@ def test_delta_chunk_of_a_query_next_to_the_end_of_f32(dk, lens):
     check(got[at, :2], exact[at, :2], tol[at, :2], "out")
     got[at, :2] = want[at, :2]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("which", ["k", "q"])
+@pytest.mark.parametrize("lens,at", [([50], 20), ([130, 70], 64)])
+def test_sums_of_squares_past_f32_are_not_finite_in_either_form(lens, at, which, dtype):
+    """A key or query of finite values that cannot be normalized in f32, in a sequence and token by token."""
+    hk, hv, dk, dv, T = 2, 4, 64, 64, sum(lens)
+    x = rule_inputs(T, hk, hv, dk, dv, dtype, seed=2, normalize=True)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+    before = pool_of(len(lens), hv, dk, dv)
+    S, S2 = torch.empty_like(before), torch.empty_like(before)
+    want = ops.delta_chunk(*x, cu, state_in=before, state_out=S, normalize=True)
+    y = [t.clone() for t in x]
+    y[which == "k"][at, 1] = 1e19
+    got = ops.delta_chunk(*y, cu, state_in=before, state_out=S2, normalize=True)
+    bad = torch.zeros(T, hv, dtype=torch.bool, device="cuda")
+    bad[at:lens[0] if which == "k" else at + 1, 2:] = True
+    assert not torch.isfinite(got[bad]).any() and torch.equal(got[~bad], want[~bad])
+    if which == "k":
+        assert not torch.isfinite(S2[0, 2:]).any()
+        S2[0, 2:] = S[0, 2:]
+    assert torch.equal(S2, S)
+    # the same token by itself
+    a, b = (before[:1].clone() for _ in range(2))
+    want, got = (ops.delta_step(*(t[at:at + 1] for t in z), s, normalize=True) for z, s in ((x, a), (y, b)))
+    assert not torch.isfinite(got[:, 2:]).any() and torch.equal(got[:, :2], want[:, :2])
+    if which == "k":
+        assert not torch.isfinite(b[0, 2:]).any()
+        b[0, 2:] = a[0, 2:]
+    assert torch.equal(a, b)
+
+
+def test_the_largest_key_that_normalizes():
+    """|k|^2 next to f32's end: still the rule's values."""
+    x = rule_inputs(100, 1, 2, 64, 64, F32, seed=4, normalize=True)
+    for t in (x[0], x[1]):
+        t *= 1.8e19 / t.norm(dim=-1, keepdim=True)
+    before = pool_of(1, 2, 64, 64)
+    S, step = torch.empty_like(before), before.clone()
+    out = ops.delta_chunk(*x, torch.tensor([0, 100], dtype=torch.int32, device="cuda"), state_in=before, state_out=S, normalize=True)
+    want, S64, tol, S_tol = ops_f64.rule(*x, before[0], normalize=True)
+    check(out, want, tol, "out")
+    check(S[0], S64, S_tol, "state")
+    for t in range(100):
+        check(ops.delta_step(*(z[t:t + 1] for z in x), step, normalize=True), want[t:t + 1], tol[t:t + 1], t)
+    check(step[0], S64, S_tol, "state by steps")
