@@ -105,9 +105,11 @@ typedef struct {
     float* scales;          /* [rows] */
 } redukt_quantize_rows;     /* any alignment that the element types have */
 
-/* The library's int8 recipe, row by row: scale = max|x| / 127 (1 for a row of zeros; NaN does
+/* The library's int8 recipe, row by row: scale = max|x| / 127 (1 where that is 0; NaN does
  * not count), code = x * (1 / scale), each step rounded to f32, to the nearest whole number
- * with halves away from zero, at most 127 in size, 0 for NaN.  x = code * scale. */
+ * with halves away from zero, at most 127 in size, 0 for NaN.  x = code * scale, but in rows
+ * whose largest magnitude is between 9e-44 and 3.7e-37: there 1 / scale passes f32's range, and
+ * what is not 0 becomes 127 or -127.  A row with an infinity has the scale inf and codes of 0. */
 int32_t redukt_op_quantize_rows(const redukt_quantize_rows* a, void* stream);
 
 typedef struct {

@@ -74,7 +74,8 @@ __global__ __launch_bounds__(kBlock) void k_quantize_rows(redukt_quantize_rows a
 #pragma unroll
         for (int w = 0; w < WAVES; w++) m = fold_abs(m, wm[w]);
     }
-    const float scale = m > 0.0f ? m / 127.0f : 1.0f;
+    float scale = m / 127.0f;
+    if (scale == 0.0f) scale = 1.0f;           // (also where the quotient rounds to 0: its inverse would make 127 of every value)
     const float inv = 1.0f / scale;
     const auto store = [&](uint32_t c, const vec& v) {
         codes y;

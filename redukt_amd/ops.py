@@ -252,7 +252,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     """int8 codes of each row of x [rows, cols] (bfloat16, float16 or float32) with the library's
-    recipe: scale = max|x| / 127 (1 for a row of zeros), code = x / scale rounded with halves away
+    recipe: scale = max|x| / 127 (1 where that is 0), code = x / scale rounded with halves away
     from zero, each step in float32; NaN counts for nothing and becomes 0.  Returns (codes int8
     [rows, cols], scales float32 [rows]), allocated if None.  Rows may be strided.
     """

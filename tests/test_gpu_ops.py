@@ -940,3 +940,19 @@ def test_the_largest_key_that_normalizes():
     for t in range(100):
         check(ops.delta_step(*(z[t:t + 1] for z in x), step, normalize=True), want[t:t + 1], tol[t:t + 1], t)
     check(step[0], S64, S_tol, "state by steps")
+
+
+def test_quantize_rows_whose_scale_rounds_to_zero():
+    """Largest values on both sides of 127 * 2^-150, half of f32's smallest step: below it the rounded scale is 0, as a row of zeros'
+    is, and 1 stands in its place."""
+    step = 2.0 ** -149
+    most = [0, 1, 2, 17, 63, 64, 127, 200]
+    x = torch.zeros(len(most), 70, device="cuda")
+    for r, m in enumerate(most):
+        x[r, 0], x[r, 3], x[r, 69] = m * step, -m * step, (m // 2) * step
+    codes, scales = ops.quantize_rows(x)
+    for r, m in enumerate(most):
+        if m < 64:
+            assert scales[r] == 1.0 and not codes[r].any(), m
+        else:
+            assert scales[r] == round(m / 127) * step and codes[r, 0] == 127 and codes[r, 3] == -127, m
