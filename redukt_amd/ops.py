@@ -6,7 +6,8 @@ channel (`int8_matmul`).  Arguments are torch tensors on one GPU; work is queued
 current stream of that GPU, or on `stream`, a hipStream_t's value.  Outputs and workspaces that a
 call allocates belong to torch's current stream, so for another one they are passed in.  Outputs
 overlap no input (but a state pool its own next states).  No model needs to be open.  The
-operators have no gradients: inputs that ask for one are refused while torch records them.
+operators have no gradients: tensors that ask for one, states and outputs among them, are refused
+while torch records them.
 Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch nothing; there is no CPU
 fallback.
 """
@@ -107,7 +108,7 @@ def _stream(op: str, stream: Optional[int], device: int, allocates: bool) -> int
 
 def _no_gradients(op: str, asked: bool) -> None:
     if asked and torch.is_grad_enabled():
-        _refuse(f"{op}: an input asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
+        _refuse(f"{op}: a tensor asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
 
 
 def _row_stride(op: str, name: str, t, width: int) -> int:
@@ -148,6 +149,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
     else:
         _check(op, device, "out", out, dtype, wide)
+        _no_gradients(op, out.requires_grad)
     wk, wv = hk * dk, hv * dv
     if scale is None:
         scale = dk ** -0.5 if dk else 0.0
@@ -161,6 +163,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
 def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
     try:
         if (t.dtype is torch.float32 and t.shape[1:] == (a.hv, a.dk, a.dv) and t.is_contiguous() and t.get_device() == device):
+            _no_gradients(op, t.requires_grad)
             return
     except AttributeError:
         pass
@@ -271,6 +274,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
     else:
         _check(op, device, "scales", scales, torch.float32, (rows,))
+        _no_gradients(op, scales.requires_grad)
         if not scales.is_contiguous():
             _refuse(f"{op}: scales is not contiguous")
     a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
@@ -315,6 +319,7 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         if out.dtype not in DTYPES:
             _refuse(f"{op}: out is bfloat16, float16 or float32")
         _check(op, device, "out", out, out.dtype, (m, n))
+        _no_gradients(op, out.requires_grad)
     a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))

@@ -195,3 +195,33 @@ def test_a_workspace_that_is_not_one_block_is_refused(recorded):
     assert not recorded.calls
     ops.delta_chunk(*x, cu, workspace=torch.zeros(2 * need, dtype=torch.uint8)[need:])
     assert len(recorded.calls) == 1
+
+
+def pools_and_calls():
+    """Each operator on tensors of its own: (floating-point inputs and outputs by name, a call of them)."""
+    f32, bf16 = torch.float32, torch.bfloat16
+    rows = dict(zip(("q", "k", "v", "g", "beta"), rule_tensors()), out=torch.zeros(3, 4, 64, dtype=bf16))
+    cu = torch.tensor([0, 3], dtype=torch.int32)
+    step = dict(rows, states=torch.zeros(3, 4, 64, 64))
+    chunk = dict(rows, state_in=torch.zeros(1, 4, 64, 64), state_out=torch.zeros(1, 4, 64, 64))
+    codes = torch.zeros(3, 16, dtype=torch.int8)
+    return {"delta_step": (step, lambda t: ops.delta_step(**t)),
+            "delta_chunk": (chunk, lambda t: ops.delta_chunk(cu_seqlens=cu, **t)),
+            "quantize_rows": (dict(x=torch.zeros(3, 16), scales=torch.zeros(3)), lambda t: ops.quantize_rows(codes=codes, **t)),
+            "int8_matmul": (dict(x_scales=torch.ones(3), w_scales=torch.ones(3), bias=torch.zeros(3), out=torch.zeros(3, 3, dtype=f32)),
+                            lambda t: ops.int8_matmul(x=codes, w=codes, **t))}
+
+
+TENSORS = [(op, name) for op, (t, _) in pools_and_calls().items() for name in t]
+
+
+@pytest.mark.parametrize("op,name", TENSORS)
+def test_every_tensor_that_asks_for_a_gradient_is_refused(recorded, op, name):
+    tensors, call = pools_and_calls()[op]
+    call(tensors)
+    tensors[name].requires_grad_()
+    refused(lambda: call(tensors))
+    assert len(recorded.calls) == 1
+    with torch.no_grad():
+        call(tensors)
+    assert len(recorded.calls) == 2
