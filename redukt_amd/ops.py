@@ -7,7 +7,7 @@ current stream of that GPU, or on `stream`, a hipStream_t's value.  Outputs and 
 call allocates belong to torch's current stream, so for another one they are passed in.  Outputs
 overlap no input (but a state pool its own next states).  No model needs to be open.  The
 operators have no gradients: tensors that ask for one, states and outputs among them, are refused
-while torch records them.
+while torch records them, and tensors with a tangent always.
 Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch nothing; there is no CPU
 fallback.
 """
@@ -17,6 +17,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import ffi
 
@@ -106,9 +107,14 @@ def _stream(op: str, stream: Optional[int], device: int, allocates: bool) -> int
     return stream
 
 
-def _no_gradients(op: str, asked: bool) -> None:
+def _no_gradients(op: str, asked: bool, *tensors) -> None:
+    """asked: one of `tensors` requires a gradient."""
     if asked and torch.is_grad_enabled():
         _refuse(f"{op}: a tensor asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
+    if forward_ad._current_level >= 0:         # (-1: nobody computes tangents)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _refuse(f"{op}: a tensor has a tangent, which this operator would drop")
 
 
 def _row_stride(op: str, name: str, t, width: int) -> int:
@@ -143,13 +149,14 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
         _check(op, device, "g", g, torch.float32, tuple(v.shape[:2]))
         _check(op, device, "beta", beta, torch.float32, tuple(v.shape[:2]))
         _refuse(f"{op}: tensors do not belong together")
-    _no_gradients(op, q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad)
+    _no_gradients(op, q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad,
+                  q, k, v, g, beta)
     _, hv, dv = wide
     if out is None:
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
     else:
         _check(op, device, "out", out, dtype, wide)
-        _no_gradients(op, out.requires_grad)
+        _no_gradients(op, out.requires_grad, out)
     wk, wv = hk * dk, hv * dv
     if scale is None:
         scale = dk ** -0.5 if dk else 0.0
@@ -163,7 +170,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
 def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
     try:
         if (t.dtype is torch.float32 and t.shape[1:] == (a.hv, a.dk, a.dv) and t.is_contiguous() and t.get_device() == device):
-            _no_gradients(op, t.requires_grad)
+            _no_gradients(op, t.requires_grad, t)
             return
     except AttributeError:
         pass
@@ -263,7 +270,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     device = _device(op, x)
     if x.dtype not in DTYPES or x.dim() != 2:
         _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
-    _no_gradients(op, x.requires_grad)
+    _no_gradients(op, x.requires_grad, x)
     on = _stream(op, stream, device, codes is None or scales is None)
     rows, cols = x.shape
     if codes is None:
@@ -274,7 +281,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
     else:
         _check(op, device, "scales", scales, torch.float32, (rows,))
-        _no_gradients(op, scales.requires_grad)
+        _no_gradients(op, scales.requires_grad, scales)
         if not scales.is_contiguous():
             _refuse(f"{op}: scales is not contiguous")
     a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
@@ -309,7 +316,8 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         if bias is not None:
             _check(op, device, "bias", bias, f32, (w.shape[0],))
         _refuse(f"{op}: scales and bias are contiguous")
-    _no_gradients(op, x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad))
+    _no_gradients(op, x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad),
+                  x_scales, w_scales, bias)
     on = _stream(op, stream, device, out is None)
     if out is None:
         if dtype not in DTYPES:
@@ -319,7 +327,7 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         if out.dtype not in DTYPES:
             _refuse(f"{op}: out is bfloat16, float16 or float32")
         _check(op, device, "out", out, out.dtype, (m, n))
-        _no_gradients(op, out.requires_grad)
+        _no_gradients(op, out.requires_grad, out)
     a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))

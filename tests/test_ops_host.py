@@ -225,3 +225,16 @@ def test_every_tensor_that_asks_for_a_gradient_is_refused(recorded, op, name):
     with torch.no_grad():
         call(tensors)
     assert len(recorded.calls) == 2
+
+
+@pytest.mark.parametrize("op,name", TENSORS)
+def test_every_tensor_with_a_tangent_is_refused(recorded, op, name):
+    from torch.autograd import forward_ad
+
+    tensors, call = pools_and_calls()[op]
+    with forward_ad.dual_level():
+        call(tensors)                                                     # (a level alone is nothing to refuse)
+        dual = dict(tensors, **{name: forward_ad.make_dual(tensors[name], torch.ones_like(tensors[name]))})
+        refused(lambda: call(dual))
+    refused(lambda: torch.func.jvp(lambda t: call(dict(tensors, **{name: t})), (tensors[name],), (torch.ones_like(tensors[name]),)))
+    assert len(recorded.calls) == 1
