@@ -74,9 +74,11 @@ def _refuse(what: str) -> None:
     raise ffi.BackendError(ffi.BackendResult.INVALID_ARGUMENT, what)
 
 
-def _done(code: int, what: str) -> None:
+def _done(code: int, what: str, written) -> None:
+    """The end of a call that writes the tensors `written`, unseen by torch: it counts their writes, for what autograd has saved."""
     if code:
         raise ffi.BackendError(ffi.BackendResult.from_code(code), what)
+    torch.autograd.graph.increment_version(written)
 
 
 def _check(op: str, device: int, name: str, t, dtype, shape) -> None:
@@ -207,7 +209,7 @@ def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[f
     _pool(op, device, "states", states, a)
     code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
                                         _slots(op, device, slots, a.rows), on)
-    _done(code, op)
+    _done(code, op, (states, out))
     return out
 
 
@@ -256,7 +258,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
                                    None if state_in is None else state_in.data_ptr(),
                                    None if state_out is None else state_out.data_ptr(), n_slots,
                                    _slots(op, device, slots, n), workspace.data_ptr(), workspace.numel(), on)
-    _done(code, op)
+    _done(code, op, (out, workspace) if state_out is None else (out, workspace, state_out))
     return out
 
 
@@ -286,7 +288,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
             _refuse(f"{op}: scales is not contiguous")
     a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
                      _row_stride(op, "codes", codes, cols), scales.data_ptr())
-    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), on), op)
+    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), on), op, (codes, scales))
     return codes, scales
 
 
@@ -331,5 +333,5 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
     a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))
-    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op)
+    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op, (out,))
     return out

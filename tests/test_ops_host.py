@@ -238,3 +238,36 @@ def test_every_tensor_with_a_tangent_is_refused(recorded, op, name):
         refused(lambda: call(dual))
     refused(lambda: torch.func.jvp(lambda t: call(dict(tensors, **{name: t})), (tensors[name],), (torch.ones_like(tensors[name]),)))
     assert len(recorded.calls) == 1
+
+
+@pytest.mark.parametrize("op,written", [("delta_step", ["states", "out"]), ("delta_chunk", ["state_out", "out"]),
+                                        ("quantize_rows", ["scales"]), ("int8_matmul", ["out"])])
+def test_what_a_call_writes_is_counted_as_written(recorded, op, written):
+    """A tensor that autograd has saved and a call overwrites is noticed by backward."""
+    tensors, call = pools_and_calls()[op]
+    before = {n: t._version for n, t in tensors.items()}
+    call(tensors)
+    for n, t in tensors.items():
+        assert (t._version > before[n]) == (n in written), n
+    w = torch.ones((), requires_grad=True)
+    loss = (w * tensors[written[0]]).sum()
+    call(tensors)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_codes_and_workspaces_are_counted_as_written(recorded):
+    codes = torch.zeros(3, 16, dtype=torch.int8)
+    ops.quantize_rows(torch.zeros(3, 16), codes=codes)
+    work = torch.zeros(ops.delta_chunk_workspace(3, 1, 2, 4, 64, 64, torch.bfloat16), dtype=torch.uint8)
+    ops.delta_chunk(*rule_tensors(), torch.tensor([0, 3], dtype=torch.int32), workspace=work)
+    assert codes._version == 1 and work._version == 1
+
+
+def test_tensors_of_inference_mode(recorded):
+    """They keep no count of writes, and none is missed."""
+    with torch.inference_mode():
+        tensors, call = pools_and_calls()["delta_step"]
+    with torch.no_grad():
+        call(tensors)
+    assert len(recorded.calls) == 1
