@@ -81,6 +81,12 @@ def _done(code: int, what: str, written) -> None:
     torch.autograd.graph.increment_version(written)
 
 
+def _sizes(op: str, *sizes: int) -> None:
+    """The library's fields for sizes have 32 bits, and ctypes would drop what is above."""
+    if max(sizes) > 0x7fffffff or min(sizes) < 0:
+        _refuse(f"{op}: sizes {sizes} are not within 2^31 - 1")
+
+
 def _check(op: str, device: int, name: str, t, dtype, shape) -> None:
     """t is a tensor on GPU `device` of this type and shape (None: any size)."""
     if not isinstance(t, torch.Tensor):
@@ -154,6 +160,7 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
     _no_gradients(op, q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad,
                   q, k, v, g, beta)
     _, hv, dv = wide
+    _sizes(op, T, hk, dk, hv, dv)
     if out is None:
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
     else:
@@ -217,6 +224,7 @@ def delta_chunk_workspace(tokens: int, sequences: int, hk: int, hv: int, dk: int
     """Bytes of workspace that `delta_chunk` needs for these sizes."""
     if dtype not in DTYPES:
         _refuse("delta_chunk_workspace: bfloat16, float16 or float32")
+    _sizes("delta_chunk_workspace", tokens, sequences, hk, hv, dk, dv)
     return _load().redukt_op_delta_chunk_workspace(ctypes.byref(DeltaRows(DTYPES[dtype], tokens, hk, hv, dk, dv)), sequences)
 
 
@@ -239,6 +247,7 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     n = cu_seqlens.shape[0] - 1
     if n < 0 or not cu_seqlens.is_contiguous():
         _refuse(f"{op}: cu_seqlens holds one value more than there are sequences")
+    _sizes(op, n)
     n_slots = 0
     for name, pool in (("state_in", state_in), ("state_out", state_out)):
         if pool is not None:
@@ -275,6 +284,7 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     _no_gradients(op, x.requires_grad, x)
     on = _stream(op, stream, device, codes is None or scales is None)
     rows, cols = x.shape
+    _sizes(op, rows, cols)
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     else:
@@ -320,6 +330,7 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         _refuse(f"{op}: scales and bias are contiguous")
     _no_gradients(op, x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad),
                   x_scales, w_scales, bias)
+    _sizes(op, m, n, k)
     on = _stream(op, stream, device, out is None)
     if out is None:
         if dtype not in DTYPES:

@@ -271,3 +271,31 @@ def test_tensors_of_inference_mode(recorded):
     with torch.no_grad():
         call(tensors)
     assert len(recorded.calls) == 1
+
+
+# ---------------------------------------------------------------- sizes that do not fit the library's fields
+
+BIG = 2 ** 32 + 5
+
+
+def test_sizes_past_32_bits_are_refused(recorded):
+    """They would arrive as what is left of them modulo 2^32.  (Tensors of stride 0: no memory is behind them.)"""
+    byte, one = torch.zeros(1, 1, dtype=torch.int8), torch.ones(1)
+    codes, scales = byte.expand(BIG, 1), one.expand(BIG)
+    for rows, cols in ((BIG, 1), (1, BIG), (2 ** 31, 1)):
+        refused(lambda: ops.quantize_rows(torch.zeros(1, 1).expand(rows, cols), codes=byte.expand(rows, cols)))
+    refused(lambda: ops.int8_matmul(codes, scales, byte, one, out=torch.zeros(1, 1).expand(BIG, 1)))
+    refused(lambda: ops.int8_matmul(byte, one, codes, scales, out=torch.zeros(1, 1).expand(1, BIG)))
+    refused(lambda: ops.int8_matmul(byte.expand(1, BIG), one, byte.expand(1, BIG), one))
+    x = [t[:1].expand(BIG, *t.shape[1:]) for t in rule_tensors(1, 1, 1, 64, 32)]
+    refused(lambda: ops.delta_step(*x, torch.zeros(1, 1, 64, 32), out=x[2]))
+    refused(lambda: ops.delta_chunk(*x, torch.zeros(2, dtype=torch.int32), out=x[2]))
+    assert not recorded.calls
+
+
+def test_sizes_of_a_workspace_past_32_bits_are_refused(lib):
+    sizes = (100, 2, 2, 4, 64, 64)
+    assert ops.delta_chunk_workspace(*sizes, torch.bfloat16) > 0
+    for i, size in enumerate(sizes):
+        for wrong in (size + 2 ** 32, size - 2 ** 32, -1, 2 ** 31):
+            refused(lambda: ops.delta_chunk_workspace(*sizes[:i], wrong, *sizes[i + 1:], torch.bfloat16))
