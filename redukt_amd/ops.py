@@ -337,7 +337,7 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
             _refuse(f"{op}: dtype is bfloat16, float16 or float32")
         out = torch.empty((m, n), dtype=dtype, device=x.device)
     else:
-        if out.dtype not in DTYPES:
+        if not isinstance(out, torch.Tensor) or out.dtype not in DTYPES:
             _refuse(f"{op}: out is bfloat16, float16 or float32")
         _check(op, device, "out", out, out.dtype, (m, n))
         _no_gradients(op, out.requires_grad, out)

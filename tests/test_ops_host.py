@@ -169,7 +169,7 @@ class Recorded:
 def recorded(lib, monkeypatch):
     """The operators on CPU tensors, with nothing behind the checks of arguments."""
     r = Recorded(lib)
-    monkeypatch.setattr(ops, "_device", lambda op, t: t.get_device())
+    monkeypatch.setattr(ops, "_device", lambda op, t: t.get_device() if isinstance(t, torch.Tensor) else ops._refuse(op))
     monkeypatch.setattr(ops, "_stream", lambda *a: None)
     monkeypatch.setattr(ops, "_load", lambda: r)
     return r
@@ -299,3 +299,10 @@ def test_sizes_of_a_workspace_past_32_bits_are_refused(lib):
     for i, size in enumerate(sizes):
         for wrong in (size + 2 ** 32, size - 2 ** 32, -1, 2 ** 31):
             refused(lambda: ops.delta_chunk_workspace(*sizes[:i], wrong, *sizes[i + 1:], torch.bfloat16))
+
+
+@pytest.mark.parametrize("op,name", TENSORS)
+def test_what_is_no_tensor_is_refused(recorded, op, name):
+    tensors, call = pools_and_calls()[op]
+    refused(lambda: call(dict(tensors, **{name: 5})))
+    assert not recorded.calls
