@@ -418,7 +418,10 @@ struct PrepLds {
 // Four waves make the units of one chunk, `len` rows from t0 on, and of `per` value heads of one key head.  (I + A)^-1 is solved by
 // blocks: 16 by substitution, all four of a chunk side by side in one wave, then 32 and 64 by products, which keeps it as exact as
 // substitution (a product of powers of A would not be, where keys are alike and the powers are large).
-constexpr int kPrepBarriers = 9;               // that prepare() passes for one head
+// A barrier that prepare() passes for its first head.  They are counted as they are written, because waves that have no part in it
+// (k_delta_chunks) meet its four waves at each of them: every wave must pass it exactly once, in no loop and under no condition.
+#define PREP_MEET() (__syncthreads(), (void)__COUNTER__)
+constexpr int kPrepFirst = __COUNTER__;
 template <typename T, int DK>
 __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds, uint32_t slot, uint32_t t0, uint32_t len, uint32_t h0,
                                         uint32_t per) {
@@ -470,7 +473,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
             *(u32x4*)((unsigned char*)sQ + id / kPer * (PK * SZ) + id % kPer * 16) = qv[u];
         }
     }
-    __syncthreads();
+    PREP_MEET();
 
     // k.k and q.k: wave w the tiles (w, 0 .. w)
     f32x4 kk[4] = {}, qk[4] = {};
@@ -500,7 +503,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
         sU[16 * wave + l16] = norm ? unit_factor(k2) : 1.0f + 0.0f * k2;
         sP[16 * wave + l16] = r.scale * (norm ? unit_factor(q2) : 1.0f);
     }
-    __syncthreads();                           // k and q are done with; sU, sP are written
+    PREP_MEET();                               // k and q are done with; sU, sP are written
 
     int here = threadIdx.x;
     for (uint32_t h = h0; h < h0 + per; h++) {
@@ -548,7 +551,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
                 }
             }
         }
-        __syncthreads();
+        PREP_MEET();
         if (wave == 0) {   // the diagonal blocks: column l16 of block g4 of (I + A)^-1 by substitution
             const float* A = sA + (16 * g4) * kPitchA + 16 * g4;
             float t[16];
@@ -574,7 +577,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
             vec[kChunk + lane] = sP[lane] * eg;
             vec[2 * kChunk + lane] = exp2_hw(last);
         }
-        __syncthreads();
+        PREP_MEET();
         // [[T1, 0], [-T2 A21 T1, T2]]: from blocks of 16 to 32
         // (inner indices in the order 4 g + s: a lane's left elements are neighbours, and no bank is met twice on the right)
         const auto at = [&](const float* m, int tr, int tc, int row, int col) { return m[(16 * tr + row) * kPitchA + 16 * tc + col]; };
@@ -592,7 +595,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
 #pragma unroll
             for (int x = 0; x < 4; x++) sT[(16 * i + 4 * g4 + x) * kPitchA + 16 * (i + 1) + l16] = 0.0f;
         }
-        __syncthreads();
+        PREP_MEET();
         {   // from 32 to 64: wave w block (2 + w / 2, w % 2)
             const int i = wave / 2, j = wave % 2;
             f32x4 y = {};
@@ -609,7 +612,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
 #pragma unroll
                 for (int s = 0; s < 4; s++) y = mma4(at(sT, 2 + i, 2 + p, l16, 4 * g4 + s), m[s], y);
             }
-            __syncthreads();                       // A is done with: P takes its place
+            PREP_MEET();                           // A is done with: P takes its place
 #pragma unroll
             for (int x = 0; x < 4; x++) sT[(32 + 16 * i + 4 * g4 + x) * kPitchA + 16 * j + l16] = -y[x];
 #pragma unroll
@@ -617,7 +620,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
 #pragma unroll
                 for (int x = 0; x < 4; x++) sA[(16 * wave + 4 * g4 + x) * kPitchA + 16 * k + l16] = vp[k][x];
         }
-        __syncthreads();
+        PREP_MEET();
         // P (I + A)^-1 by tiles (row, column), whose products' lengths are row - column + 1: five for each wave
         const uint32_t tiles = (uint32_t)(0xFA5400E8009D000Cull >> 16 * wave) & 0xFFFF;      // 4 row + column, a nibble each
         f32x4 y[4] = {};
@@ -630,7 +633,7 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
                 for (int s = 0; s < 4; s++) y[q] = mma4(at(sA, i, k, l16, 4 * g4 + s), at(sT, k, j, 4 * g4 + s, l16), y[q]);
             }
         }
-        __syncthreads();                           // P and (I + A)^-1 have been read: their columns take beta
+        PREP_MEET();                               // P and (I + A)^-1 have been read: their columns take beta
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             if (q > 1 && wave < 3) break;
@@ -646,13 +649,16 @@ __device__ __forceinline__ void prepare(const ChunkArgs& a, PrepLds<T, DK>& lds,
 #pragma unroll
             for (int x = 0; x < 4; x++) sT[(16 * wave + 4 * g4 + x) * kPitchA + 16 * j + l16] *= bj;
         }
-        __syncthreads();
+        PREP_MEET();
         for (int x = wave; x < 2 * kTri; x += 4) {
             if (x < kTri) store_fragment<3>(sT, sW, unit, x, lane);
             else store_fragment<LO>(sA, nullptr, unit + kTri * 3 * kFrag, x - kTri, lane);
         }
     }
 }
+
+constexpr int kPrepBarriers = __COUNTER__ - kPrepFirst - 1;
+#undef PREP_MEET
 
 // A workgroup a chunk and `per` value heads, for all chunks and heads side by side.
 // Bound by the chain of its steps, with four workgroups a CU beside each other: of 128 chunks of 32 heads, two to a key head, 50 us,
@@ -725,7 +731,7 @@ __global__ __launch_bounds__(512, 2) void k_delta_chunks(ChunkArgs a) {
                 prepare<T, DK>(a, lds, first, b, e - b, h, 1);
                 __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0): the unit is written before it is read
             } else {
-                for (int x = 0; x < kPrepBarriers; x++) __syncthreads();
+                for (int x = 0; x < kPrepBarriers; x++) __syncthreads();       // prepare()'s
             }
             __syncthreads();
         }
