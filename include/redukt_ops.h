@@ -39,16 +39,18 @@ extern "C" {
  * Each of hv value heads keeps a state S [dk][dv] in f32.  A token with key k and query q
  * [dk] (of key head h / (hv / hk)), value v [dv], log decay g and write strength beta makes
  *     S <- e^g S + beta k (v - e^g S^T k)^T        o = scale S^T q
- * in f32 arithmetic.  g may be -inf (the state is dropped).  The rule is stable for |k| <= 1,
- * g <= 0 and beta in [0, 2]; with REDUKT_DELTA_NORMALIZE, k and q are divided by
- * sqrt(sum of squares + 1e-6) first.
+ * in f32 arithmetic.  (The factors of delta_chunk's 16-bit outputs are taken with 16 bits: beside
+ * its rounding to `dtype` such an output is off by at most 2^-15 of the magnitudes that it sums.
+ * States and f32 outputs are as exact as f32 sums are.)  g may be -inf (the state is dropped).  The
+ * rule is stable for |k| <= 1, g <= 0 and beta in [0, 2]; with REDUKT_DELTA_NORMALIZE, k and q are
+ * divided by sqrt(sum of squares + 1e-6) first.
  *
  * A value that is not finite goes where the rule takes it: one of v into its column, one of k,
  * g or beta into its head, from its token on; one of q into its token.  What it reaches is then
  * not finite, inf or NaN.  To normalize, a key or query whose sum of squares passes f32's range
- * (|k| from about 1.8e19 on) counts as one that is not finite.  (In delta_chunk, a sum that passes f32's range from finite inputs,
- * which a stable rule has none of (the sum of squares of a key is one), may also reach up to 63 tokens back, and a decay over several
- * tokens that is below 2^-126 is 0.) */
+ * (a length of about 1.8e19) counts as one that is not finite.  In delta_chunk, a sum that passes
+ * f32's range from finite inputs may also reach up to 63 tokens back (a stable rule has none, but
+ * of values and states next to that range), and a decay over several tokens below 2^-126 is 0. */
 #define REDUKT_DELTA_NORMALIZE 1u
 
 typedef struct {

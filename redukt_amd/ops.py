@@ -236,8 +236,9 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     not wanted; state_in itself: in place).  cu_seqlens int32, none decreasing, within the rows.
     A slot of -1 leaves the sequence out; slots out of range, or named before while state_out
     is given, give NaN rows.  Returns out [rows, value heads, dv]; rows of no sequence are not
-    written.  At most 65,536 sequences.  workspace: a uint8 tensor of `delta_chunk_workspace` bytes that nothing else uses
-    meanwhile (allocated if None).
+    written.  At most 65,536 sequences.  States and float32 outputs are as exact as float32 sums,
+    16-bit outputs are summed from factors of 16 bits.  workspace: a uint8 tensor of
+    `delta_chunk_workspace` bytes that nothing else uses meanwhile (allocated if None).
     """
     op = "delta_chunk"
     allocates = out is None or workspace is None
