@@ -18,6 +18,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import ffi
 
@@ -74,17 +75,19 @@ def _refuse(what: str) -> None:
     raise ffi.BackendError(ffi.BackendResult.INVALID_ARGUMENT, what)
 
 
-def _done(code: int, what: str, written) -> None:
-    """The end of a call that writes the tensors `written`, unseen by torch: it counts their writes, for what autograd has saved."""
+# (Operators write the caller's tensors unseen by torch; increment_version counts these writes, for what autograd has saved.)
+def _done(code: int, what: str) -> None:
     if code:
         raise ffi.BackendError(ffi.BackendResult.from_code(code), what)
-    torch.autograd.graph.increment_version(written)
 
 
 def _sizes(op: str, *sizes: int) -> None:
     """The library's fields for sizes have 32 bits, and ctypes would drop what is above."""
-    if max(sizes) > 0x7fffffff or min(sizes) < 0:
-        _refuse(f"{op}: sizes {sizes} are not within 2^31 - 1")
+    bits = 0
+    for s in sizes:
+        bits |= s
+    if bits >> 31:
+        _refuse(f"{op}: sizes {sizes} are not within 0 and 2^31 - 1")
 
 
 def _check(op: str, device: int, name: str, t, dtype, shape) -> None:
@@ -115,14 +118,17 @@ def _stream(op: str, stream: Optional[int], device: int, allocates: bool) -> int
     return stream
 
 
-def _no_gradients(op: str, asked: bool, *tensors) -> None:
-    """asked: one of `tensors` requires a gradient."""
-    if asked and torch.is_grad_enabled():
+def _no_gradients(op: str, *tensors) -> None:
+    """Refuses tensors (None: left out) that ask for a gradient while torch records them, or have a tangent.  Called where one
+    requires a gradient or somebody computes tangents (_tangents)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         _refuse(f"{op}: a tensor asks for a gradient, which this operator has not (detach it, or use torch.no_grad())")
-    if forward_ad._current_level >= 0:         # (-1: nobody computes tangents)
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                _refuse(f"{op}: a tensor has a tangent, which this operator would drop")
+    if _tangents() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _refuse(f"{op}: a tensor has a tangent, which this operator would drop")
+
+
+def _tangents() -> bool:
+    return forward_ad._current_level >= 0
 
 
 def _row_stride(op: str, name: str, t, width: int) -> int:
@@ -157,15 +163,16 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
         _check(op, device, "g", g, torch.float32, tuple(v.shape[:2]))
         _check(op, device, "beta", beta, torch.float32, tuple(v.shape[:2]))
         _refuse(f"{op}: tensors do not belong together")
-    _no_gradients(op, q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad,
-                  q, k, v, g, beta)
+    if q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad or _tangents():
+        _no_gradients(op, q, k, v, g, beta)
     _, hv, dv = wide
-    _sizes(op, T, hk, dk, hv, dv)
+    if (T | hk | dk | hv | dv) >> 31:
+        _sizes(op, T, hk, dk, hv, dv)
     if out is None:
         out = torch.empty_like(v) if v.is_contiguous() else torch.empty(wide, dtype=dtype, device=q.device)
     else:
         _check(op, device, "out", out, dtype, wide)
-        _no_gradients(op, out.requires_grad, out)
+        _no_gradients(op, out)
     wk, wv = hk * dk, hv * dv
     if scale is None:
         scale = dk ** -0.5 if dk else 0.0
@@ -179,7 +186,8 @@ def _rows(op: str, q, k, v, g, beta, out, scale, normalize) -> Tuple[DeltaRows, 
 def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
     try:
         if (t.dtype is torch.float32 and t.shape[1:] == (a.hv, a.dk, a.dv) and t.is_contiguous() and t.get_device() == device):
-            _no_gradients(op, t.requires_grad, t)
+            if t.requires_grad or _tangents():
+                _no_gradients(op, t)
             return
     except AttributeError:
         pass
@@ -216,7 +224,8 @@ def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[f
     _pool(op, device, "states", states, a)
     code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
                                         _slots(op, device, slots, a.rows), on)
-    _done(code, op, (states, out))
+    _done(code, op)
+    increment_version(states if allocates else (states, out))
     return out
 
 
@@ -242,13 +251,15 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     """
     op = "delta_chunk"
     allocates = out is None or workspace is None
+    given = () if out is None and workspace is None else [t for t in (out, workspace) if t is not None]
     a, out, device = _rows(op, q, k, v, g, beta, out, scale, normalize)
     on = _stream(op, stream, device, allocates)
     _check(op, device, "cu_seqlens", cu_seqlens, torch.int32, (None,))
     n = cu_seqlens.shape[0] - 1
     if n < 0 or not cu_seqlens.is_contiguous():
         _refuse(f"{op}: cu_seqlens holds one value more than there are sequences")
-    _sizes(op, n)
+    if n > 65536:
+        _refuse(f"{op}: more than 65,536 sequences")
     n_slots = 0
     for name, pool in (("state_in", state_in), ("state_out", state_out)):
         if pool is not None:
@@ -268,7 +279,11 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
                                    None if state_in is None else state_in.data_ptr(),
                                    None if state_out is None else state_out.data_ptr(), n_slots,
                                    _slots(op, device, slots, n), workspace.data_ptr(), workspace.numel(), on)
-    _done(code, op, (out, workspace) if state_out is None else (out, workspace, state_out))
+    _done(code, op)
+    if state_out is not None:
+        increment_version(state_out)
+    if given:
+        increment_version(given)
     return out
 
 
@@ -282,8 +297,10 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
     device = _device(op, x)
     if x.dtype not in DTYPES or x.dim() != 2:
         _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
-    _no_gradients(op, x.requires_grad, x)
+    if x.requires_grad or _tangents():
+        _no_gradients(op, x)
     on = _stream(op, stream, device, codes is None or scales is None)
+    given = [t for t in (codes, scales) if t is not None]
     rows, cols = x.shape
     _sizes(op, rows, cols)
     if codes is None:
@@ -294,12 +311,14 @@ def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
         scales = torch.empty((rows,), dtype=torch.float32, device=x.device)
     else:
         _check(op, device, "scales", scales, torch.float32, (rows,))
-        _no_gradients(op, scales.requires_grad, scales)
+        _no_gradients(op, scales)
         if not scales.is_contiguous():
             _refuse(f"{op}: scales is not contiguous")
     a = QuantizeRows(DTYPES[x.dtype], rows, cols, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
                      _row_stride(op, "codes", codes, cols), scales.data_ptr())
-    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), on), op, (codes, scales))
+    _done(_load().redukt_op_quantize_rows(ctypes.byref(a), on), op)
+    if given:
+        increment_version(given)
     return codes, scales
 
 
@@ -329,11 +348,12 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         if bias is not None:
             _check(op, device, "bias", bias, f32, (w.shape[0],))
         _refuse(f"{op}: scales and bias are contiguous")
-    _no_gradients(op, x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad),
-                  x_scales, w_scales, bias)
+    if x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad) or _tangents():
+        _no_gradients(op, x_scales, w_scales, bias)
     _sizes(op, m, n, k)
-    on = _stream(op, stream, device, out is None)
-    if out is None:
+    allocates = out is None
+    on = _stream(op, stream, device, allocates)
+    if allocates:
         if dtype not in DTYPES:
             _refuse(f"{op}: dtype is bfloat16, float16 or float32")
         out = torch.empty((m, n), dtype=dtype, device=x.device)
@@ -341,9 +361,11 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
         if not isinstance(out, torch.Tensor) or out.dtype not in DTYPES:
             _refuse(f"{op}: out is bfloat16, float16 or float32")
         _check(op, device, "out", out, out.dtype, (m, n))
-        _no_gradients(op, out.requires_grad, out)
+        _no_gradients(op, out)
     a = Int8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))
-    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op, (out,))
+    _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op)
+    if not allocates:
+        increment_version(out)
     return out
