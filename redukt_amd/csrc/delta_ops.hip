@@ -38,7 +38,9 @@ __device__ __forceinline__ int entry_slot(const int32_t* slots, uint32_t n_slots
     if (s == -1) return kSkip;
     if (s < 0 || (uint32_t)s >= n_slots) return kBad;
     if (!writes) return s;
-    // (four loads at once where the loop is long: 16,384 entries 344 -> 247 us; 500 of 32 heads 399 one by one, 405 by four)
+    // Every wave of an entry looks through all slots before its own; four loads at once where the loop is long.  us by four, one by
+    // one, and of a call without slots: 500 entries of 32 heads of 128 x 128 398, 401 and 400; 4,096 of 32 heads of 64 x 64 863, 880 and
+    // 836; 16,384 of 12 1,470, 1,946 and 1,255; 65,536 of 4 3,647, 6,801 and 1,674.
     bool earlier = false;
     for (uint32_t c = lane; c < min(i, 1024u); c += kWave) earlier |= slots[c] == s;
     for (uint32_t c = 1024 + lane; c < i; c += 4 * kWave) {
@@ -150,8 +152,10 @@ const void* delta_step_fn(uint32_t dtype, uint32_t dk) {
 // own operand (f16: two limbs, f32: three, exact); S, X and diag() T are f32 split into three
 // limbs of 8 bits, and products of limbs are kept down to 2^-24 of the whole, so the state is as
 // exact as f32 sums are (two limbs leave about 4e-6).  P T, and S and X where only a 16-bit output
-// comes of them, are two limbs (2^-17 against an output's half step of 2^-8 or 2^-11).  G is
-// summed in 64 bits: the decays are e to small differences of sums that may be large.
+// comes of them, are two limbs (2^-17 against an output's half step of 2^-8 or 2^-11).  A third one of
+// P T and X there takes the outputs' error before their rounding from 3.7e-6 to 0.7e-6, and both forms are
+// off by 1.7e-3 behind it in bf16; but 6 KB more a chunk go through L1: 8,192 tokens 259 -> 293 us, 37 ragged
+// prompts 183 -> 191.  G is summed in 64 bits: the decays are e to small differences of sums that may be large.
 //
 // What is not finite.  A matrix product would spread one over rows it does not reach by the rule
 // (0 times it), so rows of X from a column's first such value on are taken as zeros, and the column's
@@ -273,7 +277,8 @@ __device__ __forceinline__ uint32_t row_of(const ChunkArgs& a, uint32_t i) {
 }
 
 // The sequence that is the pos-th by length, longest first (n <= 64; every lane of the wave takes part).  Workgroups that wait for a
-// CU start in this order, so that no long sequence begins last (37 of 3 to 932 tokens: 203 -> 194 us).
+// CU start in this order, so that no long sequence begins last (37 of 3 to 932 tokens: 203 -> 194 us).  More than 64 sequences, which
+// one wave does not hold, start in the order of their numbers.
 __device__ __forceinline__ uint32_t by_length(const ChunkArgs& a, uint32_t pos, int lane) {
     const bool in = (uint32_t)lane < a.d.n;
     const uint32_t b = in ? row_of(a, lane) : 0, len = in ? max(row_of(a, lane + 1), b) - b : 0;

@@ -109,7 +109,8 @@ __device__ __forceinline__ float scaled(const redukt_int8_matmul& a, int sum, ui
 }
 
 // Codes of any alignment: 64 x 64 outputs a workgroup, 64 columns at a time staged byte by byte
-// with zeros outside the operands.  For odd sizes and strides, not for speed: 16-byte accesses need rows that begin on 16 bytes.
+// with zeros outside the operands.  For odd sizes and strides, not for speed: 16-byte accesses need rows that begin on 16 bytes
+// (100 tokens of 4,096 x 1,530: 92 us; of 4,096 x 1,536, by the kernels below, 5).
 constexpr int kTile = 64, kPitch = kTile + 16;
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
@@ -142,10 +143,11 @@ __global__ __launch_bounds__(kBlock) void k_int8_bytes(redukt_int8_matmul a) {
     }
 }
 
-// Up to 16 tokens: the weights are read once, straight into registers, and nothing else costs much (one token of 50,280 x 768:
-// 38.6 MB in 10.2 us, 3.8 TB/s with the launch; of 8,192 x 8,192 67 MB in 13.8, 4.9).  Workgroups begin at different columns: rows of a
-// power of two put the same columns into the same channel of a cache, where all would wait at once (8,192 x 8,192: 17.6 -> 13.8 us).  Of a workgroup's eight waves `split` share 16 channels, each taking every split-th line
-// of 128 columns; their sums meet in LDS.
+// Few tokens (up to 16, of many channels up to 3: redukt_op_int8_matmul): the weights are read once, straight into registers, and
+// nothing else costs much (one token of 50,280 x 768: 38.6 MB in 10.3 us, 3.7 TB/s with the launch; of 8,192 x 8,192 67 MB in 12.7,
+// 5.3).  Workgroups begin at different columns: rows of a power of two put the same columns into the same channel of a cache, where all
+// would wait at once (8,192 x 8,192: 17.6 -> 13.8 us).  Of a workgroup's eight waves `split` share 16 channels, each taking every
+// split-th line of 128 columns; their sums meet in LDS.
 struct Int8Few {
     redukt_int8_matmul a;
     uint32_t split;
@@ -201,8 +203,8 @@ __global__ __launch_bounds__(512) void k_int8_few(Int8Few f) {
 // lane picks the piece that belongs to its place.
 //
 // Tiles of 256 x 256 are bound by the matrix cores and the LDS reads beside them: 8,192 of 8,192 x 4,096 in 249 us, 2.2 POP/s (the
-// library's int8 product 250).  The smaller ones by the columns on their way: 64 of 8,192 x 8,192 in 15.2, 67 MB at 4.4 TB/s; 100 of
-// 4,096 x 1,536 in 6.5, the launch and twelve steps.
+// library's int8 product 250).  The smaller ones by the columns on their way: 64 of 8,192 x 8,192 in 14.0, 67 MB at 4.8 TB/s; 100 of
+// 4,096 x 1,536 in 5.1, the launch and twelve steps.
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 typedef __attribute__((address_space(3))) void lds_void;
@@ -461,7 +463,8 @@ int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream) {
     if (a->m <= (a->n >= 8192 ? 3 : 16)) return few(*a, stream);
     // Tiles of 256 once they fill the CUs (8,192 of 8,192 x 4,096: 249, tiles of 128: 291; 2,048 of 4,096 x 1,536, 128 tiles: 27.8 and
     // 20.9), of 128 once they nearly do (4,096 of 768 x 768, 192 tiles: 10.3, tiles of 64: 10.8; 1,000 of 1,536 x 768, 96 tiles:
-    // 9.4 and 7.0), else of 64, by 32 channels where half of the CUs would have none (64 of 8,192 x 8,192: 15.2, by 64 16.4).  Where no CU has
+    // 9.4 and 7.0), else of 64, by 32 channels where half of the CUs would have none (64 of 8,192 x 8,192: 13.2, by 64
+    // 14.8; 128 of 4,096 x 4,096 8.0 and 8.1; 100 of 4,096 x 1,536 5.0 both).  Where no CU has
     // two workgroups, each keeps more columns on their way (1,024 of 4,096 x 4,096, 256 tiles of 128: 28.2 with two stages, 25.3 with three;
     // 2,048 of 4,096 x 1,536, 512 tiles: 21.4 and 25.3; 128 of 8,192 x 8,192, 256 of 64: 26.3 with two of 256 columns, 17.6 with four
     // of 128; 512 of 4,096 x 4,096, 512 of 64: 16.4 and 17.8).

@@ -4,12 +4,12 @@ The gated delta rule for one token (`delta_step`) and for whole sequences (`delt
 codes of activation rows (`quantize_rows`) and the product of codes with a scale per token and
 channel (`int8_matmul`).  Arguments are torch tensors on one GPU; work is queued on torch's
 current stream of that GPU, or on `stream`, a hipStream_t's value.  Outputs and workspaces that a
-call allocates belong to torch's current stream, so for another one they are passed in.  Outputs
-overlap no input (but a state pool its own next states).  No model needs to be open.  The
-operators have no gradients: tensors that ask for one, states and outputs among them, are refused
-while torch records them, and tensors with a tangent always.
-Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch nothing; there is no CPU
-fallback.
+call allocates belong to torch's current stream, so for another one they are passed in, and the
+caller keeps all tensors until that stream is done with them.  Outputs overlap no input (but a state
+pool its own next states).  No model needs to be open.  The operators have no gradients: tensors
+that ask for one, states and outputs among them, are refused while torch records them, and tensors
+with a tangent always.  Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch
+nothing; there is no CPU fallback.
 """
 from __future__ import annotations
 
