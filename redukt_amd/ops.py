@@ -75,7 +75,6 @@ def _refuse(what: str) -> None:
     raise ffi.BackendError(ffi.BackendResult.INVALID_ARGUMENT, what)
 
 
-# (Operators write the caller's tensors unseen by torch; increment_version counts these writes, for what autograd has saved.)
 def _done(code: int, what: str) -> None:
     if code:
         raise ffi.BackendError(ffi.BackendResult.from_code(code), what)
@@ -225,6 +224,7 @@ def delta_step(q, k, v, g, beta, states, slots=None, out=None, scale: Optional[f
     code = _load().redukt_op_delta_step(ctypes.byref(a), states.data_ptr(), states.shape[0],
                                         _slots(op, device, slots, a.rows), on)
     _done(code, op)
+    # (these were written unseen by torch, which counts writes for what autograd has saved)
     increment_version(states if allocates else (states, out))
     return out
 
