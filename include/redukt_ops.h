@@ -3,7 +3,8 @@
  * The plugin ABI (redukt_backend.h) steps the models that the library loads.  The entry
  * points below are the parts of such a layer as operators of their own, for programs that hold
  * activations, weights and recurrent states themselves: the gated delta rule for one token
- * and for whole sequences, and the int8 product with the pass that makes its codes.
+ * and for whole sequences, the selective scan likewise and with its gradients, and the int8
+ * product with the pass that makes its codes.
  *
  * Contract:
  *   - no model is needed (nothing here touches what redukt_backend_init made), and calls from
@@ -94,6 +95,74 @@ int32_t redukt_op_delta_chunk(const redukt_delta_rows* a, const int32_t* cu, uin
 /* The bytes of workspace for these rows (only the sizes and the element type are read); 0 if
  * the sizes are not ones that delta_chunk takes, or need none. */
 uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_seq);
+
+/* ---------------- the selective scan ----------------
+ *
+ * Each channel keeps a state h [n] in f32.  A token with input x, time step dt, gate z (of the
+ * channel), B and C [n] (of the channel's group) makes, with s = ln(1 + e^(dt + dt_bias)),
+ *     h <- e^(s a) h + s x B        out = (C . h + d x) z / (1 + e^-z)
+ * in f32, rounded once to `dtype`; without z its factor is 1, without d or dt_bias they are 0.  A dt of
+ * -inf leaves the state as it is.  The rule is stable for a <= 0.  A value that is not finite goes where
+ * the rule takes it: one of x or dt into its channel, one of B into its group's channels, from its
+ * token on; one of C or z into its token.  A power below 2^-126 is 0. */
+typedef struct {
+    uint32_t dtype;         /* of x, dt, z, b, c and out */
+    uint32_t rows;          /* tokens */
+    uint32_t channels;      /* at most 1,048,576; with several groups a multiple of 64 each */
+    uint32_t groups;        /* of B and C: channel i has those of group i / (channels / groups) */
+    uint32_t n;             /* 8, 16, 32 or 64 */
+    const void* x;          /* row t: `channels` elements at x + t * x_stride */
+    const void* dt;
+    const void* z;          /* or NULL */
+    const void* b;          /* row t: groups * n elements */
+    const void* c;
+    void* out;
+    int64_t x_stride, dt_stride, z_stride, b_stride, c_stride, out_stride;   /* elements from a row to the next, at most 2^22 */
+    const float* a;         /* [channels][n] */
+    const float* d;         /* [channels], or NULL */
+    const float* dt_bias;   /* [channels], or NULL */
+} redukt_scan_rows;         /* any alignment that the element types have; states: 16-byte aligned */
+
+/* One token for each of `rows` entries (at most 65,536), as redukt_op_delta_step has it: entry i steps
+ * slot slots[i] (NULL: i) of states [n_slots][channels][n] in place; -1 leaves the entry's output and
+ * state as they are; a slot out of range, or that an earlier entry names, touches no state and its
+ * output row becomes NaN. */
+int32_t redukt_op_scan_step(const redukt_scan_rows* a, float* states, uint32_t n_slots, const int32_t* slots, void* stream);
+
+/* Whole sequences: cu, slots, state_in, state_out, workspace and rows of no sequence are
+ * redukt_op_delta_chunk's.  A sequence's results depend on nothing else in the call. */
+int32_t redukt_op_scan_chunk(const redukt_scan_rows* a, const int32_t* cu, uint32_t n_seq, const float* state_in,
+                             float* state_out, uint32_t n_slots, const int32_t* slots, void* workspace,
+                             uint64_t workspace_bytes, void* stream);
+
+/* The bytes of workspace for these rows (only the sizes are read); 0 if the sizes are not ones that
+ * scan_chunk takes, or need none. */
+uint64_t redukt_op_scan_chunk_workspace(const redukt_scan_rows* a, uint32_t n_seq);
+
+/* What the backward pass reads and writes beside the rows: arrays like the ones that they are gradients
+ * of, in their types. */
+typedef struct {
+    const void* dout;       /* row t: `channels` elements */
+    void* dx;
+    void* ddt;
+    void* dz;               /* NULL without z */
+    void* db;               /* row t: groups * n elements */
+    void* dc;
+    int64_t dout_stride, dx_stride, ddt_stride, dz_stride, db_stride, dc_stride;    /* at most 2^22 */
+    float* da;              /* [channels][n] */
+    float* dd;              /* [channels]; NULL without d */
+    float* ddt_bias;        /* [channels]; NULL without dt_bias */
+} redukt_scan_grads;
+
+/* The gradients of sum(dout * out) + sum(dstate_out * last states) for the sequences cu from the states
+ * state_in [n_seq][channels][n] (NULL: zeros), dstate_out alike (NULL: zeros); `out` of the rows is not
+ * read.  dstate_in (NULL: not wanted; not one of the others) takes that of the first states.  Rows of no
+ * sequence get gradients of zero.  Everything is formed anew from the inputs, sums over channels, tokens
+ * and sequences in f32 in a fixed order.  workspace: redukt_op_scan_grad_workspace(a, n_seq) bytes. */
+int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* g, const int32_t* cu, uint32_t n_seq,
+                            const float* state_in, const float* dstate_out, float* dstate_in, void* workspace,
+                            uint64_t workspace_bytes, void* stream);
+uint64_t redukt_op_scan_grad_workspace(const redukt_scan_rows* a, uint32_t n_seq);
 
 /* ---------------- int8 codes and their product ---------------- */
 

@@ -29,27 +29,6 @@ struct DeltaArgs {
     uint32_t n;                // entries
 };
 
-// What becomes of entry i: its slot, or kSkip (padded, nothing is touched) or kBad (out of range, or named
-// by an earlier entry while states are written).  Every lane of the wave takes part.
-constexpr int kSkip = -1, kBad = -2;
-__device__ __forceinline__ int entry_slot(const int32_t* slots, uint32_t n_slots, uint32_t i, bool writes, int lane) {
-    if (!slots) return (int)i;
-    const int s = __builtin_amdgcn_readfirstlane(slots[i]);
-    if (s == -1) return kSkip;
-    if (s < 0 || (uint32_t)s >= n_slots) return kBad;
-    if (!writes) return s;
-    // Every wave of an entry looks through all slots before its own; four loads at once where the loop is long.  us by four, one by
-    // one, and of a call without slots: 500 entries of 32 heads of 128 x 128 398, 401 and 400; 4,096 of 32 heads of 64 x 64 863, 880 and
-    // 836; 16,384 of 12 1,470, 1,946 and 1,255; 65,536 of 4 3,647, 6,801 and 1,674.
-    bool earlier = false;
-    for (uint32_t c = lane; c < min(i, 1024u); c += kWave) earlier |= slots[c] == s;
-    for (uint32_t c = 1024 + lane; c < i; c += 4 * kWave) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) earlier |= slots[min(c + u * kWave, i - 1)] == s;
-    }
-    return __any(earlier) ? kBad : s;
-}
-
 // v summed over the lanes that differ in bits 3, 4 and 5, the same bits in every one of them.
 __device__ __forceinline__ float rows_sum(float v) {
     v += __shfl_xor(v, 8, kWave);
@@ -1166,12 +1145,6 @@ bool rows_ok(const redukt_delta_rows* a) {
     }
     return a->g && a->beta && op_aligned(a->g, 4) && op_aligned(a->beta, 4) &&
            (a->rows <= 1 || (a->g_stride >= 0 && a->beta_stride >= 0));
-}
-
-// Whether two pools of n bytes are the same one or have nothing in common.
-bool apart(const void* a, const void* b, size_t n) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return x == y || (x < y ? y - x : x - y) >= n;
 }
 
 // The rows with a step from one to the next that is a row's width where there is one row only.

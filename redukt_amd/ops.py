@@ -14,7 +14,7 @@ nothing; there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
@@ -34,6 +34,24 @@ class DeltaRows(ctypes.Structure):
                 ("q_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
                 ("out_stride", ctypes.c_int64), ("g", ctypes.c_void_p), ("beta", ctypes.c_void_p),
                 ("g_stride", ctypes.c_int64), ("beta_stride", ctypes.c_int64)]
+
+
+class ScanRows(ctypes.Structure):
+    """redukt_scan_rows."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("channels", ctypes.c_uint32), ("groups", ctypes.c_uint32),
+                ("n", ctypes.c_uint32), ("x", ctypes.c_void_p), ("dt", ctypes.c_void_p), ("z", ctypes.c_void_p),
+                ("b", ctypes.c_void_p), ("c", ctypes.c_void_p), ("out", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("dt_stride", ctypes.c_int64), ("z_stride", ctypes.c_int64), ("b_stride", ctypes.c_int64),
+                ("c_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("a", ctypes.c_void_p), ("d", ctypes.c_void_p),
+                ("dt_bias", ctypes.c_void_p)]
+
+
+class ScanGradients(ctypes.Structure):
+    """redukt_scan_grads."""
+    _fields_ = [("dout", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("ddt", ctypes.c_void_p), ("dz", ctypes.c_void_p),
+                ("db", ctypes.c_void_p), ("dc", ctypes.c_void_p), ("dout_stride", ctypes.c_int64), ("dx_stride", ctypes.c_int64),
+                ("ddt_stride", ctypes.c_int64), ("dz_stride", ctypes.c_int64), ("db_stride", ctypes.c_int64),
+                ("dc_stride", ctypes.c_int64), ("da", ctypes.c_void_p), ("dd", ctypes.c_void_p), ("ddt_bias", ctypes.c_void_p)]
 
 
 class QuantizeRows(ctypes.Structure):
@@ -65,7 +83,14 @@ def _load() -> ctypes.CDLL:
         L.redukt_op_delta_chunk_workspace.restype = u64
         L.redukt_op_quantize_rows.argtypes = [ctypes.POINTER(QuantizeRows), p]
         L.redukt_op_int8_matmul.argtypes = [ctypes.POINTER(Int8Matmul), p]
-        for f in ("delta_step", "delta_chunk", "quantize_rows", "int8_matmul"):
+        L.redukt_op_scan_step.argtypes = [ctypes.POINTER(ScanRows), p, u32, p, p]
+        L.redukt_op_scan_chunk.argtypes = [ctypes.POINTER(ScanRows), p, u32, p, p, u32, p, p, u64, p]
+        L.redukt_op_scan_chunk_workspace.argtypes = [ctypes.POINTER(ScanRows), u32]
+        L.redukt_op_scan_chunk_workspace.restype = u64
+        L.redukt_op_scan_grad.argtypes = [ctypes.POINTER(ScanRows), ctypes.POINTER(ScanGradients), p, u32, p, p, p, p, u64, p]
+        L.redukt_op_scan_grad_workspace.argtypes = [ctypes.POINTER(ScanRows), u32]
+        L.redukt_op_scan_grad_workspace.restype = u64
+        for f in ("delta_step", "delta_chunk", "scan_step", "scan_chunk", "scan_grad", "quantize_rows", "int8_matmul"):
             getattr(L, "redukt_op_" + f).restype = ctypes.c_int32
         _lib = L
     return _lib
@@ -285,6 +310,270 @@ def delta_chunk(q, k, v, g, beta, cu_seqlens, state_in=None, state_out=None, slo
     if given:
         increment_version(given)
     return out
+
+
+def _scan_rows(op: str, x, dt, a, b, c, d, z, dt_bias, out) -> Tuple[ScanRows, int]:
+    """The rows, with every tensor checked (out None: none is written)."""
+    device = _device(op, x)
+    f32, dtype = torch.float32, x.dtype
+    if dtype not in DTYPES or x.dim() != 2:
+        _refuse(f"{op}: x [rows, channels] is bfloat16, float16 or float32")
+    shape = x.shape
+    T, channels = shape
+    try:       # (all at once; what is wrong is looked for only if something is)
+        bc, n = b.shape, a.shape[1]
+        fine = (dt.shape == shape and bc == c.shape and len(bc) == 3 and bc[0] == T and bc[2] == n and a.shape == (channels, n)
+                and dt.dtype is dtype and b.dtype is dtype and c.dtype is dtype and a.dtype is f32 and a.is_contiguous()
+                and dt.get_device() == a.get_device() == b.get_device() == c.get_device() == device
+                and (z is None or (z.shape == shape and z.dtype is dtype and z.get_device() == device))
+                and (d is None or (d.shape == shape[1:] and d.dtype is f32 and d.get_device() == device and d.is_contiguous()))
+                and (dt_bias is None or (dt_bias.shape == shape[1:] and dt_bias.dtype is f32 and dt_bias.get_device() == device
+                                         and dt_bias.is_contiguous())))
+    except (AttributeError, IndexError, TypeError):
+        fine = False
+    if not fine:
+        _check(op, device, "dt", dt, dtype, (T, channels))
+        _check(op, device, "a", a, f32, (channels, None))
+        _check(op, device, "b", b, dtype, (T, None, a.shape[1]))
+        _check(op, device, "c", c, dtype, tuple(b.shape))
+        for name, t, of, want in (("z", z, dtype, (T, channels)), ("d", d, f32, (channels,)), ("dt_bias", dt_bias, f32, (channels,))):
+            if t is not None:
+                _check(op, device, name, t, of, want)
+        _refuse(f"{op}: a, d and dt_bias are contiguous")
+    groups = bc[1]
+    if (T | channels | groups | n) >> 31:
+        _sizes(op, T, channels, groups, n)
+    if out is not None:
+        _check(op, device, "out", out, dtype, shape)
+    wide = groups * n
+    return ScanRows(DTYPES[dtype], T, channels, groups, n, x.data_ptr(), dt.data_ptr(), None if z is None else z.data_ptr(), b.data_ptr(),
+                    c.data_ptr(), None if out is None else out.data_ptr(), _row_stride(op, "x", x, channels),
+                    _row_stride(op, "dt", dt, channels), 0 if z is None else _row_stride(op, "z", z, channels),
+                    _row_stride(op, "b", b, wide), _row_stride(op, "c", c, wide),
+                    0 if out is None else _row_stride(op, "out", out, channels), a.data_ptr(), None if d is None else d.data_ptr(),
+                    None if dt_bias is None else dt_bias.data_ptr()), device
+
+
+def _scan_pool(op: str, device: int, name: str, t, a: ScanRows, slots: Optional[int] = None) -> None:
+    _check(op, device, name, t, torch.float32, (slots, a.channels, a.n))
+    if not t.is_contiguous():
+        _refuse(f"{op}: {name} is not contiguous")
+
+
+def _sequences(op: str, device: int, cu_seqlens) -> int:
+    _check(op, device, "cu_seqlens", cu_seqlens, torch.int32, (None,))
+    n = cu_seqlens.shape[0] - 1
+    if n < 0 or not cu_seqlens.is_contiguous():
+        _refuse(f"{op}: cu_seqlens holds one value more than there are sequences")
+    if n > 65536:
+        _refuse(f"{op}: more than 65,536 sequences")
+    return n
+
+
+def _workspace(op: str, device: int, workspace, need: int):
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", device) if device >= 0 else "cpu")
+    _check(op, device, "workspace", workspace, torch.uint8, (None,))
+    if not workspace.is_contiguous():      # (its bytes are counted by its elements)
+        _refuse(f"{op}: workspace is not contiguous")
+    return workspace
+
+
+def _asks(*tensors) -> bool:
+    return _tangents() or any(t is not None and t.requires_grad for t in tensors)
+
+
+def scan_step(x, dt, a, b, c, states, d=None, z=None, dt_bias=None, slots=None, out=None, stream: Optional[int] = None):
+    """The selective scan for one token of each of n entries (at most 65,536); states are stepped in place.
+
+    With s = softplus(dt + dt_bias), a channel's state h takes a token as h <- e^(s a) h + s x B and
+    gives out = (C . h + d x) silu(z).  x, dt, z [n, channels] and b, c [n, groups, size] in bfloat16,
+    float16 or float32 (one type); a [channels, size], d and dt_bias [channels] and states [slots,
+    channels, size] float32.  z, d and dt_bias may be left out.  size is 8, 16, 32 or 64; with several
+    groups each has a multiple of 64 channels.  Entry i steps slot slots[i] (int32; None: slot i); -1 leaves
+    entry i's output and state as they are; a slot out of range, or named by an earlier entry, gives NaN
+    outputs and touches no state.  Returns out [n, channels] (allocated if None); rows may be strided.
+    """
+    op = "scan_step"
+    allocates = out is None
+    if allocates:
+        _device(op, x)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    r, device = _scan_rows(op, x, dt, a, b, c, d, z, dt_bias, out)
+    on = _stream(op, stream, device, allocates)
+    _scan_pool(op, device, "states", states, r)
+    if _asks(x, dt, a, b, c, d, z, dt_bias, states, out):
+        _no_gradients(op, x, dt, a, b, c, d, z, dt_bias, states, out)
+    code = _load().redukt_op_scan_step(ctypes.byref(r), states.data_ptr(), states.shape[0], _slots(op, device, slots, r.rows), on)
+    _done(code, op)
+    increment_version(states if allocates else (states, out))
+    return out
+
+
+def _scan_sizes(op: str, tokens: int, sequences: int, channels: int, groups: int, size: int) -> ScanRows:
+    _sizes(op, tokens, sequences, channels, groups, size)
+    return ScanRows(0, tokens, channels, groups, size)
+
+
+def scan_chunk_workspace(tokens: int, sequences: int, channels: int, groups: int, size: int) -> int:
+    """Bytes of workspace that `scan_chunk` needs for these sizes."""
+    a = _scan_sizes("scan_chunk_workspace", tokens, sequences, channels, groups, size)
+    return _load().redukt_op_scan_chunk_workspace(ctypes.byref(a), sequences)
+
+
+def scan_chunk(x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_in=None, state_out=None, slots=None, out=None,
+               workspace=None, stream: Optional[int] = None):
+    """The selective scan over packed sequences: rows cu_seqlens[i] to cu_seqlens[i + 1] of x, dt, z, b
+    and c (as in `scan_step`) are sequence i, from the state in slot slots[i] (None: i) of state_in (None:
+    zeros); its final state goes to that slot of state_out (None: not wanted; state_in itself: in
+    place).  cu_seqlens int32, none decreasing, within the rows.  A slot of -1 leaves the sequence out;
+    slots out of range, or named before while state_out is given, give NaN rows.  Returns out [rows,
+    channels]; rows of no sequence are not written.  At most 65,536 sequences, whose results depend on
+    nothing else in the call.  workspace: a uint8 tensor of `scan_chunk_workspace` bytes that nothing else
+    uses meanwhile (allocated if None).  For training, `scan` is the same with gradients.
+    """
+    op = "scan_chunk"
+    allocates = out is None or workspace is None
+    given = [t for t in (state_out, out, workspace) if t is not None]
+    if out is None:
+        _device(op, x)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    r, device = _scan_rows(op, x, dt, a, b, c, d, z, dt_bias, out)
+    on = _stream(op, stream, device, allocates)
+    n = _sequences(op, device, cu_seqlens)
+    n_slots = 0
+    for name, pool in (("state_in", state_in), ("state_out", state_out)):
+        if pool is not None:
+            _scan_pool(op, device, name, pool, r)
+            n_slots = pool.shape[0]
+    if state_in is not None and state_out is not None and state_in.shape[0] != state_out.shape[0]:
+        _refuse(f"{op}: state_in and state_out differ in slots")
+    if _asks(x, dt, a, b, c, d, z, dt_bias, state_in, state_out, out):
+        _no_gradients(op, x, dt, a, b, c, d, z, dt_bias, state_in, state_out, out)
+    L = _load()
+    workspace = _workspace(op, device, workspace, L.redukt_op_scan_chunk_workspace(ctypes.byref(r), n))
+    code = L.redukt_op_scan_chunk(ctypes.byref(r), cu_seqlens.data_ptr(), n, None if state_in is None else state_in.data_ptr(),
+                                  None if state_out is None else state_out.data_ptr(), n_slots, _slots(op, device, slots, n),
+                                  workspace.data_ptr(), workspace.numel(), on)
+    _done(code, op)
+    if given:
+        increment_version(given)
+    return out
+
+
+class ScanGrads(NamedTuple):
+    """Gradients of `scan_grad`'s inputs, by their names; None for what was not given."""
+    x: torch.Tensor
+    dt: torch.Tensor
+    a: torch.Tensor
+    b: torch.Tensor
+    c: torch.Tensor
+    d: Optional[torch.Tensor]
+    z: Optional[torch.Tensor]
+    dt_bias: Optional[torch.Tensor]
+    state_in: Optional[torch.Tensor]
+
+
+def scan_grad_workspace(tokens: int, sequences: int, channels: int, groups: int, size: int) -> int:
+    """Bytes of workspace that `scan_grad` needs for these sizes."""
+    a = _scan_sizes("scan_grad_workspace", tokens, sequences, channels, groups, size)
+    return _load().redukt_op_scan_grad_workspace(ctypes.byref(a), sequences)
+
+
+def scan_grad(dout, x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_in=None, dstate_out=None, grads=None,
+              workspace=None, stream: Optional[int] = None) -> ScanGrads:
+    """The backward pass of the selective scan over packed sequences: the gradients of sum(dout * out) +
+    sum(dstate_out * final states) by everything that goes in.  Inputs as in `scan_chunk`; state_in and
+    dstate_out [sequences, channels, size] or None for zeros (without state_in, its gradient is None).
+    Gradients have their inputs' types; rows of no sequence have gradients of zero.  Everything is formed anew from
+    the inputs: nothing of the forward pass is needed.  grads: a ScanGrads of tensors to write (allocated if
+    None).  workspace: a uint8 tensor of `scan_grad_workspace` bytes that nothing else uses meanwhile (allocated
+    if None).
+    """
+    op = "scan_grad"
+    allocates = grads is None or workspace is None
+    r, device = _scan_rows(op, x, dt, a, b, c, d, z, dt_bias, None)
+    on = _stream(op, stream, device, allocates)
+    n = _sequences(op, device, cu_seqlens)
+    _check(op, device, "dout", dout, x.dtype, (r.rows, r.channels))
+    for name, pool in (("state_in", state_in), ("dstate_out", dstate_out)):
+        if pool is not None:
+            _scan_pool(op, device, name, pool, r, n)
+    inputs = (x, dt, a, b, c, d, z, dt_bias, state_in)
+    if grads is None:
+        made = ScanGrads(*(None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in inputs))
+    else:
+        if not isinstance(grads, tuple) or len(grads) != len(inputs):
+            _refuse(f"{op}: grads is a ScanGrads")
+        made = ScanGrads(*grads)
+        for name, t, g in zip(ScanGrads._fields, inputs, made):
+            if t is None and g is None:
+                continue
+            if t is None or g is None:
+                _refuse(f"{op}: grads.{name} is given where {name} is, and only there")
+            _check(op, device, "grads." + name, g, t.dtype, t.shape)
+            if name in ("a", "d", "dt_bias", "state_in") and not g.is_contiguous():
+                _refuse(f"{op}: grads.{name} is not contiguous")
+    if _asks(dout, dstate_out, *inputs, *made):
+        _no_gradients(op, dout, dstate_out, *inputs, *made)
+
+    def at(t):
+        return None if t is None else t.data_ptr()
+
+    wide = r.groups * r.n
+    g = ScanGradients(dout.data_ptr(), made.x.data_ptr(), made.dt.data_ptr(), at(made.z), made.b.data_ptr(), made.c.data_ptr(),
+                      _row_stride(op, "dout", dout, r.channels), _row_stride(op, "grads.x", made.x, r.channels),
+                      _row_stride(op, "grads.dt", made.dt, r.channels),
+                      0 if made.z is None else _row_stride(op, "grads.z", made.z, r.channels),
+                      _row_stride(op, "grads.b", made.b, wide), _row_stride(op, "grads.c", made.c, wide), made.a.data_ptr(),
+                      at(made.d), at(made.dt_bias))
+    L = _load()
+    own = workspace is not None
+    workspace = _workspace(op, device, workspace, L.redukt_op_scan_grad_workspace(ctypes.byref(r), n))
+    code = L.redukt_op_scan_grad(ctypes.byref(r), ctypes.byref(g), cu_seqlens.data_ptr(), n, at(state_in), at(dstate_out),
+                                 at(made.state_in), workspace.data_ptr(), workspace.numel(), on)
+    _done(code, op)
+    written = ([t for t in made if t is not None] if grads is not None else []) + ([workspace] if own else [])
+    if written:
+        increment_version(written)
+    return made
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in):
+        final = torch.empty((max(cu_seqlens.shape[0] - 1, 0),) + tuple(a.shape), dtype=torch.float32, device=x.device)
+        out = scan_chunk(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in, final)
+        ctx.save_for_backward(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in)
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dfinal):
+        x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(x)
+        g = scan_grad(dout.contiguous(), x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in,
+                      None if dfinal is None else dfinal.contiguous())
+        return g.x, g.dt, g.a, g.b, g.c, None, g.d, g.z, g.dt_bias, g.state_in
+
+
+def scan(x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_in=None):
+    """`scan_chunk` for training: (out, final states), from the states state_in [sequences, channels, size]
+    (None: zeros), with gradients for every floating-point input (once; tangents are refused).  Every row
+    belongs to a sequence, or its output is unspecified.  On torch's current stream; the backward pass runs `scan_grad`
+    on the stream of the forward pass.
+    """
+    op = "scan"
+    _device(op, x)
+    n = _sequences(op, x.get_device(), cu_seqlens)
+    if _tangents():
+        with torch.no_grad():
+            _no_gradients(op, x, dt, a, b, c, d, z, dt_bias, state_in)
+    if state_in is not None:
+        _check(op, x.get_device(), "state_in", state_in, torch.float32, (n, None, None))
+    return _Scan.apply(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in)
 
 
 def quantize_rows(x, codes=None, scales=None, stream: Optional[int] = None):
