@@ -4,7 +4,7 @@
  * points below are the parts of such a layer as operators of their own, for programs that hold
  * activations, weights and recurrent states themselves: the gated delta rule for one token
  * and for whole sequences, the selective scan likewise and with its gradients, and the int8
- * product with the pass that makes its codes.
+ * and block-scaled 8-bit floating point products with the passes that make their codes.
  *
  * Contract:
  *   - no model is needed (nothing here touches what redukt_backend_init made), and calls from
@@ -201,6 +201,45 @@ typedef struct {
  * exact in 32-bit integers, the rest in f32, rounded once to `dtype`.  Fastest where x, w and
  * their strides are multiples of 16 bytes and k is a multiple of 16. */
 int32_t redukt_op_int8_matmul(const redukt_int8_matmul* a, void* stream);
+
+/* ---------------- e4m3 codes with a scale a block, and their product ---------------- */
+
+typedef struct {
+    uint32_t dtype;         /* of x */
+    uint32_t rows, cols;
+    uint32_t block_rows;    /* rows of a block of 128 columns: 1 (activations) or 128 (weights) */
+    const void* x;          /* row r: cols elements at x + r * x_stride */
+    int64_t x_stride;
+    void* codes;            /* row r: cols bytes (OCP e4m3: no infinities, at most 448) at codes + r * codes_stride */
+    int64_t codes_stride;
+    float* scales;          /* [ceil(rows / block_rows)][ceil(cols / 128)] */
+} redukt_quantize_blocks;   /* any alignment that the element types have; fastest where rows begin on 16 bytes */
+
+/* Block by block: scale = max|x| / 448, at least 2^-126 (NaN does not count), code = x * (1 / scale) to
+ * the nearest e4m3 value with halves to the even one, the scale, its inverse and the product each rounded
+ * to f32; NaN stays NaN.  x = code * scale.  A block with an infinity has the scale inf, and codes that are 0, or
+ * NaN for the infinities. */
+int32_t redukt_op_quantize_blocks(const redukt_quantize_blocks* a, void* stream);
+
+typedef struct {
+    uint32_t dtype;         /* of out */
+    uint32_t m, n, k;       /* tokens, channels, columns; k at most 1,048,576 */
+    const void* x;          /* token i: k e4m3 codes at x + i * x_stride */
+    int64_t x_stride;
+    const float* x_scales;  /* [m][ceil(k / 128)] */
+    const void* w;          /* channel j: k e4m3 codes at w + j * w_stride */
+    int64_t w_stride;
+    const float* w_scales;  /* [ceil(n / 128)][ceil(k / 128)] */
+    const float* bias;      /* [n], or NULL */
+    void* out;              /* token i: n elements at out + i * out_stride */
+    int64_t out_stride;
+} redukt_fp8_matmul;        /* any alignment that the element types have */
+
+/* out[i][j] = sum over blocks b of 128 columns (sum over c in b of x[i][c] * w[j][c]) *
+ * (x_scales[i][b] * w_scales[j / 128][b]) + bias[j], with sums in f32 in an order that the sizes
+ * choose, rounded once to `dtype`.  Fastest where x, w and their strides are multiples of 16 bytes and k is a
+ * multiple of 16. */
+int32_t redukt_op_fp8_matmul(const redukt_fp8_matmul* a, void* stream);
 
 #ifdef __cplusplus
 }

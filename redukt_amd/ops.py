@@ -69,6 +69,18 @@ class Int8Matmul(ctypes.Structure):
                 ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64)]
 
 
+class QuantizeBlocks(ctypes.Structure):
+    """redukt_quantize_blocks."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("cols", ctypes.c_uint32), ("block_rows", ctypes.c_uint32),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("codes", ctypes.c_void_p), ("codes_stride", ctypes.c_int64),
+                ("scales", ctypes.c_void_p)]
+
+
+class Fp8Matmul(ctypes.Structure):
+    """redukt_fp8_matmul."""
+    _fields_ = Int8Matmul._fields_
+
+
 _lib = None
 
 
@@ -90,7 +102,10 @@ def _load() -> ctypes.CDLL:
         L.redukt_op_scan_grad.argtypes = [ctypes.POINTER(ScanRows), ctypes.POINTER(ScanGradients), p, u32, p, p, p, p, u64, p]
         L.redukt_op_scan_grad_workspace.argtypes = [ctypes.POINTER(ScanRows), u32]
         L.redukt_op_scan_grad_workspace.restype = u64
-        for f in ("delta_step", "delta_chunk", "scan_step", "scan_chunk", "scan_grad", "quantize_rows", "int8_matmul"):
+        L.redukt_op_quantize_blocks.argtypes = [ctypes.POINTER(QuantizeBlocks), p]
+        L.redukt_op_fp8_matmul.argtypes = [ctypes.POINTER(Fp8Matmul), p]
+        for f in ("delta_step", "delta_chunk", "scan_step", "scan_chunk", "scan_grad", "quantize_rows", "int8_matmul", "quantize_blocks",
+                  "fp8_matmul"):
             getattr(L, "redukt_op_" + f).restype = ctypes.c_int32
         _lib = L
     return _lib
@@ -655,6 +670,100 @@ def int8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloa
                    _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                    out.data_ptr(), _row_stride(op, "out", out, n))
     _done(_load().redukt_op_int8_matmul(ctypes.byref(a), on), op)
+    if not allocates:
+        increment_version(out)
+    return out
+
+
+E4M3 = torch.float8_e4m3fn
+
+
+def quantize_blocks(x, block_rows: int = 1, codes=None, scales=None, stream: Optional[int] = None):
+    """e4m3 codes of x [rows, cols] (bfloat16, float16 or float32) with one scale for each 128 columns of a row
+    (block_rows 1: activations) or of 128 rows (block_rows 128: weights): scale = max|x| / 448, at least 2^-126,
+    code = x / scale to the nearest, each step in float32; NaN does not count and stays NaN.  Returns (codes
+    float8_e4m3fn [rows, cols], scales float32 [ceil(rows / block_rows), ceil(cols / 128)]), allocated if None.  Rows
+    may be strided.
+    """
+    op = "quantize_blocks"
+    device = _device(op, x)
+    if x.dtype not in DTYPES or x.dim() != 2:
+        _refuse(f"{op}: x [rows, cols] is bfloat16, float16 or float32")
+    if block_rows != 1 and block_rows != 128:
+        _refuse(f"{op}: block_rows is 1 or 128")
+    if x.requires_grad or _tangents():
+        _no_gradients(op, x)
+    on = _stream(op, stream, device, codes is None or scales is None)
+    given = [t for t in (codes, scales) if t is not None]
+    rows, cols = x.shape
+    _sizes(op, rows, cols)
+    blocks = (-(-rows // block_rows), -(-cols // 128))
+    if codes is None:
+        codes = torch.empty_like(x, dtype=E4M3, memory_format=torch.contiguous_format)
+    else:
+        _check(op, device, "codes", codes, E4M3, (rows, cols))
+        _no_gradients(op, codes)
+    if scales is None:
+        scales = torch.empty(blocks, dtype=torch.float32, device=x.device)
+    else:
+        _check(op, device, "scales", scales, torch.float32, blocks)
+        _no_gradients(op, scales)
+        if not scales.is_contiguous():
+            _refuse(f"{op}: scales is not contiguous")
+    a = QuantizeBlocks(DTYPES[x.dtype], rows, cols, block_rows, x.data_ptr(), _row_stride(op, "x", x, cols), codes.data_ptr(),
+                       _row_stride(op, "codes", codes, cols), scales.data_ptr())
+    _done(_load().redukt_op_quantize_blocks(ctypes.byref(a), on), op)
+    if given:
+        increment_version(given)
+    return codes, scales
+
+
+def fp8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloat16, stream: Optional[int] = None):
+    """The product of e4m3 codes x [tokens, k] and w [channels, k] with float32 scales for blocks of 128 columns,
+    x_scales [tokens, ceil(k / 128)] and w_scales [ceil(channels / 128), ceil(k / 128)] (`quantize_blocks` with block_rows
+    1 and 128): out[i, j] = the sum over blocks b of (x[i] . w[j] over b) x_scales[i, b] w_scales[j // 128, b], + bias[j], in
+    float32, rounded once to `dtype` (bfloat16, float16 or float32; out's type where out is given).  Any sizes, k up to
+    1,048,576; fastest where k and the strides of x and w are multiples of 16.
+    """
+    op = "fp8_matmul"
+    device = _device(op, x)
+    f32 = torch.float32
+    try:       # (all at once; what is wrong is looked for only if something is)
+        (m, k), (n, wk) = x.shape, w.shape
+        blocks = -(-k // 128)
+        fine = (x.dtype is E4M3 and w.dtype is E4M3 and wk == k and x_scales.dtype is f32 and w_scales.dtype is f32
+                and x_scales.shape == (m, blocks) and w_scales.shape == (-(-n // 128), blocks) and x_scales.is_contiguous()
+                and w_scales.is_contiguous() and w.get_device() == x_scales.get_device() == w_scales.get_device() == device
+                and (bias is None or (bias.dtype is f32 and bias.shape == (n,) and bias.is_contiguous()
+                                      and bias.get_device() == device)))
+    except (AttributeError, TypeError, ValueError):
+        fine = False
+    if not fine:
+        _check(op, device, "x", x, E4M3, (None, None))
+        _check(op, device, "w", w, E4M3, (None, x.shape[1]))
+        _check(op, device, "x_scales", x_scales, f32, (x.shape[0], -(-x.shape[1] // 128)))
+        _check(op, device, "w_scales", w_scales, f32, (-(-w.shape[0] // 128), -(-x.shape[1] // 128)))
+        if bias is not None:
+            _check(op, device, "bias", bias, f32, (w.shape[0],))
+        _refuse(f"{op}: scales and bias are contiguous")
+    if x.requires_grad or w.requires_grad or x_scales.requires_grad or w_scales.requires_grad or (bias is not None and bias.requires_grad) or _tangents():
+        _no_gradients(op, x, w, x_scales, w_scales, bias)
+    _sizes(op, m, n, k)
+    allocates = out is None
+    on = _stream(op, stream, device, allocates)
+    if allocates:
+        if dtype not in DTYPES:
+            _refuse(f"{op}: dtype is bfloat16, float16 or float32")
+        out = torch.empty((m, n), dtype=dtype, device=x.device)
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype not in DTYPES:
+            _refuse(f"{op}: out is bfloat16, float16 or float32")
+        _check(op, device, "out", out, out.dtype, (m, n))
+        _no_gradients(op, out)
+    a = Fp8Matmul(DTYPES[out.dtype], m, n, k, x.data_ptr(), _row_stride(op, "x", x, k), x_scales.data_ptr(), w.data_ptr(),
+                  _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
+                  out.data_ptr(), _row_stride(op, "out", out, n))
+    _done(_load().redukt_op_fp8_matmul(ctypes.byref(a), on), op)
     if not allocates:
         increment_version(out)
     return out
