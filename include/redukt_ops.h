@@ -4,7 +4,8 @@
  * points below are the parts of such a layer as operators of their own, for programs that hold
  * activations, weights and recurrent states themselves: the gated delta rule for one token
  * and for whole sequences, the selective scan likewise and with its gradients, and the int8
- * and block-scaled 8-bit floating point products with the passes that make their codes.
+ * and block-scaled 8-bit floating point products with the passes that make their codes, and the
+ * drawing of tokens from logits.
  *
  * Contract:
  *   - no model is needed (nothing here touches what redukt_backend_init made), and calls from
@@ -240,6 +241,35 @@ typedef struct {
  * choose, rounded once to `dtype`.  Fastest where x, w and their strides are multiples of 16 bytes and k is a
  * multiple of 16. */
 int32_t redukt_op_fp8_matmul(const redukt_fp8_matmul* a, void* stream);
+
+/* ---------------- drawing a token ---------------- */
+
+typedef struct {
+    uint32_t dtype;         /* of logits */
+    uint32_t rows, vocab;   /* vocab 1 to 1,048,576 */
+    const void* logits;     /* row r: vocab elements at logits + r * logits_stride */
+    int64_t logits_stride;
+    const float* u;         /* [rows]: random numbers in [0, 1) */
+    float temperature;      /* for every row, unless there are `temperatures` [rows]; and so on */
+    float top_p, min_p;
+    int32_t top_k;
+    const float* temperatures;
+    const float* top_ps;
+    const float* min_ps;
+    const int32_t* top_ks;
+    int32_t* tokens;        /* [rows] */
+} redukt_sample;            /* any alignment that the element types have */
+
+/* Draws one token of each row.  With l the row's logits and m the largest of them, token i weighs
+ * W_i = 2^42 e^((l_i - m) / temperature), rounded to a whole number (2^42 where l_i = m; -inf and NaN weigh
+ * nothing).  In the order of falling logits, equal ones by index, are kept: the first top_k (not over 0: all); of
+ * these, those before which less than top_p of their sum has come, the first always (not below 1: all); of these, those
+ * of W_i >= min_p 2^42 (not over 0: all; over 1: as 1).  The token is the first in the order of indexes up to which
+ * the kept weights' sum is over u times the whole one (u below 0 or NaN: as 0; 1 and more: the last kept one).
+ * Sums are exact; a sum and a limit are compared as doubles, the limits each one product of doubles.
+ * A temperature that is not over 0 takes the first of the largest logits.  A row without a logit over
+ * -inf gets the token -1. */
+int32_t redukt_op_sample(const redukt_sample* a, void* stream);
 
 #ifdef __cplusplus
 }

@@ -81,6 +81,14 @@ class Fp8Matmul(ctypes.Structure):
     _fields_ = Int8Matmul._fields_
 
 
+class Sample(ctypes.Structure):
+    """redukt_sample."""
+    _fields_ = [("dtype", ctypes.c_uint32), ("rows", ctypes.c_uint32), ("vocab", ctypes.c_uint32), ("logits", ctypes.c_void_p),
+                ("logits_stride", ctypes.c_int64), ("u", ctypes.c_void_p), ("temperature", ctypes.c_float), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float), ("top_k", ctypes.c_int32), ("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p),
+                ("min_ps", ctypes.c_void_p), ("top_ks", ctypes.c_void_p), ("tokens", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -104,8 +112,9 @@ def _load() -> ctypes.CDLL:
         L.redukt_op_scan_grad_workspace.restype = u64
         L.redukt_op_quantize_blocks.argtypes = [ctypes.POINTER(QuantizeBlocks), p]
         L.redukt_op_fp8_matmul.argtypes = [ctypes.POINTER(Fp8Matmul), p]
+        L.redukt_op_sample.argtypes = [ctypes.POINTER(Sample), p]
         for f in ("delta_step", "delta_chunk", "scan_step", "scan_chunk", "scan_grad", "quantize_rows", "int8_matmul", "quantize_blocks",
-                  "fp8_matmul"):
+                  "fp8_matmul", "sample"):
             getattr(L, "redukt_op_" + f).restype = ctypes.c_int32
         _lib = L
     return _lib
@@ -764,6 +773,56 @@ def fp8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloat
                   _row_stride(op, "w", w, k), w_scales.data_ptr(), None if bias is None else bias.data_ptr(),
                   out.data_ptr(), _row_stride(op, "out", out, n))
     _done(_load().redukt_op_fp8_matmul(ctypes.byref(a), on), op)
+    if not allocates:
+        increment_version(out)
+    return out
+
+
+def sample(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, out=None, stream: Optional[int] = None):
+    """Draws a token from each row of logits [rows, vocab] (bfloat16, float16 or float32; vocab at most 1,048,576) by the
+    random numbers u [rows] float32 in [0, 1).
+
+    Token i weighs e^((l_i - max) / temperature) in whole steps of 2^-42; -inf and NaN weigh nothing.  Kept are, by
+    falling logits and equal ones by index, the top_k first; of these, those before which less than top_p of their sum has
+    come; of these, those that weigh min_p of the largest or more.  The token is the first by index up to which the kept
+    weights' sum is over u times the whole one: sums are exact, so it depends on nothing but the row.  temperature, top_p and
+    min_p are numbers or float32 tensors [rows], top_k a number or an int32 tensor; None (and top_k <= 0, top_p >= 1, min_p <=
+    0) keeps all.  A temperature of 0 takes the first of the largest.  Rows may be strided.  Returns out int32 [rows]
+    (allocated if None); -1 for a row with no logit over -inf.
+    """
+    op = "sample"
+    device = _device(op, logits)
+    if logits.dtype not in DTYPES or logits.dim() != 2:
+        _refuse(f"{op}: logits [rows, vocab] is bfloat16, float16 or float32")
+    rows, vocab = logits.shape
+    _sizes(op, rows, vocab)
+
+    def per_row(name, t, dtype):
+        _check(op, device, name, t, dtype, (rows,))
+        if not t.is_contiguous():
+            _refuse(f"{op}: {name} is not contiguous")
+        return t.data_ptr()
+
+    a = Sample(DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(op, "logits", logits, vocab), per_row("u", u, torch.float32),
+               1.0, 1.0, 0.0, 0)
+    settings = (("temperature", temperature, "temperatures", torch.float32), ("top_p", top_p, "top_ps", torch.float32),
+                ("min_p", min_p, "min_ps", torch.float32), ("top_k", top_k, "top_ks", torch.int32))
+    for name, v, many, dtype in settings:
+        if isinstance(v, torch.Tensor):
+            setattr(a, many, per_row(name, v, dtype))
+        elif v is not None:
+            try:
+                setattr(a, name, min(max(int(v), -1), 2 ** 31 - 1) if name == "top_k" else float(v))
+            except (TypeError, ValueError):
+                _refuse(f"{op}: {name} is a number or a tensor [rows]")
+    if _asks(logits, u) or any(isinstance(v, torch.Tensor) and v.requires_grad for _, v, _, _ in settings):
+        _no_gradients(op, logits, u, *(v if isinstance(v, torch.Tensor) else None for _, v, _, _ in settings))
+    allocates = out is None
+    on = _stream(op, stream, device, allocates)
+    if allocates:
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    a.tokens = per_row("out", out, torch.int32)
+    _done(_load().redukt_op_sample(ctypes.byref(a), on), op)
     if not allocates:
         increment_version(out)
     return out
