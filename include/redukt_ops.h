@@ -122,7 +122,7 @@ typedef struct {
     const float* a;         /* [channels][n] */
     const float* d;         /* [channels], or NULL */
     const float* dt_bias;   /* [channels], or NULL */
-} redukt_scan_rows;         /* any alignment that the element types have; states: 16-byte aligned */
+} redukt_scan_rows;         /* a and states: 16-byte aligned; the others: as their element types */
 
 /* One token for each of `rows` entries (at most 65,536), as redukt_op_delta_step has it: entry i steps
  * slot slots[i] (NULL: i) of states [n_slots][channels][n] in place; -1 leaves the entry's output and
@@ -150,7 +150,7 @@ typedef struct {
     void* db;               /* row t: groups * n elements */
     void* dc;
     int64_t dout_stride, dx_stride, ddt_stride, dz_stride, db_stride, dc_stride;    /* at most 2^22 */
-    float* da;              /* [channels][n] */
+    float* da;              /* [channels][n], 16-byte aligned */
     float* dd;              /* [channels]; NULL without d */
     float* ddt_bias;        /* [channels]; NULL without dt_bias */
 } redukt_scan_grads;
@@ -265,7 +265,7 @@ typedef struct {
  * nothing).  In the order of falling logits, equal ones by index, are kept: the first top_k (not over 0: all); of
  * these, those before which less than top_p of their sum has come, the first always (not below 1: all); of these, those
  * of W_i >= min_p 2^42 (not over 0: all; over 1: as 1).  The token is the first in the order of indexes up to which
- * the kept weights' sum is over u times the whole one (u below 0 or NaN: as 0; 1 and more: the last kept one).
+ * the kept weights' sum is over u times the whole one (u below 0 or NaN: as 0; of 1 or more: as just below 1).
  * Sums are exact; a sum and a limit are compared as doubles, the limits each one product of doubles.
  * A temperature that is not over 0 takes the first of the largest logits.  A row without a logit over
  * -inf gets the token -1. */

@@ -14,7 +14,9 @@ namespace {
 constexpr double kOne = 0x1p42;
 constexpr double kLeast = -29.9;           // ln 2^-43 = -29.81: e to less than this is no whole step
 constexpr uint32_t kBins = 2048;           // of (max - l) / T, linear, down to kLeast
-constexpr uint32_t kList = 2048;           // elements that are put in order by comparing each with all
+constexpr uint32_t kList = 1024;           // elements that are put in order by comparing each with all
+constexpr uint32_t kCoarse = 512;          // bins of the threads' largest logits
+constexpr uint32_t kFewK = 512;            // top_k that the list takes in general
 constexpr uint32_t kMaxVocab = 1u << 20;   // 2^20 weights of 2^42 stay below 2^63
 
 // Logits' order as that of unsigned numbers.
@@ -22,6 +24,8 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);         // (-0 is 0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+
+__device__ __forceinline__ float value_of(uint32_t key) { return __builtin_bit_cast(float, key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 // Where the kept part of a row's order (larger values first, equal ones by index) ends: its last element.
 struct Cut {
@@ -34,12 +38,13 @@ struct SampleArgs {
     uint32_t aligned;          // rows begin on 16 bytes
 };
 
-// An element of the list.
+// An element of the list: its place in the order of values as one word (the larger comes first), and its weight.
 struct __attribute__((aligned(16))) Listed {
-    uint32_t key, index;
-    uint64_t w;
-    __device__ __forceinline__ bool before(const Listed& o) const { return key > o.key || (key == o.key && index < o.index); }
+    uint64_t order, w;
+    __device__ __forceinline__ uint32_t key() const { return (uint32_t)(order >> 32); }
+    __device__ __forceinline__ uint32_t index() const { return ~(uint32_t)order; }
 };
+__device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t index) { return (uint64_t)key << 32 | (uint32_t)~index; }
 
 template <int THREADS>
 struct SampleLds {
@@ -50,12 +55,13 @@ struct SampleLds {
     };
     uint64_t wave_sum[THREADS / kOpWave];
     float wave_max[THREADS / kOpWave];
-    uint32_t listed, least, most, bin, found_key, found_index;
-    uint64_t before;
+    uint32_t listed, least, most, bin, found_key, found_index, kept;
+    uint64_t before, sum;
+    Listed sorted[kList];
 };
 
-// A row of logits, VEC neighbouring ones of a sweep over the row a thread.  It is read again for each pass (from L2: 64 logits a thread in
-// registers, with every pass unrolled over them, spill).
+// A row of logits, VEC neighbouring ones of a sweep over the row a thread.  Passes of the general way read it again (from L2: with every
+// one of them unrolled over 64 logits in registers, they spill).
 template <typename T, int THREADS>
 struct Row {
     static constexpr int VEC = 16 / sizeof(T), kSweep = THREADS * VEC;
@@ -179,7 +185,7 @@ __device__ __forceinline__ Cut find_cut(SampleLds<THREADS>& l, const R& row, con
             const float x = (float)v[e];
             if (!m.live(x) || m.bin(x) != bin || !in(key_of(x), i0 + e)) continue;
             const uint32_t key = key_of(x), at = atomicAdd(&l.listed, 1u);
-            if (at < kList) l.list[at] = Listed{key, i0 + e, want.by_weight ? m.weight(x) : 1};
+            if (at < kList) l.list[at] = Listed{order_of(key, i0 + e), want.by_weight ? m.weight(x) : 1};
             atomicMin(&l.least, key);
             atomicMax(&l.most, key);
         }
@@ -192,8 +198,8 @@ __device__ __forceinline__ Cut find_cut(SampleLds<THREADS>& l, const R& row, con
             const Listed me = l.list[t];
             uint64_t sum = before, rank = 0;
             for (uint32_t j = 0; j < n; j++)
-                if (l.list[j].before(me)) sum += l.list[j].w, rank++;
-            if (want.keeps(sum) && (rank + 1 == n || !want.keeps(sum + me.w))) l.found_key = me.key, l.found_index = me.index;
+                if (l.list[j].order > me.order) sum += l.list[j].w, rank++;
+            if (want.keeps(sum) && (rank + 1 == n || !want.keeps(sum + me.w))) l.found_key = me.key(), l.found_index = me.index();
         }
         __syncthreads();
         return {l.found_key, l.found_index};
@@ -257,67 +263,116 @@ __device__ __forceinline__ Cut find_cut(SampleLds<THREADS>& l, const R& row, con
     return {lo, l.found_index};
 }
 
-// The limit that a running sum of kept weights passes at the drawn token: u of the whole sum (u of 1 or more: the last one's; below 0 or
-// NaN: the first one's).
+// The limit that a running sum of kept weights passes at the drawn token: u of the whole sum (u of 1 or more: just below it; below 0 or
+// NaN: 0).
 __device__ __forceinline__ double limit_of(float u, uint64_t sum) {
     const double limit = (u > 0.0f ? (double)u : 0.0) * (double)sum;
     return limit < (double)sum ? limit : (double)sum * 0.9999999999999999;
 }
 
-// Where everything that may be kept is in the list (n elements, top_k and top_p of them, `all` the sum that top_p is of if top_k keeps all):
-// each element looks at all others for its place in the order of values, and once more in that of indexes.
+// How many neighbouring threads share each of n elements: 1 to 16.
+template <int THREADS>
+__device__ __forceinline__ uint32_t sharers(uint32_t n) {
+    uint32_t share = 16;
+    while (share > 1 && n * share > THREADS) share /= 2;
+    return share;
+}
+
+__device__ __forceinline__ uint64_t shared_sum(uint64_t v, uint32_t share) {
+    for (uint32_t o = 1; o < share; o <<= 1) v += __shfl_xor(v, o, kOpWave);
+    return v;
+}
+
+// Where everything that may be kept is in the list (n > 0 elements; top_k and top_p of them, `all` the sum that top_p is of if top_k keeps
+// all): each element looks at all others for its place in the order of values, and those that are kept at each other once more in that of
+// indexes.
 template <int THREADS>
 __device__ __forceinline__ void draw_listed(SampleLds<THREADS>& l, uint32_t n, uint64_t top_k, bool by_p, double top_p, uint64_t all, double least, float u,
                                             int32_t* token) {
-    constexpr int kPer = kList / THREADS;
+    constexpr uint64_t kMark = 1ull << 53;     // an element counts as this beside its weight: 1,024 weights stay below it
+    constexpr int kPer = kList / THREADS > 1 ? kList / THREADS : 1;
+    uint32_t share = sharers<THREADS>(n), sub = threadIdx.x % share;
     Listed me[kPer];
-    uint64_t before[kPer], sum = 0;
-    bool kept[kPer];
+    uint64_t before[kPer];
+    uint32_t rank[kPer];
+    if (threadIdx.x == 0) l.kept = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-        const uint32_t t = i * THREADS + threadIdx.x;
-        kept[i] = t < n;
-        before[i] = 0;
-        if (!kept[i]) continue;
+        const uint32_t t = i * (THREADS / share) + threadIdx.x / share;
+        rank[i] = ~0u;
+        if (t >= n) continue;                  // (a shared element's threads all go or stay)
         me[i] = l.list[t];
-        uint32_t rank = 0;
-#pragma unroll 4
-        for (uint32_t j = 0; j < n; j++) {
-            const Listed o = l.list[j];
-            const bool b = o.before(me[i]);
-            rank += b;
-            before[i] += b ? o.w : 0;
-        }
-        kept[i] = rank < top_k;
-        if (kept[i]) sum += me[i].w;
+        uint64_t sum = 0;
+#pragma unroll 8
+        for (uint32_t j = sub; j < n; j += share) sum += l.list[j].order > me[i].order ? l.list[j].w + kMark : 0;
+        sum = shared_sum(sum, share);
+        if (sub != 0) continue;
+        rank[i] = (uint32_t)(sum / kMark);
+        before[i] = sum % kMark;
+        if (rank[i] + 1 == (top_k < n ? (uint32_t)top_k : n)) l.sum = before[i] + me[i].w;
     }
-    if (by_p) {
-        sum = top_k == ~0ull ? all : block_sum(l, sum);
-        const Want want{true, 0, top_p * (double)sum};
-#pragma unroll
-        for (int i = 0; i < kPer; i++) kept[i] = kept[i] && want.keeps(before[i]);
-    }
-    sum = 0;
     __syncthreads();
+    const Want want{true, 0, top_p * (double)(top_k == ~0ull ? all : l.sum)};
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-        kept[i] = kept[i] && (double)me[i].w >= least;
-        if (kept[i]) sum += me[i].w;
-        else if (i * THREADS + threadIdx.x < n) l.list[i * THREADS + threadIdx.x].w = 0;
+        if (rank[i] >= top_k || rank[i] == ~0u || (by_p && !want.keeps(before[i])) || (double)me[i].w < least) continue;
+        l.sorted[rank[i]] = me[i];
+        atomicMax(&l.kept, rank[i] + 1);
     }
-    sum = block_sum(l, sum);                   // (its barriers stand between the list's changes and the next look at it)
-    const double limit = limit_of(u, sum);
+    __syncthreads();
+    const uint32_t m = l.kept;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        if (!kept[i]) continue;
+    for (int i = 0; i < kPer; i++)
+        if (rank[i] + 1 == m) l.before = before[i] + me[i].w;        // (all kept weights)
+    __syncthreads();
+    const double limit = limit_of(u, l.before);
+    share = sharers<THREADS>(m), sub = threadIdx.x % share;
+    for (uint32_t t = threadIdx.x / share; t < m; t += THREADS / share) {
+        const Listed e = l.sorted[t];
         uint64_t upto = 0;
-#pragma unroll 4
-        for (uint32_t j = 0; j < n; j++) upto += l.list[j].index <= me[i].index ? l.list[j].w : 0;
-        if ((double)upto > limit && !((double)(upto - me[i].w) > limit) && me[i].w) *token = (int32_t)me[i].index;
+#pragma unroll 8
+        for (uint32_t j = sub; j < m; j += share) upto += (uint32_t)l.sorted[j].order >= (uint32_t)e.order ? l.sorted[j].w : 0;      // (indexes are inverted)
+        upto = shared_sum(upto, share);
+        if (sub == 0 && (double)upto > limit && !((double)(upto - e.w) > limit)) *token = (int32_t)e.index();
     }
 }
 
-template <typename T, int THREADS>
+// The coarse bin (kCoarse of them, in l.count) that the top_k-th of the threads' largest logits is in, or kCoarse if there are not so many.
+template <int THREADS>
+__device__ __forceinline__ uint32_t coarse_bin(SampleLds<THREADS>& l, uint32_t top_k, int lane) {
+    constexpr int kPer = kCoarse / kOpWave;
+    if (threadIdx.x < kOpWave) {
+        uint32_t c[kPer], mine = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) mine += c[i] = l.count[lane * kPer + i];
+        uint32_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < kOpWave; o <<= 1) {
+            const uint32_t x = __shfl_up(upto, o, kOpWave);
+            if (lane >= o) upto += x;
+        }
+        const uint64_t hit = __ballot(upto >= top_k);
+        if (lane == 0) l.bin = kCoarse;
+        if (hit && lane == (int)__builtin_ctzll(hit)) {
+            uint32_t before = upto - mine, bin = lane * kPer;
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                before += c[i];
+                if (before < top_k) bin++;
+            }
+            l.bin = bin;
+        }
+    }
+    __syncthreads();
+    return l.bin;
+}
+
+// HELD: sweeps that stay in registers, which hold the whole row; 0: none.
+//
+// With top_k the way is short.  Each thread has the largest of its logits; the top_k-th logit is no further down than the top_k-th of
+// these, and there are few others so far up: they are listed from registers and put in order by comparing each with all.  So a row is
+// read once.
+template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     typedef Row<T, THREADS> R;
     constexpr int VEC = R::VEC, kWaves = THREADS / kOpWave;
@@ -328,12 +383,28 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     const uint32_t r = blockIdx.x;
     const R row{(const T*)a.logits + (int64_t)r * a.logits_stride, a.vocab, (a.vocab + R::kSweep - 1) / R::kSweep, s.aligned != 0};
 
-    Scale m;
-    m.most = -__builtin_inff();
-    row.each([&](uint32_t, uint32_t, const typename R::vec& v) {
+    const float temperature = a.temperatures ? a.temperatures[r] : a.temperature, u = a.u[r];
+    const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+    const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p;
+
+    float mine = -__builtin_inff();
+    typename R::vec held[HELD ? HELD : 1];
+    const auto fold = [&](const typename R::vec& v) {
 #pragma unroll
-        for (int e = 0; e < VEC; e++) m.most = (float)v[e] > m.most ? (float)v[e] : m.most;        // (NaN is none)
-    });
+        for (int e = 0; e < VEC; e++) mine = (float)v[e] > mine ? (float)v[e] : mine;        // (NaN is none)
+    };
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if ((uint32_t)i < row.sweeps) held[i] = row.load(i);
+#pragma unroll
+        for (int i = 0; i < HELD; i++)
+            if ((uint32_t)i < row.sweeps) fold(held[i]);
+    } else {
+        row.each([&](uint32_t, uint32_t, const typename R::vec& v) { fold(v); });
+    }
+    Scale m;
+    m.most = mine;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m.most = fmaxf(m.most, __shfl_xor(m.most, o, kOpWave));
     if (lane == 0) l.wave_max[wave] = m.most;
@@ -345,7 +416,6 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
         if (threadIdx.x == 0) a.tokens[r] = -1;
         return;
     }
-    const float temperature = a.temperatures ? a.temperatures[r] : a.temperature;
     if (!(temperature > 0.0f)) {               // the first of the largest
         row.each([&](uint32_t, uint32_t i0, const typename R::vec& v) {
 #pragma unroll
@@ -358,11 +428,59 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     }
     m.inv = 1.0 / (double)temperature;
     m.bins = (float)((kBins - 1) / -kLeast * m.inv);
-    const int32_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-    const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p, u = a.u[r];
     const bool by_k = top_k > 0 && (uint32_t)top_k < a.vocab, by_p = top_p < 1.0f, by_min = min_p > 0.0f;
     const double least = by_min ? (double)fminf(min_p, 1.0f) * kOne : 0.0;
 
+    if constexpr (HELD > 0) {
+        if (by_k && top_k <= (int)kFewK) {
+            for (uint32_t i = threadIdx.x; i < kCoarse; i += THREADS) l.count[i] = 0;
+            if (threadIdx.x == 0) l.listed = 0;
+            __syncthreads();
+            if (m.live(mine)) atomicAdd(&l.count[m.bin(mine) / (kBins / kCoarse)], 1u);
+            __syncthreads();
+            const uint32_t bin = coarse_bin(l, (uint32_t)top_k, lane);
+            if (bin < kCoarse) {
+                // (what is a little further down may be listed too, but nothing less: the bin's end as a logit, with room for roundings)
+                float from = m.most - (float)((bin + 1) * (kBins / kCoarse)) / m.bins * 1.0001f;
+                if (!(from < m.most)) from = m.most;
+                // (counted first, so that a wave asks for its places in the list once)
+                uint32_t hits = 0;
+#pragma unroll
+                for (int i = 0; i < HELD; i++) {
+                    if ((uint32_t)i >= row.sweeps) continue;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) hits += __popcll(__ballot((float)held[i][e] >= from));
+                }
+                uint32_t at = 0;
+                if (lane == 0 && hits) at = atomicAdd(&l.listed, hits);
+                at = __builtin_amdgcn_readfirstlane(at);
+                if (hits && at + hits <= kList) {
+#pragma unroll
+                    for (int i = 0; i < HELD; i++) {
+                        if ((uint32_t)i >= row.sweeps) continue;
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) {
+                            const bool hit = (float)held[i][e] >= from;
+                            const uint64_t all = __ballot(hit);
+                            if (!all) continue;
+                            const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+                            if (hit) l.list[to].order = order_of(key_of((float)held[i][e]), (uint32_t)i * R::kSweep + threadIdx.x * VEC + e);
+                            at += __popcll(all);
+                        }
+                    }
+                }
+                __syncthreads();
+                const uint32_t n = l.listed;
+                if (n <= kList) {
+                    for (uint32_t t = threadIdx.x; t < n; t += THREADS) l.list[t].w = m.weight(value_of(l.list[t].key()));
+                    __syncthreads();
+                    draw_listed(l, n, (uint64_t)top_k, by_p, (double)top_p, 0, least, u, a.tokens + r);
+                    return;
+                }
+            }
+            __syncthreads();
+        }
+    }
     Cut cut{0, ~0u};                           // everything
     if (by_k || by_p) {
         // The bin that the cut is in: by elements, or by weight where only that counts.
@@ -399,7 +517,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
                 const float x = (float)v[e];
                 if (!(m.place(x) < (float)(bin + 1))) continue;
                 const uint32_t at = atomicAdd(&l.listed, 1u);
-                if (at < kList) l.list[at] = Listed{key_of(x), i0 + e, m.weight(x)};
+                if (at < kList) l.list[at] = Listed{order_of(key_of(x), i0 + e), m.weight(x)};
             }
         });
         __syncthreads();
@@ -469,13 +587,13 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
         before += __shfl(upto, kOpWave - 1, kOpWave);
     }
     const uint32_t i0 = cell / kWaves * R::kSweep + (cell % kWaves * kOpWave + lane) * VEC;
-    uint64_t w[VEC], mine = 0;
+    uint64_t w[VEC], own = 0;
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
         w[e] = i0 + e < a.vocab ? kept((float)row.p[i0 + e], i0 + e) : 0;
-        mine += w[e];
+        own += w[e];
     }
-    const uint64_t upto = wave_upto(mine, lane);
+    const uint64_t upto = wave_upto(own, lane);
     const uint64_t hit = __ballot((double)(before + upto) > limit);
     if (!hit || lane != (int)__builtin_ctzll(hit)) return;
     uint64_t to = before + upto;
@@ -492,12 +610,13 @@ template <typename T>
 int32_t launch(SampleArgs& k, void* stream) {
     constexpr int VEC = 16 / sizeof(T);
     const uint32_t v = k.a.vocab;
-    // A thread has at least a few loads of a row, but no fewer than 256 threads share one.
-    const bool small = v <= 4096;
-    const uint32_t threads = small ? 256 : 1024, sweeps = (v + threads * VEC - 1) / (threads * VEC);
+    // A thread has at least a few loads of a row, but no fewer than 256 threads share one; up to 64 logits a thread stay in registers.
+    const uint32_t threads = v <= 4096 ? 256 : 1024, sweeps = (v + threads * VEC - 1) / (threads * VEC);
     if (!op_grid_ok(k.a.rows, threads)) return BACKEND_INVALID_ARGUMENT;
-    return op_launch(small ? (const void*)k_sample<T, 256> : (const void*)k_sample<T, 1024>, dim3(k.a.rows), dim3(threads),
-                     sweeps * (threads / kOpWave) * 8, stream, k);
+    const void* const fn = threads == 256         ? (const void*)k_sample<T, 256, 16 / VEC>
+                           : sweeps <= 64u / VEC ? (const void*)k_sample<T, 1024, 64 / VEC>
+                                                 : (const void*)k_sample<T, 1024, 0>;
+    return op_launch(fn, dim3(k.a.rows), dim3(threads), sweeps * (threads / kOpWave) * 8, stream, k);
 }
 
 }  // namespace

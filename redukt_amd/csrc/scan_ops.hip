@@ -138,46 +138,67 @@ __device__ __forceinline__ void store_state(float* p, const float (&h)[S]) {
     *(typename Parts<S>::vec*)p = v;
 }
 
-template <typename T, int S>
+// A wave takes 64 channels of an entry, 16 at a time with their states' loads side by side (NB 4), or 16 (NB 1, while there are too few waves
+// for the device otherwise).  With NB 4 each lane of a quad does one of the four channels' softplus and gate.
+template <typename T, int S, int NB>
 __global__ __launch_bounds__(kBlock) void k_scan_step(ScanArgs a) {
+    constexpr int N = 4 * S, kWide = 16 * NB;
     const redukt_scan_rows& r = a.r;
     const int lane = threadIdx.x % kOpWave, q = lane % 4;
-    const uint32_t blocks = (r.channels + 15) / 16;
+    const uint32_t blocks = (r.channels + kWide - 1) / kWide;
     const uint64_t id = (uint64_t)blockIdx.x * (kBlock / kOpWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kOpWave);
-    const uint32_t i = (uint32_t)(id / blocks), at = (uint32_t)(id % blocks) * 16 + lane / 4;
+    const uint32_t i = (uint32_t)(id / blocks), ch0 = (uint32_t)(id % blocks) * kWide;
     if (i >= a.n) return;
+    // (the lane's own channel, for which it does what a quad shares out)
+    const uint32_t own = ch0 + lane / 4 + (NB == 4 ? 16 * q : 0), ch = min(own, r.channels - 1);
+    const bool in = own < r.channels && (NB == 4 || q == 0);
+    const uint32_t g = ch0 / (r.channels / r.groups) * N + q * S;
+    const T* const pb = (const T*)r.b + (int64_t)i * r.b_stride + g;
+    const T* const pc = (const T*)r.c + (int64_t)i * r.c_stride + g;
+    const T x0 = ((const T*)r.x)[(int64_t)i * r.x_stride + ch], t0 = ((const T*)r.dt)[(int64_t)i * r.dt_stride + ch];
+    const T z0 = r.z ? ((const T*)r.z)[(int64_t)i * r.z_stride + ch] : x0;
+    const float d = r.d ? r.d[ch] : 0.0f, bias = r.dt_bias ? r.dt_bias[ch] : 0.0f;
+    T b0[S], c0[S];
+#pragma unroll
+    for (int e = 0; e < S; e++) b0[e] = pb[e], c0[e] = pc[e];
+    float k[NB][S];
+#pragma unroll
+    for (int j = 0; j < NB; j++) load_state<S>(r.a + (size_t)min(ch0 + 16 * j + lane / 4, r.channels - 1) * N + q * S, k[j]);
     const int slot = entry_slot(a.slots, a.n_slots, i, true, lane);
     if (slot == kSkip) return;
-    const bool in = at < r.channels;
-    const uint32_t ch = in ? at : r.channels - 1;
     T* const out = (T*)r.out + (int64_t)i * r.out_stride + ch;
     if (slot == kBad) {
-        if (in && q == 0) *out = (T)__builtin_nanf("");
+        if (in) *out = (T)__builtin_nanf("");
         return;
     }
-    float* const state = a.states + ((size_t)slot * r.channels + ch) * (4 * S) + q * S;
-    float h[S];
-    load_state<S>(state, h);
-    const Channel<S> k = channel_of<S>(r, ch, q);
-    const uint32_t g = ch / (r.channels / r.groups) * (4 * S) + q * S;
-    const T* const b = (const T*)r.b + (int64_t)i * r.b_stride + g;
-    const T* const c = (const T*)r.c + (int64_t)i * r.c_stride + g;
-    const float x = (float)((const T*)r.x)[(int64_t)i * r.x_stride + ch];
-    const float s = softplus((float)((const T*)r.dt)[(int64_t)i * r.dt_stride + ch] + k.bias).s, u = s * x;
-    float p = 0.0f;
+    float* const state = a.states + (size_t)slot * r.channels * N + q * S;
+    float h[NB][S];
 #pragma unroll
-    for (int e = 0; e < S; e++) {
-        h[e] = fmaf(power(s, k.a2[e]), h[e], u * (float)b[e]);
-        p = fmaf((float)c[e], h[e], p);
-    }
-    float y = fmaf(k.d, x, quad_sum(p));
+    for (int j = 0; j < NB; j++) load_state<S>(state + (size_t)min(ch0 + 16 * j + lane / 4, r.channels - 1) * N, h[j]);
+    const float x = (float)x0, s = softplus((float)t0 + bias).s, u = s * x;
+    float p[4] = {};
+    const auto block = [&](auto J) {
+        constexpr int j = J.value;
+        if constexpr (j < NB) {
+            const float sj = NB == 4 ? quad_lane<j>(s) : s, uj = NB == 4 ? quad_lane<j>(u) : u;
+#pragma unroll
+            for (int e = 0; e < S; e++) {
+                h[j][e] = fmaf(power(sj, k[j][e] * kLog2e), h[j][e], uj * (float)b0[e]);
+                p[j] = fmaf((float)c0[e], h[j][e], p[j]);
+            }
+        }
+    };
+    block(std::integral_constant<int, 0>()), block(std::integral_constant<int, 1>());
+    block(std::integral_constant<int, 2>()), block(std::integral_constant<int, 3>());
+    float y = fmaf(d, x, NB == 4 ? quad_sums(p, q) : quad_sum(p[0]));
     if (r.z) {
-        const float z = (float)((const T*)r.z)[(int64_t)i * r.z_stride + ch];
+        const float z = (float)z0;
         y *= z * sigmoid(z);
     }
-    if (!in) return;
-    store_state<S>(state, h);
-    if (q == 0) *out = (T)y;
+#pragma unroll
+    for (int j = 0; j < NB; j++)
+        if (ch0 + 16 * j + lane / 4 < r.channels) store_state<S>(state + (size_t)(ch0 + 16 * j + lane / 4) * N, h[j]);
+    if (in) *out = (T)y;
 }
 
 // ---------------------------------------------------------------- sequences in pieces
@@ -891,12 +912,15 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_columns(GradArgs ga) {
 
 // ---------------------------------------------------------------- launches
 
-#define SCAN_BY_N(T, n, fn) \
-    ((n) == 8 ? (const void*)fn<T, 2> : (n) == 16 ? (const void*)fn<T, 4> : (n) == 32 ? (const void*)fn<T, 8> : (const void*)fn<T, 16>)
-#define SCAN_FN(r, fn) \
-    ((r).dtype == REDUKT_OP_BF16  ? SCAN_BY_N(__bf16, (r).n, fn) \
-     : (r).dtype == REDUKT_OP_F16 ? SCAN_BY_N(_Float16, (r).n, fn) \
-                                  : SCAN_BY_N(float, (r).n, fn))
+#define SCAN_BY_N(T, n, fn, ...) \
+    ((n) == 8    ? (const void*)fn<T, 2 __VA_OPT__(, ) __VA_ARGS__> \
+     : (n) == 16 ? (const void*)fn<T, 4 __VA_OPT__(, ) __VA_ARGS__> \
+     : (n) == 32 ? (const void*)fn<T, 8 __VA_OPT__(, ) __VA_ARGS__> \
+                 : (const void*)fn<T, 16 __VA_OPT__(, ) __VA_ARGS__>)
+#define SCAN_FN(r, fn, ...) \
+    ((r).dtype == REDUKT_OP_BF16  ? SCAN_BY_N(__bf16, (r).n, fn __VA_OPT__(, ) __VA_ARGS__) \
+     : (r).dtype == REDUKT_OP_F16 ? SCAN_BY_N(_Float16, (r).n, fn __VA_OPT__(, ) __VA_ARGS__) \
+                                  : SCAN_BY_N(float, (r).n, fn __VA_OPT__(, ) __VA_ARGS__))
 
 const void* join_fn(uint32_t n) {
     return n == 8 ? (const void*)k_scan_join<2> : n == 16 ? (const void*)k_scan_join<4> : n == 32 ? (const void*)k_scan_join<8> : (const void*)k_scan_join<16>;
@@ -932,7 +956,7 @@ bool rows_ok(const redukt_scan_rows* a, bool outputs) {
 }
 
 bool layer_ok(const redukt_scan_rows* a) {
-    return a->a && op_aligned(a->a, 4) && op_aligned(a->d, 4) && op_aligned(a->dt_bias, 4);
+    return a->a && op_aligned(a->a, 16) && op_aligned(a->d, 4) && op_aligned(a->dt_bias, 4);
 }
 
 // The rows with steps that are a row's width where there is one row only.
@@ -982,12 +1006,14 @@ int32_t redukt_op_scan_step(const redukt_scan_rows* a, float* states, uint32_t n
     if (a->rows == 0) return BACKEND_OK;
     if (!rows_ok(a, true) || !layer_ok(a) || !states || !op_aligned(states, 16) || !op_aligned(slots, 4)) return BACKEND_INVALID_ARGUMENT;
     if (n_slots >= (1u << 31) || (!slots && a->rows > n_slots)) return BACKEND_INVALID_ARGUMENT;
-    const uint64_t grid = ((uint64_t)a->rows * ((a->channels + 15) / 16) + 3) / 4;
+    const bool few = (uint64_t)a->rows * ((a->channels + 63) / 64) < 2048;
+    const uint32_t wide = few ? 16 : 64;
+    const uint64_t grid = ((uint64_t)a->rows * ((a->channels + wide - 1) / wide) + 3) / 4;
     if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(a->out);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     ScanArgs k{stepped(*a), states, states, n_slots, slots, nullptr, a->rows, nullptr, 0, 0};
-    return op_launch(SCAN_FN(k.r, k_scan_step), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
+    return op_launch(few ? SCAN_FN(k.r, k_scan_step, 1) : SCAN_FN(k.r, k_scan_step, 4), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
 }
 
 uint64_t redukt_op_scan_chunk_workspace(const redukt_scan_rows* a, uint32_t n_seq) {
