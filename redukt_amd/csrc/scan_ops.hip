@@ -57,21 +57,19 @@ constexpr float kLog2e = 0x1.715476p+0f, kLog2eRest = 0x1.4ae0cp-26f, kLn2 = 0x1
 
 // e^v for v <= 0: the power's argument in two parts, so its rounding does not grow with |v|.
 __device__ __forceinline__ float exp_down(float v) {
-    v = v < -200.0f ? -200.0f : v;             // (e^-inf, without inf - inf in the rest; NaN stays)
+    v = fmaxf(v, -200.0f);                     // (e^-inf, without inf - inf in the rest; of NaN as well, which callers keep)
     const float t = v * kLog2e, rest = fmaf(v, kLog2e, -t) + v * kLog2eRest, e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, rest * kLn2, e);
 }
 
-// ln(1 + e) for e in [0, 1], as 2 artanh(w) = 2 (w + w^3 / 3 + ...) with w = e / (2 + e) <= 1/3: eight terms leave 3^-17 / 17 of w.
+// ln(1 + e) for e in [0, 1], as 2 artanh(w) = 2 (w + w^3 / 3 + ...) with w = e / (2 + e) <= 1/3: the series' tail as a polynomial of
+// degree 3 in w^2, fitted so that its largest relative error on [0, 1/3] is least (4.5e-9).
 __device__ __forceinline__ float log_1p(float e) {
     const float w = e * __builtin_amdgcn_rcpf(2.0f + e), w2 = w * w;
-    float p = 1.0f / 15.0f;
-    p = fmaf(p, w2, 1.0f / 13.0f);
-    p = fmaf(p, w2, 1.0f / 11.0f);
-    p = fmaf(p, w2, 1.0f / 9.0f);
-    p = fmaf(p, w2, 1.0f / 7.0f);
-    p = fmaf(p, w2, 1.0f / 5.0f);
-    p = fmaf(p, w2, 1.0f / 3.0f);
+    float p = 0x1.1ed7bep-3f;
+    p = fmaf(p, w2, 0x1.1ebd0ep-3f);
+    p = fmaf(p, w2, 0x1.99d208p-3f);
+    p = fmaf(p, w2, 0x1.555502p-2f);
     return 2.0f * fmaf(w * w2, p, w);
 }
 
@@ -81,9 +79,10 @@ struct Step {
 };
 __device__ __forceinline__ Step softplus(float v) {
     const float e = exp_down(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
-    return {(v > 0.0f ? v : 0.0f) + log_1p(e), v > 0.0f ? r : e * r};
+    return {(v <= 0.0f ? 0.0f : v) + log_1p(e), v > 0.0f ? r : e * r};     // (s of NaN is NaN)
 }
 
+// 1 / (1 + e^-v); of NaN a number, times which it stays NaN.
 __device__ __forceinline__ float sigmoid(float v) {
     const float e = exp_down(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
     return v > 0.0f ? r : e * r;
@@ -361,14 +360,16 @@ __global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a) {
     if (q == 0) a.ws[(size_t)a.pieces * r.channels * N + (size_t)slot * r.channels + ch] = sum;
 }
 
-// The first states of all pieces of a sequence, in the places of what k_scan_pieces left there: a quad a channel.
+// The first states of all pieces of a sequence, in the places of what k_scan_pieces left there: a quad a channel.  A workgroup is one
+// wave: what it waits for is the way through its CU (8,192 tokens of 1,536 channels, gradients: 20 us with four waves).
+constexpr int kJoinCh = 16;
 template <int S>
-__global__ __launch_bounds__(kBlock) void k_scan_join(ScanArgs a) {
+__global__ __launch_bounds__(kOpWave) void k_scan_join(ScanArgs a) {
     constexpr int N = 4 * S, P = kPiece<S>;
     const redukt_scan_rows& r = a.r;
-    const int lane = threadIdx.x % kOpWave, q = lane % 4;
-    const uint32_t blocks = (r.channels + kBlockCh - 1) / kBlockCh, i = blockIdx.x / blocks;
-    const uint32_t ch = blockIdx.x % blocks * kBlockCh + threadIdx.x / 4;
+    const int lane = threadIdx.x, q = lane % 4;
+    const uint32_t blocks = (r.channels + kJoinCh - 1) / kJoinCh, i = blockIdx.x / blocks;
+    const uint32_t ch = blockIdx.x % blocks * kJoinCh + lane / 4;
     const Bounds m{a.cu, a.n, r.rows, false};
     const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = b / P + i;
     if (count < 2) return;
@@ -601,12 +602,12 @@ __device__ __forceinline__ void state_or_zeros(const float* pool, uint32_t seq, 
 
 // The first states of all pieces of a sequence (blockIdx.y 0), or what comes back behind them (1), in place.
 template <int S, bool SHORT>
-__global__ __launch_bounds__(kBlock) void k_scan_grad_join(GradArgs ga) {
+__global__ __launch_bounds__(kOpWave) void k_scan_grad_join(GradArgs ga) {
     constexpr int N = 4 * S, P = kGradPiece<S, SHORT>;
     const redukt_scan_rows& r = ga.a.r;
-    const int lane = threadIdx.x % kOpWave, q = lane % 4;
-    const uint32_t blocks = (r.channels + kBlockCh - 1) / kBlockCh, i = blockIdx.x / blocks + 1;
-    const uint32_t ch = blockIdx.x % blocks * kBlockCh + threadIdx.x / 4;
+    const int lane = threadIdx.x, q = lane % 4;
+    const uint32_t blocks = (r.channels + kJoinCh - 1) / kJoinCh, i = blockIdx.x / blocks + 1;
+    const uint32_t ch = blockIdx.x % blocks * kJoinCh + lane / 4;
     const Bounds m{ga.a.cu, ga.a.n, r.rows, true};
     const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = b / P + i;
     if (count < 2 || ch >= r.channels) return;
@@ -1052,8 +1053,8 @@ int32_t redukt_op_scan_chunk(const redukt_scan_rows* a, const int32_t* cu, uint3
     if (a->rows == 0 && !state_out) return BACKEND_OK;
     const uint64_t need = redukt_op_scan_chunk_workspace(a, n_seq);
     if (need && (!workspace || !op_aligned(workspace, 16) || workspace_bytes < need)) return BACKEND_INVALID_ARGUMENT;
-    const uint64_t pieces = chunk_pieces(*a, n_seq), blocks = (a->channels + kBlockCh - 1) / kBlockCh;
-    if (!op_grid_ok(pieces * blocks, kBlock)) return BACKEND_INVALID_ARGUMENT;
+    const uint64_t pieces = chunk_pieces(*a, n_seq), blocks = (a->channels + kBlockCh - 1) / kBlockCh, joins = (a->channels + kJoinCh - 1) / kJoinCh;
+    if (!op_grid_ok(pieces * blocks, kBlock) || !op_grid_ok(n_seq * joins, kOpWave)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     // No sequence has more pieces than the rows fill; few of them are joined by each piece itself, which saves a launch.
@@ -1062,7 +1063,7 @@ int32_t redukt_op_scan_chunk(const redukt_scan_rows* a, const int32_t* cu, uint3
     const dim3 grid((uint32_t)(pieces * blocks));
     if (need) {
         int32_t rc = op_launch(SCAN_FN(k.r, k_scan_pieces), grid, dim3(kBlock), 0, stream, k);
-        if (rc == BACKEND_OK && k.joined) rc = op_launch(join_fn(k.r.n), dim3((uint32_t)(n_seq * blocks)), dim3(kBlock), 0, stream, k);
+        if (rc == BACKEND_OK && k.joined) rc = op_launch(join_fn(k.r.n), dim3((uint32_t)(n_seq * joins)), dim3(kOpWave), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
     return op_launch(SCAN_FN(k.r, k_scan_run), grid, dim3(kBlock), 0, stream, k);
@@ -1088,9 +1089,9 @@ int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* 
         return BACKEND_INVALID_ARGUMENT;
     const GradPlan p = grad_plan(*a, n_seq);
     if (!workspace || !op_aligned(workspace, 16) || workspace_bytes < p.bytes) return BACKEND_INVALID_ARGUMENT;
-    const uint64_t blocks = (a->channels + kBlockCh - 1) / kBlockCh, sums = ((uint64_t)a->rows * a->groups * 2 * a->n + kBlock - 1) / kBlock;
+    const uint64_t blocks = (a->channels + kBlockCh - 1) / kBlockCh, joins = (a->channels + kJoinCh - 1) / kJoinCh, sums = ((uint64_t)a->rows * a->groups * 2 * a->n + kBlock - 1) / kBlock;
     const uint64_t columns = ((uint64_t)a->channels * (a->n + 2) + kOpWave - 1) / kOpWave;
-    if (!op_grid_ok(p.pieces * blocks, kBlock) || !op_grid_ok(sums, kBlock) || !op_grid_ok(n_seq * blocks, kBlock))
+    if (!op_grid_ok(p.pieces * blocks, kBlock) || !op_grid_ok(sums, kBlock) || !op_grid_ok(n_seq * joins, kOpWave))
         return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
@@ -1112,7 +1113,7 @@ int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* 
         const void* const fn = small ? SCAN_FN(k.a.r, k_scan_grad_pieces, true) : SCAN_FN(k.a.r, k_scan_grad_pieces, false);
         int32_t rc = op_launch(fn, dim3((uint32_t)(p.pieces * blocks)), dim3(kBlock), 0, stream, k);
         if (rc == BACKEND_OK && k.a.joined && n_seq)
-            rc = op_launch(small ? grad_join_fn<true>(a->n) : grad_join_fn<false>(a->n), dim3((uint32_t)(n_seq * blocks), 2), dim3(kBlock), 0, stream, k);
+            rc = op_launch(small ? grad_join_fn<true>(a->n) : grad_join_fn<false>(a->n), dim3((uint32_t)(n_seq * joins), 2), dim3(kOpWave), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
     int32_t rc = op_launch(small ? SCAN_FN(k.a.r, k_scan_grad_run, true) : SCAN_FN(k.a.r, k_scan_grad_run, false), dim3((uint32_t)(p.pieces * p.parts)), dim3(kBlock), 0,
