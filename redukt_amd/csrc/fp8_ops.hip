@@ -296,12 +296,12 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 __device__ __forceinline__ int place_of(int row, int c) { return c ^ (row / 2 % 8); }
 
-// ROWS rows of a tile into `to`, 1 KB a wave and request; `at` is the lane's place in the operand, stride the bytes of a row.
+// ROWS rows of a tile into `to`, 1 KB a wave and request; `at` are the lane's places in the operand, c the bytes behind them.
 template <int ROWS, int WAVES>
-__device__ __forceinline__ void stage_rows(__amdgpu_buffer_rsrc_t from, lds_u8* __restrict__ to, uint32_t at, uint32_t stride, int wave) {
+__device__ __forceinline__ void stage_rows(__amdgpu_buffer_rsrc_t from, lds_u8* __restrict__ to, const uint32_t (&at)[ROWS / 8 / WAVES], uint32_t c, int wave) {
 #pragma unroll
     for (int u = 0; u < ROWS / 8 / WAVES; u++)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(to + (u * WAVES + wave) * 1024), 16, (int)(at + u * (WAVES * 8) * stride), 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)(to + (u * WAVES + wave) * 1024), 16, (int)at[u], (int)c, 0, 0);
 }
 
 __device__ __forceinline__ i32x4 piece(const lds_u8* rows, int row, int c) {
@@ -349,38 +349,60 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
     const int row = wave * 8 + lane / 8;
     const uint32_t col = place_of(row, lane % 8) * 16, scale_at = (wave * kWave + lane) * blocks * 4;
     static_assert(W * 8 % 16 == 0, "a lane's rows have one order of pieces");
-    // (rows past the tile and columns past k are out of the buffers' bounds and come as zeros)
+    uint32_t at_w[TN / 8 / W], at_x[TM / 8 / W];
+#pragma unroll
+    for (int u = 0; u < TN / 8 / W; u++) at_w[u] = (row + u * (W * 8)) * ws + col;
+#pragma unroll
+    for (int u = 0; u < TM / 8 / W; u++) at_x[u] = (row + u * (W * 8)) * xs + col;
+    // Rows past the tile are out of the buffers' bounds and come as zeros.  The columns' place is the requests' scalar offset while all 128
+    // are there; a last part of them, and what would follow, goes by places out of bounds for the columns past k.
     const auto stage = [&](lds_u8* __restrict__ to, uint32_t c) {
-        const bool in = c + col < a.k;
-        stage_rows<TN, W>(rw, to, in ? row * ws + col + c : 0x80000000u, ws, wave);
-        stage_rows<TM, W>(rx, to + TN * kSide, in ? row * xs + col + c : 0x80000000u, xs, wave);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + kRows + wave * 256), 4, c < a.k ? (int)(scale_at + c / kSide * 4) : (int)0x80000000, 0, 0, 0);
+        if (c + kSide <= a.k) {
+            stage_rows<TN, W>(rw, to, at_w, c, wave);
+            stage_rows<TM, W>(rx, to + TN * kSide, at_x, c, wave);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + kRows + wave * 256), 4, (int)scale_at, (int)(c / kSide * 4), 0, 0);
+        } else {
+            uint32_t end_w[TN / 8 / W], end_x[TM / 8 / W];
+#pragma unroll
+            for (int u = 0; u < TN / 8 / W; u++) end_w[u] = c + col < a.k ? at_w[u] + c : 0x80000000u;
+#pragma unroll
+            for (int u = 0; u < TM / 8 / W; u++) end_x[u] = c + col < a.k ? at_x[u] + c : 0x80000000u;
+            stage_rows<TN, W>(rw, to, end_w, 0, wave);
+            stage_rows<TM, W>(rx, to + TN * kSide, end_x, 0, wave);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(to + kRows + wave * 256), 4, c < a.k ? (int)(scale_at + c / kSide * 4) : (int)0x80000000, 0, 0, 0);
+        }
     };
     const int rj = wave / WN * (TM / WM), ri = wave % WN * (TN / WN);
     const float* const wsc = a.w_scales + (size_t)((j0 + ri) / kSide < (a.n + kSide - 1) / kSide ? (j0 + ri) / kSide : 0) * blocks;
     f32x4 acc[NI][NJ] = {};
-    const auto step = [&](const lds_u8* __restrict__ w, const lds_u8* __restrict__ x, const float* sx, float sw) {
+    // A block of columns, in `buffer`; `ahead` asks for a later one once this one's first fragments are on their way.
+    const auto step = [&](const lds_u8* __restrict__ w, float sw, auto&& ahead) {
+        const lds_u8* const x = w + TN * kSide;
         const auto load = [&](const lds_u8* rows, int row) {
             return fragment_of<kExact<T>>(piece(rows, row + lane % 16, lane / 16), piece(rows, row + lane % 16, 4 + lane / 16));
         };
         Fragment<kExact<T>> fw[NI], fx[2];
         float s[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] = sx[rj + 16 * j + lane % 16] * sw;
-#pragma unroll
         for (int i = 0; i < NI; i++) fw[i] = load(w, ri + 16 * i);
         fx[0] = load(x, rj);
-        // (a tile's sums are added while the matrix cores work on the next one)
-        f32x4 p[2];
 #pragma unroll
-        for (int t = 0; t <= NI * NJ; t++) {
+        for (int j = 0; j < NJ; j++) s[j] = ((const __attribute__((address_space(3))) float*)(w + kRows))[rj + 16 * j + lane % 16] * sw;
+        __builtin_amdgcn_sched_barrier(0);
+        ahead();
+        __builtin_amdgcn_sched_barrier(0);
+        // (a tile's sums are added while the matrix cores work on the next ones)
+        constexpr int kLag = 2;
+        f32x4 p[kLag + 1];
+#pragma unroll
+        for (int t = 0; t < NI * NJ + kLag; t++) {
             const int i = t % NI, j = t / NI;
             if (i == 0 && j + 1 < NJ) fx[(j + 1) % 2] = load(x, rj + 16 * (j + 1));
-            if (t < NI * NJ) p[t % 2] = multiply(fw[i], fx[j % 2]);
-            if (t > 0) {
-                const int u = (t - 1) % NI, v = (t - 1) / NI;
+            if (t < NI * NJ) p[t % (kLag + 1)] = multiply(fw[i], fx[j % 2]);
+            if (t >= kLag) {
+                const int u = (t - kLag) % NI, v = (t - kLag) / NI;
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[u][v][e] = fmaf(p[(t - 1) % 2][e], s[v], acc[u][v][e]);
+                for (int e = 0; e < 4; e++) acc[u][v][e] = fmaf(p[(t - kLag) % (kLag + 1)][e], s[v], acc[u][v][e]);
                 asm volatile("" : "+v"(acc[u][v]));        // (here, and not behind the last product, where every tile's would wait in registers)
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -396,8 +418,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
             if (c + s * kSide >= a.k) break;
             const float sw = wsc[c / kSide + s];
             wait_and_meet<kPending>();
-            stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * kSide);
-            step((const lds_u8*)lds[s], (const lds_u8*)lds[s] + TN * kSide, (const float*)(lds[s] + kRows), sw);
+            step((const lds_u8*)lds[s], sw, [&] { stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * kSide); });
         }
     }
     wait_and_meet<0>();                        // (zeros may still be on their way)
