@@ -289,8 +289,9 @@ __global__ __launch_bounds__(512) void k_fp8_few(Fp8Few f) {
 // while the matrix cores work on another.  A wave takes (TN / WN) x (TM / WM) outputs in 16 x 16 tiles.
 //
 // A row of 128 codes is 8 pieces of 16 bytes; piece c of row r stands at place c ^ (r / 2 % 8), so that the 16 rows that 16 lanes read a
-// piece of meet no bank twice.  The loads write LDS in lane order, so the lane picks the piece that belongs to its place.  The tokens' scales
-// of the block come the same way, 4 bytes a lane.
+// piece of meet no bank twice.  The loads write LDS in lane order, so the lane picks the piece that belongs to its place.  The scales of
+// the block come the same way, 4 bytes a lane: a load into registers would be waited for with all that is on its way to LDS (64 of 8,192 x
+// 8,192: 42 us).
 typedef __attribute__((address_space(3))) unsigned char lds_u8;
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -325,11 +326,12 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("" ::: "memory");
 }
 
+// (two waves a SIMD: with more registers to choose from, the products go to accumulation registers, which the sums cannot read)
 template <typename T, int TM, int TN, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tiles(Fp8Tiles f) {
     constexpr int W = WM * WN, NI = TN / WN / 16, NJ = TM / WM / 16, kRows = (TM + TN) * kSide, kStage = kRows + W * kWave * 4;
     constexpr int kRequests = kRows / 1024 / W + 1, kPending = (STAGES - 2) * kRequests;        // (of a wave and stage; behind the next one)
-    static_assert(kPending < 64 && TM / 8 % W == 0 && TN / 8 % W == 0 && TM <= W * kWave && kSide % (TN / WN) == 0, "");
+    static_assert(kPending < 64 && TM / 8 % W == 0 && TN / 8 % W == 0 && TM + 2 <= W * kWave && TM % kWave == 0 && TN <= 2 * kSide && kSide % (TN / WN) == 0, "");
     __shared__ __attribute__((aligned(1024))) unsigned char lds[STAGES][kStage];
     const redukt_fp8_matmul& a = f.a;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -345,9 +347,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
     const auto rx = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)a.x + (size_t)i0 * xs), (short)0, (int)((tall - 1) * xs + a.k), 0x00020000);
     const auto rw = __builtin_amdgcn_make_buffer_rsrc((void*)((const uint8_t*)a.w + (size_t)j0 * ws), (short)0,
                                                       (int)((min(a.n - j0, (uint32_t)TN) - 1) * ws + a.k), 0x00020000);
-    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(a.x_scales + (size_t)i0 * blocks), (short)0, (int)(tall * blocks * 4), 0x00020000);
+    // (of the scales, the first waves take the tokens', the others the channels')
+    const uint32_t sides = (a.n + kSide - 1) / kSide, side0 = j0 / kSide;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void*)(wave < TM / kWave ? a.x_scales + (size_t)i0 * blocks : a.w_scales + (size_t)side0 * blocks), (short)0,
+                                                      (int)((wave < TM / kWave ? tall : min(sides - side0, 2u)) * blocks * 4), 0x00020000);
     const int row = wave * 8 + lane / 8;
-    const uint32_t col = place_of(row, lane % 8) * 16, scale_at = (wave * kWave + lane) * blocks * 4;
+    const uint32_t col = place_of(row, lane % 8) * 16, scale_at = (wave < TM / kWave ? wave * kWave + lane : (wave - TM / kWave) * kWave + lane) * blocks * 4;
     static_assert(W * 8 % 16 == 0, "a lane's rows have one order of pieces");
     uint32_t at_w[TN / 8 / W], at_x[TM / 8 / W];
 #pragma unroll
@@ -373,32 +378,38 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
         }
     };
     const int rj = wave / WN * (TM / WM), ri = wave % WN * (TN / WN);
-    const float* const wsc = a.w_scales + (size_t)((j0 + ri) / kSide < (a.n + kSide - 1) / kSide ? (j0 + ri) / kSide : 0) * blocks;
     f32x4 acc[NI][NJ] = {};
     // A block of columns, in `buffer`; `ahead` asks for a later one once this one's first fragments are on their way.
-    const auto step = [&](const lds_u8* __restrict__ w, float sw, auto&& ahead) {
+    const auto step = [&](const lds_u8* __restrict__ w, auto&& ahead) {
+        typedef const __attribute__((address_space(3))) float lds_float;
         const lds_u8* const x = w + TN * kSide;
+        lds_float* const scales = (lds_float*)(w + kRows);
         const auto load = [&](const lds_u8* rows, int row) {
             return fragment_of<kExact<T>>(piece(rows, row + lane % 16, lane / 16), piece(rows, row + lane % 16, 4 + lane / 16));
         };
-        Fragment<kExact<T>> fw[NI], fx[2];
+        constexpr int kFx = NJ > 4 ? 3 : 2;        // tokens' fragments in registers
+        Fragment<kExact<T>> fw[NI], fx[kFx];
         float s[NJ];
 #pragma unroll
         for (int i = 0; i < NI; i++) fw[i] = load(w, ri + 16 * i);
-        fx[0] = load(x, rj);
 #pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] = ((const __attribute__((address_space(3))) float*)(w + kRows))[rj + 16 * j + lane % 16] * sw;
+        for (int j = 0; j < kFx - 1 && j < NJ; j++) fx[j] = load(x, rj + 16 * j);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s[j] = scales[rj + 16 * j + lane % 16];
+        const float sw = scales[TM + ri / kSide];
         __builtin_amdgcn_sched_barrier(0);
         ahead();
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s[j] *= sw;
         // (a tile's sums are added while the matrix cores work on the next ones)
         constexpr int kLag = 2;
         f32x4 p[kLag + 1];
 #pragma unroll
         for (int t = 0; t < NI * NJ + kLag; t++) {
             const int i = t % NI, j = t / NI;
-            if (i == 0 && j + 1 < NJ) fx[(j + 1) % 2] = load(x, rj + 16 * (j + 1));
-            if (t < NI * NJ) p[t % (kLag + 1)] = multiply(fw[i], fx[j % 2]);
+            if (i == 0 && j + kFx - 1 < NJ) fx[(j + kFx - 1) % kFx] = load(x, rj + 16 * (j + kFx - 1));
+            if (t < NI * NJ) p[t % (kLag + 1)] = multiply(fw[i], fx[j % kFx]);
             if (t >= kLag) {
                 const int u = (t - kLag) % NI, v = (t - kLag) / NI;
 #pragma unroll
@@ -416,9 +427,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_tiles(Fp8Tiles f) {
 #pragma unroll
         for (int s = 0; s < STAGES; s++) {
             if (c + s * kSide >= a.k) break;
-            const float sw = wsc[c / kSide + s];
             wait_and_meet<kPending>();
-            step((const lds_u8*)lds[s], sw, [&] { stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * kSide); });
+            step((const lds_u8*)lds[s], [&] { stage((lds_u8*)lds[(s + STAGES - 1) % STAGES], c + (s + STAGES - 1) * kSide); });
         }
     }
     wait_and_meet<0>();                        // (zeros may still be on their way)
@@ -570,13 +580,22 @@ int32_t redukt_op_fp8_matmul(const redukt_fp8_matmul* a, void* stream) {
         if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
         return op_launch(OP_BY_TYPE(k.dtype, k_fp8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
-    if (k.m <= (k.n >= 8192 ? 3 : 16)) return few(k, stream);
-    const auto count = [&](uint32_t t) { return (uint64_t)((k.m + t - 1) / t) * ((k.n + t - 1) / t); };
-    if (count(256) >= 256 && k.dtype != REDUKT_OP_F32) return tiles16<256, 256, 2, 4, 2>(k, stream);
-    if (count(128) > 256) return tiles<128, 128, 2, 2, 2>(k, stream);
-    if (count(128) >= 192) return tiles<128, 128, 2, 2, 3>(k, stream);
-    if (count(64) <= 128) return tiles<64, 32, 2, 1, 6>(k, stream);
-    return tiles<64, 64, 2, 2, 4>(k, stream);
+    // The choice is by time (us on either side of each edge, bf16; n and k after m).  Few tokens: weights straight into registers (16 of 4,096 x
+    // 4,096 7.6, tiles 10.1; 8 of 768 x 4,096 5.9 and 9.8), fewer of them where the channels alone fill the CUs with tiles (8 of 8,192 x 8,192
+    // 16.7 and 17.3; 8 of 50,280 x 768 12.3 and 9.1, 1 9.9 and 9.0, with f32 outputs 10.1 and 10.4).
+    if (k.m <= (k.n >= 16384 ? 2 : k.n >= 8192 ? 8 : 16)) return few(k, stream);
+    // Tiles of 256 once they nearly fill the CUs (8,192 of 1,536 x 768, 192 tiles: 17.3, of 128: 19.8), of 128 once a CU has two (2,048 of
+    // 4,096 x 4,096, 512 tiles: 41.4, 64 x 128 50.2; 1,024 of 4,096 x 4,096, 256: 29.8 and 27.3), of 64 x 128 once each CU has one (512 of
+    // 4,096 x 4,096, 256 tiles: 17.2, of 64 18.5; 1,000 of 1,536 x 768, 192: 6.0 and 5.4), else of 64, with more stages where a CU has
+    // one workgroup only (128 of 8,192 x 8,192, 256 tiles: four stages 21.2, two 37.1; 1,000 of 1,536 x 768, 384: 6.2 and 5.4), by 32 channels
+    // where half of the CUs would have none (64 of 8,192 x 8,192: 18.0, by 64 20.0; 128 of 768 x 4,096 10.0 and 10.8).
+    const auto count = [&](uint32_t tm, uint32_t tn) { return (uint64_t)((k.m + tm - 1) / tm) * ((k.n + tn - 1) / tn); };
+    if (count(256, 256) >= 160 && k.dtype != REDUKT_OP_F32) return tiles16<256, 256, 2, 4, 2>(k, stream);
+    if (count(128, 128) >= 384) return tiles<128, 128, 2, 2, 2>(k, stream);
+    if (count(64, 128) >= 256) return tiles<64, 128, 2, 2, 3>(k, stream);
+    if (count(64, 64) > 256) return tiles<64, 64, 2, 2, 2>(k, stream);
+    if (count(64, 64) > 128) return tiles<64, 64, 2, 2, 4>(k, stream);
+    return tiles<64, 32, 2, 1, 4>(k, stream);
 }
 
 }  // extern "C"
