@@ -6,7 +6,7 @@
 
 #include "op_common.h"
 
-#pragma clang fp contract(off)
+#pragma clang fp contract(fast)
 
 namespace rdk {
 namespace {
@@ -14,7 +14,8 @@ namespace {
 constexpr double kOne = 0x1p42;
 constexpr double kLeast = -29.9;           // ln 2^-43 = -29.81: e to less than this is no whole step
 constexpr uint32_t kBins = 2048;           // of (max - l) / T, linear, down to kLeast
-constexpr uint32_t kList = 1024;           // elements that are put in order by comparing each with all
+constexpr uint32_t kList = 1024;           // elements that are put in order in LDS
+constexpr int kPowerBits = 7, kPowers = 1 << kPowerBits;
 constexpr uint32_t kCoarse = 512;          // bins of the threads' largest logits
 constexpr uint32_t kFewK = 512;            // top_k that the list takes in general
 constexpr uint32_t kMaxVocab = 1u << 20;   // 2^20 weights of 2^42 stay below 2^63
@@ -48,7 +49,8 @@ __device__ __forceinline__ uint64_t order_of(uint32_t key, uint32_t index) { ret
 
 template <int THREADS>
 struct SampleLds {
-    Listed list[kList];
+    double powers[kPowers];    // 2^(i / kPowers)
+    Listed list[kList], sorted[kList];
     union {
         uint64_t weight[kBins];
         uint32_t count[kBins];
@@ -57,7 +59,6 @@ struct SampleLds {
     float wave_max[THREADS / kOpWave];
     uint32_t listed, least, most, bin, found_key, found_index, kept;
     uint64_t before, sum;
-    Listed sorted[kList];
 };
 
 // A row of logits, VEC neighbouring ones of a sweep over the row a thread.  Passes of the general way read it again (from L2: with every
@@ -70,8 +71,8 @@ struct Row {
     uint32_t n, sweeps;
     bool aligned;
 
-    __device__ __forceinline__ vec load(uint32_t s) const {
-        const uint32_t i = s * kSweep + threadIdx.x * VEC;
+    __device__ __forceinline__ vec load(uint32_t s) const { return at(s * kSweep + threadIdx.x * VEC); }
+    __device__ __forceinline__ vec at(uint32_t i) const {
         vec v;
         if (aligned && i + VEC <= n) return *(const vec*)(p + i);
 #pragma unroll
@@ -94,34 +95,54 @@ struct Row {
 struct Scale {
     float most;
     float bins;                // bins a unit of logits
-    double inv;                // 1 / T
+    double steps;              // kPowers log2(e) / T: steps of 2^(1 / kPowers) a unit of logits
+    const double* powers;
     // Where l is below the largest, in bins: falls with l, and is below kBins for all that weigh anything (kLeast leaves 6 bins to
     // spare for the rounding).  NaN and -inf are nowhere.
     __device__ __forceinline__ float place(float l) const { return l == most ? 0.0f : (most - l) * bins; }
     __device__ __forceinline__ bool live(float l) const { return place(l) < (float)kBins; }
     __device__ __forceinline__ uint32_t bin(float l) const { return (uint32_t)place(l); }
+    // 2^42 e^((l - most) / T) to the nearest whole number, of a live l.  The power's argument in steps of 2^(1 / 128) is a whole number (added
+    // to 1.5 * 2^52 it stands in the sum's last bits) and a rest of at most half a step, |rest ln 2 / 128| <= 0.0028; of its power's series five
+    // terms leave 1.4e-15.  Adding 2^52 leaves the whole number in the last bits again.
     __device__ __forceinline__ uint64_t weight(float l) const {
         if (l == most) return (uint64_t)kOne;
-        const double x = ((double)l - (double)most) * inv;
-        return x >= kLeast ? (uint64_t)__builtin_rint(exp(x) * kOne) : 0;
+        constexpr double kWhole = 0x1.8p52, kRest = 0x1.62e42fefa39efp-1 / kPowers;
+        const double x = ((double)l - (double)most) * steps, whole = x + kWhole;
+        const int k = (int)(uint32_t)__builtin_bit_cast(uint64_t, whole);
+        const double r = (x - (whole - kWhole)) * kRest;
+        const double p = 1.0 + r * (1.0 + r * (0.5 + r * (1.0 / 6.0 + r * (1.0 / 24.0))));
+        const double w = __builtin_ldexp(powers[k & (kPowers - 1)] * p, (k >> kPowerBits) + 42);
+        return x >= kLeast * (kPowers * 0x1.71547652b82fep+0) ? __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xfffffffffffffull : 0;
     }
 };
 
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kOpWave);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_or_0(uint64_t v) {
+    return (uint64_t)dpp_or_0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp_or_0<CTRL, ROWS>((uint32_t)v);
+}
+
+// v summed over the lanes up to this one: within rows of 16 by moves of 1, 2, 4 and 8 lanes, then a row's last lane into the next row, and
+// lane 31 into the upper half.
+template <typename V>
+__device__ __forceinline__ V wave_upto(V v) {
+    v += dpp_or_0<0x111, 0xf>(v);
+    v += dpp_or_0<0x112, 0xf>(v);
+    v += dpp_or_0<0x114, 0xf>(v);
+    v += dpp_or_0<0x118, 0xf>(v);
+    v += dpp_or_0<0x142, 0xa>(v);
+    v += dpp_or_0<0x143, 0xc>(v);
     return v;
 }
 
-// v summed over the lanes up to this one.
-__device__ __forceinline__ uint64_t wave_upto(uint64_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < kOpWave; o <<= 1) {
-        const uint64_t x = __shfl_up(v, o, kOpWave);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) { return (uint64_t)from_lane((uint32_t)(v >> 32), lane) << 32 | from_lane((uint32_t)v, lane); }
+
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return from_lane(wave_upto(v), kOpWave - 1); }
 
 template <int THREADS>
 __device__ __forceinline__ uint64_t block_sum(SampleLds<THREADS>& l, uint64_t v) {
@@ -152,7 +173,7 @@ __device__ __forceinline__ void find_bin(SampleLds<THREADS>& l, const V* value, 
     uint64_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) mine += value[threadIdx.x * kPer + i];
-    const uint64_t upto = wave_upto(mine, lane);
+    const uint64_t upto = wave_upto(mine);
     if (threadIdx.x == 0) l.bin = kBins;
     if (lane == kOpWave - 1) l.wave_sum[wave] = upto;
     __syncthreads();
@@ -238,7 +259,7 @@ __device__ __forceinline__ Cut find_cut(SampleLds<THREADS>& l, const R& row, con
             w[e] = !hit ? 0 : want.by_weight ? m.weight(x) : 1;
             mine += w[e];
         }
-        const uint64_t upto = wave_upto(mine, lane);
+        const uint64_t upto = wave_upto(mine);
         __syncthreads();
         if (lane == kOpWave - 1) l.wave_sum[wave] = upto;
         __syncthreads();
@@ -270,70 +291,105 @@ __device__ __forceinline__ double limit_of(float u, uint64_t sum) {
     return limit < (double)sum ? limit : (double)sum * 0.9999999999999999;
 }
 
-// How many neighbouring threads share each of n elements: 1 to 16.
-template <int THREADS>
-__device__ __forceinline__ uint32_t sharers(uint32_t n) {
-    uint32_t share = 16;
-    while (share > 1 && n * share > THREADS) share /= 2;
-    return share;
-}
+// What draw_listed keeps in the bins' place.
+constexpr uint32_t kFine = 256;            // its bins
+struct Ordered {
+    uint32_t first[kFine + 1];             // elements of a bin, then the place of its first one
+    uint32_t place[kList];                 // an element's bin, and behind 16 bits its number there
+    uint64_t weight[kFine];                // kept weights by index
+};
+static_assert(sizeof(Ordered) <= kBins * 8, "");
 
-__device__ __forceinline__ uint64_t shared_sum(uint64_t v, uint32_t share) {
-    for (uint32_t o = 1; o < share; o <<= 1) v += __shfl_xor(v, o, kOpWave);
-    return v;
-}
-
-// Where everything that may be kept is in the list (n > 0 elements; top_k and top_p of them, `all` the sum that top_p is of if top_k keeps
-// all): each element looks at all others for its place in the order of values, and those that are kept at each other once more in that of
-// indexes.
+// Where everything that may be kept is in the list (n elements, none further than `reach` below the largest; top_k and top_p of them, `all` the
+// sum that top_p is of if top_k keeps all).  Elements go to 256 bins by value, and within a bin each looks at the others for its place.  From there
+// one wave goes on without waiting for others: sums along the order say who is kept, their weights go to 256 bins by index, and the bin that the
+// limit falls into is looked through.  (Each element against all others took 5 us with 150 of them, 100 with 1,000.)
 template <int THREADS>
-__device__ __forceinline__ void draw_listed(SampleLds<THREADS>& l, uint32_t n, uint64_t top_k, bool by_p, double top_p, uint64_t all, double least, float u,
-                                            int32_t* token) {
-    constexpr uint64_t kMark = 1ull << 53;     // an element counts as this beside its weight: 1,024 weights stay below it
-    constexpr int kPer = kList / THREADS > 1 ? kList / THREADS : 1;
-    uint32_t share = sharers<THREADS>(n), sub = threadIdx.x % share;
-    Listed me[kPer];
-    uint64_t before[kPer];
-    uint32_t rank[kPer];
+__device__ __forceinline__ void draw_listed(SampleLds<THREADS>& l, const Scale& m, uint32_t n, float reach, uint32_t vocab, uint64_t top_k, bool by_p, double top_p,
+                                            uint64_t all, uint64_t least, float u, int32_t* token) {
+    constexpr uint32_t kPer = kFine / kOpWave;
+    Ordered& o = *(Ordered*)l.weight;
+    const int lane = threadIdx.x % kOpWave;
+    const float fine = (float)(kFine - 1) / reach;
+    for (uint32_t i = threadIdx.x; i < kFine; i += THREADS) o.first[i] = 0, o.weight[i] = 0;
     if (threadIdx.x == 0) l.kept = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        const uint32_t t = i * (THREADS / share) + threadIdx.x / share;
-        rank[i] = ~0u;
-        if (t >= n) continue;                  // (a shared element's threads all go or stay)
-        me[i] = l.list[t];
-        uint64_t sum = 0;
-#pragma unroll 8
-        for (uint32_t j = sub; j < n; j += share) sum += l.list[j].order > me[i].order ? l.list[j].w + kMark : 0;
-        sum = shared_sum(sum, share);
-        if (sub != 0) continue;
-        rank[i] = (uint32_t)(sum / kMark);
-        before[i] = sum % kMark;
-        if (rank[i] + 1 == (top_k < n ? (uint32_t)top_k : n)) l.sum = before[i] + me[i].w;
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < n; t += THREADS) {
+        const float v = value_of(l.list[t].key());
+        const uint32_t bin = v == m.most ? 0u : (uint32_t)fminf((m.most - v) * fine, (float)(kFine - 1));
+        l.list[t].w = m.weight(v);
+        o.place[t] = bin | atomicAdd(&o.first[bin], 1u) << 16;
     }
     __syncthreads();
-    const Want want{true, 0, top_p * (double)(top_k == ~0ull ? all : l.sum)};
+    if (threadIdx.x < kOpWave) {
+        uint32_t c[kPer], mine = 0;
 #pragma unroll
-    for (int i = 0; i < kPer; i++) {
-        if (rank[i] >= top_k || rank[i] == ~0u || (by_p && !want.keeps(before[i])) || (double)me[i].w < least) continue;
-        l.sorted[rank[i]] = me[i];
-        atomicMax(&l.kept, rank[i] + 1);
+        for (uint32_t i = 0; i < kPer; i++) mine += c[i] = o.first[lane * kPer + i];
+        uint32_t before = wave_upto(mine) - mine;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; i++) {
+            o.first[lane * kPer + i] = before;
+            before += c[i];
+        }
+        if (lane == 0) o.first[kFine] = n;
     }
     __syncthreads();
-    const uint32_t m = l.kept;
-#pragma unroll
-    for (int i = 0; i < kPer; i++)
-        if (rank[i] + 1 == m) l.before = before[i] + me[i].w;        // (all kept weights)
+    for (uint32_t t = threadIdx.x; t < n; t += THREADS) l.sorted[o.first[o.place[t] & 0xffff] + (o.place[t] >> 16)] = l.list[t];
     __syncthreads();
-    const double limit = limit_of(u, l.before);
-    share = sharers<THREADS>(m), sub = threadIdx.x % share;
-    for (uint32_t t = threadIdx.x / share; t < m; t += THREADS / share) {
+    for (uint32_t t = threadIdx.x; t < n; t += THREADS) {
+        const uint32_t bin = o.place[t] & 0xffff, first = o.first[bin], end = o.first[bin + 1], at = first + (o.place[t] >> 16);
+        const Listed me = l.sorted[at];
+        uint32_t rank = first;
+        for (uint32_t j = first; j < end; j++) rank += l.sorted[j].order > me.order;
+        l.list[rank] = me;                     // (all are in `sorted`)
+    }
+    __syncthreads();
+    if (threadIdx.x >= kOpWave) return;
+    // In order now: a lane takes `per` neighbouring ones.
+    const uint32_t per = (n + kOpWave - 1) / kOpWave, t0 = lane * per, t1 = min(t0 + per, n);
+    uint64_t sum = 0;
+    for (uint32_t t = t0; t < t1; t++) sum += t < top_k ? l.list[t].w : 0;
+    uint64_t upto = wave_upto(sum);
+    const Want want{true, 0, top_p * (double)(top_k == ~0ull ? all : from_lane(upto, kOpWave - 1))};
+    const uint32_t wide = (vocab + kFine - 1) / kFine;
+    uint64_t before = upto - sum;
+    sum = 0;
+    for (uint32_t t = t0; t < t1; t++) {
+        const Listed e = l.list[t];
+        const bool kept = t < top_k && (!by_p || want.keeps(before)) && e.w >= least;
+        before += e.w;
+        if (kept) {
+            sum += e.w;
+            atomicAdd((unsigned long long*)&o.weight[e.index() / wide], (unsigned long long)e.w);
+        } else {
+            l.list[t].w = 0;
+        }
+    }
+    sum = wave_sum(sum);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const double limit = limit_of(u, sum);
+    uint64_t w[kPer], mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPer; i++) mine += w[i] = o.weight[lane * kPer + i];
+    upto = wave_upto(mine);
+    const int at = __builtin_ctzll(__ballot((double)upto > limit) | 1ull << 63);        // (the last lane's is)
+    before = upto - mine;
+    uint32_t bin = lane * kPer;
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < kPer; i++)
+        if (bin == lane * kPer + i && !((double)(before + w[i]) > limit)) before += w[i], bin++;
+    before = from_lane(before, at), bin = from_lane(bin, at);
+    for (uint32_t t = t0; t < t1; t++)
+        if (l.list[t].w && l.list[t].index() / wide == bin) l.sorted[atomicAdd(&l.kept, 1u)] = l.list[t];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const uint32_t few = l.kept;
+    for (uint32_t t = lane; t < few; t += kOpWave) {
         const Listed e = l.sorted[t];
-        uint64_t upto = 0;
-#pragma unroll 8
-        for (uint32_t j = sub; j < m; j += share) upto += (uint32_t)l.sorted[j].order >= (uint32_t)e.order ? l.sorted[j].w : 0;      // (indexes are inverted)
-        upto = shared_sum(upto, share);
-        if (sub == 0 && (double)upto > limit && !((double)(upto - e.w) > limit)) *token = (int32_t)e.index();
+        uint64_t s = before;
+        for (uint32_t j = 0; j < few; j++) s += l.sorted[j].index() <= e.index() ? l.sorted[j].w : 0;
+        if ((double)s > limit && !((double)(s - e.w) > limit)) *token = (int32_t)e.index();
     }
 }
 
@@ -345,12 +401,7 @@ __device__ __forceinline__ uint32_t coarse_bin(SampleLds<THREADS>& l, uint32_t t
         uint32_t c[kPer], mine = 0;
 #pragma unroll
         for (int i = 0; i < kPer; i++) mine += c[i] = l.count[lane * kPer + i];
-        uint32_t upto = mine;
-#pragma unroll
-        for (int o = 1; o < kOpWave; o <<= 1) {
-            const uint32_t x = __shfl_up(upto, o, kOpWave);
-            if (lane >= o) upto += x;
-        }
+        const uint32_t upto = wave_upto(mine);
         const uint64_t hit = __ballot(upto >= top_k);
         if (lane == 0) l.bin = kCoarse;
         if (hit && lane == (int)__builtin_ctzll(hit)) {
@@ -367,11 +418,11 @@ __device__ __forceinline__ uint32_t coarse_bin(SampleLds<THREADS>& l, uint32_t t
     return l.bin;
 }
 
-// HELD: sweeps that stay in registers, which hold the whole row; 0: none.
+// HELD: sweeps whose loads go out together, which cover the row; 0: one after the other.
 //
 // With top_k the way is short.  Each thread has the largest of its logits; the top_k-th logit is no further down than the top_k-th of
-// these, and there are few others so far up: they are listed from registers and put in order by comparing each with all.  So a row is
-// read once.
+// these, and there are few others so far up: they are listed and put in order.  A row is read once, and of it again what the threads read
+// that have such a logit.
 template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     typedef Row<T, THREADS> R;
@@ -409,6 +460,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     for (int o = 32; o > 0; o >>= 1) m.most = fmaxf(m.most, __shfl_xor(m.most, o, kOpWave));
     if (lane == 0) l.wave_max[wave] = m.most;
     if (threadIdx.x == 0) l.found_index = ~0u;
+    if (threadIdx.x < kPowers) l.powers[threadIdx.x] = exp2((double)threadIdx.x / kPowers);
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kWaves; w++) m.most = fmaxf(m.most, l.wave_max[w]);
@@ -426,10 +478,12 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
         if (threadIdx.x == 0) a.tokens[r] = (int32_t)l.found_index;
         return;
     }
-    m.inv = 1.0 / (double)temperature;
-    m.bins = (float)((kBins - 1) / -kLeast * m.inv);
+    const double inverse = 1.0 / (double)temperature;
+    m.bins = (float)((kBins - 1) / -kLeast * inverse);
+    m.steps = kPowers * 0x1.71547652b82fep+0 * inverse;
+    m.powers = l.powers;
     const bool by_k = top_k > 0 && (uint32_t)top_k < a.vocab, by_p = top_p < 1.0f, by_min = min_p > 0.0f;
-    const double least = by_min ? (double)fminf(min_p, 1.0f) * kOne : 0.0;
+    const uint64_t least = by_min ? (uint64_t)__builtin_ceil((double)fminf(min_p, 1.0f) * kOne) : 1;       // (the limit is exact, and weights are whole)
 
     if constexpr (HELD > 0) {
         if (by_k && top_k <= (int)kFewK) {
@@ -443,38 +497,54 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
                 // (what is a little further down may be listed too, but nothing less: the bin's end as a logit, with room for roundings)
                 float from = m.most - (float)((bin + 1) * (kBins / kCoarse)) / m.bins * 1.0001f;
                 if (!(from < m.most)) from = m.most;
-                // (counted first, so that a wave asks for its places in the list once)
-                uint32_t hits = 0;
+                // The threads that have one, and then all threads over what those read: a row's other logits are not looked at again.
+                if (threadIdx.x == 0) l.kept = 0;
+                __syncthreads();
+                uint32_t* const who = (uint32_t*)l.sorted;
+                const uint64_t some = __ballot(mine >= from);
+                uint32_t to = 0;
+                if (lane == 0 && some) to = atomicAdd(&l.kept, (uint32_t)__popcll(some));
+                to = from_lane(to, 0) + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+                if (mine >= from) who[to] = threadIdx.x;
+                __syncthreads();
+                constexpr uint32_t kAbreast = THREADS / 4;
+                const uint32_t many = l.kept;
+                for (uint32_t j0 = 0; j0 < many; j0 += kAbreast) {
+                    const uint32_t j = j0 + threadIdx.x % kAbreast, first = who[min(j, many - 1)] * VEC;
+                    // (four loads at once, in a row's first part where they would pass its end)
+                    for (uint32_t s0 = wave * kOpWave / kAbreast; s0 < row.sweeps; s0 += 16) {
+                        typename R::vec v[4];
+                        uint32_t i[4], hits = 0;
+                        const bool vectors = row.aligned && a.vocab >= (uint32_t)VEC;
 #pragma unroll
-                for (int i = 0; i < HELD; i++) {
-                    if ((uint32_t)i >= row.sweeps) continue;
-#pragma unroll
-                    for (int e = 0; e < VEC; e++) hits += __popcll(__ballot((float)held[i][e] >= from));
-                }
-                uint32_t at = 0;
-                if (lane == 0 && hits) at = atomicAdd(&l.listed, hits);
-                at = __builtin_amdgcn_readfirstlane(at);
-                if (hits && at + hits <= kList) {
-#pragma unroll
-                    for (int i = 0; i < HELD; i++) {
-                        if ((uint32_t)i >= row.sweeps) continue;
-#pragma unroll
-                        for (int e = 0; e < VEC; e++) {
-                            const bool hit = (float)held[i][e] >= from;
-                            const uint64_t all = __ballot(hit);
-                            if (!all) continue;
-                            const uint32_t to = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-                            if (hit) l.list[to].order = order_of(key_of((float)held[i][e]), (uint32_t)i * R::kSweep + threadIdx.x * VEC + e);
-                            at += __popcll(all);
+                        for (int k = 0; k < 4; k++) {
+                            i[k] = (s0 + 4 * k) * R::kSweep + first;
+                            if (vectors) v[k] = *(const typename R::vec*)(row.p + (i[k] + VEC <= a.vocab ? i[k] : 0));
                         }
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            if (!vectors || i[k] + VEC > a.vocab) v[k] = row.at(min(i[k], a.vocab));      // (-inf behind the row)
+#pragma unroll
+                            for (int e = 0; e < VEC; e++) hits += (float)v[k][e] >= from;
+                        }
+                        if (j >= many) hits = 0;
+                        // (places in the list for a whole wave at once: an atomic a logit costs more than all else here)
+                        const uint32_t upto = wave_upto(hits), all = from_lane(upto, kOpWave - 1);
+                        uint32_t at = 0;
+                        if (lane == 0 && all) at = atomicAdd(&l.listed, all);
+                        at = from_lane(at, 0) + upto - hits;
+                        if (!hits || at + hits > kList) continue;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+#pragma unroll
+                            for (int e = 0; e < VEC; e++)
+                                if ((float)v[k][e] >= from) l.list[at++].order = order_of(key_of((float)v[k][e]), i[k] + e);
                     }
                 }
                 __syncthreads();
                 const uint32_t n = l.listed;
                 if (n <= kList) {
-                    for (uint32_t t = threadIdx.x; t < n; t += THREADS) l.list[t].w = m.weight(value_of(l.list[t].key()));
-                    __syncthreads();
-                    draw_listed(l, n, (uint64_t)top_k, by_p, (double)top_p, 0, least, u, a.tokens + r);
+                    draw_listed(l, m, n, m.most - from, a.vocab, (uint64_t)top_k, by_p, (double)top_p, 0, least, u, a.tokens + r);
                     return;
                 }
             }
@@ -517,12 +587,12 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
                 const float x = (float)v[e];
                 if (!(m.place(x) < (float)(bin + 1))) continue;
                 const uint32_t at = atomicAdd(&l.listed, 1u);
-                if (at < kList) l.list[at] = Listed{order_of(key_of(x), i0 + e), m.weight(x)};
+                if (at < kList) l.list[at].order = order_of(key_of(x), i0 + e);
             }
         });
         __syncthreads();
         if (l.listed <= kList) {
-            draw_listed(l, l.listed, by_k ? (uint64_t)top_k : ~0ull, by_p, (double)top_p, sum, least, u, a.tokens + r);
+            draw_listed(l, m, l.listed, (float)(bin + 1) / m.bins, a.vocab, by_k ? (uint64_t)top_k : ~0ull, by_p, (double)top_p, sum, least, u, a.tokens + r);
             return;
         }
         __syncthreads();                       // (find_cut begins the list anew)
@@ -550,10 +620,11 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
         cut = find_cut(l, row, m, want, [&](uint32_t k, uint32_t i) { return upto.keeps(k, i); });
     }
     // Kept weights, by sweep and wave, and their sum.
+    const bool whole = cut.key == 0;
     const auto kept = [&](float x, uint32_t i) {
-        if (!m.live(x) || !cut.keeps(key_of(x), i)) return (uint64_t)0;
+        if (!m.live(x) || !(whole || cut.keeps(key_of(x), i))) return (uint64_t)0;
         const uint64_t w = m.weight(x);
-        return (double)w >= least ? w : 0;
+        return w >= least ? w : 0;
     };
     uint64_t sum = 0;
     row.each([&](uint32_t sweep, uint32_t i0, const typename R::vec& v) {
@@ -576,7 +647,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     uint32_t cell = 0;
     for (uint32_t c0 = 0; c0 < row.sweeps * kWaves; c0 += kOpWave) {
         const uint32_t c = c0 + lane;
-        const uint64_t w = c < row.sweeps * kWaves ? cells[c] : 0, upto = wave_upto(w, lane);
+        const uint64_t w = c < row.sweeps * kWaves ? cells[c] : 0, upto = wave_upto(w);
         const uint64_t hit = __ballot((double)(before + upto) > limit);
         if (hit) {
             const int at = __builtin_ctzll(hit);
@@ -593,7 +664,7 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
         w[e] = i0 + e < a.vocab ? kept((float)row.p[i0 + e], i0 + e) : 0;
         own += w[e];
     }
-    const uint64_t upto = wave_upto(own, lane);
+    const uint64_t upto = wave_upto(own);
     const uint64_t hit = __ballot((double)(before + upto) > limit);
     if (!hit || lane != (int)__builtin_ctzll(hit)) return;
     uint64_t to = before + upto;

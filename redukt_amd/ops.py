@@ -246,7 +246,8 @@ def _pool(op: str, device: int, name: str, t, a: DeltaRows) -> None:
 def _slots(op: str, device: int, slots, n: int) -> Optional[int]:
     if slots is None:
         return None
-    _check(op, device, "slots", slots, torch.int32, (n,))
+    if not isinstance(slots, torch.Tensor) or slots.dtype is not torch.int32 or slots.shape != (n,) or slots.get_device() != device:
+        _check(op, device, "slots", slots, torch.int32, (n,))
     if not slots.is_contiguous():
         _refuse(f"{op}: slots is not contiguous")
     return slots.data_ptr()
@@ -367,21 +368,30 @@ def _scan_rows(op: str, x, dt, a, b, c, d, z, dt_bias, out) -> Tuple[ScanRows, i
     groups = bc[1]
     if (T | channels | groups | n) >> 31:
         _sizes(op, T, channels, groups, n)
-    if out is not None:
+    if out is not None and (not isinstance(out, torch.Tensor) or out.shape != shape or out.dtype is not dtype or out.get_device() != device):
         _check(op, device, "out", out, dtype, shape)
-    wide = groups * n
-    return ScanRows(DTYPES[dtype], T, channels, groups, n, x.data_ptr(), dt.data_ptr(), None if z is None else z.data_ptr(), b.data_ptr(),
-                    c.data_ptr(), None if out is None else out.data_ptr(), _row_stride(op, "x", x, channels),
-                    _row_stride(op, "dt", dt, channels), 0 if z is None else _row_stride(op, "z", z, channels),
-                    _row_stride(op, "b", b, wide), _row_stride(op, "c", c, wide),
-                    0 if out is None else _row_stride(op, "out", out, channels), a.data_ptr(), None if d is None else d.data_ptr(),
-                    None if dt_bias is None else dt_bias.data_ptr()), device
+    wide, null = groups * n, None
+    # (rows that are not contiguous have their steps looked up)
+    return ScanRows(DTYPES[dtype], T, channels, groups, n, x.data_ptr(), dt.data_ptr(), z.data_ptr() if z is not null else null, b.data_ptr(),
+                    c.data_ptr(), out.data_ptr() if out is not null else null,
+                    channels if x.is_contiguous() else _row_stride(op, "x", x, channels),
+                    channels if dt.is_contiguous() else _row_stride(op, "dt", dt, channels),
+                    channels if z is null or z.is_contiguous() else _row_stride(op, "z", z, channels),
+                    wide if b.is_contiguous() else _row_stride(op, "b", b, wide), wide if c.is_contiguous() else _row_stride(op, "c", c, wide),
+                    channels if out is null or out.is_contiguous() else _row_stride(op, "out", out, channels), a.data_ptr(),
+                    d.data_ptr() if d is not null else null, dt_bias.data_ptr() if dt_bias is not null else null), device
 
 
 def _scan_pool(op: str, device: int, name: str, t, a: ScanRows, slots: Optional[int] = None) -> None:
+    try:
+        got = t.shape
+        if (t.dtype is torch.float32 and got[1:] == (a.channels, a.n) and (slots is None or got[0] == slots) and t.is_contiguous()
+                and t.get_device() == device):
+            return
+    except (AttributeError, IndexError):
+        pass
     _check(op, device, name, t, torch.float32, (slots, a.channels, a.n))
-    if not t.is_contiguous():
-        _refuse(f"{op}: {name} is not contiguous")
+    _refuse(f"{op}: {name} is not contiguous")
 
 
 def _sequences(op: str, device: int, cu_seqlens) -> int:
@@ -404,7 +414,11 @@ def _workspace(op: str, device: int, workspace, need: int):
 
 
 def _asks(*tensors) -> bool:
-    return _tangents() or any(t is not None and t.requires_grad for t in tensors)
+    """Whether one (None: left out) requires a gradient, or somebody computes tangents."""
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return forward_ad._current_level >= 0
 
 
 def scan_step(x, dt, a, b, c, states, d=None, z=None, dt_bias=None, slots=None, out=None, stream: Optional[int] = None):
@@ -422,11 +436,11 @@ def scan_step(x, dt, a, b, c, states, d=None, z=None, dt_bias=None, slots=None, 
     allocates = out is None
     if allocates:
         _device(op, x)
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     r, device = _scan_rows(op, x, dt, a, b, c, d, z, dt_bias, out)
     on = _stream(op, stream, device, allocates)
     _scan_pool(op, device, "states", states, r)
-    if _asks(x, dt, a, b, c, d, z, dt_bias, states, out):
+    if _asks(x, dt, a, b, c, states, d, z, dt_bias, out):
         _no_gradients(op, x, dt, a, b, c, d, z, dt_bias, states, out)
     code = _load().redukt_op_scan_step(ctypes.byref(r), states.data_ptr(), states.shape[0], _slots(op, device, slots, r.rows), on)
     _done(code, op)
@@ -461,7 +475,7 @@ def scan_chunk(x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_i
     given = [t for t in (state_out, out, workspace) if t is not None]
     if out is None:
         _device(op, x)
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        out = torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     r, device = _scan_rows(op, x, dt, a, b, c, d, z, dt_bias, out)
     on = _stream(op, stream, device, allocates)
     n = _sequences(op, device, cu_seqlens)
@@ -797,31 +811,40 @@ def sample(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, out=N
     rows, vocab = logits.shape
     _sizes(op, rows, vocab)
 
+    asks = logits.requires_grad or _tangents()
+
     def per_row(name, t, dtype):
-        _check(op, device, name, t, dtype, (rows,))
+        nonlocal asks
+        if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != (rows,) or t.get_device() != device:
+            _check(op, device, name, t, dtype, (rows,))
         if not t.is_contiguous():
             _refuse(f"{op}: {name} is not contiguous")
+        asks = asks or t.requires_grad
         return t.data_ptr()
 
-    a = Sample(DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(op, "logits", logits, vocab), per_row("u", u, torch.float32),
-               1.0, 1.0, 0.0, 0)
-    settings = (("temperature", temperature, "temperatures", torch.float32), ("top_p", top_p, "top_ps", torch.float32),
-                ("min_p", min_p, "min_ps", torch.float32), ("top_k", top_k, "top_ks", torch.int32))
-    for name, v, many, dtype in settings:
+    def setting(name, v, dtype, none):
+        """(the number for all rows, the address of one for each)"""
+        if v is None:
+            return none, None
         if isinstance(v, torch.Tensor):
-            setattr(a, many, per_row(name, v, dtype))
-        elif v is not None:
-            try:
-                setattr(a, name, min(max(int(v), -1), 2 ** 31 - 1) if name == "top_k" else float(v))
-            except (TypeError, ValueError):
-                _refuse(f"{op}: {name} is a number or a tensor [rows]")
-    if _asks(logits, u) or any(isinstance(v, torch.Tensor) and v.requires_grad for _, v, _, _ in settings):
-        _no_gradients(op, logits, u, *(v if isinstance(v, torch.Tensor) else None for _, v, _, _ in settings))
+            return none, per_row(name, v, dtype)
+        try:
+            return (min(max(int(v), -1), 2 ** 31 - 1) if dtype is torch.int32 else float(v)), None
+        except (TypeError, ValueError):
+            _refuse(f"{op}: {name} is a number or a tensor [rows]")
+
+    f32 = torch.float32
+    at_u = per_row("u", u, f32)
+    (t, ts), (p, ps), (m, ms) = setting("temperature", temperature, f32, 1.0), setting("top_p", top_p, f32, 1.0), setting("min_p", min_p, f32, 0.0)
+    k, ks = setting("top_k", top_k, torch.int32, 0)
+    if asks:
+        _no_gradients(op, logits, u, *(v if isinstance(v, torch.Tensor) else None for v in (temperature, top_p, min_p)))
     allocates = out is None
     on = _stream(op, stream, device, allocates)
     if allocates:
         out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    a.tokens = per_row("out", out, torch.int32)
+    a = Sample(DTYPES[logits.dtype], rows, vocab, logits.data_ptr(), _row_stride(op, "logits", logits, vocab), at_u, t, p, m, k, ts, ps, ms, ks,
+               per_row("out", out, torch.int32))
     _done(_load().redukt_op_sample(ctypes.byref(a), on), op)
     if not allocates:
         increment_version(out)

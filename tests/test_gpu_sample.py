@@ -204,3 +204,15 @@ def test_sample_captured_and_on_another_stream():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, ops.sample(x, u, top_k=k, top_p=0.9))
+
+
+@types
+@pytest.mark.parametrize("vocab", [2, 3, 900, 5001, 50280])
+def test_sample_infinite_temperature_of_masked_rows(vocab, dtype):
+    """All tokens that are not masked weigh the same, with every filter; the row's end is no token."""
+    x = logits_of(5, vocab, dtype, seed=vocab)
+    x[:, 1::2] = -INF
+    t = torch.full((5,), INF, device="cuda")
+    for i, s in enumerate([{}, dict(top_k=1), dict(top_k=300), dict(top_k=vocab - 1), dict(top_p=0.6), dict(top_k=40, top_p=0.5, min_p=1.0)]):
+        got = same(x, uniform(5, seed=i), temperature=t, **s)
+        assert (got % 2 == 0).all()
