@@ -151,9 +151,10 @@ def test_sample_strided_and_unaligned(off, pad, dtype):
     same(logits_of(1, vocab, dtype).expand(rows, vocab), uniform(rows))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=NAMES.get)
 @pytest.mark.parametrize("vocab", [131072, 1 << 20])
-def test_sample_large_vocabularies(vocab):
-    x = logits_of(2, vocab, BF16, spread=0.3)
+def test_sample_large_vocabularies(vocab, dtype):
+    x = logits_of(2, vocab, dtype, spread=0.3)
     for s in ({}, dict(top_k=100), dict(top_p=0.9), dict(top_k=vocab // 2, top_p=0.99)):
         same(x, uniform(2), **s)
 
