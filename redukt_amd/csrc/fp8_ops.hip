@@ -390,18 +390,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tiles(Fp8Tiles f) {
         constexpr int kFx = NJ > 4 ? 3 : 2;        // tokens' fragments in registers
         Fragment<kExact<T>> fw[NI], fx[kFx];
         float s[NJ];
+        // (in the order of their use: the first product waits for two fragments only)
+        fw[0] = load(w, ri);
+        fx[0] = load(x, rj);
 #pragma unroll
-        for (int i = 0; i < NI; i++) fw[i] = load(w, ri + 16 * i);
+        for (int i = 1; i < NI; i++) fw[i] = load(w, ri + 16 * i);
 #pragma unroll
-        for (int j = 0; j < kFx - 1 && j < NJ; j++) fx[j] = load(x, rj + 16 * j);
+        for (int j = 1; j < kFx - 1 && j < NJ; j++) fx[j] = load(x, rj + 16 * j);
 #pragma unroll
         for (int j = 0; j < NJ; j++) s[j] = scales[rj + 16 * j + lane % 16];
         const float sw = scales[TM + ri / kSide];
         __builtin_amdgcn_sched_barrier(0);
         ahead();
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int j = 0; j < NJ; j++) s[j] *= sw;
         // (a tile's sums are added while the matrix cores work on the next ones)
         constexpr int kLag = 2;
         f32x4 p[kLag + 1];
@@ -412,6 +413,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tiles(Fp8Tiles f) {
             if (t < NI * NJ) p[t % (kLag + 1)] = multiply(fw[i], fx[j % kFx]);
             if (t >= kLag) {
                 const int u = (t - kLag) % NI, v = (t - kLag) / NI;
+                if (u == 0) s[v] *= sw;
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[u][v][e] = fmaf(p[(t - kLag) % (kLag + 1)][e], s[v], acc[u][v][e]);
                 asm volatile("" : "+v"(acc[u][v]));        // (here, and not behind the last product, where every tile's would wait in registers)

@@ -139,6 +139,8 @@ __device__ __forceinline__ void store_state(float* p, const float (&h)[S]) {
 
 // A wave takes 64 channels of an entry, 16 at a time with their states' loads side by side (NB 4), or 16 (NB 1, while there are too few waves
 // for the device otherwise).  With NB 4 each lane of a quad does one of the four channels' softplus and gate.
+// Bound by the states' bytes, read and written once: 1,000 entries of 1,536 channels of 16, 206 MB, 33 us in a row of calls on the same states
+// (in part from cache) and 46 where states change from call to call (4.5 TB/s; a large copy moves 5.2).  One entry is the launch, 3.3 us.
 template <typename T, int S, int NB>
 __global__ __launch_bounds__(kBlock) void k_scan_step(ScanArgs a) {
     constexpr int N = 4 * S, kWide = 16 * NB;
@@ -493,10 +495,13 @@ __global__ __launch_bounds__(kBlock) void k_scan_run(ScanArgs a) {
 // the same joining as of the states, from the other end.  k_scan_grad_pieces makes l_p, S_p and r_p, going forward (r_p = sum of
 // dy_t C_t e^((s_t0 + ... + s_t) a)).  k_scan_grad_run then goes through a piece forward, keeping the states every L tokens, and backward over
 // these, L at a time: once more forward with the powers and e^(s a) h_(t-1) of all L tokens in registers, then backward.
+//
+// Bound by the vector unit as well: k_scan_grad_run issues 135 vector instructions for a token of 16 channels of 16 parts, a fifth of them to sum dB
+// and dC over channels.  8,192 tokens of 1,536 channels in bf16: pieces 71 us, joining 18, k_scan_grad_run 236, the sums over workgroups and
+// pieces 9 (the bytes alone would take 35).
 
-// Pieces are as long as scan_chunk's, or (SHORT) of 16 tokens in calls too small to fill the device with those.
-constexpr int kShort = 16;
-template <int S, bool SHORT> constexpr int kGradPiece = SHORT ? kShort : kPiece<S>;
+// Pieces are as long as scan_chunk's, or (SHORT) half of that in calls too small to fill the device with those.
+template <int S, bool SHORT> constexpr int kGradPiece = SHORT ? kPiece<S> / 2 : kPiece<S>;
 
 struct GradArgs {
     ScanArgs a;                // in: the first states; states: null
@@ -891,6 +896,7 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_rows(GradArgs ga) {
     if (t >= r.rows) return;
     const uint32_t gr = e / wide, i = e % wide;
     float v = 0.0f;
+#pragma unroll 4
     for (uint32_t p = 0; p < ga.parts_g; p++) v += ga.bc[((size_t)(gr * ga.parts_g + p) * r.rows + t) * wide + i];
     if (i < r.n) ((T*)ga.g.db)[(int64_t)t * ga.g.db_stride + gr * r.n + i] = (T)v;
     else ((T*)ga.g.dc)[(int64_t)t * ga.g.dc_stride + gr * r.n + i - r.n] = (T)v;
@@ -987,6 +993,7 @@ uint64_t chunk_floats(const redukt_scan_rows& a, uint32_t n_seq) { return chunk_
 
 struct GradPlan {
     uint32_t piece, per, parts_g, parts;
+    bool small;
     uint64_t pieces, bc, tok, bytes;
 };
 
@@ -994,7 +1001,11 @@ GradPlan grad_plan(const redukt_scan_rows& a, uint32_t n_seq) {
     GradPlan p;
     const uint32_t blocks = (a.channels / a.groups + kBlockCh - 1) / kBlockCh;
     p.piece = piece_rows(a.n);
-    if (((uint64_t)a.rows / p.piece + n_seq) * blocks * a.groups < 768) p.piece = kShort;
+    // Shorter pieces while there are less than one and a half workgroups a CU of the others (us with short and long ones: 512 tokens of
+    // 1,536 channels, 216 workgroups, 43.8 and 52.4; four segments of 1,030 in all and 768 channels, 240, 49.9 and 55.3; 2,048 of 768, 396, 73.9
+    // and 74.0; the four segments of 1,536, 480, 79.0 and 70.8).
+    p.small = ((uint64_t)a.rows / p.piece + n_seq) * blocks * a.groups < 384;
+    if (p.small) p.piece /= 2;
     p.pieces = (uint64_t)a.rows / p.piece + n_seq + 2;
     // A workgroup takes up to four blocks of channels one after the other, whose dB and dC it adds, while there are workgroups enough without.
     p.per = 4;
@@ -1022,7 +1033,8 @@ int32_t redukt_op_scan_step(const redukt_scan_rows* a, float* states, uint32_t n
     if (a->rows == 0) return BACKEND_OK;
     if (!rows_ok(a, true) || !layer_ok(a) || !states || !op_aligned(states, 16) || !op_aligned(slots, 4)) return BACKEND_INVALID_ARGUMENT;
     if (n_slots >= (1u << 31) || (!slots && a->rows > n_slots)) return BACKEND_INVALID_ARGUMENT;
-    const bool few = (uint64_t)a->rows * ((a->channels + 63) / 64) < 2048;
+    // (us with 16 and 64 channels a wave, 1,536 channels: 20 entries 5.6 and 6.1, 40 5.1 and 4.7, 400 22.8 and 16.3)
+    const bool few = (uint64_t)a->rows * ((a->channels + 63) / 64) < 768;
     const uint32_t wide = few ? 16 : 64;
     const uint64_t grid = ((uint64_t)a->rows * ((a->channels + wide - 1) / wide) + 3) / 4;
     if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
@@ -1108,15 +1120,14 @@ int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* 
     k.tok = k.back + states;
     k.bc = k.tok + round4(p.tok);
     k.per = p.per, k.parts = p.parts, k.parts_g = p.parts_g;
-    const bool small = p.piece == kShort;
     if (a->rows > p.piece) {
-        const void* const fn = small ? SCAN_FN(k.a.r, k_scan_grad_pieces, true) : SCAN_FN(k.a.r, k_scan_grad_pieces, false);
+        const void* const fn = p.small ? SCAN_FN(k.a.r, k_scan_grad_pieces, true) : SCAN_FN(k.a.r, k_scan_grad_pieces, false);
         int32_t rc = op_launch(fn, dim3((uint32_t)(p.pieces * blocks)), dim3(kBlock), 0, stream, k);
         if (rc == BACKEND_OK && k.a.joined && n_seq)
-            rc = op_launch(small ? grad_join_fn<true>(a->n) : grad_join_fn<false>(a->n), dim3((uint32_t)(n_seq * joins), 2), dim3(kOpWave), 0, stream, k);
+            rc = op_launch(p.small ? grad_join_fn<true>(a->n) : grad_join_fn<false>(a->n), dim3((uint32_t)(n_seq * joins), 2), dim3(kOpWave), 0, stream, k);
         if (rc != BACKEND_OK) return rc;
     }
-    int32_t rc = op_launch(small ? SCAN_FN(k.a.r, k_scan_grad_run, true) : SCAN_FN(k.a.r, k_scan_grad_run, false), dim3((uint32_t)(p.pieces * p.parts)), dim3(kBlock), 0,
+    int32_t rc = op_launch(p.small ? SCAN_FN(k.a.r, k_scan_grad_run, true) : SCAN_FN(k.a.r, k_scan_grad_run, false), dim3((uint32_t)(p.pieces * p.parts)), dim3(kBlock), 0,
                            stream, k);
     if (rc == BACKEND_OK && a->rows) {
         const void* const fn = a->dtype == REDUKT_OP_BF16  ? (const void*)k_scan_grad_rows<__bf16>
