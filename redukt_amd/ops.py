@@ -1,12 +1,14 @@
 """Operators of libredukt_gpu.so on the caller's own device tensors (include/redukt_ops.h).
 
-The gated delta rule for one token (`delta_step`) and for whole sequences (`delta_chunk`), int8
+The gated delta rule for one token (`delta_step`) and for whole sequences (`delta_chunk`), the
+selective scan likewise (`scan_step`, `scan_chunk`) and its gradients (`scan_grad`, `scan`), int8
 codes of activation rows (`quantize_rows`) and the product of codes with a scale per token and
-channel (`int8_matmul`).  Arguments are torch tensors on one GPU; work is queued on torch's
+channel (`int8_matmul`), e4m3 codes with a scale for blocks of 128 (`quantize_blocks`) and their
+product (`fp8_matmul`), and tokens drawn from logits (`sample`).  Arguments are torch tensors on one GPU; work is queued on torch's
 current stream of that GPU, or on `stream`, a hipStream_t's value.  Outputs and workspaces that a
 call allocates belong to torch's current stream, so for another one they are passed in, and the
 caller keeps all tensors until that stream is done with them.  Outputs overlap no input (but a state
-pool its own next states).  No model needs to be open.  The operators have no gradients: tensors
+pool its own next states).  No model needs to be open.  The operators but `scan` have no gradients: tensors
 that ask for one, states and outputs among them, are refused while torch records them, and tensors
 with a tangent always.  Wrong arguments raise `ffi.BackendError` (INVALID_ARGUMENT) and launch
 nothing; there is no CPU fallback.
