@@ -432,7 +432,8 @@ def scan_step(x, dt, a, b, c, states, d=None, z=None, dt_bias=None, slots=None, 
     channels, size] float32.  z, d and dt_bias may be left out.  size is 8, 16, 32 or 64; with several
     groups each has a multiple of 64 channels.  Entry i steps slot slots[i] (int32; None: slot i); -1 leaves
     entry i's output and state as they are; a slot out of range, or named by an earlier entry, gives NaN
-    outputs and touches no state.  Returns out [n, channels] (allocated if None); rows may be strided.
+    outputs and touches no state.  Returns out [n, channels] (allocated if None); rows may be strided, a and states
+    begin on 16 bytes.
     """
     op = "scan_step"
     allocates = out is None
@@ -583,7 +584,9 @@ class _Scan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in):
         final = torch.empty((max(cu_seqlens.shape[0] - 1, 0),) + tuple(a.shape), dtype=torch.float32, device=x.device)
-        out = scan_chunk(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in, final)
+        # (a row of no sequence is a zero: what is left out of a loss by a factor of 0 may not be NaN)
+        out = torch.zeros_like(x, memory_format=torch.contiguous_format)
+        scan_chunk(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in, final, out=out)
         ctx.save_for_backward(x, dt, a, b, c, cu_seqlens, d, z, dt_bias, state_in)
         ctx.set_materialize_grads(False)
         return out, final
@@ -601,9 +604,9 @@ class _Scan(torch.autograd.Function):
 
 def scan(x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_in=None):
     """`scan_chunk` for training: (out, final states), from the states state_in [sequences, channels, size]
-    (None: zeros), with gradients for every floating-point input (once; tangents are refused).  Every row
-    belongs to a sequence, or its output is unspecified.  On torch's current stream; the backward pass runs `scan_grad`
-    on the stream of the forward pass.
+    (None: zeros), with gradients for every floating-point input (once; tangents are refused).  Rows of no
+    sequence have outputs and gradients of zero.  On torch's current stream; the backward pass runs `scan_grad`
+    on the stream of the forward pass.  To capture it, let no graph of an eager pass over the same leaves live.
     """
     op = "scan"
     _device(op, x)
@@ -832,7 +835,7 @@ def sample(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None, out=N
             return none, per_row(name, v, dtype)
         try:
             return (min(max(int(v), -1), 2 ** 31 - 1) if dtype is torch.int32 else float(v)), None
-        except (TypeError, ValueError):
+        except (OverflowError, TypeError, ValueError):
             _refuse(f"{op}: {name} is a number or a tensor [rows]")
 
     f32 = torch.float32

@@ -513,6 +513,78 @@ def test_scan_notices_what_was_overwritten():
         out.sum().backward()
 
 
+def test_scan_of_a_padded_batch():
+    """Rows of no sequence: zeros, with gradients of zero, whatever was in the memory and is in their inputs."""
+    lens, before, behind, ch = [70, 0, 9], 3, 40, 48
+    T = before + sum(lens) + behind
+    x = layer(T, ch, 16, 1, F32)
+    live = slice(before, before + sum(lens))
+    for k in ("x", "dt", "z", "b", "c"):
+        x[k][:before] = x[k][live.stop:] = float("nan")
+    filler = torch.full((T, ch), float("nan"), device="cuda")
+    del filler                               # (its memory is likely the output's)
+    leaves = {k: v.clone().requires_grad_() for k, v in x.items()}
+    out, _ = ops.scan(cu_seqlens=cu_of(lens, before), **leaves)
+    assert (out[:before] == 0).all() and (out[live.stop:] == 0).all()
+    assert torch.equal(out[live], ops.scan_chunk(cu_seqlens=cu_of(lens), **rows_of(x, live)))
+    mask = torch.zeros(T, 1, device="cuda")
+    mask[live] = 1.0
+    (out * mask).square().sum().backward()
+    for k, v in leaves.items():
+        assert v.grad.isfinite().all(), k
+        if k in ("x", "dt", "z", "b", "c"):
+            assert (v.grad[:before] == 0).all() and (v.grad[live.stop:] == 0).all(), k
+
+
+def test_scan_captured_with_its_backward_pass():
+    """Leaves that no eager pass has seen; every replay against the operators themselves."""
+    lens = [150, 1, 40]
+    T, ch = sum(lens), 64
+    x = layer(T, ch, 16, 1, F32)
+    cu, dout = cu_of(lens), torch.randn(T, ch, device="cuda")
+    names = [k for k in GRADS if k != "state_in"]
+    leaves = {k: x[k].clone().requires_grad_() for k in names}
+    ops.scan_grad(dout, cu_seqlens=cu, **x)  # (kernels are loaded by their first call)
+    ops.scan_chunk(cu_seqlens=cu, **x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, last = ops.scan(cu_seqlens=cu, **leaves)
+        grads = torch.autograd.grad([out], [leaves[k] for k in names], [dout])
+    for i in range(4):
+        with torch.no_grad():
+            leaves["x"].normal_(), leaves["b"].normal_(), dout.normal_()
+        g.replay()
+        torch.cuda.synchronize()
+        now = {k: v.detach() for k, v in leaves.items()}
+        final = torch.empty_like(last)
+        assert torch.equal(out.detach(), ops.scan_chunk(cu_seqlens=cu, state_out=final, **now)) and torch.equal(last.detach(), final), i
+        want = ops.scan_grad(dout, cu_seqlens=cu, **now)
+        assert all(torch.equal(p, getattr(want, k)) for k, p in zip(names, grads)), i
+
+
+def test_scan_on_two_streams_at_once():
+    lens = [2100, 300]
+    T, ch, n = sum(lens), 200, 16
+    both = []
+    for seed in (1, 2):
+        x = layer(T, ch, n, 1, BF16, seed=seed)
+        dout = torch.randn(T, ch, generator=gen(seed + 20), device="cuda").to(BF16)
+        want = ops.scan_grad(dout, cu_seqlens=cu_of(lens), **x)
+        both.append((x, dout, cu_of(lens), ops.scan_chunk(cu_seqlens=cu_of(lens), **x), want, torch.zeros(T, ch, dtype=BF16, device="cuda"),
+                     ops.ScanGrads(*(None if g is None else torch.zeros_like(g) for g in want)),
+                     torch.empty(ops.scan_chunk_workspace(T, 2, ch, 1, n), dtype=torch.uint8, device="cuda"),
+                     torch.empty(ops.scan_grad_workspace(T, 2, ch, 1, n), dtype=torch.uint8, device="cuda"), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x, dout, cu, _, _, out, grads, work, back, on in both:
+            ops.scan_chunk(cu_seqlens=cu, out=out, workspace=work, stream=on.cuda_stream, **x)
+            ops.scan_grad(dout, cu_seqlens=cu, grads=grads, workspace=back, stream=on.cuda_stream, **x)
+    torch.cuda.synchronize()
+    for _, _, _, first, want, out, grads, *_ in both:
+        assert torch.equal(out, first) and all(p is None and q is None or torch.equal(p, q) for p, q in zip(want, grads))
+
+
 def test_a_prompt_and_the_tokens_after_it():
     """scan_chunk, then scan_step from the states that it left."""
     ch, n, T = 96, 16, 200

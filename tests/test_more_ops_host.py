@@ -421,3 +421,9 @@ def test_drawing_by_hand():
     assert f64.draw(l, 0.999) == 3 and f64.draw(l, 0.3, top_k=1) == 1 and f64.draw(l, 0.6, top_k=2) == 3
     assert f64.draw(l, 0.3, temperature=0.0) == 1 and f64.draw([float("-inf")] * 3, 0.5) == -1
     assert f64.draw(l, 0.99, top_p=0.3) == 1 and f64.draw(l, 0.99, min_p=0.5) == 3
+
+
+def test_settings_that_are_no_numbers_are_refused(recorded):
+    for over in (dict(top_k=float("inf")), dict(top_k=float("nan")), dict(temperature=10 ** 400), dict(top_p="half"), dict(min_p=[0.1])):
+        refused(lambda: ops.sample(torch.zeros(3, 9), torch.zeros(3), out=torch.zeros(3, dtype=torch.int32), **over))
+    assert not recorded.calls
