@@ -303,7 +303,7 @@ static_assert(sizeof(Ordered) <= kBins * 8, "");
 // Where everything that may be kept is in the list (n elements, none further than `reach` below the largest; top_k and top_p of them, `all` the
 // sum that top_p is of if top_k keeps all).  Elements go to 256 bins by value, and within a bin each looks at the others for its place.  From there
 // one wave goes on without waiting for others: sums along the order say who is kept, their weights go to 256 bins by index, and the bin that the
-// limit falls into is looked through.  (Each element against all others took 5 us with 150 of them, 100 with 1,000.)
+// limit falls into is looked through.  (1,000 rows of 1,000 logits by workgroups of 256: 21 us, with each element against all others 130.)
 template <int THREADS>
 __device__ __forceinline__ void draw_listed(SampleLds<THREADS>& l, const Scale& m, uint32_t n, float reach, uint32_t vocab, uint64_t top_k, bool by_p, double top_p,
                                             uint64_t all, uint64_t least, float u, int32_t* token) {
@@ -418,16 +418,17 @@ __device__ __forceinline__ uint32_t coarse_bin(SampleLds<THREADS>& l, uint32_t t
     return l.bin;
 }
 
-// HELD: sweeps whose loads go out together, which cover the row; 0: one after the other.
+// HELD: sweeps whose loads go out together; WHOLE: they cover the row.
 //
 // With top_k the way is short.  Each thread has the largest of its logits; the top_k-th logit is no further down than the top_k-th of
 // these, and there are few others so far up: they are listed and put in order.  A row is read once, and of it again what the threads read
 // that have such a logit.
-// Bound by the steps of a row, one workgroup a CU: 50,280 logits in f32 take 24,000 cycles, 5,700 of them to read the row, 3,400 for its largest
-// values, 6,000 to list what may be kept, 8,000 to order it and draw.  One row 10.5 us, 1,000 in bf16, 100 MB, 51 (2 TB/s).  Without top_k all
-// weights are formed, in 64 bits: 1,000 rows 103 us, and with top_p, whose sums by bin are atomics in LDS, 275.
-template <typename T, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
+// Bound by the steps of a row, one after the other: 50,280 logits in f32 take 1,024 threads 24,000 cycles, 5,700 of them to read the row, 3,400 for
+// its largest values, 6,000 to list what may be kept, 8,000 to order it and draw.  One row 10.5 us; 1,000 in bf16, 100 MB, two workgroups a CU, 38
+// (2.6 TB/s), in f32 61 (3.3).  Without top_k all weights are formed, in 64 bits: 1,000 rows 81 us, and with top_p, whose sums by bin are atomics
+// in LDS, 220.
+template <typename T, int THREADS, int HELD, bool WHOLE>
+__global__ __launch_bounds__(THREADS, 4) void k_sample(SampleArgs s) {
     typedef Row<T, THREADS> R;
     constexpr int VEC = R::VEC, kWaves = THREADS / kOpWave;
     __shared__ SampleLds<THREADS> l;
@@ -442,20 +443,17 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     const float top_p = a.top_ps ? a.top_ps[r] : a.top_p, min_p = a.min_ps ? a.min_ps[r] : a.min_p;
 
     float mine = -__builtin_inff();
-    typename R::vec held[HELD ? HELD : 1];
-    const auto fold = [&](const typename R::vec& v) {
-#pragma unroll
-        for (int e = 0; e < VEC; e++) mine = (float)v[e] > mine ? (float)v[e] : mine;        // (NaN is none)
-    };
-    if constexpr (HELD > 0) {
+    for (uint32_t s0 = 0; s0 < (WHOLE ? 1 : row.sweeps); s0 += HELD) {
+        typename R::vec held[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; i++)
-            if ((uint32_t)i < row.sweeps) held[i] = row.load(i);
+            if (s0 + i < row.sweeps) held[i] = row.load(s0 + i);
 #pragma unroll
         for (int i = 0; i < HELD; i++)
-            if ((uint32_t)i < row.sweeps) fold(held[i]);
-    } else {
-        row.each([&](uint32_t, uint32_t, const typename R::vec& v) { fold(v); });
+            if (s0 + i < row.sweeps) {
+#pragma unroll
+                for (int e = 0; e < VEC; e++) mine = (float)held[i][e] > mine ? (float)held[i][e] : mine;        // (NaN is none)
+            }
     }
     Scale m;
     m.most = mine;
@@ -488,71 +486,69 @@ __global__ __launch_bounds__(THREADS) void k_sample(SampleArgs s) {
     const bool by_k = top_k > 0 && (uint32_t)top_k < a.vocab, by_p = top_p < 1.0f, by_min = min_p > 0.0f;
     const uint64_t least = by_min ? (uint64_t)__builtin_ceil((double)fminf(min_p, 1.0f) * kOne) : 1;       // (the limit is exact, and weights are whole)
 
-    if constexpr (HELD > 0) {
-        if (by_k && top_k <= (int)kFewK) {
-            for (uint32_t i = threadIdx.x; i < kCoarse; i += THREADS) l.count[i] = 0;
-            if (threadIdx.x == 0) l.listed = 0;
+    if (by_k && top_k <= (int)kFewK) {
+        for (uint32_t i = threadIdx.x; i < kCoarse; i += THREADS) l.count[i] = 0;
+        if (threadIdx.x == 0) l.listed = 0;
+        __syncthreads();
+        if (m.live(mine)) atomicAdd(&l.count[m.bin(mine) / (kBins / kCoarse)], 1u);
+        __syncthreads();
+        const uint32_t bin = coarse_bin(l, (uint32_t)top_k, lane);
+        if (bin < kCoarse) {
+            // (what is a little further down may be listed too, but nothing less: the bin's end as a logit, with room for roundings)
+            float from = m.most - (float)((bin + 1) * (kBins / kCoarse)) / m.bins * 1.0001f;
+            if (!(from < m.most)) from = m.most;
+            // The threads that have one, and then all threads over what those read: a row's other logits are not looked at again.
+            if (threadIdx.x == 0) l.kept = 0;
             __syncthreads();
-            if (m.live(mine)) atomicAdd(&l.count[m.bin(mine) / (kBins / kCoarse)], 1u);
+            uint32_t* const who = (uint32_t*)l.sorted;
+            const uint64_t some = __ballot(mine >= from);
+            uint32_t to = 0;
+            if (lane == 0 && some) to = atomicAdd(&l.kept, (uint32_t)__popcll(some));
+            to = from_lane(to, 0) + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
+            if (mine >= from) who[to] = threadIdx.x;
             __syncthreads();
-            const uint32_t bin = coarse_bin(l, (uint32_t)top_k, lane);
-            if (bin < kCoarse) {
-                // (what is a little further down may be listed too, but nothing less: the bin's end as a logit, with room for roundings)
-                float from = m.most - (float)((bin + 1) * (kBins / kCoarse)) / m.bins * 1.0001f;
-                if (!(from < m.most)) from = m.most;
-                // The threads that have one, and then all threads over what those read: a row's other logits are not looked at again.
-                if (threadIdx.x == 0) l.kept = 0;
-                __syncthreads();
-                uint32_t* const who = (uint32_t*)l.sorted;
-                const uint64_t some = __ballot(mine >= from);
-                uint32_t to = 0;
-                if (lane == 0 && some) to = atomicAdd(&l.kept, (uint32_t)__popcll(some));
-                to = from_lane(to, 0) + __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
-                if (mine >= from) who[to] = threadIdx.x;
-                __syncthreads();
-                constexpr uint32_t kAbreast = THREADS / 4;
-                const uint32_t many = l.kept;
-                for (uint32_t j0 = 0; j0 < many; j0 += kAbreast) {
-                    const uint32_t j = j0 + threadIdx.x % kAbreast, first = who[min(j, many - 1)] * VEC;
-                    // (four loads at once, in a row's first part where they would pass its end)
-                    for (uint32_t s0 = wave * kOpWave / kAbreast; s0 < row.sweeps; s0 += 16) {
-                        typename R::vec v[4];
-                        uint32_t i[4], hits = 0;
-                        const bool vectors = row.aligned && a.vocab >= (uint32_t)VEC;
+            constexpr uint32_t kAbreast = THREADS / 4;
+            const uint32_t many = l.kept;
+            for (uint32_t j0 = 0; j0 < many; j0 += kAbreast) {
+                const uint32_t j = j0 + threadIdx.x % kAbreast, first = who[min(j, many - 1)] * VEC;
+                // (four loads at once, in a row's first part where they would pass its end)
+                for (uint32_t s0 = wave * kOpWave / kAbreast; s0 < row.sweeps; s0 += 16) {
+                    typename R::vec v[4];
+                    uint32_t i[4], hits = 0;
+                    const bool vectors = row.aligned && a.vocab >= (uint32_t)VEC;
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            i[k] = (s0 + 4 * k) * R::kSweep + first;
-                            if (vectors) v[k] = *(const typename R::vec*)(row.p + (i[k] + VEC <= a.vocab ? i[k] : 0));
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            if (!vectors || i[k] + VEC > a.vocab) v[k] = row.at(min(i[k], a.vocab));      // (-inf behind the row)
-#pragma unroll
-                            for (int e = 0; e < VEC; e++) hits += (float)v[k][e] >= from;
-                        }
-                        if (j >= many) hits = 0;
-                        // (places in the list for a whole wave at once: an atomic a logit costs more than all else here)
-                        const uint32_t upto = wave_upto(hits), all = from_lane(upto, kOpWave - 1);
-                        uint32_t at = 0;
-                        if (lane == 0 && all) at = atomicAdd(&l.listed, all);
-                        at = from_lane(at, 0) + upto - hits;
-                        if (!hits || at + hits > kList) continue;
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-#pragma unroll
-                            for (int e = 0; e < VEC; e++)
-                                if ((float)v[k][e] >= from) l.list[at++].order = order_of(key_of((float)v[k][e]), i[k] + e);
+                    for (int k = 0; k < 4; k++) {
+                        i[k] = (s0 + 4 * k) * R::kSweep + first;
+                        if (vectors) v[k] = *(const typename R::vec*)(row.p + (i[k] + VEC <= a.vocab ? i[k] : 0));
                     }
-                }
-                __syncthreads();
-                const uint32_t n = l.listed;
-                if (n <= kList) {
-                    draw_listed(l, m, n, m.most - from, a.vocab, (uint64_t)top_k, by_p, (double)top_p, 0, least, u, a.tokens + r);
-                    return;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (!vectors || i[k] + VEC > a.vocab) v[k] = row.at(min(i[k], a.vocab));      // (-inf behind the row)
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) hits += (float)v[k][e] >= from;
+                    }
+                    if (j >= many) hits = 0;
+                    // (places in the list for a whole wave at once: an atomic a logit costs more than all else here)
+                    const uint32_t upto = wave_upto(hits), all = from_lane(upto, kOpWave - 1);
+                    uint32_t at = 0;
+                    if (lane == 0 && all) at = atomicAdd(&l.listed, all);
+                    at = from_lane(at, 0) + upto - hits;
+                    if (!hits || at + hits > kList) continue;
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+#pragma unroll
+                        for (int e = 0; e < VEC; e++)
+                            if ((float)v[k][e] >= from) l.list[at++].order = order_of(key_of((float)v[k][e]), i[k] + e);
                 }
             }
             __syncthreads();
+            const uint32_t n = l.listed;
+            if (n <= kList) {
+                draw_listed(l, m, n, m.most - from, a.vocab, (uint64_t)top_k, by_p, (double)top_p, 0, least, u, a.tokens + r);
+                return;
+            }
         }
+        __syncthreads();
     }
     Cut cut{0, ~0u};                           // everything
     if (by_k || by_p) {
@@ -684,12 +680,14 @@ template <typename T>
 int32_t launch(SampleArgs& k, void* stream) {
     constexpr int VEC = 16 / sizeof(T);
     const uint32_t v = k.a.vocab;
-    // A thread has at least a few loads of a row, but no fewer than 256 threads share one; up to 64 logits a thread stay in registers.
-    const uint32_t threads = v <= 4096 ? 256 : 1024, sweeps = (v + threads * VEC - 1) / (threads * VEC);
+    // With more rows than CUs two workgroups share one, and one works while the other waits for its single wave (us with 1,024 and 512 threads:
+    // 200 rows of 50,280 in bf16 13.8 and 15.2, 300 24.5 and 17.9, 1,000 53 and 38, 1,000 of 1,000 40 and 21; one row in f32 10.5 and 12.6).
+    // A row's loads go out all at once where 16 vectors of a thread cover it (64 registers; in f32 32 of them spill), else by turns.
+    const uint32_t threads = k.a.rows <= 256 ? 1024 : 512, sweeps = (v + threads * VEC - 1) / (threads * VEC);
     if (!op_grid_ok(k.a.rows, threads)) return BACKEND_INVALID_ARGUMENT;
-    const void* const fn = threads == 256         ? (const void*)k_sample<T, 256, 16 / VEC>
-                           : sweeps <= 64u / VEC ? (const void*)k_sample<T, 1024, 64 / VEC>
-                                                 : (const void*)k_sample<T, 1024, 0>;
+    const void* const fn = threads == 1024 ? sweeps <= 64u / VEC ? (const void*)k_sample<T, 1024, 64 / VEC, true> : (const void*)k_sample<T, 1024, 64 / VEC, false>
+                           : sweeps <= 16  ? (const void*)k_sample<T, 512, 16, true>
+                                           : (const void*)k_sample<T, 512, 64 / VEC, false>;
     return op_launch(fn, dim3(k.a.rows), dim3(threads), sweeps * (threads / kOpWave) * 8, stream, k);
 }
 

@@ -159,6 +159,26 @@ def test_sample_large_vocabularies(vocab, dtype):
         same(x, uniform(2), **s)
 
 
+@types
+@pytest.mark.parametrize("vocab", [1, 7, 1000, 5003, 50280, 70001, 131072])
+def test_sample_of_few_rows_and_of_many(vocab, dtype):
+    """A row's token does not depend on how many there are: masked rows, ties and nearly equal values, strided as well."""
+    rows, times = 8, 40
+    wide = logits_of(rows, vocab + 8, dtype, seed=vocab)
+    x = wide[:, :vocab]
+    x[1] = -INF
+    x[2, ::2] = -INF
+    x[3] = 1.5
+    x[4] = torch.linspace(1.0, 1.01, vocab, device="cuda").to(dtype)
+    x[5, ::3] = NAN
+    for i, s in enumerate(SETTINGS):
+        u = uniform(rows, seed=i)
+        few = ops.sample(x, u, **s)
+        many = ops.sample(wide.repeat(times, 1)[:, :vocab] if i % 2 else x.repeat(times, 1), u.repeat(times), **s)
+        assert torch.equal(many, few.repeat(times)), s
+        assert few.tolist() == drawn(x, u, **s) or vocab > 5003, s
+
+
 def test_sample_offsets_past_32_bits():
     rows, vocab = 70000, 1 << 15
     x = torch.full((rows, vocab), -INF, dtype=BF16, device="cuda")
