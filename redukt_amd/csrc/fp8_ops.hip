@@ -412,6 +412,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_fp8_tiles(Fp8Tiles f) {
             const int i = t % NI, j = t / NI;
             if (i == 0 && j + kFx - 1 < NJ) fx[(j + kFx - 1) % kFx] = load(x, rj + 16 * (j + kFx - 1));
             if (t < NI * NJ) p[t % (kLag + 1)] = multiply(fw[i], fx[j % kFx]);
+            __builtin_amdgcn_sched_barrier(0);                 // (the product first: left to itself, the compiler lets it wait for the sums of the one before)
             if (t >= kLag) {
                 const int u = (t - kLag) % NI, v = (t - kLag) / NI;
                 if (u == 0) s[v] *= sw;
