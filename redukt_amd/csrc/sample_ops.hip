@@ -426,7 +426,7 @@ __device__ __forceinline__ uint32_t coarse_bin(SampleLds<THREADS>& l, uint32_t t
 // Bound by the steps of a row, one after the other: 50,280 logits in f32 take 1,024 threads 24,000 cycles, 5,700 of them to read the row, 3,400 for
 // its largest values, 6,000 to list what may be kept, 8,000 to order it and draw.  One row 10.5 us; 1,000 in bf16, 100 MB, two workgroups a CU, 38
 // (2.6 TB/s), in f32 61 (3.3).  Without top_k all weights are formed, in 64 bits: 1,000 rows 81 us, and with top_p, whose sums by bin are atomics
-// in LDS, 220.
+// in LDS, 211.
 template <typename T, int THREADS, int HELD, bool WHOLE>
 __global__ __launch_bounds__(THREADS, 4) void k_sample(SampleArgs s) {
     typedef Row<T, THREADS> R;
@@ -581,13 +581,17 @@ __global__ __launch_bounds__(THREADS, 4) void k_sample(SampleArgs s) {
         // What may be kept, if it fits the list.
         const uint32_t bin = l.bin;
         row.each([&](uint32_t, uint32_t i0, const typename R::vec& v) {
+            uint32_t hits = 0;                 // (places for a whole wave at once, as above)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float x = (float)v[e];
-                if (!(m.place(x) < (float)(bin + 1))) continue;
-                const uint32_t at = atomicAdd(&l.listed, 1u);
-                if (at < kList) l.list[at].order = order_of(key_of(x), i0 + e);
-            }
+            for (int e = 0; e < VEC; e++) hits += m.place((float)v[e]) < (float)(bin + 1);
+            const uint32_t upto = wave_upto(hits), all = from_lane(upto, kOpWave - 1);
+            uint32_t at = 0;
+            if (lane == 0 && all) at = atomicAdd(&l.listed, all);
+            at = from_lane(at, 0) + upto - hits;
+            if (!hits || at + hits > kList) return;
+#pragma unroll
+            for (int e = 0; e < VEC; e++)
+                if (m.place((float)v[e]) < (float)(bin + 1)) l.list[at++].order = order_of(key_of((float)v[e]), i0 + e);
         });
         __syncthreads();
         if (l.listed <= kList) {
