@@ -93,13 +93,14 @@ struct Row {
 
 // The row's measure: what its values mean once the largest one is known.
 struct Scale {
-    float most;
-    float bins;                // bins a unit of logits
+    float most, half;          // the largest, and half of it
+    float bins;                // bins a unit of logits, at most half of f32's range (of less than a T of 2e-37; what weighs anything is below 30 T)
+    float half_bins;           // twice that: bins a unit of half logits
     double steps;              // kPowers log2(e) / T: steps of 2^(1 / kPowers) a unit of logits
     const double* powers;
     // Where l is below the largest, in bins: falls with l, and is below kBins for all that weigh anything (kLeast leaves 6 bins to
-    // spare for the rounding).  NaN and -inf are nowhere.
-    __device__ __forceinline__ float place(float l) const { return l == most ? 0.0f : (most - l) * bins; }
+    // spare for the rounding).  NaN and -inf are nowhere.  It goes by half of the difference, which has no overflow.
+    __device__ __forceinline__ float place(float l) const { return l == most ? 0.0f : fmaf(l, -0.5f, half) * half_bins; }
     __device__ __forceinline__ bool live(float l) const { return place(l) < (float)kBins; }
     __device__ __forceinline__ uint32_t bin(float l) const { return (uint32_t)place(l); }
     // 2^42 e^((l - most) / T) to the nearest whole number, of a live l.  The power's argument in steps of 2^(1 / 128) is a whole number (added
@@ -480,7 +481,9 @@ __global__ __launch_bounds__(THREADS, 4) void k_sample(SampleArgs s) {
         return;
     }
     const double inverse = 1.0 / (double)temperature;
-    m.bins = (float)((kBins - 1) / -kLeast * inverse);
+    m.half = 0.5f * m.most;
+    m.bins = fminf((float)((kBins - 1) / -kLeast * inverse), 0x1p126f);
+    m.half_bins = 2.0f * m.bins;
     m.steps = kPowers * 0x1.71547652b82fep+0 * inverse;
     m.powers = l.powers;
     const bool by_k = top_k > 0 && (uint32_t)top_k < a.vocab, by_p = top_p < 1.0f, by_min = min_p > 0.0f;
