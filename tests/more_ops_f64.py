@@ -262,3 +262,33 @@ def draw(l, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not limit < float(total):
         limit = math.nextafter(float(total), 0.0)
     return int(next(i for i, s in zip(keep, sums) if float(s) > limit))
+
+
+def draw_fast(l, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """draw by sums of whole arrays, for long rows."""
+    l = np.asarray(l, np.float64)
+    clean = np.where(np.isnan(l), -np.inf, l)
+    if np.isneginf(clean.max()):
+        return -1
+    temperature, top_p, min_p, u = (float(np.float32(v)) for v in (temperature, top_p, min_p, u))
+    if not temperature > 0:
+        return int(np.argmax(clean))
+    l, w = weights(l, temperature)
+    keep = np.flatnonzero(w)
+    if top_k > 0 or top_p < 1.0:
+        keep = keep[np.argsort(-l[keep], kind="stable")]
+        if top_k > 0:
+            keep = keep[:top_k]
+        if top_p < 1.0:
+            sums = np.cumsum(w[keep])
+            before = sums - w[keep]
+            keep = keep[(before == 0) | (before.astype(np.float64) < top_p * float(sums[-1]))]
+    if min_p > 0.0:
+        keep = keep[w[keep].astype(np.float64) >= min(min_p, 1.0) * ONE]
+    keep = np.sort(keep)
+    sums = np.cumsum(w[keep])
+    total = float(sums[-1])
+    limit = (u if u > 0 else 0.0) * total
+    if not limit < total:
+        limit = math.nextafter(total, 0.0)
+    return int(keep[np.argmax(sums.astype(np.float64) > limit)])

@@ -1,0 +1,103 @@
+"""Every way that the sizes of a call choose through scan_grad, fp8_matmul and sample, on the GPU, against the 64-bit
+statements of tests/more_ops_f64.py.  (That the shapes here choose those ways: test_op_ways_host.py.)"""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from redukt_amd import ops  # noqa: E402
+from tests import more_ops_f64 as f64  # noqa: E402
+from tests.test_gpu_fp8_ops import check, product  # noqa: E402
+from tests.test_gpu_sample import SETTINGS, logits_of, uniform  # noqa: E402
+from tests.test_gpu_scan_ops import gradients  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+TYPES = [BF16, F16, F32]
+NAMES = {BF16: "bf16", F16: "f16", F32: "f32"}
+types = pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
+INF, NAN = float("inf"), float("nan")
+
+# ---------------------------------------------------------------- gradients of the scan
+
+# lengths, channels, groups; then by states of up to 16 parts and of more: blocks of channels that a workgroup takes, whether a launch
+# of its own joins the pieces.  None is small enough for the shorter pieces.
+GRAD_WAYS = {
+    "four-blocks": ([5] * 200 + [150, 0, 64, 65, 200], 1100, 1, ((4, False), (4, True))),
+    "four-blocks-few-rows": ([2] * 250 + [100, 64, 33, 250], 1100, 1, ((4, False), (4, False))),
+    "four-blocks-of-two-groups": ([4] * 250 + [130, 70], 768, 2, ((4, False), (4, True))),
+    "two-or-four-blocks-joined": ([1] * 450 + [1100, 130, 700, 129], 500, 1, ((2, True), (4, True))),
+    "a-block-each-joined": ([70] * 40, 640, 1, ((1, True), (1, True))),
+    "a-block-each": ([100] * 10, 1100, 1, ((1, False), (1, False))),
+}
+
+
+def grad_way(lens, ch, groups, n):
+    """(short pieces, blocks of a workgroup, joined by a launch, bytes of workspace) as scan_grad's plan has them."""
+    rows, blocks, piece = sum(lens), -(-(ch // groups) // 64), 64 if n <= 16 else 32
+    short = (rows // piece + len(lens)) * blocks * groups < 384
+    piece //= 2 if short else 1
+    pieces, per = rows // piece + len(lens) + 2, 4
+    while per > 1 and pieces * groups * -(-blocks // per) < 1024:
+        per //= 2
+    floats = pieces * ch * (3 * n + 3) + -(-blocks // per) * groups * rows * 2 * n + 12
+    return short, per, rows > 32 * piece, 4 * floats
+
+
+@types
+@pytest.mark.parametrize("n", [8, 16, 32, 64])
+def test_scan_grad_of_four_blocks_a_workgroup(n, dtype):
+    lens, ch, groups, _ = GRAD_WAYS["four-blocks"]
+    gradients(lens, ch, n, groups, dtype, before_rows=3, behind=70, seed=n)
+
+
+@pytest.mark.parametrize("i,n", enumerate([8, 16, 32, 64]))
+@pytest.mark.parametrize("j,way", enumerate(w for w in GRAD_WAYS if w != "four-blocks"))
+def test_scan_grad_ways(way, n, i, j):
+    lens, ch, groups, _ = GRAD_WAYS[way]
+    gradients(lens, ch, n, groups, TYPES[(i + j) % 3], seed=n + j)
+
+
+# ---------------------------------------------------------------- products
+
+# More blocks of 128 columns than any tile has stages, and a part of one at the end.
+DEEP = [(16, 200, 1040), (2, 20000, 656), (100, 400, 1168), (600, 1200, 1168), (600, 1700, 1168), (1000, 2100, 1168), (2048, 4096, 1040),
+        (4100, 4200, 656), (130, 257, 650)]
+
+
+@types
+@pytest.mark.parametrize("m,n,k", DEEP)
+def test_fp8_matmul_of_many_blocks(m, n, k, dtype):
+    x = product(m, n, k, seed=m + n)
+    bias = torch.randn(n, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    check(ops.fp8_matmul(*x, bias=bias, dtype=dtype), x, bias, dtype)
+
+
+# ---------------------------------------------------------------- sampling
+
+def drawn(logits, u, **settings):
+    rows = logits.float().cpu().numpy()
+    return [f64.draw_fast(rows[i], float(u[i]), **{k: v[i].item() if isinstance(v, torch.Tensor) else v for k, v in settings.items()})
+            for i in range(len(rows))]
+
+
+@types
+@pytest.mark.parametrize("vocab", [50280, 70001, 131072])
+def test_sample_of_large_vocabularies_few_rows_and_many(vocab, dtype):
+    """Masked, tied and nearly equal logits and NaN, in rows that begin at any place, for workgroups of either size."""
+    rows, times = 8, 40
+    wide = logits_of(rows, vocab + 3, dtype, seed=vocab)
+    x = wide[:, 1:vocab + 1]
+    x[1] = -INF
+    x[2, ::2] = -INF
+    x[3] = 1.5
+    x[4] = torch.linspace(1.0, 1.01, vocab, device="cuda").to(dtype)
+    x[5, ::3] = NAN
+    x[6] = torch.arange(vocab, device="cuda").remainder(7).to(dtype)
+    y = x.contiguous()
+    for i, s in enumerate(SETTINGS):
+        u = uniform(rows, seed=i)
+        want = drawn(x, u, **s)
+        for t in (x, y):
+            assert ops.sample(t, u, **s).tolist() == want, s
+            assert ops.sample(t.repeat(times, 1), u.repeat(times), **s).tolist() == want * times, s
