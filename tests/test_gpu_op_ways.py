@@ -1,4 +1,4 @@
-"""Every way that the sizes of a call choose through scan_grad, fp8_matmul and sample, on the GPU, against the 64-bit
+"""Every way that the sizes of a call choose through the scan and its gradients, fp8_matmul and sample, on the GPU, against the 64-bit
 statements of tests/more_ops_f64.py.  (That the shapes here choose those ways: test_op_ways_host.py.)"""
 import numpy as np
 import pytest
@@ -9,7 +9,7 @@ from redukt_amd import ops  # noqa: E402
 from tests import more_ops_f64 as f64  # noqa: E402
 from tests.test_gpu_fp8_ops import check, product  # noqa: E402
 from tests.test_gpu_sample import SETTINGS, logits_of, uniform  # noqa: E402
-from tests.test_gpu_scan_ops import gradients  # noqa: E402
+from tests.test_gpu_scan_ops import check as scan_check, gradients, layer, pool_of, rows_of, sequences  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -17,6 +17,43 @@ TYPES = [BF16, F16, F32]
 NAMES = {BF16: "bf16", F16: "f16", F32: "f32"}
 types = pytest.mark.parametrize("dtype", TYPES, ids=NAMES.get)
 INF, NAN = float("inf"), float("nan")
+
+# ---------------------------------------------------------------- the scan
+
+STEPS = [(45, 1100, 1), (70, 768, 2), (800, 17, 1)]        # entries, channels, groups: enough of them for 64 channels a wave
+
+
+@types
+@pytest.mark.parametrize("n", [8, 16, 32, 64])
+@pytest.mark.parametrize("rows,ch,groups", STEPS)
+def test_scan_step_of_many_channels(rows, ch, groups, n, dtype):
+    """Channels past the last whole 64, padded entries, slots out of range and named twice, states that no entry names."""
+    x = layer(rows, ch, n, groups, dtype, seed=rows + n)
+    slots = np.random.default_rng(rows).permutation(rows + 2)[:rows].astype(np.int32)
+    slots[5], slots[7], slots[8], slots[11] = -1, rows + 2, -9, slots[3]
+    pool = pool_of(rows + 2, ch, n)
+    before = pool.clone()
+    out = torch.full((rows, ch), 7.0, dtype=dtype, device="cuda")
+    ops.scan_step(states=pool, slots=torch.from_numpy(slots).cuda(), out=out, **x)
+    assert (out[5] == 7.0).all() and out[[7, 8, 11]].isnan().all()
+    named = sorted(set(range(rows)) - {5, 7, 8, 11})
+    free = sorted(set(range(rows + 2)) - {int(slots[i]) for i in named})
+    assert torch.equal(pool[free], before[free])
+    for i in named[::max(1, rows // 40)] + [named[-1]]:
+        want, h = f64.scan(h0=before[int(slots[i])], **rows_of(x, slice(i, i + 1)))
+        scan_check(out[i:i + 1], want, dtype, ("out", i))
+        scan_check(pool[int(slots[i])], h, F32, ("state", i))
+
+
+CHUNKS = [([2200, 0, 70, 3], True), ([900, 64, 1, 33], False)]      # lengths; whether a launch of its own joins the pieces
+
+
+@types
+@pytest.mark.parametrize("n", [8, 16, 32, 64])
+@pytest.mark.parametrize("lens,joined", CHUNKS, ids=["joined", "by-themselves"])
+def test_scan_chunk_of_many_pieces(lens, joined, n, dtype):
+    sequences(lens, 70, n, 1, dtype, initial=True, before_rows=2, behind=3, seed=n)
+
 
 # ---------------------------------------------------------------- gradients of the scan
 

@@ -70,6 +70,14 @@ for op, v in json.loads(sys.stdin.read()):
         dtype, m, n, k = v
         a = ops.Fp8Matmul(dtype, m, n, k, P, k, P, P, k, P, None, P, n)
         out.append(recorded(lambda: L.redukt_op_fp8_matmul(ctypes.byref(a), None)))
+    elif op == "step":
+        rows, ch, groups, n, dtype = v
+        a = ops.ScanRows(dtype, rows, ch, groups, n, P, P, P, P, P, P, ch, ch, ch, groups * n, groups * n, ch, P, P, P)
+        out.append(recorded(lambda: L.redukt_op_scan_step(ctypes.byref(a), P, rows + 2, P, None)))
+    elif op == "chunk":
+        rows, n_seq, ch, groups, n, dtype = v
+        a = ops.ScanRows(dtype, rows, ch, groups, n, P, P, P, P, P, P, ch, ch, ch, groups * n, groups * n, ch, P, P, P)
+        out.append(recorded(lambda: L.redukt_op_scan_chunk(ctypes.byref(a), P, n_seq, P, P, n_seq + 2, P, P, 1 << 40, None)))
     elif op == "grad":
         rows, n_seq, ch, groups, n, dtype = v
         a = ops.ScanRows(dtype, rows, ch, groups, n, P, P, P, P, P, None, ch, ch, ch, groups * n, groups * n, 0, P, P, P)
@@ -114,6 +122,15 @@ def test_the_products_shapes_reach_every_kernel_with_more_blocks_than_it_has_sta
         assert {fn for fn, _ in met} == {"k_fp8_tiles", "k_fp8_few", "k_fp8_bytes"}
         assert all(max(blocks) > t[4] + 1 for (fn, t), blocks in met.items() if fn == "k_fp8_tiles")
         assert len([s for s in ways.DEEP if s[2] % 128 == 0]) == 0
+
+
+def test_the_scans_shapes_choose_their_ways(launched):
+    sizes = (8, 16, 32, 64)
+    for (((name, *_),), n) in zip(launched([["step", [*s, n, 2]] for s in ways.STEPS for n in sizes]), sizes * len(ways.STEPS)):
+        assert kernel(name) == ("k_scan_step", (n // 4, 4))
+    calls = [(lens, joined, n) for lens, joined in ways.CHUNKS for n in sizes]
+    for (lens, joined, n), launches in zip(calls, launched([["chunk", [sum(l), len(l), 70, 1, n, 2]] for l, _, n in calls])):
+        assert [kernel(l[0]) for l in launches] == [(f, (n // 4,)) for f in ["k_scan_pieces"] + ["k_scan_join"] * joined + ["k_scan_run"]]
 
 
 def test_the_gradients_shapes_choose_their_ways(launched):
