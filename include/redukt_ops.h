@@ -237,9 +237,15 @@ typedef struct {
 } redukt_fp8_matmul;        /* any alignment that the element types have */
 
 /* out[i][j] = sum over blocks b of 128 columns (sum over c in b of x[i][c] * w[j][c]) *
- * (x_scales[i][b] * w_scales[j / 128][b]) + bias[j], with sums in f32 in an order that the sizes
- * choose, rounded once to `dtype`.  Fastest where x, w and their strides are multiples of 16 bytes and k is a
- * multiple of 16. */
+ * (x_scales[i][b] * w_scales[j / 128][b]) + bias[j], in an order that the sizes choose, rounded once to `dtype`.
+ * f32 outputs: every product is exact, and sums are f32's.
+ * 16-bit outputs: the products of columns 8 c to 8 c + 7 are added together, each cut off (toward zero) 13 bits
+ * below the exponent of the largest of the eight; all other sums are f32's.  Beside its rounding such an output
+ * is off by at most 7 * 2^-13 of the largest product of each eight, times the block's scales, summed over all
+ * eights.  Of random codes that is 1.5e-5 of a result; where large products of one eight cancel each other, or
+ * the bias cancels them, it can be all that the small ones beside them come to.  Ask for f32 outputs where
+ * that matters.
+ * Fastest where x, w and their strides are multiples of 16 bytes and k is a multiple of 16. */
 int32_t redukt_op_fp8_matmul(const redukt_fp8_matmul* a, void* stream);
 
 /* ---------------- drawing a token ---------------- */

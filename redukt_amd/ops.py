@@ -749,8 +749,12 @@ def quantize_blocks(x, block_rows: int = 1, codes=None, scales=None, stream: Opt
 def fp8_matmul(x, x_scales, w, w_scales, bias=None, out=None, dtype=torch.bfloat16, stream: Optional[int] = None):
     """The product of e4m3 codes x [tokens, k] and w [channels, k] with float32 scales for blocks of 128 columns,
     x_scales [tokens, ceil(k / 128)] and w_scales [ceil(channels / 128), ceil(k / 128)] (`quantize_blocks` with block_rows
-    1 and 128): out[i, j] = the sum over blocks b of (x[i] . w[j] over b) x_scales[i, b] w_scales[j // 128, b], + bias[j], in
-    float32, rounded once to `dtype` (bfloat16, float16 or float32; out's type where out is given).  Any sizes, k up to
+    1 and 128): out[i, j] = the sum over blocks b of (x[i] . w[j] over b) x_scales[i, b] w_scales[j // 128, b], + bias[j], rounded
+    once to `dtype` (bfloat16, float16 or float32; out's type where out is given).  float32 outputs are as exact as float32
+    sums of exact products.  For 16-bit outputs the products of eight neighbouring columns are added with 13 bits below the largest one's
+    exponent, and all else in float32: beside the rounding they are off by at most 7 * 2^-13 of the largest product of each
+    eight, times its scales (about 1.5e-5 of a result with random codes; more of one that large products cancel out in, for
+    which float32 outputs are the way).  Any sizes, k up to
     1,048,576; fastest where k and the strides of x and w are multiples of 16.
     """
     op = "fp8_matmul"

@@ -110,6 +110,44 @@ def test_fp8_matmul_of_many_blocks(m, n, k, dtype):
     check(ops.fp8_matmul(*x, bias=bias, dtype=dtype), x, bias, dtype)
 
 
+def any_codes(rows, k, seed):
+    """Codes of every finite value alike: products next to each other differ by up to 2^35, subnormal ones among them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    c = torch.randint(0, 254, (rows, k), generator=g, device="cuda", dtype=torch.int16)
+    return (c + (c >= 127).to(torch.int16)).to(torch.uint8).view(torch.float8_e4m3fn)      # (0x7f and 0xff are NaN)
+
+
+@types
+@pytest.mark.parametrize("m,n,k", [(5, 300, 768), (40, 300, 768), (300, 520, 784), (600, 1200, 400), (33, 70, 401)])
+def test_fp8_matmul_of_codes_of_all_sizes(m, n, k, dtype):
+    x = product(m, n, k)
+    x[0], x[2] = any_codes(m, k, 1), any_codes(n, k, 2)
+    check(ops.fp8_matmul(*x, dtype=dtype), x, None, dtype)
+
+
+@types
+@pytest.mark.parametrize("m", [3, 70, 2100])
+def test_fp8_matmul_of_large_codes_that_cancel(m, dtype):
+    """448 x 448 twice, with both signs, and small products whose sum is 6: in the same eight columns as those, where 16-bit outputs may be off
+    by what seven products are cut off by; then each of the three in an eight of its own, where nothing is."""
+    n, k = 200 if m < 2000 else 4200, 144
+    one = torch.ones(m, 2, device="cuda"), torch.ones(-(-n // 128), 2, device="cuda")
+    for apart in (1, 8):
+        for first in (0, 96, 120, 128 - 16):
+            x, w = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+            x[:, first], x[:, first + apart] = 448.0, -448.0
+            w[:, first], w[:, first + apart] = 448.0, 448.0
+            at = slice(first + 2, first + 8) if apart == 1 else slice(first + 16, first + 22)
+            x[:, at] = w[:, at] = 1.0
+            args = x.to(torch.float8_e4m3fn), one[0], w.to(torch.float8_e4m3fn), one[1]
+            got = ops.fp8_matmul(*args, dtype=dtype)
+            if dtype == F32 or apart == 8:
+                assert (got == 6.0).all(), (apart, first)
+            else:
+                check(got, args, None, dtype, first)
+                assert (got <= 6.0).all()
+
+
 # ---------------------------------------------------------------- sampling
 
 def drawn(logits, u, **settings):
