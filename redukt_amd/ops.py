@@ -611,6 +611,7 @@ def scan(x, dt, a, b, c, cu_seqlens, d=None, z=None, dt_bias=None, state_in=None
     op = "scan"
     _device(op, x)
     n = _sequences(op, x.get_device(), cu_seqlens)
+    _check(op, x.get_device(), "a", a, torch.float32, (None, None))      # (the final states take their size from it)
     if _tangents():
         with torch.no_grad():
             _no_gradients(op, x, dt, a, b, c, d, z, dt_bias, state_in)
