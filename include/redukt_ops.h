@@ -137,7 +137,8 @@ int32_t redukt_op_scan_chunk(const redukt_scan_rows* a, const int32_t* cu, uint3
                              uint64_t workspace_bytes, void* stream);
 
 /* The bytes of workspace for these rows (only the sizes are read); 0 if the sizes are not ones that
- * scan_chunk takes, or need none. */
+ * scan_chunk takes, or need none.  With pieces of 64 rows (32 from n = 32 on) at most 4 channels (n + 1) times the smaller of
+ * 2 rows / piece and rows / piece + n_seq. */
 uint64_t redukt_op_scan_chunk_workspace(const redukt_scan_rows* a, uint32_t n_seq);
 
 /* What the backward pass reads and writes beside the rows: arrays like the ones that they are gradients
@@ -159,7 +160,8 @@ typedef struct {
  * state_in [n_seq][channels][n] (NULL: zeros), dstate_out alike (NULL: zeros); `out` of the rows is not
  * read.  dstate_in (NULL: not wanted; not one of the others) takes that of the first states.  Rows of no
  * sequence get gradients of zero.  Everything is formed anew from the inputs, sums over channels, tokens
- * and sequences in f32 in a fixed order.  workspace: redukt_op_scan_grad_workspace(a, n_seq) bytes. */
+ * and sequences in f32 in a fixed order.  workspace: redukt_op_scan_grad_workspace(a, n_seq) bytes, which are about
+ * 12 channels (n + 1) for each sequence and each 64 rows (16 to 64), and 8 groups n for each row and 64 to 256 channels. */
 int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* g, const int32_t* cu, uint32_t n_seq,
                             const float* state_in, const float* dstate_out, float* dstate_in, void* workspace,
                             uint64_t workspace_bytes, void* stream);

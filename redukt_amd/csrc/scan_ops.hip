@@ -101,8 +101,9 @@ struct ScanArgs {
     const int32_t* cu;         // null: one row an entry
     uint32_t n;                // entries
     float* ws;                 // pieces: states [pieces][channels][n], then the sums of their time steps [pieces][channels]
-    uint32_t pieces;
+    uint32_t pieces;           // places in ws
     uint32_t joined;           // the first states of all pieces are in ws (k_scan_join)
+    uint32_t spread;           // which place a piece has (place_of)
 };
 
 // A lane's parts of its channel's a (times log2 e), and d and dt_bias.
@@ -232,8 +233,9 @@ struct Bounds {
 // A piece: rows [t0, t0 + len) are number `index` of `count` pieces of sequence seq, whose first one is in slot `first`.  Sequence i's pieces
 // have the slots from rows / P + i on (its first row's), so those of one are consecutive, those of the next begin after them, and
 // rows / P + n slots are enough.  len is 0 in the slot of a sequence without rows (index 0, count 0) and in unused ones (index > 0).
+// Row `begin` is the sequence's first one.
 struct Piece {
-    uint32_t seq, t0, len, index, count, first;
+    uint32_t seq, t0, len, index, count, first, begin;
 };
 
 template <int P>
@@ -245,13 +247,21 @@ __device__ __forceinline__ Piece piece_of(const Bounds& m, uint32_t slot) {
         else hi = mid - 1;
     }
     const uint32_t b = m.at(lo), e = max(m.at(lo + 1), b), first = b / P + lo;
-    Piece k{lo, 0, 0, slot - first, (e - b + P - 1) / P, first};
+    Piece k{lo, 0, 0, slot - first, (e - b + P - 1) / P, first, b};
     if (slot < first) k.index = ~0u, k.count = 0;          // (boundaries that decrease)
     if (k.index < k.count) {
         k.t0 = b + k.index * P;
         k.len = min(e - k.t0, (uint32_t)P);
     }
     return k;
+}
+
+// The place in ws of the first piece of sequence `seq`, whose first row is `begin`.  Only sequences of two pieces and more have places there, so
+// where there are many sequences they are given out by rows alone: with more than P rows a sequence's two places for each P of them are as many
+// as its pieces at least, from floor(2 begin / P) on, so those of sequences that follow each other do not meet and 2 rows / P are enough.
+template <int P>
+__device__ __forceinline__ uint32_t place_of(const ScanArgs& a, uint32_t begin, uint32_t seq) {
+    return a.spread ? 2 * begin / P : begin / P + seq;
 }
 
 // Rows of B (or C) of a piece in LDS, as f32.
@@ -321,7 +331,8 @@ __global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a) {
     const uint32_t at = ch0 + threadIdx.x / 4;
     const bool in = at < r.channels;
     const uint32_t ch = in ? at : r.channels - 1;
-    float* const mine = a.ws + ((size_t)slot * r.channels + ch) * N + q * S;
+    const size_t place = (size_t)(place_of<P>(a, m.begin, m.seq) + m.index) * r.channels + ch;
+    float* const mine = a.ws + place * N + q * S;
     float h[S];
     if (m.index + 1 == m.count) {
         first_state<S>(a, st, ch, q, h);
@@ -359,7 +370,7 @@ __global__ __launch_bounds__(kBlock) void k_scan_pieces(ScanArgs a) {
     sum = quad_sum(sum);
     if (!in) return;
     store_state<S>(mine, h);
-    if (q == 0) a.ws[(size_t)a.pieces * r.channels * N + (size_t)slot * r.channels + ch] = sum;
+    if (q == 0) a.ws[(size_t)a.pieces * r.channels * N + place] = sum;
 }
 
 // The first states of all pieces of a sequence, in the places of what k_scan_pieces left there: a quad a channel.  A workgroup is one
@@ -373,7 +384,7 @@ __global__ __launch_bounds__(kOpWave) void k_scan_join(ScanArgs a) {
     const uint32_t blocks = (r.channels + kJoinCh - 1) / kJoinCh, i = blockIdx.x / blocks;
     const uint32_t ch = blockIdx.x % blocks * kJoinCh + lane / 4;
     const Bounds m{a.cu, a.n, r.rows, false};
-    const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = b / P + i;
+    const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = place_of<P>(a, b, i);
     if (count < 2) return;
     const int st = entry_slot(a.slots, a.n_slots, i, a.states != nullptr, lane);
     if (st < 0 || ch >= r.channels) return;
@@ -439,8 +450,9 @@ __global__ __launch_bounds__(kBlock) void k_scan_run(ScanArgs a) {
     if (m.count == 1) {
         first_state<S>(a, st, ch, q, h);
     } else {
-        load_state<S>(a.ws + ((size_t)(a.joined ? slot : m.first + m.count - 1) * r.channels + ch) * N + q * S, h);
-        if (!a.joined) join<S>(a, k, ch, q, m.first, m.index, h);
+        const uint32_t first = place_of<P>(a, m.begin, m.seq);
+        load_state<S>(a.ws + ((size_t)(first + (a.joined ? m.index : m.count - 1)) * r.channels + ch) * N + q * S, h);
+        if (!a.joined) join<S>(a, k, ch, q, first, m.index, h);
     }
     __syncthreads();
     for (uint32_t t0 = 0; t0 < m.len; t0 += kSpan) {
@@ -989,7 +1001,10 @@ redukt_scan_rows stepped(redukt_scan_rows a) {
 }
 
 uint64_t chunk_pieces(const redukt_scan_rows& a, uint32_t n_seq) { return (uint64_t)a.rows / piece_rows(a.n) + n_seq; }
-uint64_t chunk_floats(const redukt_scan_rows& a, uint32_t n_seq) { return chunk_pieces(a, n_seq) * a.channels * (a.n + 1ull); }
+// Places in ws: by sequences, or by rows alone where that takes fewer (65,536 tokens of as many sequences, 1,536 channels of 16: 6.9 GB and 214 MB).
+bool chunk_spread(const redukt_scan_rows& a, uint32_t n_seq) { return 2ull * a.rows / piece_rows(a.n) < chunk_pieces(a, n_seq); }
+uint64_t chunk_places(const redukt_scan_rows& a, uint32_t n_seq) { return chunk_spread(a, n_seq) ? 2ull * a.rows / piece_rows(a.n) : chunk_pieces(a, n_seq); }
+uint64_t chunk_floats(const redukt_scan_rows& a, uint32_t n_seq) { return chunk_places(a, n_seq) * a.channels * (a.n + 1ull); }
 
 struct GradPlan {
     uint32_t piece, per, parts_g, parts;
@@ -1040,7 +1055,7 @@ int32_t redukt_op_scan_step(const redukt_scan_rows* a, float* states, uint32_t n
     if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
     OpDevice dev(a->out);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
-    ScanArgs k{stepped(*a), states, states, n_slots, slots, nullptr, a->rows, nullptr, 0, 0};
+    ScanArgs k{stepped(*a), states, states, n_slots, slots, nullptr, a->rows, nullptr, 0, 0, 0};
     return op_launch(few ? SCAN_FN(k.r, k_scan_step, 1) : SCAN_FN(k.r, k_scan_step, 4), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
 }
 
@@ -1070,8 +1085,8 @@ int32_t redukt_op_scan_chunk(const redukt_scan_rows* a, const int32_t* cu, uint3
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     // No sequence has more pieces than the rows fill; few of them are joined by each piece itself, which saves a launch.
-    ScanArgs k{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq, (float*)workspace, (uint32_t)pieces,
-               a->rows > kJoinHere * piece_rows(a->n)};
+    ScanArgs k{stepped(*a), state_in, state_out, n_slots, slots, cu, n_seq, (float*)workspace, (uint32_t)chunk_places(*a, n_seq),
+               a->rows > kJoinHere * piece_rows(a->n), chunk_spread(*a, n_seq)};
     const dim3 grid((uint32_t)(pieces * blocks));
     if (need) {
         int32_t rc = op_launch(SCAN_FN(k.r, k_scan_pieces), grid, dim3(kBlock), 0, stream, k);
@@ -1108,7 +1123,7 @@ int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* 
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     GradArgs k{};
-    k.a = ScanArgs{stepped(*a), state_in, nullptr, n_seq, nullptr, cu, n_seq, (float*)workspace, (uint32_t)p.pieces, a->rows > kJoinHere * p.piece};
+    k.a = ScanArgs{stepped(*a), state_in, nullptr, n_seq, nullptr, cu, n_seq, (float*)workspace, (uint32_t)p.pieces, a->rows > kJoinHere * p.piece, 0};
     k.g = *g;
     if (a->rows == 1) {
         k.g.dout_stride = k.g.dx_stride = k.g.ddt_stride = k.g.dz_stride = a->channels;

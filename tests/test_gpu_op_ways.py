@@ -55,6 +55,35 @@ def test_scan_chunk_of_many_pieces(lens, joined, n, dtype):
     sequences(lens, 70, n, 1, dtype, initial=True, before_rows=2, behind=3, seed=n)
 
 
+# Many sequences, most of them of one piece: places in the workspace go by rows.  (The second half: those of more follow each other closely.)
+SPREAD = [([1] * 300 + [130, 64, 65, 0, 200, 33] + [2] * 40, False), ([1] * 200 + [2200, 3, 65, 66] + [0] * 30, True),
+          ([65, 65, 66, 129, 65] * 3 + [1] * 40, False), ([33, 33, 34, 65, 33] * 4 + [0, 1] * 30, False)]
+
+
+@types
+@pytest.mark.parametrize("n", [16, 64])
+@pytest.mark.parametrize("way", range(len(SPREAD)))
+def test_scan_chunk_of_many_sequences(way, n, dtype):
+    sequences(SPREAD[way][0], 70, n, 1, dtype, initial=True, before_rows=way, behind=3, seed=n)
+
+
+@pytest.mark.parametrize("way", range(len(SPREAD)))
+def test_scan_chunk_of_many_sequences_in_place_and_alone(way):
+    """The same bits in place, and of each long sequence in a call of its own (whose places go by sequences)."""
+    lens = SPREAD[way][0]
+    x = layer(sum(lens), 70, 16, 1, BF16)
+    cu = torch.from_numpy(np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)).cuda()
+    first, last = pool_of(len(lens), 70, 16), torch.empty(len(lens), 70, 16, device="cuda")
+    want = ops.scan_chunk(cu_seqlens=cu, state_in=first, state_out=last, **x)
+    pool = first.clone()
+    assert torch.equal(ops.scan_chunk(cu_seqlens=cu, state_in=pool, state_out=pool, **x), want) and torch.equal(pool, last)
+    for i, n in enumerate(lens):
+        if n > 64:
+            r, one = slice(int(cu[i]), int(cu[i + 1])), torch.empty(1, 70, 16, device="cuda")
+            alone = ops.scan_chunk(cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device="cuda"), state_in=first[i:i + 1], state_out=one, **rows_of(x, r))
+            assert torch.equal(alone, want[r]) and torch.equal(one[0], last[i]), i
+
+
 # ---------------------------------------------------------------- gradients of the scan
 
 # lengths, channels, groups; then by states of up to 16 parts and of more: blocks of channels that a workgroup takes, whether a launch

@@ -128,9 +128,12 @@ def test_the_scans_shapes_choose_their_ways(launched):
     sizes = (8, 16, 32, 64)
     for (((name, *_),), n) in zip(launched([["step", [*s, n, 2]] for s in ways.STEPS for n in sizes]), sizes * len(ways.STEPS)):
         assert kernel(name) == ("k_scan_step", (n // 4, 4))
-    calls = [(lens, joined, n) for lens, joined in ways.CHUNKS for n in sizes]
+    calls = [(lens, joined, n) for lens, joined in ways.CHUNKS for n in sizes] + [(lens, joined, 16) for lens, joined in ways.SPREAD]
     for (lens, joined, n), launches in zip(calls, launched([["chunk", [sum(l), len(l), 70, 1, n, 2]] for l, _, n in calls])):
         assert [kernel(l[0]) for l in launches] == [(f, (n // 4,)) for f in ["k_scan_pieces"] + ["k_scan_join"] * joined + ["k_scan_run"]]
+    for lens, _ in ways.SPREAD:
+        for n, piece in ((16, 64), (64, 32)):
+            assert ops.scan_chunk_workspace(sum(lens), len(lens), 70, 1, n) == 2 * sum(lens) // piece * 70 * (n + 1) * 4
 
 
 def test_the_gradients_shapes_choose_their_ways(launched):
