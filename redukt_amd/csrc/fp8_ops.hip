@@ -586,18 +586,23 @@ int32_t redukt_op_fp8_matmul(const redukt_fp8_matmul* a, void* stream) {
         if (!op_grid_ok(grid, kBlock)) return BACKEND_INVALID_ARGUMENT;
         return op_launch(OP_BY_TYPE(k.dtype, k_fp8_bytes), dim3((uint32_t)grid), dim3(kBlock), 0, stream, k);
     }
-    // The choice is by time (us on either side of each edge, bf16; n and k after m).  Few tokens: weights straight into registers (16 of 4,096 x
-    // 4,096 7.6, tiles 10.1; 8 of 768 x 4,096 5.9 and 9.8), fewer of them where the channels alone fill the CUs with tiles (8 of 8,192 x 8,192
-    // 16.7 and 17.3; 8 of 50,280 x 768 12.3 and 9.1, 1 9.9 and 9.0, with f32 outputs 10.1 and 10.4).
-    if (k.m <= (k.n >= 16384 ? 2 : k.n >= 8192 ? 8 : 16)) return few(k, stream);
-    // Tiles of 256 once they nearly fill the CUs (8,192 of 1,536 x 768, 192 tiles: 17.3, of 128: 19.8), of 128 once a CU has two (2,048 of
-    // 4,096 x 4,096, 512 tiles: 41.4, 64 x 128 50.2; 1,024 of 4,096 x 4,096, 256: 29.8 and 27.3), of 64 x 128 once each CU has one (512 of
-    // 4,096 x 4,096, 256 tiles: 17.2, of 64 18.5; 1,000 of 1,536 x 768, 192: 6.0 and 5.4), else of 64, with more stages where a CU has
-    // one workgroup only (128 of 8,192 x 8,192, 256 tiles: four stages 21.2, two 37.1; 1,000 of 1,536 x 768, 384: 6.2 and 5.4), by 32 channels
-    // where half of the CUs would have none (64 of 8,192 x 8,192: 18.0, by 64 20.0; 128 of 768 x 4,096 10.0 and 10.8).
+    // The choice is by time (us on either side of each edge, bf16 where nothing else is said, weights from memory; n x k after m).  Few tokens:
+    // weights straight into registers (8 of 768 x 4,096 6.1, tiles 9.4; of 8,192 x 8,192 17.9 and 19.5; of 16,384 x 4,096 17.4 and 17.1, f32 17.3 and
+    // 19.1; of 50,280 x 768 12.6 and 14.2, 4 of 50,280 x 4,096 51 and 60).  More of them where the channels alone give too few CUs a tile (16 of 4,096 x
+    // 8,192 14.3 and 16.9, of 8,192 x 8,192 20.6 and 19.6), longer with f32 outputs, whose tiles take twice the matrix work (16 of 8,192 x 8,192 20.6
+    // and 30.3, of 16,384 x 4,096 20.7 and 19.4).
+    if (k.m <= 8 || (k.m <= 16 && k.n < (k.dtype == REDUKT_OP_F32 ? 16384 : 8192))) return few(k, stream);
+    // Tiles of 256 once they nearly fill the CUs (8,192 of 1,536 x 768, 192 tiles: 16.0, of 128: 16.9), of 128 once a CU has two (2,048 of
+    // 4,096 x 4,096, 512 tiles: 38.3, 64 x 128 47.5; 1,024 of 4,096 x 4,096, 256: 28.9 and 26.2; f32 64.6 and 75.6, 42.8 and 40.7), either with more
+    // tokens than half of a tile's (160 of 50,280 x 768 16.1, of 128 19.0; 128 of them 15.3 and 12.2; 80 of them 11.6, 64 x 128 13.9; 64 of them 11.3 and
+    // 10.4, f32 17.3 and 14.1), of 64 x 128 once each CU has one (512 of
+    // 4,096 x 4,096, 256 tiles: 16.5, of 64 17.8; 1,000 of 1,536 x 768, 192: 6.3 and 6.2; f32 28.6 and 27.5, 8.7 and 7.9), else of 64, with more stages
+    // where a CU has one workgroup only (128 of 8,192 x 8,192, 256 tiles: four stages 28.5, two 52.4, f32 36.3 and 53.0; 1,000 of 1,536 x 768, 384: 6.4
+    // and 6.2), by 32 channels where half of the CUs would have none (64 of 8,192 x 8,192: 23.1, by 64 29.1; 128 of 768 x 4,096 9.7 and 11.0, f32
+    // 17.1 and 18.9).
     const auto count = [&](uint32_t tm, uint32_t tn) { return (uint64_t)((k.m + tm - 1) / tm) * ((k.n + tn - 1) / tn); };
-    if (count(256, 256) >= 160 && k.dtype != REDUKT_OP_F32) return tiles16<256, 256, 2, 4, 2>(k, stream);
-    if (count(128, 128) >= 384) return tiles<128, 128, 2, 2, 2>(k, stream);
+    if (k.m > 128 && count(256, 256) >= 160 && k.dtype != REDUKT_OP_F32) return tiles16<256, 256, 2, 4, 2>(k, stream);
+    if (k.m > 64 && count(128, 128) >= 384) return tiles<128, 128, 2, 2, 2>(k, stream);
     if (count(64, 128) >= 256) return tiles<64, 128, 2, 2, 3>(k, stream);
     if (count(64, 64) > 256) return tiles<64, 64, 2, 2, 2>(k, stream);
     if (count(64, 64) > 128) return tiles<64, 64, 2, 2, 4>(k, stream);

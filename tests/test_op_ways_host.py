@@ -124,6 +124,17 @@ def test_the_products_shapes_reach_every_kernel_with_more_blocks_than_it_has_sta
         assert len([s for s in ways.DEEP if s[2] % 128 == 0]) == 0
 
 
+def test_products_of_few_tokens_take_no_tiles_that_are_mostly_empty(launched):
+    shapes = [(m, n, k) for m in (1, 2, 4, 8, 9, 16, 17, 32, 64, 65, 100, 128, 129, 200) for n, k in ((4096, 4096), (8192, 768), (50280, 768), (131072, 4096))]
+    for dtype in (0, 2):
+        for (m, n, k), ((name, *_),) in zip(shapes, launched([["fp8", [dtype, *s]] for s in shapes])):
+            fn, t = kernel(name)
+            if m <= 8:
+                assert fn == "k_fp8_few", (m, n, k, dtype)
+            elif m > 16 or fn != "k_fp8_few":
+                assert fn == "k_fp8_tiles" and (t[0] == 64 or m > t[0] // 2), (m, n, k, dtype)
+
+
 def test_the_scans_shapes_choose_their_ways(launched):
     sizes = (8, 16, 32, 64)
     for (((name, *_),), n) in zip(launched([["step", [*s, n, 2]] for s in ways.STEPS for n in sizes]), sizes * len(ways.STEPS)):
