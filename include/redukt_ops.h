@@ -103,7 +103,9 @@ uint64_t redukt_op_delta_chunk_workspace(const redukt_delta_rows* a, uint32_t n_
  * channel), B and C [n] (of the channel's group) makes, with s = ln(1 + e^(dt + dt_bias)),
  *     h <- e^(s a) h + s x B        out = (C . h + d x) z / (1 + e^-z)
  * in f32, rounded once to `dtype`; without z its factor is 1, without d or dt_bias they are 0.  A dt of
- * -inf leaves the state as it is.  The rule is stable for a <= 0.  A value that is not finite goes where
+ * -inf leaves the state as it is.  The rule is stable for a <= 0.  (With a > 0, scan_chunk and scan_grad form powers over up to
+ * 64 tokens at once: where one passes f32's range, states and gradients become inf or NaN, zeros among them, that token by
+ * token would be finite.)  A value that is not finite goes where
  * the rule takes it: one of x or dt into its channel, one of B into its group's channels, from its
  * token on; one of C or z into its token.  A power below 2^-126 is 0. */
 typedef struct {

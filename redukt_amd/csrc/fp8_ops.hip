@@ -238,7 +238,7 @@ __global__ __launch_bounds__(kBlock) void k_fp8_bytes(redukt_fp8_matmul a) {
 // Few tokens: the weights are read once, straight into registers.  Of a workgroup's eight waves `split` share 16 channels, each
 // taking every split-th block of columns; their sums meet in LDS.  Workgroups begin at different columns, so that rows of a power of two do
 // not all wait for one channel of a cache.  Bound by the weights' bytes: one token of 50,280 x 768, 38.6 MB, 9.9 us with the launch (3.9 TB/s), of
-// 8,192 x 8,192 67 MB in 13.6 (4.9).
+// 8,192 x 8,192 67 MB in 16.4 (4.1; where part of it is still in cache 13.6).
 struct Fp8Few {
     redukt_fp8_matmul a;
     uint32_t split;
