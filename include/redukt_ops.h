@@ -163,8 +163,8 @@ typedef struct {
  * read.  dstate_in (NULL: not wanted; not one of the others) takes that of the first states.  Rows of no
  * sequence get gradients of zero.  Everything is formed anew from the inputs, sums over channels, tokens
  * and sequences in f32 in a fixed order.  workspace: redukt_op_scan_grad_workspace(a, n_seq) bytes, which are about
- * 12 channels (n + 1) for each sequence and each 64 rows (16 to 64 of them in small calls), and 8 n for each row and
- * 64 to 256 channels. */
+ * 4 channels (n + 2) for each sequence, 20 channels (n + 1) at most for each 64 rows (16 to 64 of them in small calls), and 8 n
+ * for each row and 64 to 256 channels. */
 int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* g, const int32_t* cu, uint32_t n_seq,
                             const float* state_in, const float* dstate_out, float* dstate_in, void* workspace,
                             uint64_t workspace_bytes, void* stream);

@@ -230,12 +230,12 @@ struct Bounds {
     }
 };
 
-// A piece: rows [t0, t0 + len) are number `index` of `count` pieces of sequence seq, whose first one is in slot `first`.  Sequence i's pieces
+// A piece: rows [t0, t0 + len) are number `index` of `count` pieces of sequence seq.  Sequence i's pieces
 // have the slots from rows / P + i on (its first row's), so those of one are consecutive, those of the next begin after them, and
 // rows / P + n slots are enough.  len is 0 in the slot of a sequence without rows (index 0, count 0) and in unused ones (index > 0).
 // Row `begin` is the sequence's first one.
 struct Piece {
-    uint32_t seq, t0, len, index, count, first, begin;
+    uint32_t seq, t0, len, index, count, begin;
 };
 
 template <int P>
@@ -247,7 +247,7 @@ __device__ __forceinline__ Piece piece_of(const Bounds& m, uint32_t slot) {
         else hi = mid - 1;
     }
     const uint32_t b = m.at(lo), e = max(m.at(lo + 1), b), first = b / P + lo;
-    Piece k{lo, 0, 0, slot - first, (e - b + P - 1) / P, first, b};
+    Piece k{lo, 0, 0, slot - first, (e - b + P - 1) / P, b};
     if (slot < first) k.index = ~0u, k.count = 0;          // (boundaries that decrease)
     if (k.index < k.count) {
         k.t0 = b + k.index * P;
@@ -520,9 +520,10 @@ struct GradArgs {
     redukt_scan_grads g;
     const float* dlast;        // null: zeros
     float* dfirst;             // null: not wanted
-    float* back;               // r_p [pieces][channels][n] (joined: R_(p+1))
+    float* back;               // r_p [places][channels][n] (joined: R_(p+1))
     float* bc;                 // dB, dC of a workgroup's channels: [parts][rows][2 n]
-    float* tok;                // da, then dd and ddt_bias of a piece: [pieces][channels][n], [pieces][channels][2]
+    float* tok;                // da, then dd and ddt_bias of a piece: [slots][channels][n], [slots][channels][2]
+    uint32_t slots;            // of pieces
     uint32_t per;              // blocks of 64 channels of a workgroup
     uint32_t parts, parts_g;   // workgroups along the channels, of all groups and of one
 };
@@ -588,20 +589,20 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_pieces(GradArgs ga) {
     }
     sum = quad_sum(sum);
     if (!in) return;
-    const size_t mine = ((size_t)slot * r.channels + ch) * N + q * S;
-    store_state<S>(a.ws + mine, h);
-    store_state<S>(ga.back + mine, back);
-    if (q == 0) a.ws[(size_t)a.pieces * r.channels * N + (size_t)slot * r.channels + ch] = sum;
+    const size_t place = (size_t)(place_of<P>(a, m.begin, m.seq) + m.index) * r.channels + ch;
+    store_state<S>(a.ws + place * N + q * S, h);
+    store_state<S>(ga.back + place * N + q * S, back);
+    if (q == 0) a.ws[(size_t)a.pieces * r.channels * N + place] = sum;
 }
 
 // R_(p+1) of piece p, from the pieces behind it.
 template <int S>
-__device__ __forceinline__ void join_back(const GradArgs& g, const Channel<S>& k, uint32_t ch, int q, const Piece& m, float (&R)[S]) {
+__device__ __forceinline__ void join_back(const GradArgs& g, const Channel<S>& k, uint32_t ch, int q, const Piece& m, uint32_t first, float (&R)[S]) {
     const redukt_scan_rows& r = g.a.r;
     const float* const sums = g.a.ws + (size_t)g.a.pieces * r.channels * (4 * S);
 #pragma unroll 4
     for (uint32_t p = m.count - 1; p > m.index; p--) {
-        const size_t at = (size_t)(m.first + p) * r.channels + ch;
+        const size_t at = (size_t)(first + p) * r.channels + ch;
         float l[S];
         load_state<S>(g.back + at * (4 * S) + q * S, l);
         const float s = sums[at];
@@ -626,7 +627,7 @@ __global__ __launch_bounds__(kOpWave) void k_scan_grad_join(GradArgs ga) {
     const uint32_t blocks = (r.channels + kJoinCh - 1) / kJoinCh, i = blockIdx.x / blocks + 1;
     const uint32_t ch = blockIdx.x % blocks * kJoinCh + lane / 4;
     const Bounds m{ga.a.cu, ga.a.n, r.rows, true};
-    const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = b / P + i;
+    const uint32_t b = m.at(i), e = max(m.at(i + 1), b), count = (e - b + P - 1) / P, first = place_of<P>(ga.a, b, i);
     if (count < 2 || ch >= r.channels) return;
     const bool backward = blockIdx.y;
     const Channel<S> k = channel_of<S>(r, ch, q);
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_run(GradArgs ga) {
     const Piece m = piece_of<P>(Bounds{a.cu, a.n, r.rows, true}, slot);
     const bool none = m.len == 0 || m.seq == 0 || m.seq == a.n + 1;
     float* const tok_a = ga.tok;
-    float* const tok_d = ga.tok + (size_t)a.pieces * r.channels * N;
+    float* const tok_d = ga.tok + (size_t)ga.slots * r.channels * N;
     if (!none) {
         stage<T, N>(sb, r.b, r.b_stride, m.t0, m.len, gr);
         stage<T, N>(sc, r.c, r.c_stride, m.t0, m.len, gr);
@@ -750,14 +751,16 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_run(GradArgs ga) {
         } else {
             const Channel<S> k = channel_of<S>(r, ch, q);
             float h[S];
+            const uint32_t first = place_of<P>(a, m.begin, m.seq);
             if (a.joined && m.count > 1) {
-                load_state<S>(a.ws + mine * N + q * S, h);
-                load_state<S>(ga.back + mine * N + q * S, G);
+                const size_t place = (size_t)(first + m.index) * r.channels + ch;
+                load_state<S>(a.ws + place * N + q * S, h);
+                load_state<S>(ga.back + place * N + q * S, G);
             } else {
                 state_or_zeros<S>(a.in, m.seq - 1, r.channels, ch, q, h);
                 state_or_zeros<S>(ga.dlast, m.seq - 1, r.channels, ch, q, G);
-                join<S>(a, k, ch, q, m.first, m.index, h);
-                join_back<S>(ga, k, ch, q, m, G);
+                join<S>(a, k, ch, q, first, m.index, h);
+                join_back<S>(ga, k, ch, q, m, first, G);
             }
             if (!in) {
 #pragma unroll
@@ -921,12 +924,12 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_columns(GradArgs ga) {
     const uint64_t wide = (uint64_t)r.channels * r.n, narrow = (uint64_t)r.channels * 2;
     const uint64_t col = (uint64_t)blockIdx.x * kOpWave + threadIdx.x % kOpWave;
     const bool in = col < wide + narrow, of_a = col < wide;
-    const float* const from = of_a ? ga.tok + col : ga.tok + (uint64_t)ga.a.pieces * wide + (col - wide);
+    const float* const from = of_a ? ga.tok + col : ga.tok + (uint64_t)ga.slots * wide + (col - wide);
     const uint64_t step = of_a ? wide : narrow;
     float v = 0.0f;
     if (in) {
 #pragma unroll 8
-        for (uint32_t p = threadIdx.x / kOpWave; p < ga.a.pieces; p += kBlock / kOpWave) v += from[p * step];
+        for (uint32_t p = threadIdx.x / kOpWave; p < ga.slots; p += kBlock / kOpWave) v += from[p * step];
     }
     half[threadIdx.x] = v;
     __syncthreads();
@@ -1008,8 +1011,8 @@ uint64_t chunk_floats(const redukt_scan_rows& a, uint32_t n_seq) { return chunk_
 
 struct GradPlan {
     uint32_t piece, per, parts_g, parts;
-    bool small;
-    uint64_t pieces, bc, tok, bytes;
+    bool small, spread;
+    uint64_t pieces, places, bc, tok, bytes;
 };
 
 GradPlan grad_plan(const redukt_scan_rows& a, uint32_t n_seq) {
@@ -1027,10 +1030,12 @@ GradPlan grad_plan(const redukt_scan_rows& a, uint32_t n_seq) {
     while (p.per > 1 && p.pieces * a.groups * ((blocks + p.per - 1) / p.per) < 1024) p.per /= 2;
     p.parts_g = (blocks + p.per - 1) / p.per;
     p.parts = p.parts_g * a.groups;
-    const uint64_t states = p.pieces * a.channels * a.n;
+    p.spread = 2ull * a.rows / p.piece < p.pieces;
+    p.places = p.spread ? 2ull * a.rows / p.piece : p.pieces;
+    const uint64_t states = p.places * a.channels * a.n;
     p.bc = (uint64_t)p.parts * a.rows * 2 * a.n;
-    p.tok = states + p.pieces * a.channels * 2;
-    p.bytes = 4 * (states + p.pieces * a.channels + states + p.tok + p.bc + 12);
+    p.tok = p.pieces * a.channels * (a.n + 2ull);
+    p.bytes = 4 * (states + p.places * a.channels + states + p.tok + p.bc + 12);
     return p;
 }
 
@@ -1123,17 +1128,18 @@ int32_t redukt_op_scan_grad(const redukt_scan_rows* a, const redukt_scan_grads* 
     OpDevice dev(cu);
     if (!dev.ok) return BACKEND_INVALID_ARGUMENT;
     GradArgs k{};
-    k.a = ScanArgs{stepped(*a), state_in, nullptr, n_seq, nullptr, cu, n_seq, (float*)workspace, (uint32_t)p.pieces, a->rows > kJoinHere * p.piece, 0};
+    k.a = ScanArgs{stepped(*a), state_in, nullptr, n_seq, nullptr, cu, n_seq, (float*)workspace, (uint32_t)p.places, a->rows > kJoinHere * p.piece, p.spread};
     k.g = *g;
     if (a->rows == 1) {
         k.g.dout_stride = k.g.dx_stride = k.g.ddt_stride = k.g.dz_stride = a->channels;
         k.g.db_stride = k.g.dc_stride = bc;
     }
     k.dlast = dstate_out, k.dfirst = dstate_in;
-    const uint64_t states = p.pieces * a->channels * a->n;
-    k.back = k.a.ws + round4(states + p.pieces * a->channels);
+    const uint64_t states = p.places * a->channels * a->n;
+    k.back = k.a.ws + round4(states + p.places * a->channels);
     k.tok = k.back + states;
     k.bc = k.tok + round4(p.tok);
+    k.slots = (uint32_t)p.pieces;
     k.per = p.per, k.parts = p.parts, k.parts_g = p.parts_g;
     if (a->rows > p.piece) {
         const void* const fn = p.small ? SCAN_FN(k.a.r, k_scan_grad_pieces, true) : SCAN_FN(k.a.r, k_scan_grad_pieces, false);

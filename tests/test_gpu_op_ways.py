@@ -87,7 +87,7 @@ def test_scan_chunk_of_many_sequences_in_place_and_alone(way):
 # ---------------------------------------------------------------- gradients of the scan
 
 # lengths, channels, groups; then by states of up to 16 parts and of more: blocks of channels that a workgroup takes, whether a launch
-# of its own joins the pieces.  None is small enough for the shorter pieces.
+# of its own joins the pieces.  None is small enough for the shorter pieces, but the last two.
 GRAD_WAYS = {
     "four-blocks": ([5] * 200 + [150, 0, 64, 65, 200], 1100, 1, ((4, False), (4, True))),
     "four-blocks-few-rows": ([2] * 250 + [100, 64, 33, 250], 1100, 1, ((4, False), (4, False))),
@@ -95,7 +95,10 @@ GRAD_WAYS = {
     "two-or-four-blocks-joined": ([1] * 450 + [1100, 130, 700, 129], 500, 1, ((2, True), (4, True))),
     "a-block-each-joined": ([70] * 40, 640, 1, ((1, True), (1, True))),
     "a-block-each": ([100] * 10, 1100, 1, ((1, False), (1, False))),
+    "many-in-short-pieces": ([1] * 30 + [33, 65, 0, 40, 66] + [2] * 9, 70, 1, ((1, False), (1, False))),
+    "many-in-short-pieces-joined": ([1] * 50 + [1100, 33], 70, 1, ((1, True), (1, True))),
 }
+SHORT_WAYS = {"many-in-short-pieces", "many-in-short-pieces-joined"}
 
 
 def grad_way(lens, ch, groups, n):
@@ -106,7 +109,8 @@ def grad_way(lens, ch, groups, n):
     pieces, per = rows // piece + len(lens) + 2, 4
     while per > 1 and pieces * groups * -(-blocks // per) < 1024:
         per //= 2
-    floats = pieces * ch * (3 * n + 3) + -(-blocks // per) * groups * rows * 2 * n + 12
+    places = min(pieces, 2 * rows // piece)     # (for sequences of more than one piece)
+    floats = places * ch * (2 * n + 1) + pieces * ch * (n + 2) + -(-blocks // per) * groups * rows * 2 * n + 12
     return short, per, rows > 32 * piece, 4 * floats
 
 

@@ -153,12 +153,12 @@ def test_the_gradients_shapes_choose_their_ways(launched):
     for (name, n), launches in zip(calls, launched(args)):
         lens, ch, groups, want = ways.GRAD_WAYS[name]
         short, per, joined, size = ways.grad_way(lens, ch, groups, n)
-        assert not short and (per, joined) == want[n > 16], (name, n)
+        assert short == (name in ways.SHORT_WAYS) and (per, joined) == want[n > 16], (name, n)
         assert size == ops.scan_grad_workspace(sum(lens), len(lens), ch, groups, n)
         fns = [kernel(l[0]) for l in launches]
         assert [f for f, _ in fns] == ["k_scan_grad_pieces"] + ["k_scan_grad_join"] * joined + ["k_scan_grad_run", "k_scan_grad_rows", "k_scan_grad_columns"]
-        assert all(t == (n // 4, 0) for f, t in fns[:-2])
-        pieces = sum(lens) // (64 if n <= 16 else 32) + len(lens) + 2
+        assert all(t == (n // 4, int(short)) for f, t in fns[:-2])
+        pieces = sum(lens) // ((64 if n <= 16 else 32) // (1 + short)) + len(lens) + 2
         assert int(launches[-3][1]) == pieces * groups * -(-(-(-(ch // groups) // 64)) // per)
 
 
