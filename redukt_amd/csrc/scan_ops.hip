@@ -100,10 +100,10 @@ struct ScanArgs {
     const int32_t* slots;
     const int32_t* cu;         // null: one row an entry
     uint32_t n;                // entries
-    float* ws;                 // pieces: states [pieces][channels][n], then the sums of their time steps [pieces][channels]
-    uint32_t pieces;           // places in ws
-    uint32_t joined;           // the first states of all pieces are in ws (k_scan_join)
-    uint32_t spread;           // which place a piece has (place_of)
+    float* ws;                 // pieces: states [places][channels][n], then the sums of their time steps [places][channels]
+    uint32_t pieces;           // places
+    uint16_t joined;           // the first states of all pieces are in ws (k_scan_join)
+    uint16_t spread;           // which place a piece has (place_of)
 };
 
 // A lane's parts of its channel's a (times log2 e), and d and dt_bias.
@@ -261,7 +261,7 @@ __device__ __forceinline__ Piece piece_of(const Bounds& m, uint32_t slot) {
 // as its pieces at least, from floor(2 begin / P) on, so those of sequences that follow each other do not meet and 2 rows / P are enough.
 template <int P>
 __device__ __forceinline__ uint32_t place_of(const ScanArgs& a, uint32_t begin, uint32_t seq) {
-    return a.spread ? 2 * begin / P : begin / P + seq;
+    return __builtin_amdgcn_readfirstlane(a.spread ? 2 * begin / P : begin / P + seq);      // (a wave has one sequence)
 }
 
 // Rows of B (or C) of a piece in LDS, as f32.
@@ -718,6 +718,7 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_run(GradArgs ga) {
     const uint32_t block0 = part % ga.parts_g * ga.per, block1 = min(block0 + ga.per, blocks_g);
     const Piece m = piece_of<P>(Bounds{a.cu, a.n, r.rows, true}, slot);
     const bool none = m.len == 0 || m.seq == 0 || m.seq == a.n + 1;
+    const uint32_t first = place_of<P>(a, m.begin, m.seq);
     float* const tok_a = ga.tok;
     float* const tok_d = ga.tok + (size_t)ga.slots * r.channels * N;
     if (!none) {
@@ -751,7 +752,6 @@ __global__ __launch_bounds__(kBlock) void k_scan_grad_run(GradArgs ga) {
         } else {
             const Channel<S> k = channel_of<S>(r, ch, q);
             float h[S];
-            const uint32_t first = place_of<P>(a, m.begin, m.seq);
             if (a.joined && m.count > 1) {
                 const size_t place = (size_t)(first + m.index) * r.channels + ch;
                 load_state<S>(a.ws + place * N + q * S, h);
